@@ -35,7 +35,8 @@ typedef enum mllmb200_status {
   MLLMB200_CUDA_ERROR = 3,    /* a CUDA runtime call failed; see mllmb200_last_cuda_error() */
   MLLMB200_TIMEOUT = 4,       /* a bounded device-side wait ran out (reported by mllmb200_check_device_status) */
   MLLMB200_BAD_BLOB = 5,      /* pre-pack blob header does not match (magic, version, sizes) */
-  MLLMB200_TOO_LARGE = 6      /* request exceeds a fixed capacity (static scratch entry point) */
+  MLLMB200_TOO_LARGE = 6,     /* request exceeds a fixed capacity (static scratch entry point) */
+  MLLMB200_BAD_PAGE = 7       /* a page number or a length outside of a paged cache (reported by mllmb200_lm_operator_status) */
 } mllmb200_status;
 
 /* How the 2-byte per-group scale is encoded.

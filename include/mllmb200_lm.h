@@ -122,6 +122,81 @@ MLLMB200_API void* mllmb200_lm_stream(void* handle);
 MLLMB200_API const char* mllmb200_lm_last_error(void* handle);
 MLLMB200_API int mllmb200_lm_check_device_status(void* handle);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Operators on the caller's device memory, on the caller's stream and the current device: a key-value cache in pages,
+ * attention of new tokens over it, and verification of drafted tokens.  They allocate nothing and never synchronize (they
+ * can be captured into a CUDA graph, every call of it with a workspace of its own); results are valid when the stream
+ * reaches them.  Tables, lengths and row starts are device memory and may change between replays of a graph. */
+
+enum { MLLMB200_LM_F16 = 2 };  /* caches and queries in fp16 (beside MLLMB200_LM_BF16) */
+
+/* A layer's cache: position j of sequence s lies in page table[s * ld_table + j / page], row j % page.  Pages may lie in
+ * any order; strides are in elements (multiples of 8; rows are contiguous), pointers 16-byte aligned.
+ * Sequence s brings the rows [q_start[s], q_start[s + 1]) of a call (q_start NULL: rows / seqs each) and is
+ * lengths[s] tokens long with them: its row t stands at position lengths[s] - n + t.  Rows at negative positions see nothing
+ * (attention: zeros) and are not stored; rows from q_start[seqs] on are neither read nor written.
+ * A page number outside [0, pages): what the page would hold is taken as zeros and is not stored.  A length beyond
+ * max_pages pages counts as max_pages pages.  Both make mllmb200_lm_operator_status report MLLMB200_BAD_PAGE.  Page numbers of
+ * positions that no row of the call sees are not read. */
+typedef struct mllmb200_lm_pages {
+  void *k, *v;                       /* dim numbers per key, vdim per value */
+  long long k_page, k_head, k_row, v_page, v_head, v_row;
+  const int *table, *lengths, *q_start;
+  int dtype;                         /* MLLMB200_LM_BF16 or MLLMB200_LM_F16 */
+  int pages, page;                   /* their number, and tokens in each: a multiple of 16 */
+  int kv_heads, dim, vdim;           /* sizes: multiples of 16 up to 256 */
+  int ld_table, max_pages;           /* row stride of the table, and the pages that a row names at most */
+  int seqs, rows;
+} mllmb200_lm_pages;
+
+/* Attention of the rows' queries (same dtype) over the pages.  A row at position i sees key j if j <= i and (window == 0
+ * or j > i - window or j < keep); scores are scale q.k + bias[h][min(i - j, bias_max)]; with `sink` the softmax of head h
+ * has one more score, sink[h], without a value.  A row that sees no key gives zeros.  Scores, weights' sums and outputs are
+ * summed in fp32. */
+typedef struct mllmb200_lm_look {
+  const void* q;                     /* [rows][heads][dim] */
+  void* out;                         /* [rows][heads][vdim] */
+  long long q_row, q_head, out_row, out_head;
+  const float* sink;                 /* [heads] or NULL */
+  const float* bias;                 /* [heads][bias_max + 1] or NULL */
+  int heads;                         /* a multiple of kv_heads, at most 64 per key head */
+  int bias_max, window, keep;
+  float scale;
+} mllmb200_lm_look;
+
+/* New keys [rows][kv_heads][dim] and values [rows][kv_heads][vdim] into the pages (strides as above). */
+MLLMB200_API int mllmb200_lm_pages_append(const mllmb200_lm_pages* pages, const void* k, long long k_row, long long k_head,
+                                          const void* v, long long v_row, long long v_head, void* stream);
+
+/* A few tokens of every sequence (q_start NULL, rows / seqs <= 16): the lengths are split over the GPU and joined. */
+MLLMB200_API int mllmb200_lm_attn_decode_workspace(const mllmb200_lm_pages* pages, const mllmb200_lm_look* look, size_t* bytes);
+MLLMB200_API int mllmb200_lm_attn_decode(const mllmb200_lm_pages* pages, const mllmb200_lm_look* look, void* workspace, void* stream);
+
+/* Any number of tokens of every sequence. */
+MLLMB200_API int mllmb200_lm_attn_prompt_workspace(const mllmb200_lm_pages* pages, const mllmb200_lm_look* look, size_t* bytes);
+MLLMB200_API int mllmb200_lm_attn_prompt(const mllmb200_lm_pages* pages, const mllmb200_lm_look* look, void* workspace, void* stream);
+
+/* Rows of logits to probabilities: exp((z - max z) / temperature) over their sum; temperature 0: 1 at the first largest.
+ * -inf gives 0; a row of nothing but -inf, zeros; a row with NaN or +inf, NaN (temperature 0: NaN is passed over).
+ * dtype: MLLMB200_LM_F32, _BF16 or _F16; out fp32. */
+MLLMB200_API int mllmb200_lm_probabilities(const void* logits, int dtype, long long ld, int rows, int vocab, float temperature,
+                                           float* out, long long ld_out, void* stream);
+
+/* Drafted tokens against the target's probabilities.  target: fp32 [seqs][drafts + 1][vocab], draft: fp32
+ * [seqs][drafts][vocab], tokens: [seqs][drafts], accept: uniform numbers in [0, 1) per draft, pick: one per sequence.  Token x
+ * at place i is accepted while accept q(x) < p(x) (products and sums in 64 bits); at the first refused place the next token
+ * comes from max(p - q, 0) (from p where that has no mass), behind the last draft from p: the lowest index whose running sum
+ * exceeds pick times the whole.  A token outside [0, vocab) ends a sequence's drafts: the next token comes from p there.
+ * Negative numbers and NaN count as 0.  accepted[s]: accepted drafts; out [seqs][drafts + 1]: these, the next token (-1 where
+ * p has no mass), and -1 behind it.  drafts may be 0: a plain draw from p. */
+MLLMB200_API int mllmb200_lm_verify(const float* target, long long t_seq, long long t_row, const float* draft, long long d_seq,
+                                    long long d_row, const int* tokens, long long ld_tokens, const float* accept,
+                                    long long ld_accept, const float* pick, int seqs, int drafts, int vocab, int* accepted,
+                                    int* out, long long ld_out, void* stream);
+
+/* Synchronizes the stream; reads and clears what these operators found wrong on the device. */
+MLLMB200_API int mllmb200_lm_operator_status(void* stream);
+
 /* Host only: the distance buckets of a bias table, out[n] for n in [0, count). */
 MLLMB200_API int mllmb200_lm_distance_buckets(int bias_rows, int bias_max, int count, int* out);
 

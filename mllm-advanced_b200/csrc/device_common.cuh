@@ -13,6 +13,7 @@ namespace mllmb200 {
 enum : unsigned {
   kDevStatusTimeout = 1u,    // a bounded wait on an mbarrier ran out
   kDevStatusBadHeader = 2u,  // tiled buffer header does not match the call's N/K
+  kDevStatusBadPage = 4u,    // page number or length outside of a paged cache
 };
 
 extern __device__ unsigned int g_device_status;

@@ -15,7 +15,10 @@ cudaError_t read_device_status(cudaStream_t st, int* status) {
     const unsigned int zero = 0;
     e = cudaMemcpyToSymbol(g_device_status, &zero, sizeof(zero));
   }
-  *status = (word & kDevStatusTimeout) ? MLLMB200_TIMEOUT : (word & kDevStatusBadHeader) ? MLLMB200_BAD_BLOB : MLLMB200_OK;
+  *status = (word & kDevStatusTimeout)     ? MLLMB200_TIMEOUT
+            : (word & kDevStatusBadHeader) ? MLLMB200_BAD_BLOB
+            : (word & kDevStatusBadPage)   ? MLLMB200_BAD_PAGE
+                                           : MLLMB200_OK;
   return e;
 }
 

@@ -181,6 +181,7 @@ const char* mllmb200_status_str(int status) {
     case MLLMB200_TIMEOUT: return "device-side wait timed out";
     case MLLMB200_BAD_BLOB: return "pre-pack blob header mismatch";
     case MLLMB200_TOO_LARGE: return "request exceeds a fixed capacity";
+    case MLLMB200_BAD_PAGE: return "page number or length outside of the cache";
     default: return "unknown status";
   }
 }

@@ -1,0 +1,843 @@
+// Operators over a key-value cache in pages (include/mllmb200_lm.h): storing new rows, attention of a few tokens per
+// sequence with the lengths split over the GPU, attention of prompts.
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+
+#include "lm_paged.h"
+
+namespace mllmb200 {
+cudaError_t read_device_status(cudaStream_t, int* status);
+
+namespace lm {
+namespace {
+
+// ------------------------------------------------------------------------------------------ append
+// One thread copies 16 bytes; grid (rows, pieces / 128).
+__global__ void __launch_bounds__(128) lm_pages_append_kernel(Paged a, const void* k, long long k_row, long long k_head, const void* v,
+                                                              long long v_row, long long v_head, uint16_t* pool_k, uint16_t* pool_v) {
+  pdl_launch_dependents();
+  pdl_wait_prior();
+  const int row = blockIdx.x, kp = a.dim / 8, vp = a.vdim / 8, i = blockIdx.y * 128 + threadIdx.x;
+  if (i >= a.kv_heads * (kp + vp)) return;
+  int s, t, n;
+  if (!a.q_start) {
+    s = row / a.tokens, t = row - s * a.tokens, n = a.tokens;
+  } else {
+    int lo = 0, hi = a.seqs;  // last s with q_start[s] <= row
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (a.q_start[mid] <= row) lo = mid;
+      else hi = mid;
+    }
+    const int2 r = paged_rows(a, lo);
+    s = lo, t = row - r.x, n = r.y;
+    if (t < 0 || t >= n) return;  // behind the last sequence
+  }
+  const int pos = paged_length(a, s) - n + t;
+  if (pos < 0) return;
+  const int place = pos / a.page, page = paged_page(a, s, place), inside = pos - place * a.page;
+  if (page < 0) return;
+  if (i < a.kv_heads * kp) {
+    const int g = i / kp, c = (i - g * kp) * 8;
+    const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(k) + row * k_row + g * k_head + c);
+    *reinterpret_cast<uint4*>(pool_k + page * a.k_page + g * a.k_head + inside * a.k_row + c) = x;
+  } else {
+    const int j = i - a.kv_heads * kp, g = j / vp, c = (j - g * vp) * 8;
+    const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(v) + row * v_row + g * v_head + c);
+    *reinterpret_cast<uint4*>(pool_v + page * a.v_page + g * a.v_head + inside * a.v_row + c) = x;
+  }
+}
+
+// ------------------------------------------------------------------------------------------ shared by the attentions
+// o += P V for 16 keys at j0 held as B fragments (mv: address of the first), P = hi + lo of the type (its rounding to 16 bits
+// would cost as much as the output's; two halves keep 2^-17 and better).  EDGE: some of the keys are not seen by some of the
+// warp's rows, and what their values hold (infinities, NaN) must not reach those rows through a weight of 0: one token
+// of the rows after the other, with the keys that it does not see as zeros.
+template <class T, int DV, bool EDGE>
+__device__ __forceinline__ void weigh_values(const Paged& a, float (&o)[DV / 8][4], const uint32_t (&hi)[4], const uint32_t (&lo)[4],
+                                             uint32_t v_addr, int j0, int lane, const int (&pos)[2], int first, int last) {
+  if constexpr (!EDGE) {
+#pragma unroll
+    for (int n = 0; n < DV / 16; ++n)
+      if (n * 16 < a.vdim) {
+        uint32_t b[4];
+        paged_ldsm_t(b, v_addr + n * 32);
+        Num<T>::mma(o[2 * n], hi, b[0], b[1]);
+        Num<T>::mma(o[2 * n + 1], hi, b[2], b[3]);
+        Num<T>::mma(o[2 * n], lo, b[0], b[1]);
+        Num<T>::mma(o[2 * n + 1], lo, b[2], b[3]);
+      }
+    return;
+  } else {
+  for (int p = first; p <= last; ++p) {
+    uint32_t keep[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int j = j0 + u * 8 + (lane & 3) * 2;
+      keep[u] = (seen_by(a, p, j) ? 0xffffu : 0u) | (seen_by(a, p, j + 1) ? 0xffff0000u : 0u);
+    }
+#pragma unroll
+    for (int n = 0; n < DV / 16; ++n)
+      if (n * 16 < a.vdim) {
+        uint32_t b[4];
+        paged_ldsm_t(b, v_addr + n * 32);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          Num<T>::mma(t, hi, b[2 * u] & keep[0], b[2 * u + 1] & keep[1]);
+          Num<T>::mma(t, lo, b[2 * u] & keep[0], b[2 * u + 1] & keep[1]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (pos[i >> 1] == p) o[2 * n + u][i] += t[i];
+        }
+      }
+  }
+  }
+}
+
+// Scores (base 2) of 16 x 8 N products of one warp for keys from j0 on: scale, bias, mask; the rows' running maxima and sums,
+// the weights in place of the scores.  ALL: every row sees every key.
+template <int N, bool ALL>
+__device__ __forceinline__ void weigh_keys(const Paged& a, float (&s)[N][4], float (&m)[2], float (&l)[2], float (&alpha)[2], int j0, int lane,
+                                           const int (&pos)[2], const float* const (&bias)[2]) {
+  float mx[2] = {m[0], m[1]};
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = j0 + n * 8 + (lane & 3) * 2 + (i & 1), r = i >> 1;
+      float x = s[n][i] * a.scale2;
+      if (a.bias && bias[r]) x = fmaf(__ldg(bias[r] + max(0, min(pos[r] - j, a.bias_max))), kPagedLog2e, x);
+      s[n][i] = ALL || seen_by(a, pos[r], j) ? x : -INFINITY;
+      mx[r] = fmaxf(mx[r], s[n][i]);
+    }
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+    const float base = mx[r] == -INFINITY ? 0.0f : mx[r];  // (nothing seen yet: every weight is 0)
+    alpha[r] = paged_exp2(m[r] - base);
+    m[r] = mx[r];
+    l[r] *= alpha[r];
+    mx[r] = base;
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[n][i] = paged_exp2(s[n][i] - mx[i >> 1]);
+      l[i >> 1] += s[n][i];
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void split_weights(const float (&s0)[4], const float (&s1)[4], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float p0 = (i >> 1 ? s1 : s0)[(i & 1) * 2], p1 = (i >> 1 ? s1 : s0)[(i & 1) * 2 + 1];
+    hi[i] = Num<T>::pack(p0, p1);
+    const float2 h = Num<T>::unpack(hi[i]);
+    lo[i] = Num<T>::pack(p0 - h.x, p1 - h.y);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ decode
+constexpr int kDecSeqs = 512;  // sequences of a launch
+constexpr int kDecCtas = kSms;
+
+// An item is (sequence, kv head, block of 16 MT rows); its keys are walked in blocks of 16 per warp.  The blocks of all
+// items, one after the other, are dealt out evenly: CTA c takes [c T / G, (c + 1) T / G).  An item that lies in one CTA is
+// finished there; of the others every CTA leaves the maximum, the sum and the unnormalized output of its share: in place 2 c + 1 where
+// the item begins in it, else in place 2 c.
+struct DecodeWork {
+  float* part_o;    // [2 G][16 MT][vdim]
+  float2* part_ml;  // [2 G][16 MT]
+  long long* base;  // [seqs + 1] blocks of a kv head and row block before every sequence
+  int row_blocks;
+};
+__device__ __forceinline__ int owner_of(long long b, long long total, int ctas) { return (int)(((b + 1) * ctas - 1) / total); }
+
+template <class T, int DV, int MT, int STAGES, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, 1) lm_paged_decode_kernel(Paged a, DecodeWork w) {
+  constexpr int kDecWarps = WARPS, kDecThreads = 32 * WARPS, kDecB = 16 * WARPS;
+  extern __shared__ __align__(16) uint8_t pd_smem[];
+  __shared__ long long s_base[kDecSeqs + 1], s_warp[kDecWarps];
+  __shared__ float s_m[kDecWarps][16 * MT], s_l[kDecWarps][16 * MT];
+  constexpr int kRows = 16 * MT;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int ldk = a.dim + 8, ldv = a.vdim + 8;
+  T* sQ = reinterpret_cast<T*>(pd_smem);
+  T* ring = sQ + kRows * ldk;                            // [warps][stages][16 keys | 16 values]
+  float* sO = reinterpret_cast<float*>(ring);            // [warps][rows][vdim], when a share is used up
+  const int stage_elems = 16 * (ldk + ldv);
+  T* mine = ring + (size_t)warp * STAGES * stage_elems;
+  pdl_launch_dependents();
+  pdl_wait_prior();
+  {  // blocks of every sequence, summed up
+    constexpr int kEach = kDecSeqs / kDecThreads;
+    long long sum[kEach], run = 0;
+    const int s0 = tid * kEach;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (s0 + i < a.seqs) {
+        const int len = paged_length(a, s0 + i);
+        run += paged_seen<kDecB>(a, len - a.tokens, len - 1).blocks;
+      }
+      sum[i] = run;
+    }
+    long long up = run;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += v;
+    }
+    if (lane == 31) s_warp[warp] = up;
+    __syncthreads();
+    up -= run;
+    for (int i = 0; i < warp; ++i) up += s_warp[i];
+    if (tid == 0) s_base[0] = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (s0 + i < a.seqs) s_base[s0 + i + 1] = up + sum[i];
+    __syncthreads();
+    if (blockIdx.x == 0)
+      for (int i = tid; i <= a.seqs; i += kDecThreads) w.base[i] = s_base[i];
+  }
+  const int items = a.kv_heads * w.row_blocks, rows = a.group * a.tokens;  // per sequence; per kv head
+  const long long total = s_base[a.seqs] * items;
+  const int ctas = (int)min((long long)gridDim.x, total);  // (every one of them has something)
+  if ((int)blockIdx.x >= ctas) return;
+  long long b = total * blockIdx.x / ctas;
+  const long long end = total * (blockIdx.x + 1) / ctas;
+  const int mat = lane >> 3, ml = lane & 7, cr = lane >> 3, cc = lane & 7;
+  const uint32_t q_addr = smem_u32(sQ + ((mat & 1) * 8 + ml) * ldk + (mat >> 1) * 8);
+
+  while (b < end) {
+    int s = 0;
+    for (int step = kDecSeqs / 2; step; step /= 2)
+      if (s + step < a.seqs && s_base[s + step] * items <= b) s += step;
+    const int len = paged_length(a, s), p_first = len - a.tokens, p_last = len - 1;
+    const Seen seen = paged_seen<kDecB>(a, p_first, p_last);
+    const long long in_seq = b - s_base[s] * items;
+    const int item = (int)(in_seq / seen.blocks), blk0 = (int)(in_seq - (long long)item * seen.blocks);
+    const int n_blk = (int)min(end - b, (long long)(seen.blocks - blk0));
+    const bool begins = blk0 == 0, whole = begins && n_blk == seen.blocks;
+    const int kvh = item / w.row_blocks, r0 = (item - kvh * w.row_blocks) * kRows;
+    const int2 q_rows = paged_rows(a, s);
+    const T* kb = static_cast<const T*>(a.k) + kvh * a.k_head;
+    const T* vb = static_cast<const T*>(a.v) + kvh * a.v_head;
+
+    int pids = -1;  // lane i: page of this warp's slice i of 32
+    auto fetch = [&](int it) {
+      if (it < n_blk) {
+        if ((it & 31) == 0) {
+          const int j = block_key<kDecB>(seen, blk0 + it + lane) + warp * 16;
+          pids = it + lane < n_blk && j <= seen.last && (j + 15 >= seen.lo || j < seen.head) ? paged_page(a, s, j / a.page) : -1;
+        }
+        const int page = __shfl_sync(0xffffffffu, pids, it & 31), j = block_key<kDecB>(seen, blk0 + it) + warp * 16, at = j % a.page;
+        T* dk = mine + (size_t)(it % STAGES) * stage_elems;
+        T* dv = dk + 16 * ldk;
+        const T* ks = kb + (page < 0 ? 0 : page * a.k_page + at * a.k_row);
+        const T* vs = vb + (page < 0 ? 0 : page * a.v_page + at * a.v_row);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int r = cr + u * 4;
+          const bool ok = page >= 0 && seen_by_some(seen, j + r);
+          for (int c = cc * 8; c < a.dim; c += 64) paged_copy16(smem_u32(dk + r * ldk + c), ok ? ks + r * a.k_row + c : kb, ok);
+          for (int c = cc * 8; c < a.vdim; c += 64) paged_copy16(smem_u32(dv + r * ldv + c), ok ? vs + r * a.v_row + c : vb, ok);
+        }
+      }
+      paged_commit();
+    };
+#pragma unroll
+    for (int it = 0; it < STAGES - 1; ++it) fetch(it);
+    for (int i = tid; i < kRows * (a.dim / 8); i += kDecThreads) {
+      const int r = i / (a.dim / 8), c = (i - r * (a.dim / 8)) * 8, tok = (r0 + r) / a.group, hg = r0 + r - tok * a.group;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (r0 + r < rows && tok < q_rows.y)
+        x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (q_rows.x + tok) * a.q_row + (kvh * a.group + hg) * a.q_head + c);
+      *reinterpret_cast<uint4*>(sQ + r * ldk + c) = x;
+    }
+    float m[MT][2], l[MT][2], o[MT][DV / 8][4];
+    int pos[MT][2];
+    const float* bias[MT][2];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = r0 + t * 16 + (lane >> 2) + i * 8, tok = r / a.group;
+        m[t][i] = -INFINITY, l[t][i] = 0.0f;
+        pos[t][i] = r < rows ? p_first + tok : -1;
+        bias[t][i] = a.bias && r < rows ? a.bias + (size_t)(kvh * a.group + r - tok * a.group) * (a.bias_max + 1) : nullptr;
+      }
+#pragma unroll
+      for (int n = 0; n < DV / 8; ++n) o[t][n][0] = o[t][n][1] = o[t][n][2] = o[t][n][3] = 0.0f;
+    }
+    __syncthreads();
+    for (int it = 0; it < n_blk; ++it) {
+      fetch(it + STAGES - 1);
+      paged_wait<STAGES - 1>();
+      __syncwarp();
+      const int j0 = block_key<kDecB>(seen, blk0 + it) + warp * 16;
+      if (j0 <= seen.last && (j0 + 15 >= seen.lo || j0 < seen.head)) {
+        const T* tk = mine + (size_t)(it % STAGES) * stage_elems;
+        const uint32_t k_addr = smem_u32(tk + ((mat >> 1) * 8 + ml) * ldk + (mat & 1) * 8);
+        const uint32_t v_addr = smem_u32(tk + 16 * ldk + ((mat & 1) * 8 + ml) * ldv + (mat >> 1) * 8);
+        float sc[MT][2][4] = {};
+#pragma unroll 4
+        for (int kk = 0; kk < a.dim; kk += 16) {
+          uint32_t kf[4];
+          paged_ldsm(kf, k_addr + kk * 2);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            uint32_t qf[4];
+            paged_ldsm(qf, q_addr + (t * 16 * ldk + kk) * 2);
+            Num<T>::mma(sc[t][0], qf, kf[0], kf[1]);
+            Num<T>::mma(sc[t][1], qf, kf[2], kf[3]);
+          }
+        }
+        const bool all = seen_by_all(a, p_first, p_last, j0, j0 + 15);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          float alpha[2];
+          if (all) weigh_keys<2, true>(a, sc[t], m[t], l[t], alpha, j0, lane, pos[t], bias[t]);
+          else weigh_keys<2, false>(a, sc[t], m[t], l[t], alpha, j0, lane, pos[t], bias[t]);
+          if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+#pragma unroll
+            for (int n = 0; n < DV / 8; ++n) o[t][n][0] *= alpha[0], o[t][n][1] *= alpha[0], o[t][n][2] *= alpha[1], o[t][n][3] *= alpha[1];
+          }
+          uint32_t hi[4], lo[4];
+          split_weights<T>(sc[t][0], sc[t][1], hi, lo);
+          // (keys that no row sees are zeros; with one token a sequence those are all that are masked)
+          if (all || a.tokens == 1) weigh_values<T, DV, false>(a, o[t], hi, lo, v_addr, j0, lane, pos[t], 0, 0);
+          else weigh_values<T, DV, true>(a, o[t], hi, lo, v_addr, j0, lane, pos[t], max(0, p_first), p_last);
+        }
+      }
+      __syncwarp();
+    }
+    paged_wait<0>();
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], 1);
+        l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], 2);
+      }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = t * 16 + (lane >> 2) + i * 8;
+        if ((lane & 3) == 0) s_m[warp][r] = m[t][i], s_l[warp][r] = l[t][i];
+        float* so = sO + ((size_t)warp * kRows + r) * a.vdim + (lane & 3) * 2;
+#pragma unroll
+        for (int n = 0; n < DV / 8; ++n)
+          if (n * 8 < a.vdim) *reinterpret_cast<float2*>(so + n * 8) = make_float2(o[t][n][2 * i], o[t][n][2 * i + 1]);
+      }
+    __syncthreads();
+    const int slot = 2 * blockIdx.x + begins, n_rows = min(kRows, rows - r0);
+    for (int i = tid; i < n_rows * a.vdim; i += kDecThreads) {
+      const int r = i / a.vdim, d = i - r * a.vdim, tok = (r0 + r) / a.group, h = kvh * a.group + r0 + r - tok * a.group;
+      const float sink = whole && a.sink ? a.sink[h] * kPagedLog2e : -INFINITY;
+      float mx = sink;
+#pragma unroll
+      for (int u = 0; u < kDecWarps; ++u) mx = fmaxf(mx, s_m[u][r]);
+      const float base = mx == -INFINITY ? 0.0f : mx;
+      float sum = whole && a.sink ? exp2f(sink - base) : 0.0f, v = 0.0f;
+#pragma unroll
+      for (int u = 0; u < kDecWarps; ++u) {
+        const float f = exp2f(s_m[u][r] - base);
+        sum = fmaf(f, s_l[u][r], sum);
+        v = fmaf(f, sO[(size_t)u * kRows * a.vdim + i], v);
+      }
+      if (whole) {
+        if (tok < q_rows.y) {
+          T* out = static_cast<T*>(a.out) + (q_rows.x + tok) * a.out_row + h * a.out_head + d;
+          *out = T(p_first + tok < 0 ? 0.0f : v / sum);
+        }
+      } else {
+        w.part_o[((size_t)slot * kRows + r) * a.vdim + d] = v;
+        if (d == 0) w.part_ml[(size_t)slot * kRows + r] = make_float2(mx, sum);
+      }
+    }
+    b += n_blk;
+    __syncthreads();
+  }
+}
+
+// grid (items of all sequences, rows of an item): joins the shares of items that lie in several CTAs; zeros for those
+// without keys.
+template <class T>
+__global__ void __launch_bounds__(128) lm_paged_join_kernel(Paged a, DecodeWork w, int item_rows, int grid) {
+  __shared__ float s_f[kDecCtas], s_inv;
+  pdl_launch_dependents();
+  pdl_wait_prior();
+  const int items = a.kv_heads * w.row_blocks, s = blockIdx.x / items, item = blockIdx.x - s * items;
+  const int kvh = item / w.row_blocks, r = blockIdx.y, row = (item - kvh * w.row_blocks) * item_rows + r, tid = threadIdx.x;
+  if (row >= a.group * a.tokens) return;
+  const long long b0 = w.base[s] * items, nb = w.base[s + 1] - w.base[s], first = b0 + item * nb, total = w.base[a.seqs] * items;
+  const int tok = row / a.group, h = kvh * a.group + row - tok * a.group;
+  const int2 q_rows = paged_rows(a, s);
+  if (tok >= q_rows.y) return;
+  T* out = static_cast<T*>(a.out) + (q_rows.x + tok) * a.out_row + h * a.out_head;
+  if (nb == 0) {
+    for (int d = tid; d < a.vdim; d += 128) out[d] = T(0.0f);
+    return;
+  }
+  const int ctas = (int)min((long long)grid, total);
+  const int c0 = owner_of(first, total, ctas), c1 = owner_of(first + nb - 1, total, ctas), n = c1 - c0 + 1;
+  if (n == 1) return;  // finished there
+  const bool nothing = paged_length(a, s) - a.tokens + tok < 0;
+  auto slot = [&](int i) { return (size_t)(2 * (c0 + i) + (i == 0)) * item_rows + r; };
+  if (tid < 32) {
+    const float sink = a.sink ? a.sink[h] * kPagedLog2e : -INFINITY;
+    float mx = sink;
+    for (int i = tid; i < n; i += 32) mx = fmaxf(mx, w.part_ml[slot(i)].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float base = mx == -INFINITY ? 0.0f : mx;
+    float sum = 0.0f;
+    for (int i = tid; i < n; i += 32) {
+      const float2 v = w.part_ml[slot(i)];
+      const float f = exp2f(v.x - base);
+      s_f[i] = f;
+      sum = fmaf(f, v.y, sum);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (tid == 0) s_inv = 1.0f / (sum + (a.sink ? exp2f(sink - base) : 0.0f));
+  }
+  __syncthreads();
+  for (int d = tid; d < a.vdim; d += 128) {
+    float v = 0.0f;
+    for (int i0 = 0; i0 < n; i0 += 8) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = w.part_o[slot(min(i0 + j, n - 1)) * a.vdim + d];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v = fmaf(i0 + j < n ? s_f[i0 + j] : 0.0f, x[j], v);
+    }
+    out[d] = T(nothing ? 0.0f : v * s_inv);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ prompts, any head size
+constexpr int kPpRows = 64, kPpKeys = 64, kPpThreads = 256;
+
+size_t prompt_smem(int dim, int vdim) {
+  return (size_t)kPpRows * (dim + 8) * 2 + std::max((size_t)2 * kPpKeys * (dim + vdim + 16) * 2, (size_t)kPpRows * vdim * 4);
+}
+
+// Which sequence and which of its tiles of `toks` rows a CTA has: {sequence, tile}, sequence -1 past the last one.  All
+// threads call it; a sequence's last tiles (the longest) come first.
+__device__ __forceinline__ int2 paged_tile(const Paged& a, int index, int toks) {
+  __shared__ int2 s_tile;
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    int2 found = make_int2(-1, 0);
+    for (int s0 = 0; s0 < a.seqs; s0 += 32) {
+      const int n = s0 + lane < a.seqs ? (paged_rows(a, s0 + lane).y + toks - 1) / toks : 0;
+      int up = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, up, o);
+        if (lane >= o) up += v;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, index < up);
+      if (hit) {
+        const int who = __ffs(hit) - 1;
+        found = make_int2(s0 + who, __shfl_sync(0xffffffffu, up, who) - 1 - index);
+        break;
+      }
+      index -= __shfl_sync(0xffffffffu, up, 31);
+    }
+    if (lane == 0) s_tile = found;
+  }
+  __syncthreads();
+  return s_tile;
+}
+
+// grid (tiles, kv heads): 64 rows (token, query head of one kv head).  Eight warps: warp w and w + 4 own the same 16 rows
+// and one half each of every block of 64 keys; their states meet at the end.
+template <class T, int DV>
+__global__ void __launch_bounds__(kPpThreads) lm_paged_prompt_kernel(Paged a) {
+  extern __shared__ __align__(16) uint8_t pp_smem[];
+  __shared__ float s_m[kPpRows], s_l[kPpRows];
+  constexpr int kHalf = kPpKeys / 2, kEach = kPpKeys / (kPpThreads / 8);
+  pdl_launch_dependents();
+  pdl_wait_prior();
+  const int D = a.dim, toks = kPpRows / a.group, kvh = blockIdx.y;
+  const int2 tile = paged_tile(a, blockIdx.x, toks);
+  if (tile.x < 0) return;
+  const int2 rows = paged_rows(a, tile.x);
+  const int row0 = rows.x + tile.y * toks, ntok = min(toks, rows.y - tile.y * toks);
+  const int pos0 = paged_length(a, tile.x) - rows.y + tile.y * toks, p_last = pos0 + ntok - 1;
+  const Seen seen = paged_seen<kPpKeys>(a, pos0, p_last);
+  const int ldk = D + 8, ldv = a.vdim + 8, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, half = warp >> 2, wrow = (warp & 3) * 16;
+  T* sQ = reinterpret_cast<T*>(pp_smem);
+  T* sK = sQ + kPpRows * ldk;
+  T* sV = sK + 2 * kPpKeys * ldk;
+  float* sO = reinterpret_cast<float*>(sK);
+  const T* kb = static_cast<const T*>(a.k) + kvh * a.k_head;
+  const T* vb = static_cast<const T*>(a.v) + kvh * a.v_head;
+  const int cr = tid >> 3, cc = tid & 7;  // copies: eight threads per row of 16-byte pieces
+  for (int r = cr; r < kPpRows; r += kPpThreads / 8) {
+    const int tok = r / a.group, hg = r - tok * a.group;
+    const bool ok = tok < ntok;
+    const T* src = static_cast<const T*>(a.q) + (row0 + (ok ? tok : 0)) * a.q_row + (kvh * a.group + hg) * a.q_head;
+    for (int c = cc * 8; c < D; c += 64) paged_copy16(smem_u32(sQ + r * ldk + c), ok ? src + c : static_cast<const T*>(a.q), ok);
+  }
+  auto page_of = [&](int b, int u) {  // page of this thread's row u of block b
+    const int j = b < seen.blocks ? block_key<kPpKeys>(seen, b) + cr + u * (kPpThreads / 8) : -1;
+    return j >= 0 && seen_by_some(seen, j) ? paged_page(a, tile.x, j / a.page) : -1;
+  };
+  int next[kEach];
+#pragma unroll
+  for (int u = 0; u < kEach; ++u) next[u] = page_of(0, u);
+  auto fetch = [&](int b, int buf) {
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+      const int r = cr + u * (kPpThreads / 8), at = (block_key<kPpKeys>(seen, b) + r) % a.page;
+      const bool ok = next[u] >= 0;
+      const T* ks = ok ? kb + next[u] * a.k_page + at * a.k_row : kb;
+      const T* vs = ok ? vb + next[u] * a.v_page + at * a.v_row : vb;
+      const uint32_t dk = smem_u32(sK + (buf * kPpKeys + r) * ldk), dv = smem_u32(sV + (buf * kPpKeys + r) * ldv);
+      for (int c = cc * 8; c < D; c += 64) paged_copy16(dk + c * 2, ok ? ks + c : kb, ok);
+      for (int c = cc * 8; c < a.vdim; c += 64) paged_copy16(dv + c * 2, ok ? vs + c : vb, ok);
+      next[u] = page_of(b + 1, u);
+    }
+    paged_commit();
+  };
+  if (seen.blocks) fetch(0, 0);
+  int pos[2], tok_r[2], hg_r[2];
+  const float* bias[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = wrow + (lane >> 2) + i * 8;
+    tok_r[i] = r / a.group;
+    hg_r[i] = r - tok_r[i] * a.group;
+    pos[i] = tok_r[i] < ntok ? pos0 + tok_r[i] : -1;
+    bias[i] = a.bias && tok_r[i] < ntok ? a.bias + (size_t)(kvh * a.group + hg_r[i]) * (a.bias_max + 1) : nullptr;
+  }
+  // positions of this warp's rows
+  const int w_first = pos0 + wrow / a.group, w_last = min(p_last, pos0 + (wrow + 15) / a.group);
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[DV / 8][4];
+#pragma unroll
+  for (int n = 0; n < DV / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+  const int mat = lane >> 3, ml = lane & 7;
+  const uint32_t q_addr = smem_u32(sQ + (wrow + (mat & 1) * 8 + ml) * ldk + (mat >> 1) * 8);
+  const uint32_t k_addr = smem_u32(sK + (half * kHalf + (mat >> 1) * 8 + ml) * ldk + (mat & 1) * 8);
+  const uint32_t v_addr = smem_u32(sV + (half * kHalf + (mat & 1) * 8 + ml) * ldv + (mat >> 1) * 8);
+
+  for (int blk = 0; blk < seen.blocks; ++blk) {
+    const int buf = blk & 1, j0 = block_key<kPpKeys>(seen, blk);
+    paged_wait<0>();
+    __syncthreads();
+    if (blk + 1 < seen.blocks) fetch(blk + 1, buf ^ 1);
+    // values that only some rows see, and that a weight of 0 would not keep from the others
+    bool edge = false;
+    if (!seen_by_all(a, max(pos0, 0), p_last, j0, j0 + kPpKeys - 1)) {
+      for (int r = cr; r < kPpKeys; r += kPpThreads / 8)
+        for (int c = cc * 8; c < a.vdim; c += 64) {
+          const uint4 x = *reinterpret_cast<const uint4*>(sV + (buf * kPpKeys + r) * ldv + c);
+          edge = edge || not_finite2<T>(x.x) || not_finite2<T>(x.y) || not_finite2<T>(x.z) || not_finite2<T>(x.w);
+        }
+      edge = __syncthreads_or(edge);
+    }
+    if (w_first > p_last) continue;  // (no row of this warp is there)
+    const int jw = j0 + half * kHalf;
+    float s[kHalf / 8][4];
+#pragma unroll
+    for (int n = 0; n < kHalf / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll 4
+    for (int kk = 0; kk < D; kk += 16) {
+      uint32_t qa[4];
+      paged_ldsm(qa, q_addr + kk * 2);
+#pragma unroll
+      for (int n = 0; n < kHalf / 16; ++n) {
+        uint32_t b[4];
+        paged_ldsm(b, k_addr + ((buf * kPpKeys + n * 16) * ldk + kk) * 2);
+        Num<T>::mma(s[2 * n], qa, b[0], b[1]);
+        Num<T>::mma(s[2 * n + 1], qa, b[2], b[3]);
+      }
+    }
+    float alpha[2];
+    if (w_first >= 0 && seen_by_all(a, w_first, w_last, jw, jw + kHalf - 1)) weigh_keys<kHalf / 8, true>(a, s, m, l, alpha, jw, lane, pos, bias);
+    else weigh_keys<kHalf / 8, false>(a, s, m, l, alpha, jw, lane, pos, bias);
+#pragma unroll
+    for (int n = 0; n < DV / 8; ++n) o[n][0] *= alpha[0], o[n][1] *= alpha[0], o[n][2] *= alpha[1], o[n][3] *= alpha[1];
+#pragma unroll
+    for (int kk = 0; kk < kHalf / 16; ++kk) {
+      uint32_t hi[4], lo[4];
+      split_weights<T>(s[2 * kk], s[2 * kk + 1], hi, lo);
+      const uint32_t at = v_addr + (uint32_t)(buf * kPpKeys + kk * 16) * ldv * 2;
+      if (!edge) weigh_values<T, DV, false>(a, o, hi, lo, at, jw + kk * 16, lane, pos, 0, 0);
+      else weigh_values<T, DV, true>(a, o, hi, lo, at, jw + kk * 16, lane, pos, max(0, w_first), w_last);
+    }
+  }
+  paged_wait<0>();
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+  }
+  __syncthreads();
+  if (half == 1) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = wrow + (lane >> 2) + r * 8;
+      if ((lane & 3) == 0) s_m[row] = m[r], s_l[row] = l[r];
+      float* so = sO + (size_t)row * a.vdim + (lane & 3) * 2;
+#pragma unroll
+      for (int n = 0; n < DV / 8; ++n)
+        if (n * 8 < a.vdim) *reinterpret_cast<float2*>(so + n * 8) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+    }
+  }
+  __syncthreads();
+  if (half == 1) return;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    if (tok_r[r] >= ntok) continue;
+    const int row = wrow + (lane >> 2) + r * 8, h = kvh * a.group + hg_r[r];
+    const float sink = a.sink ? a.sink[h] * kPagedLog2e : -INFINITY, mt = fmaxf(fmaxf(m[r], s_m[row]), sink);
+    const float base = mt == -INFINITY ? 0.0f : mt, f0 = exp2f(m[r] - base), f1 = exp2f(s_m[row] - base);
+    const float sum = l[r] * f0 + s_l[row] * f1 + exp2f(sink - base), inv = pos[r] < 0 ? 0.0f : 1.0f / sum;
+    const float* so = sO + (size_t)row * a.vdim + (lane & 3) * 2;
+    T* out = static_cast<T*>(a.out) + (row0 + tok_r[r]) * a.out_row + h * a.out_head + (lane & 3) * 2;
+#pragma unroll
+    for (int n = 0; n < DV / 8; ++n)
+      if (n * 8 < a.vdim) {
+        const float2 x = *reinterpret_cast<const float2*>(so + n * 8);
+        const float v0 = fmaf(o[n][2 * r], f0, x.x * f1) * inv, v1 = fmaf(o[n][2 * r + 1], f0, x.y * f1) * inv;
+        *reinterpret_cast<uint32_t*>(out + n * 8) = pos[r] < 0 ? 0u : Num<T>::pack(v0, v1);
+      }
+  }
+}
+
+// ------------------------------------------------------------------------------------------ host
+constexpr int kPagedSmemMax = 220 * 1024;
+
+int dec_stages(const Paged& a) { return a.dim + a.vdim <= 128 ? 5 : 3; }
+int dec_warps(const Paged& a) { return a.vdim <= 128 && a.dim + a.vdim <= 256 ? 8 : 4; }
+int dec_rows(const Paged& a) { return a.vdim <= 128 && a.group * a.tokens > 16 ? 32 : 16; }
+size_t decode_smem(const Paged& a) {
+  const size_t rows = dec_rows(a), ring = (size_t)dec_warps(a) * dec_stages(a) * 16 * (a.dim + a.vdim + 16) * 2;
+  return rows * (a.dim + 8) * 2 + std::max(ring, dec_warps(a) * rows * a.vdim * 4);
+}
+size_t up16(size_t n) { return (n + 15) / 16 * 16; }
+
+// Kernel attributes are set once per device.
+template <class F>
+cudaError_t once_per_device(std::atomic<unsigned long long>* done, F f) {
+  int dev = 0;
+  cudaError_t r = cudaGetDevice(&dev);
+  if (r != cudaSuccess) return r;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (dev < 64 && (done->load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  r = f();
+  if (r == cudaSuccess && dev < 64) done->fetch_or(bit, std::memory_order_release);
+  return r;
+}
+cudaError_t configure_prompt() {
+  static std::atomic<unsigned long long> done{0};
+  return once_per_device(&done, [] {
+    cudaError_t r = cudaSuccess;
+    auto set = [&](auto f) {
+      if (r == cudaSuccess) r = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kPagedSmemMax);
+    };
+    set(lm_paged_prompt_kernel<__nv_bfloat16, 64>), set(lm_paged_prompt_kernel<__nv_bfloat16, 128>), set(lm_paged_prompt_kernel<__nv_bfloat16, 256>);
+    set(lm_paged_prompt_kernel<__half, 64>), set(lm_paged_prompt_kernel<__half, 128>), set(lm_paged_prompt_kernel<__half, 256>);
+    return r;
+  });
+}
+// f(kernel) for the instance that serves these sizes
+template <class T, int DV, int MT, class F>
+auto with_decode_rows(const Paged& a, F f) {
+  if (dec_warps(a) == 4) return f(lm_paged_decode_kernel<T, DV, MT, 3, 4>);
+  return dec_stages(a) == 5 ? f(lm_paged_decode_kernel<T, DV, MT, 5, 8>) : f(lm_paged_decode_kernel<T, DV, MT, 3, 8>);
+}
+template <class T, class F>
+auto with_decode(const Paged& a, F f) {
+  const bool two = dec_rows(a) == 32;
+  if (a.vdim <= 64) return two ? with_decode_rows<T, 64, 2>(a, f) : with_decode_rows<T, 64, 1>(a, f);
+  if (a.vdim <= 128) return two ? with_decode_rows<T, 128, 2>(a, f) : with_decode_rows<T, 128, 1>(a, f);
+  return f(lm_paged_decode_kernel<T, 256, 1, 3, 4>);
+}
+cudaError_t configure_decode() {
+  static std::atomic<unsigned long long> done{0};
+  return once_per_device(&done, [] {
+    cudaError_t r = cudaSuccess;
+    auto set = [&](auto f) {
+      if (r == cudaSuccess) r = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kPagedSmemMax);
+      return r;
+    };
+    for (int vdim : {64, 80, 128, 256})  // (reaches every instance)
+      for (int dim : {16, 128, 256})
+        for (int tokens : {1, 32}) {
+          Paged a{};
+          a.vdim = vdim, a.dim = dim, a.group = 1, a.tokens = tokens;
+          with_decode<__nv_bfloat16>(a, set);
+          with_decode<__half>(a, set);
+        }
+    return r;
+  });
+}
+
+// Layout of the decode workspace for `seqs` sequences of a launch.
+struct DecodeSpace {
+  size_t ml, base, bytes;
+};
+DecodeSpace decode_space(const Paged& a, int seqs) {
+  DecodeSpace d;
+  const size_t rows = (size_t)2 * kDecCtas * dec_rows(a);
+  d.ml = up16(rows * a.vdim * 4);
+  d.base = d.ml + up16(rows * sizeof(float2));
+  d.bytes = d.base + up16((size_t)(seqs + 1) * sizeof(long long));
+  return d;
+}
+
+bool aligned(const void* p, long long a, long long b, long long c = 0) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && a % 8 == 0 && b % 8 == 0 && c % 8 == 0;
+}
+
+int check_pages(const mllmb200_lm_pages* p, Paged* a) {
+  if (!p || p->seqs < 0 || p->rows < 0) return MLLMB200_INVALID_ARG;
+  if (p->dtype != MLLMB200_LM_BF16 && p->dtype != MLLMB200_LM_F16) return MLLMB200_UNSUPPORTED;
+  if (p->pages < 1 || p->page < 1 || p->kv_heads < 1 || p->dim < 1 || p->vdim < 1 || p->max_pages < 0 || p->ld_table < 0) return MLLMB200_INVALID_ARG;
+  if (p->page % 16 || p->dim % 16 || p->vdim % 16 || p->dim > 256 || p->vdim > 256) return MLLMB200_UNSUPPORTED;
+  if ((long long)p->max_pages * p->page > kLongest) return MLLMB200_UNSUPPORTED;
+  if (p->seqs && (!p->k || !p->v || !p->lengths || (!p->table && p->max_pages))) return MLLMB200_INVALID_ARG;
+  if (!aligned(p->k, p->k_page, p->k_head, p->k_row) || !aligned(p->v, p->v_page, p->v_head, p->v_row)) return MLLMB200_INVALID_ARG;
+  if (!p->q_start && p->seqs && p->rows % p->seqs) return MLLMB200_INVALID_ARG;
+  *a = Paged{};
+  a->k = p->k, a->v = p->v;
+  a->k_page = p->k_page, a->k_head = p->k_head, a->k_row = p->k_row, a->v_page = p->v_page, a->v_head = p->v_head, a->v_row = p->v_row;
+  a->table = p->table, a->lengths = p->lengths, a->q_start = p->q_start;
+  a->pages = p->pages, a->page = p->page, a->kv_heads = p->kv_heads, a->dim = p->dim, a->vdim = p->vdim;
+  a->ld_table = p->ld_table, a->max_pages = p->max_pages, a->seqs = p->seqs, a->rows = p->rows;
+  a->tokens = p->q_start || !p->seqs ? 0 : p->rows / p->seqs;
+  return MLLMB200_OK;
+}
+int check_look(const mllmb200_lm_pages* p, const mllmb200_lm_look* l, Paged* a) {
+  const int st = check_pages(p, a);
+  if (st != MLLMB200_OK) return st;
+  if (!l || l->heads < 1 || l->heads % a->kv_heads || l->window < 0 || l->keep < 0 || !(std::fabs(l->scale) <= 3.402823466e+38f)) return MLLMB200_INVALID_ARG;
+  if (l->heads / a->kv_heads > 64) return MLLMB200_UNSUPPORTED;
+  if (l->bias && l->bias_max < 0) return MLLMB200_INVALID_ARG;
+  if (a->rows && (!l->q || !l->out)) return MLLMB200_INVALID_ARG;
+  if (!aligned(l->q, l->q_row, l->q_head) || !aligned(l->out, l->out_row, l->out_head)) return MLLMB200_INVALID_ARG;
+  a->q = l->q, a->out = l->out;
+  a->q_row = l->q_row, a->q_head = l->q_head, a->out_row = l->out_row, a->out_head = l->out_head;
+  a->sink = l->sink, a->bias = l->bias;
+  a->heads = l->heads, a->group = l->heads / a->kv_heads, a->bias_max = l->bias_max, a->window = l->window, a->keep = l->keep;
+  a->scale2 = l->scale * kPagedLog2e;
+  return MLLMB200_OK;
+}
+int check_decode(const mllmb200_lm_pages* p, const mllmb200_lm_look* l, Paged* a) {
+  const int st = check_look(p, l, a);
+  if (st != MLLMB200_OK) return st;
+  if (a->q_start) return MLLMB200_INVALID_ARG;
+  return a->tokens > 16 ? MLLMB200_UNSUPPORTED : MLLMB200_OK;
+}
+
+template <class T>
+cudaError_t launch_decode(Paged a, uint8_t* ws, cudaStream_t s) {
+  const int all = a.seqs, item_rows = dec_rows(a);
+  const DecodeSpace d = decode_space(a, std::min(all, kDecSeqs));
+  DecodeWork w{reinterpret_cast<float*>(ws), reinterpret_cast<float2*>(ws + d.ml), reinterpret_cast<long long*>(ws + d.base),
+               (a.group * a.tokens + item_rows - 1) / item_rows};
+  const size_t smem = decode_smem(a);
+  for (int s0 = 0; s0 < all; s0 += kDecSeqs) {
+    Paged b = a;
+    b.seqs = std::min(kDecSeqs, all - s0);
+    b.lengths += s0;
+    b.table += (size_t)s0 * a.ld_table;
+    if (b.q_start) b.q_start += s0, b.q_count += s0;
+    else b.q = static_cast<const T*>(a.q) + (long long)s0 * a.tokens * a.q_row, b.out = static_cast<T*>(a.out) + (long long)s0 * a.tokens * a.out_row;
+    cudaError_t r = with_decode<T>(b, [&](auto f) { return launch_pdl(f, dim3(kDecCtas), dim3(32 * dec_warps(b)), smem, s, b, w); });
+    if (r != cudaSuccess) return r;
+    r = launch_pdl(lm_paged_join_kernel<T>, dim3(b.seqs * b.kv_heads * w.row_blocks, std::min(item_rows, b.group * b.tokens)), dim3(128), 0, s, b, w,
+                   item_rows, kDecCtas);
+    if (r != cudaSuccess) return r;
+  }
+  return cudaSuccess;
+}
+template <class T>
+cudaError_t launch_prompt(const Paged& a, cudaStream_t s) {
+  const int toks = kPpRows / a.group;
+  const long long tiles = std::min((long long)a.rows, a.rows / toks + (long long)a.seqs);
+  const size_t smem = prompt_smem(a.dim, a.vdim);
+  auto go = [&](auto f) { return launch_pdl(f, dim3((unsigned)tiles, a.kv_heads), dim3(kPpThreads), smem, s, a); };
+  return a.vdim <= 64 ? go(lm_paged_prompt_kernel<T, 64>) : a.vdim <= 128 ? go(lm_paged_prompt_kernel<T, 128>) : go(lm_paged_prompt_kernel<T, 256>);
+}
+int status_of(cudaError_t r) { return r == cudaSuccess ? MLLMB200_OK : MLLMB200_CUDA_ERROR; }
+
+}  // namespace
+}  // namespace lm
+}  // namespace mllmb200
+
+using namespace mllmb200;
+using namespace mllmb200::lm;
+
+extern "C" {
+
+int mllmb200_lm_pages_append(const mllmb200_lm_pages* pages, const void* k, long long k_row, long long k_head, const void* v, long long v_row,
+                             long long v_head, void* stream) {
+  Paged a;
+  const int st = check_pages(pages, &a);
+  if (st != MLLMB200_OK) return st;
+  if (!a.seqs || !a.rows) return MLLMB200_OK;
+  if (!k || !v || !aligned(k, k_row, k_head) || !aligned(v, v_row, v_head)) return MLLMB200_INVALID_ARG;
+  const int pieces = a.kv_heads * (a.dim + a.vdim) / 8;
+  return status_of(launch_pdl(lm_pages_append_kernel, dim3(a.rows, (pieces + 127) / 128), dim3(128), 0, static_cast<cudaStream_t>(stream), a, k, k_row,
+                              k_head, v, v_row, v_head, static_cast<uint16_t*>(pages->k), static_cast<uint16_t*>(pages->v)));
+}
+
+int mllmb200_lm_attn_decode_workspace(const mllmb200_lm_pages* pages, const mllmb200_lm_look* look, size_t* bytes) {
+  Paged a;
+  if (!bytes) return MLLMB200_INVALID_ARG;
+  const int st = check_decode(pages, look, &a);
+  if (st != MLLMB200_OK) return st;
+  *bytes = decode_space(a, std::min(a.seqs, kDecSeqs)).bytes;
+  return MLLMB200_OK;
+}
+int mllmb200_lm_attn_decode(const mllmb200_lm_pages* pages, const mllmb200_lm_look* look, void* workspace, void* stream) {
+  Paged a;
+  const int st = check_decode(pages, look, &a);
+  if (st != MLLMB200_OK) return st;
+  if (!a.seqs || !a.rows) return MLLMB200_OK;
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u)) return MLLMB200_INVALID_ARG;
+  cudaError_t r = configure_decode();
+  if (r != cudaSuccess) return MLLMB200_CUDA_ERROR;
+  auto* ws = static_cast<uint8_t*>(workspace);
+  auto s = static_cast<cudaStream_t>(stream);
+  return status_of(pages->dtype == MLLMB200_LM_F16 ? launch_decode<__half>(a, ws, s) : launch_decode<__nv_bfloat16>(a, ws, s));
+}
+
+int mllmb200_lm_attn_prompt_workspace(const mllmb200_lm_pages* pages, const mllmb200_lm_look* look, size_t* bytes) {
+  Paged a;
+  if (!bytes) return MLLMB200_INVALID_ARG;
+  const int st = check_look(pages, look, &a);
+  if (st != MLLMB200_OK) return st;
+  *bytes = 0;
+  return MLLMB200_OK;
+}
+int mllmb200_lm_attn_prompt(const mllmb200_lm_pages* pages, const mllmb200_lm_look* look, void* workspace, void* stream) {
+  Paged a;
+  const int st = check_look(pages, look, &a);
+  if (st != MLLMB200_OK) return st;
+  if (!a.seqs || !a.rows) return MLLMB200_OK;
+  (void)workspace;
+  if (configure_prompt() != cudaSuccess) return MLLMB200_CUDA_ERROR;
+  auto s = static_cast<cudaStream_t>(stream);
+  return status_of(pages->dtype == MLLMB200_LM_F16 ? launch_prompt<__half>(a, s) : launch_prompt<__nv_bfloat16>(a, s));
+}
+
+int mllmb200_lm_operator_status(void* stream) {
+  int status = MLLMB200_OK;
+  return read_device_status(static_cast<cudaStream_t>(stream), &status) == cudaSuccess ? status : MLLMB200_CUDA_ERROR;
+}
+
+}  // extern "C"

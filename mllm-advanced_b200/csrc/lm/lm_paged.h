@@ -1,0 +1,146 @@
+// A key-value cache in pages: what the operators over it share (include/mllmb200_lm.h says what they compute).
+#pragma once
+#include <cuda_fp16.h>
+
+#include "../device_common.cuh"
+#include "lm_state.h"
+
+namespace mllmb200 {
+namespace lm {
+
+// The public structures as the kernels use them.
+struct Paged {
+  const void *k, *v;
+  long long k_page, k_head, k_row, v_page, v_head, v_row;
+  const int *table, *lengths, *q_start;
+  const int* q_count;  // rows of every sequence; nullptr: q_start[s + 1] - q_start[s]
+  int pages, page, kv_heads, dim, vdim, ld_table, max_pages, seqs, rows;
+  int tokens;          // rows of every sequence where q_start is nullptr
+  const void* q;
+  void* out;
+  long long q_row, q_head, out_row, out_head;
+  const float *sink, *bias;
+  int heads, group, bias_max, window, keep;
+  float scale2;        // scale log2(e): scores are in base 2
+};
+
+constexpr float kPagedLog2e = 1.4426950408889634f;
+constexpr int kLongest = 1 << 30;  // positions that a table's row can name, at most
+
+// A sequence's length, cut to what its row of the table can name.
+__device__ __forceinline__ int paged_length(const Paged& a, int s) {
+  const int n = a.lengths[s], most = a.max_pages * a.page;
+  if (n > most) atomicOr(&g_device_status, kDevStatusBadPage);
+  return max(0, min(n, most));
+}
+// Page number of a table place, or -1.
+__device__ __forceinline__ int paged_page(const Paged& a, int s, int place) {
+  int p = place < a.max_pages ? __ldg(a.table + (size_t)s * a.ld_table + place) : -1;
+  if (p < 0 || p >= a.pages) {
+    atomicOr(&g_device_status, kDevStatusBadPage);
+    p = -1;
+  }
+  return p;
+}
+// First row and number of rows of a sequence, inside [0, rows).
+__device__ __forceinline__ int2 paged_rows(const Paged& a, int s) {
+  if (!a.q_start) return make_int2(s * a.tokens, a.tokens);
+  const int r0 = a.q_start[s], n = a.q_count ? a.q_count[s] : a.q_start[s + 1] - r0;
+  if (r0 < 0 || r0 >= a.rows) return make_int2(0, 0);
+  return make_int2(r0, max(0, min(n, a.rows - r0)));
+}
+
+// What rows at positions [first, last] see of a sequence: keys [0, head) and [lo, last].  Walked in blocks of B keys (B a
+// multiple of 16): `front` blocks from 0, the others from block lo / B on.
+struct Seen {
+  int head, lo, last, front, blocks;
+};
+template <int B>
+__device__ __forceinline__ Seen paged_seen(const Paged& a, int first, int last) {
+  Seen v;
+  v.last = last;
+  v.lo = a.window ? max(0, first - a.window + 1) : 0;
+  v.head = a.window ? min(a.keep, v.lo) : 0;
+  v.front = min((v.head + B - 1) / B, v.lo / B);
+  v.blocks = last < 0 ? 0 : v.front + last / B + 1 - v.lo / B;
+  return v;
+}
+template <int B>
+__device__ __forceinline__ int block_key(const Seen& v, int b) {  // first key of block b
+  return (b < v.front ? b : v.lo / B + b - v.front) * B;
+}
+__device__ __forceinline__ bool seen_by_some(const Seen& v, int j) { return j <= v.last && (j >= v.lo || j < v.head); }
+__device__ __forceinline__ bool seen_by(const Paged& a, int pos, int j) {
+  return j <= pos && (a.window == 0 || j > pos - a.window || j < a.keep);
+}
+// keys [j0, j1] are all seen by every row at positions [first, last]
+__device__ __forceinline__ bool seen_by_all(const Paged& a, int first, int last, int j0, int j1) {
+  return j1 <= first && (a.window == 0 || j0 > last - a.window || j1 < a.keep);
+}
+
+// Numbers of 16 bits on the tensor cores of a warp.
+template <class T>
+struct Num;
+template <>
+struct Num<__nv_bfloat16> {
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+  static constexpr uint32_t kExponent = 0x7f807f80u;
+};
+template <>
+struct Num<__half> {
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t w) {
+    const __half2 h = *reinterpret_cast<const __half2*>(&w);
+    return __half22float2(h);
+  }
+  static constexpr uint32_t kExponent = 0x7c007c00u;
+};
+// infinity or NaN in either half
+template <class T>
+__device__ __forceinline__ bool not_finite2(uint32_t w) {
+  constexpr uint32_t lo = Num<T>::kExponent & 0xffffu, hi = Num<T>::kExponent & 0xffff0000u;
+  return (w & lo) == lo || (w & hi) == hi;
+}
+
+__device__ __forceinline__ void paged_ldsm(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void paged_ldsm_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void paged_copy16(uint32_t dst, const void* src, bool valid) {  // zeros where not valid (src: any address then)
+  const int n = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void paged_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void paged_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float paged_exp2(float x) {  // results below 2^-126 are 0; 2^-22 of the result off at most
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+}  // namespace lm
+}  // namespace mllmb200

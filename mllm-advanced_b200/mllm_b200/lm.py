@@ -8,7 +8,9 @@ import subprocess
 import numpy as np
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
-BF16, F32 = 0, 1
+BF16, F32, F16 = 0, 1, 2  # (F16: the operators' caches and logits)
+STATUS = {1: "invalid argument", 2: "unsupported shape or mode", 3: "CUDA runtime error", 4: "device-side wait timed out",
+          6: "request exceeds a fixed capacity", 7: "page number or length outside of the cache"}
 ATTENTION, RETENTION, LATENT = 0, 1, 2
 CLAMPED, GELU, SILU = 0, 1, 2  # gated feed-forwards
 NORM_SANDWICH, NORM_POST = 0, 1
@@ -55,13 +57,19 @@ def lib():
     if not os.path.exists(lib_path()):
         raise ImportError(f"{lib_path()} is missing: build it with mllm-advanced_b200/build.sh lm; there is no CPU fallback")
     L = C.CDLL(lib_path())
-    vp, ci = C.c_void_p, C.c_int
+    vp, ci, ll = C.c_void_p, C.c_int, C.c_longlong
     sig = {"create": [C.POINTER(Config), C.POINTER(Layer), C.POINTER(vp)], "set_tensor": [vp, ci, ci, vp, ci, ci],
            "set_expert": [vp, ci, ci, ci, vp, ci, ci],
            "step": [vp, ci, vp, vp, vp, ci, vp, vp, ci], "decode": [vp, ci, vp, ci], "free_slot": [vp, ci],
            "read": [vp, ci, ci, ci, vp, vp], "keep_residual": [vp, ci], "read_residual": [vp, ci, ci, vp],
            "stats": [vp, C.POINTER(C.c_size_t), C.POINTER(C.c_longlong)], "synchronize": [vp], "check_device_status": [vp],
-           "distance_buckets": [ci, ci, ci, vp]}
+           "distance_buckets": [ci, ci, ci, vp],
+           # operators (structures as packed bytes)
+           "pages_append": [C.c_char_p, vp, ll, ll, vp, ll, ll, vp],
+           "attn_decode_workspace": [C.c_char_p, C.c_char_p, vp], "attn_decode": [C.c_char_p, C.c_char_p, vp, vp],
+           "attn_prompt_workspace": [C.c_char_p, C.c_char_p, vp], "attn_prompt": [C.c_char_p, C.c_char_p, vp, vp],
+           "probabilities": [vp, ci, ll, ci, ci, C.c_float, vp, ll, vp],
+           "verify": [vp, ll, ll, vp, ll, ll, vp, ll, vp, ll, vp, ci, ci, ci, vp, vp, ll, vp], "operator_status": [vp]}
     for name, args in sig.items():
         fn = getattr(L, "mllmb200_lm_" + name)
         fn.argtypes, fn.restype = args, ci
