@@ -2,6 +2,9 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <atomic>
+#include <type_traits>
+
 #include "../device_common.cuh"
 #include "lm_state.h"
 
@@ -141,6 +144,21 @@ __device__ __forceinline__ float paged_exp2(float x) {  // results below 2^-126 
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// Kernel attributes are set once per device.
+template <class F>
+cudaError_t once_per_device(std::atomic<unsigned long long>* done, F f) {
+  int dev = 0;
+  cudaError_t r = cudaGetDevice(&dev);
+  if (r != cudaSuccess) return r;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (dev < 64 && (done->load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  r = f();
+  if (r == cudaSuccess && dev < 64) done->fetch_or(bit, std::memory_order_release);
+  return r;
+}
+
+bool launch_paged_prompt_tc(const Paged& a, bool f16, cudaStream_t s, cudaError_t* launched);
 
 }  // namespace lm
 }  // namespace mllmb200

@@ -1,0 +1,450 @@
+// Prompt attention over pages on the 5th-generation tensor cores, heads of 64 or 128 (include/mllmb200_lm.h has the mathematics).
+//
+// A CTA owns two tiles of 128 rows; a row is (token, query head) of one kv head, so that all heads of a group share every key
+// and value that is fetched.  Per block of 128 keys and tile: S = Q K^T into tensor memory, softmax weights P in 16 bits over
+// S's own columns, O += P V.  While the weights of one tile are made, the products of the other run:
+//   warps 0-3, 4-7  weights of tile 0 and 1, a row per thread; O is rescaled (tensor memory) only when a row's maximum has grown by
+//                   more than 2^8 - weights up to 2^8 are as exact in 16 bits, and their fp32 sum is kept under the same base
+//   warp 8          copies: TMA, pieces of a block that lie in one page, into a ring of keys and one of values
+//   warp 9          MMA issue, tensor-memory owner
+//   warps 10-11     values of blocks that some rows do not see in full: rows that no row sees (page tails, other sequences' data) are
+//                   made zeros; where what only some rows see is not finite, a weight of 0 would not hide it: the tile is
+//                   done again row-block by row-block on mma.sync (paged_prompt_rows), which can.
+// The weights' rounding to 16 bits (2^-9 of each, independent) is of the size of the output's own; everything else is fp32.
+#include <algorithm>
+#include <atomic>
+#include <mutex>
+
+#include "../tcgen05_common.cuh"
+#include "lm_paged_rows.cuh"
+
+namespace mllmb200 {
+namespace lm {
+namespace {
+
+constexpr int kTcKeys = 128, kTcThreads = 384;
+
+template <int D>
+struct TcLayout {
+  static constexpr int kTile = 128 * D * 2;                 // a block of keys or values, and a tile of queries
+  static constexpr int kK = D == 128 ? 3 : 4, kV = D == 128 ? 2 : 4;  // blocks of keys, of values
+  static constexpr int kBytes = (2 + kK + kV) * kTile + 1024;  // (queries and ring on 1024 bytes)
+};
+
+template <class T>
+__device__ __forceinline__ uint32_t tc_idesc(int n, bool b_mn) {  // fp32 sums, M = 128
+  const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (type << 7) | (type << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+// Operand in the 128-byte swizzle, rows of 64 numbers, groups of 8 rows 1024 bytes apart; `lead`: bytes between chunks of 64
+// numbers where those run along M or N (values)
+__device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t lead) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
+               "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
+               "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
+      "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+      "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+
+struct TcBarriers {
+  uint64_t q_full, k_full[4], k_free[4], v_full[4], v_free[4], v_fixed[4], s_full[2], p_ready[2], o_done[2];
+};
+
+template <class T, int D, bool BIAS>
+__global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const __grid_constant__ Paged a, const __grid_constant__ CUtensorMap qmap,
+                                                                           const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                                                                           int piece) {
+  using L = TcLayout<D>;
+  extern __shared__ uint8_t tc_smem_raw[];
+  __shared__ TcBarriers bars;
+  __shared__ uint32_t s_tmem;
+  __shared__ volatile int s_bad, s_gave_up;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const uint32_t smem0 = (smem_u32(tc_smem_raw) + 1023u) & ~1023u, keys0 = smem0 + 2 * L::kTile, values0 = keys0 + L::kK * L::kTile;
+  pdl_launch_dependents();
+  pdl_wait_prior();
+  const int toks = 128 / a.group, kvh = blockIdx.x % a.kv_heads;
+  const int2 tile = paged_tile(a, blockIdx.x / a.kv_heads, 2 * toks);
+  if (tile.x < 0) return;
+  const int2 seq_rows = paged_rows(a, tile.x);
+  const int row0 = seq_rows.x + tile.y * 2 * toks, ntok = min(2 * toks, seq_rows.y - tile.y * 2 * toks);
+  const int pos0 = paged_length(a, tile.x) - seq_rows.y + tile.y * 2 * toks, p_last = pos0 + ntok - 1;
+  const Seen seen = paged_seen<kTcKeys>(a, pos0, p_last);
+  const int nt = seen.blocks, tiles = ntok > toks ? 2 : 1;
+  if (tid == 0) {
+    mbar_init(&bars.q_full, 1);
+    for (int i = 0; i < L::kK; ++i) mbar_init(&bars.k_full[i], 1), mbar_init(&bars.k_free[i], 1);
+    for (int i = 0; i < L::kV; ++i) mbar_init(&bars.v_full[i], 1), mbar_init(&bars.v_free[i], 1), mbar_init(&bars.v_fixed[i], 2);
+    for (int i = 0; i < 2; ++i) mbar_init(&bars.s_full[i], 1), mbar_init(&bars.p_ready[i], 4), mbar_init(&bars.o_done[i], 1);
+    s_bad = s_gave_up = 0;
+    mbar_fence_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(&s_tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+  auto turn = [](int j, int n) { return (uint32_t)(j / n) & 1u; };  // parity of a ring's pass
+  auto partly = [&](int j) {  // some row does not see some key of block j
+    const int j0 = block_key<kTcKeys>(seen, j);
+    return pos0 < 0 || !seen_by_all(a, pos0, p_last, j0, j0 + kTcKeys - 1);
+  };
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (s_gave_up) return false;
+    if (mbar_wait_bounded(bar, parity)) return true;
+    s_gave_up = 1;
+    return false;
+  };
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (warp == 8) {
+      // ---------------------------------------------------------- copies
+      if (nt) {
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&bars.q_full, (uint32_t)(tiles * toks * a.group * D * 2));
+          for (int t = 0; t < tiles; ++t)
+            for (int c = 0; c < D / 64; ++c) tma_load_3d(smem0 + t * L::kTile + c * 16384, &qmap, c * 64, kvh * a.group, row0 + t * toks, &bars.q_full);
+        }
+        const int pieces = kTcKeys / piece;
+        int n_k = 0, n_v = 0;
+        bool ok = true;
+        auto page_of = [&](int j) {  // lane i: page of piece i of block j, a.pages (zeros) where nothing of it is seen
+          int page = a.pages;
+          if (j < nt && lane < pieces) {
+            const int key = block_key<kTcKeys>(seen, j) + lane * piece;
+            if (key <= seen.last && (key + piece > seen.lo || key < seen.head)) {
+              const int p = paged_page(a, tile.x, key / a.page);
+              if (p >= 0) page = p;
+            }
+          }
+          return page;
+        };
+        int pages = page_of(0);
+        for (int j = 0; j < nt && ok; ++j) {
+          const int next = page_of(j + 1), j0 = block_key<kTcKeys>(seen, j);
+          auto copy = [&](const CUtensorMap* map, uint32_t block, uint64_t* full) {
+            if (lane == 0) mbar_arrive_expect_tx(full, L::kTile);
+            __syncwarp();
+            if (lane < pieces) {
+              const int at = (j0 + lane * piece) % a.page;
+#pragma unroll
+              for (int c = 0; c < D / 64; ++c) tma_load_4d(block + lane * piece * 128 + c * 16384, map, c * 64, at, kvh, pages, full);
+            }
+            __syncwarp();
+          };
+          const int ks = j % L::kK, vs = j % L::kV;
+          if (j >= L::kK) ok = __all_sync(0xffffffffu, wait(&bars.k_free[ks], turn(j, L::kK) ^ 1u));
+          if (!ok) break;
+          copy(&kmap, keys0 + ks * L::kTile, &bars.k_full[ks]);
+          ++n_k;
+          if (j >= L::kV) ok = __all_sync(0xffffffffu, wait(&bars.v_free[vs], turn(j, L::kV) ^ 1u));
+          if (!ok) break;
+          copy(&vmap, values0 + vs * L::kTile, &bars.v_full[vs]);
+          ++n_v;
+          pages = next;
+        }
+        if (!ok) {  // nothing in flight when the CTA leaves
+          mbar_wait_bounded(&bars.q_full, 0);
+          for (int j = max(0, n_k - L::kK); j < n_k; ++j) mbar_wait_bounded(&bars.k_full[j % L::kK], turn(j, L::kK));
+          for (int j = max(0, n_v - L::kV); j < n_v; ++j) mbar_wait_bounded(&bars.v_full[j % L::kV], turn(j, L::kV));
+        }
+      }
+    } else if (warp == 9) {
+      // ---------------------------------------------------------- MMA issue
+      if (nt) {
+        const bool issuer = elect_one_sync();
+        const uint32_t idesc_s = tc_idesc<T>(kTcKeys, false), idesc_o = tc_idesc<T>(D, true);
+        auto all_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+        auto scores = [&](int t, int j, bool last) {
+          if (issuer) {
+            const uint64_t q = tc_desc(smem0 + t * L::kTile, 16), k = tc_desc(keys0 + j % L::kK * L::kTile, 16);
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) {
+              const uint64_t off = (uint64_t)((ks / 4) * 1024 + (ks % 4) * 2);
+              tc_mma_f16(tmem + t * 128, q + off, k + off, idesc_s, ks > 0);
+            }
+            tc_commit(&bars.s_full[t]);
+            if (last) tc_commit(&bars.k_free[j % L::kK]);
+          }
+          __syncwarp();
+        };
+        bool ok = all_wait(&bars.q_full, 0) && all_wait(&bars.k_full[0], 0);
+        if (ok) {
+          tc_fence_after();
+          for (int t = 0; t < tiles; ++t) scores(t, 0, t == tiles - 1);
+        }
+        for (int j = 0; j < nt && ok; ++j) {
+          for (int t = 0; t < tiles && ok; ++t) {
+            ok = all_wait(&bars.p_ready[t], (uint32_t)j & 1u);
+            if (t == 0 && ok) {
+              ok = all_wait(&bars.v_full[j % L::kV], turn(j, L::kV)) && all_wait(&bars.v_fixed[j % L::kV], turn(j, L::kV));
+            }
+            if (!ok) break;
+            tc_fence_after();
+            if (issuer) {
+              const uint64_t v = tc_desc(values0 + j % L::kV * L::kTile, 16384);
+#pragma unroll
+              for (int ks = 0; ks < kTcKeys / 16; ++ks)
+                tc_mma_f16_ts(tmem + 256 + t * D, tmem + t * 128 + ks * 8, v + (uint64_t)(ks * 128), idesc_o, j > 0 || ks > 0);
+              if (t == tiles - 1) tc_commit(&bars.v_free[j % L::kV]);
+              if (j == nt - 1) tc_commit(&bars.o_done[t]);
+            }
+            __syncwarp();
+            if (j + 1 < nt) {
+              if (t == 0) ok = all_wait(&bars.k_full[(j + 1) % L::kK], turn(j + 1, L::kK));
+              if (ok) {
+                tc_fence_after();
+                scores(t, j + 1, t == tiles - 1);
+              }
+            }
+          }
+        }
+      }
+    } else {
+      // ---------------------------------------------------------- values that not every row sees
+      bool ok = true;
+      for (int j = 0; j < nt && ok; ++j) {
+        ok = wait(&bars.v_full[j % L::kV], turn(j, L::kV));
+        if (!ok) break;
+        const int j0 = block_key<kTcKeys>(seen, j);
+        const uint32_t block = values0 + j % L::kV * L::kTile;
+        bool bad = false;
+        for (int r = partly(j) ? tid - 320 : kTcKeys; r < kTcKeys; r += 64) {
+          const bool some = seen_by_some(seen, j0 + r);
+          if (some && pos0 >= 0 && seen_by_all(a, pos0, p_last, j0 + r, j0 + r)) continue;
+          for (int c = 0; c < D / 8; ++c) {
+            const uint32_t at = block + (c / 8) * 16384 + r * 128 + (c % 8) * 16;  // (any order: every piece of the row is visited)
+            if (some) {
+              uint4 x;
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory");
+              bad = bad || not_finite2<T>(x.x) || not_finite2<T>(x.y) || not_finite2<T>(x.z) || not_finite2<T>(x.w);
+            } else {
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
+            }
+          }
+        }
+        if (bad) s_bad = 1;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.v_fixed[j % L::kV]);
+      }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+      tc_fence_after();
+      tmem_dealloc(tmem, 512);
+    }
+    return;
+  }
+
+  // ------------------------------------------------------------ weights: one row per thread
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+  {
+    const int t = warp >> 2, r = tid & 127, tok = r / a.group, hg = r - tok * a.group, head = kvh * a.group + hg;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_col = tmem + t * 128 + lanes, o_col = tmem + 256 + t * D + lanes;
+    const bool live = tok < toks && t * toks + tok < ntok;
+    const int pos = live ? pos0 + t * toks + tok : -1;
+    const int first = pos0 + t * toks, last = min(p_last, first + toks - 1);  // of this tile
+    const float* bias = BIAS && live ? a.bias + (size_t)head * (a.bias_max + 1) : nullptr;
+    const float sink = a.sink && live ? a.sink[head] * kPagedLog2e : -INFINITY;
+    const float scale = BIAS ? 1.0f : a.scale2, grown = 8.0f / scale;  // BIAS: scores are scaled before their maximum
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    const int n = t < tiles ? nt : 0;
+    for (int j = 0; j < n; ++j) {
+      ok = ok && __all_sync(0xffffffffu, wait(&bars.s_full[t], (uint32_t)j & 1u));
+      tc_fence_after();
+      uint32_t v[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(s_col + c * 32, v[c]);
+      tmem_ld_wait();
+      const int j0 = block_key<kTcKeys>(seen, j);
+      if (BIAS) {
+        const float far = bias ? bias[a.bias_max] * kPagedLog2e : 0.0f;
+        const bool near = first - (j0 + kTcKeys - 1) < a.bias_max;  // some distance has a bias of its own
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float b = near && bias ? __ldg(bias + max(0, min(pos - (j0 + c * 32 + i), a.bias_max))) * kPagedLog2e : far;
+            v[c][i] = __float_as_uint(fmaf(__uint_as_float(v[c][i]), a.scale2, b));
+          }
+      }
+      if (first < 0 || !seen_by_all(a, first, last, j0, j0 + kTcKeys - 1)) {
+        const int hi = pos - j0, lo = a.window ? hi - a.window : -1, kp = a.window ? a.keep - j0 : 0;  // column i: i <= hi and (i > lo or i < kp)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int col = c * 32 + i;
+            if (!(col <= hi && (col > lo || col < kp))) v[c][i] = 0xff800000u;
+          }
+      }
+      float mx[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        mx[c] = __uint_as_float(v[c][0]);
+#pragma unroll
+        for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(v[c][i]));
+      }
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      if (__any_sync(0xffffffffu, top > m + grown)) {
+        const float m_new = fmaxf(m, top), alpha = m_new == -INFINITY ? 1.0f : paged_exp2((m - m_new) * scale);
+        m = m_new;
+        if (j > 0) {
+          l *= alpha;
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {  // (the products before S of this block are done)
+            uint32_t o[32];
+            tmem_ld32(o_col + c * 32, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st32(o_col + c * 32, o);
+          }
+        }
+      }
+      const float base = m == -INFINITY ? 0.0f : -m * scale;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p0 = paged_exp2(fmaf(__uint_as_float(v[c][2 * i]), scale, base)), p1 = paged_exp2(fmaf(__uint_as_float(v[c][2 * i + 1]), scale, base));
+          sum[i & 3] += p0 + p1;
+          w[i] = Num<T>::pack(p0, p1);
+        }
+        tmem_st16(s_col + c * 16, w);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.p_ready[t]);
+    }
+    if (n) ok = ok && __all_sync(0xffffffffu, wait(&bars.o_done[t], 0));
+    tc_fence_after();
+    if (live && n == 0) {
+      T* out = static_cast<T*>(a.out) + (row0 + t * toks + tok) * a.out_row + head * a.out_head;
+      for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(out + d) = make_uint4(0, 0, 0, 0);
+    }
+    if (n) {
+      const float total = l + paged_exp2(sink - (m == -INFINITY ? 0.0f : m * scale)), inv = pos < 0 ? 0.0f : 1.0f / total;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(o_col + c * 32, o);
+        tmem_ld_wait();
+        if (live && ok) {
+          T* out = static_cast<T*>(a.out) + (row0 + t * toks + tok) * a.out_row + head * a.out_head + c * 32;
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = pos < 0 ? 0u : Num<T>::pack(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(out + i * 8) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (!s_bad) return;
+  struct Cta {
+    __device__ void sync() const { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+    __device__ bool any(bool v) const {
+      int r;
+      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 256, p;\n\tselp.b32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"((int)v) : "memory");
+      return r != 0;
+    }
+  };
+  const Cta cta{};
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int few = kPpRows / a.group;
+  for (int t = 0; t < ntok; t += few) {
+    cta.sync();
+    paged_prompt_rows<T, D>(a, smem, cta, tid, tile.x, row0 + t, min(few, ntok - t), pos0 + t, kvh);
+  }
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                              CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static std::atomic<EncodeFn> fn{nullptr};
+  EncodeFn f = fn.load(std::memory_order_acquire);
+  if (!f) {
+    cudaDriverEntryPointQueryResult q;
+    void* p = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || !p) return nullptr;
+    f = reinterpret_cast<EncodeFn>(p);
+    fn.store(f, std::memory_order_release);
+  }
+  return f;
+}
+template <int N>
+bool encode(CUtensorMap* map, CUtensorMapDataType type, const void* base, const cuuint64_t (&dims)[N], const cuuint64_t (&strides)[N - 1], const cuuint32_t (&box)[N]) {
+  const EncodeFn fn = encode_fn();
+  cuuint32_t one[N];
+  for (auto& o : one) o = 1;
+  return fn && fn(map, type, N, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class T, int D, bool BIAS>
+cudaError_t configure() {
+  static std::atomic<unsigned long long> done{0};
+  return once_per_device(&done, [] { return cudaFuncSetAttribute(lm_paged_prompt_tc_kernel<T, D, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<D>::kBytes); });
+}
+template <class T, int D>
+cudaError_t launch(const Paged& a, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, int piece, cudaStream_t s) {
+  const int toks = 2 * (128 / a.group);
+  const long long tiles = std::min((long long)a.rows, a.rows / toks + (long long)a.seqs);
+  auto go = [&](auto kernel, cudaError_t r) {
+    return r != cudaSuccess ? r : launch_pdl(kernel, dim3((unsigned)(tiles * a.kv_heads)), dim3(kTcThreads), TcLayout<D>::kBytes, s, a, q, k, v, piece);
+  };
+  return a.bias ? go(lm_paged_prompt_tc_kernel<T, D, true>, configure<T, D, true>()) : go(lm_paged_prompt_tc_kernel<T, D, false>, configure<T, D, false>());
+}
+
+}  // namespace
+
+// Whether the kernel takes these sizes (and the tensor maps, these addresses and strides); `launched` says what became of it.
+bool launch_paged_prompt_tc(const Paged& a, bool f16, cudaStream_t s, cudaError_t* launched) {
+  if (a.dim != a.vdim || (a.dim != 64 && a.dim != 128) || !(a.scale2 > 1e-30f) || !(a.scale2 < 1e30f)) return false;
+  const int toks = 128 / a.group;
+  if (((long long)a.rows / (2 * toks) + a.seqs) * a.kv_heads > 0x7fffffffll) return false;
+  int piece = 16;
+  while (piece < kTcKeys && a.page % (2 * piece) == 0) piece *= 2;
+  const auto type = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  CUtensorMap q, k, v;
+  const cuuint32_t q_box[3] = {64, (cuuint32_t)a.group, (cuuint32_t)toks}, box[4] = {64, (cuuint32_t)piece, 1, 1};
+  const cuuint64_t D = a.dim, dims[4] = {D, (cuuint64_t)a.page, (cuuint64_t)a.kv_heads, (cuuint64_t)a.pages};
+  if (!encode<3>(&q, type, a.q, {D, (cuuint64_t)a.heads, (cuuint64_t)a.rows}, {(cuuint64_t)a.q_head * 2, (cuuint64_t)a.q_row * 2}, q_box) ||
+      !encode<4>(&k, type, a.k, dims, {(cuuint64_t)a.k_row * 2, (cuuint64_t)a.k_head * 2, (cuuint64_t)a.k_page * 2}, box) ||
+      !encode<4>(&v, type, a.v, dims, {(cuuint64_t)a.v_row * 2, (cuuint64_t)a.v_head * 2, (cuuint64_t)a.v_page * 2}, box))
+    return false;
+  *launched = f16 ? (a.dim == 64 ? launch<__half, 64>(a, q, k, v, piece, s) : launch<__half, 128>(a, q, k, v, piece, s))
+                  : (a.dim == 64 ? launch<__nv_bfloat16, 64>(a, q, k, v, piece, s) : launch<__nv_bfloat16, 128>(a, q, k, v, piece, s));
+  return true;
+}
+
+}  // namespace lm
+}  // namespace mllmb200
