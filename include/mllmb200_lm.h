@@ -42,6 +42,8 @@ typedef struct mllmb200_lm_config {
   float logit_scale;
   int norm_place;   /* MLLMB200_LM_NORM_* */
   float residual_scale; /* POST only */
+  int page, pages;  /* 0: a contiguous cache of max_ctx positions per slot; else attention layers keep their keys and values in
+                       `pages` pages of `page` tokens (a multiple of 16; BF16 only), which slots take as they grow */
 } mllmb200_lm_config;
 
 typedef struct mllmb200_lm_layer {
@@ -60,6 +62,7 @@ typedef struct mllmb200_lm_layer {
   int kv_from;               /* latent attention: -1, or the earlier layer whose cached rows this one uses */
   int act;                   /* MLLMB200_LM_ACT_* */
   int experts, top;          /* mixture of experts: their number and how many a token uses; experts 0 = a dense feed-forward */
+  int window, keep;          /* attention, with pages: position i sees j > i - window and j < keep alone; window 0 = everything */
 } mllmb200_lm_layer;
 
 /* Tensors of a layer; linear maps are bf16 [out, in] row-major. */
@@ -94,9 +97,23 @@ MLLMB200_API int mllmb200_lm_set_expert(void* handle, int layer, int expert, int
  * step).  tokens: all entries' tokens one after the other (host).  want: places among these sum(counts) rows whose
  * logits are copied to logits_out (host, fp32 [n_want, vocab], in the order of want).  sample != 0: the greedy next
  * token of every entry's last row is kept on the device as the slot's current token (see decode and read).
- * Synchronizes when logits are wanted.  MLLMB200_TOO_LARGE: more than max_rows rows, or a slot beyond max_ctx. */
+ * Synchronizes when logits are wanted.  MLLMB200_TOO_LARGE: more than max_rows rows, a slot beyond max_ctx, or more pages
+ * than are free (nothing is changed then). */
 MLLMB200_API int mllmb200_lm_step(void* handle, int entries, const int* slots, const int* counts, const int* tokens,
                                   int n_want, const int* want, float* logits_out, int sample);
+
+/* The same with the probabilities of the wanted rows instead of their logits (mllmb200_lm_probabilities), to device memory, fp32
+ * [n_want][ld]; nothing is sampled and nothing synchronizes: they are valid when the engine's stream reaches them. */
+MLLMB200_API int mllmb200_lm_step_probabilities(void* handle, int entries, const int* slots, const int* counts, const int* tokens,
+                                                int n_want, const int* want, float temperature, float* probabilities, long long ld);
+
+/* Takes a slot back to its first `length` tokens (drafted tokens that did not stand).  MLLMB200_UNSUPPORTED where layers
+ * have state that cannot go back (retention, an input convolution); MLLMB200_INVALID_ARG beyond the slot's tokens, or where
+ * pages that the tokens would see again have been given up. */
+MLLMB200_API int mllmb200_lm_truncate(void* handle, int slot, int length);
+
+/* Pages that no slot holds (0 without pages). */
+MLLMB200_API int mllmb200_lm_free_pages(void* handle, int* pages);
 
 /* `steps` greedy steps for `count` slots together, each feeding the slot's current token; the last call on every slot
  * must have been a sampling step or a decode.  One CUDA graph replay per step. */

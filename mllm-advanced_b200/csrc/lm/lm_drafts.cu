@@ -234,6 +234,11 @@ cudaError_t launch_probabilities(const void* logits, long long ld, int rows, int
 }
 
 }  // namespace
+
+cudaError_t launch_probability_rows(const float* logits, long long ld, int rows, int vocab, float temperature, float* out, long long ld_out, cudaStream_t s) {
+  return launch_probabilities<float>(logits, ld, rows, vocab, temperature, out, ld_out, s);
+}
+
 }  // namespace lm
 }  // namespace mllmb200
 

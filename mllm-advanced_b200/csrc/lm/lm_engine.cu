@@ -14,7 +14,7 @@
 #include <cstring>
 #include <tuple>
 
-#include "lm_state.h"
+#include "lm_paged.h"
 
 namespace mllmb200 {
 __global__ void sample_advance_batched_kernel(const float2*, int, int*, int*, int*, int, const int*, int*);
@@ -58,6 +58,13 @@ struct StepCtx {
   std::map<int, std::pair<const int4*, int>> tiles;
   const int2 *chunks = nullptr, *entry_chunks = nullptr;
   int n_chunks = 0;
+  // pages: where every row's keys and values go, and the sequences of one token and of more, each with its rows, length and
+  // row of the table
+  const int2* row_page = nullptr;
+  struct PagedRows {
+    int n = 0;
+    const int *first = nullptr, *count = nullptr, *lengths = nullptr, *table = nullptr;
+  } page_single, page_prompt;
   // latent attention: rows that attend through the latent (nullptr: all), a bound of their contexts, and the others
   const int* latent_rows = nullptr;
   int n_latent = 0, latent_ctx = 1;
@@ -97,6 +104,15 @@ struct Engine {
   int *d_slots = nullptr, *d_row_token = nullptr, *d_row_entry = nullptr, *d_identity = nullptr;
   int2* d_row_sp = nullptr;
   Entry* d_entries = nullptr;
+  // pages: their numbers per slot (-1: given up, behind the windows), those that no slot holds; tables of decode steps
+  bool paged = false;
+  int max_pages = 0, window = 0, keep_first = 0;  // window, keep_first: what every layer has let go of lies outside of them
+  std::vector<std::vector<int>> slot_pages;
+  std::vector<int> free_pages;
+  int *d_table = nullptr, *d_len = nullptr;
+  int2* d_row_page = nullptr;
+  float* zero_sinks = nullptr;
+  void* page_ws = nullptr;
   std::vector<int> cur_slots;
   std::vector<int> meta;
   int *meta_h = nullptr, *meta_d = nullptr;
@@ -202,6 +218,7 @@ int check_layer(Engine* e, int i, const mllmb200_lm_layer& d) {
     if (d.experts < 1 || d.top < 1 || d.top > d.experts || d.ff < 1) return fail(e, MLLMB200_INVALID_ARG, "layer %d: %d of %d experts", i, d.top, d.experts);
     if (d.experts > kMaxExperts || d.top > kMaxTop) return fail(e, MLLMB200_UNSUPPORTED, "layer %d: more than %d experts or %d at a time", i, kMaxExperts, kMaxTop);
   }
+  if (d.mixer == MLLMB200_LM_LATENT && (d.window || d.keep)) return fail(e, MLLMB200_UNSUPPORTED, "layer %d: a window in latent attention", i);
   if (d.mixer == MLLMB200_LM_LATENT) return check_latent(e, i, d);
   if (d.mixer == MLLMB200_LM_RETENTION) {
     if (d.kv_heads != d.heads) return fail(e, MLLMB200_UNSUPPORTED, "layer %d: retention has as many key as query heads", i);
@@ -211,6 +228,8 @@ int check_layer(Engine* e, int i, const mllmb200_lm_layer& d) {
       return fail(e, MLLMB200_INVALID_ARG, "layer %d: distance bias needs at least two rows and a largest distance beyond half of them", i);
     if (d.rot_dims) return fail(e, MLLMB200_UNSUPPORTED, "layer %d: rotation in attention", i);
   }
+  if (d.window < 0 || d.keep < 0) return fail(e, MLLMB200_INVALID_ARG, "layer %d: window %d, first tokens %d", i, d.window, d.keep);
+  if (d.window && (d.mixer != MLLMB200_LM_ATTENTION || !e->paged)) return fail(e, MLLMB200_UNSUPPORTED, "layer %d: a window needs attention over pages", i);
   if (d.weights_of >= 0) {
     if (d.weights_of >= i) return fail(e, MLLMB200_INVALID_ARG, "layer %d: weights of a later layer", i);
     const mllmb200_lm_layer &o = e->layers[d.weights_of].d, &m = d;
@@ -231,6 +250,9 @@ int create(Engine* e, const mllmb200_lm_layer* descs) {
   if (e->post && c.conv_taps) return fail(e, MLLMB200_UNSUPPORTED, "an input convolution with norms behind the residual sum");
   e->f32 = c.dtype == MLLMB200_LM_F32;
   e->elt = e->f32 ? 4 : 2;
+  if (c.page < 0 || c.pages < 0 || (c.page == 0) != (c.pages == 0)) return fail(e, MLLMB200_INVALID_ARG, "%d pages of %d tokens", c.pages, c.page);
+  e->paged = c.page > 0;
+  if (e->paged && (e->f32 || c.page % 16)) return fail(e, MLLMB200_UNSUPPORTED, "pages hold bf16, a multiple of 16 tokens each");
   e->widthp = pad_to(c.width, 64);
   if (e->widthp > 8192 || (size_t)c.conv_taps * e->widthp * 4 > kNormSmemMax) return fail(e, MLLMB200_UNSUPPORTED, "width %d with %d taps", c.width, c.conv_taps);
   LM_CUDA(cudaStreamCreateWithFlags(&e->stream, cudaStreamNonBlocking));
@@ -286,8 +308,9 @@ int create(Engine* e, const mllmb200_lm_layer* descs) {
       if (L.d.mixer == MLLMB200_LM_RETENTION) LM_OK(dalloc(e, &L.w.decay, (size_t)L.d.heads * (kChunk + 1)));
     }
     if (is_attn(L)) {
-      LM_OK(dalloc_bytes(e, &L.kc, slots * G * c.max_ctx * L.dimp * e->elt, true));
-      LM_OK(dalloc_bytes(e, &L.vc, slots * G * c.max_ctx * L.vdimp * e->elt, true));
+      const size_t positions = e->paged ? (size_t)c.pages * c.page : slots * c.max_ctx;
+      LM_OK(dalloc_bytes(e, &L.kc, positions * G * L.dimp * e->elt, true));
+      LM_OK(dalloc_bytes(e, &L.vc, positions * G * L.vdimp * e->elt, true));
       proj_bytes = std::max(proj_bytes, rows * qk_cols(L) * e->elt);
       part = std::max(part, (size_t)mix_cols(L));
       heads = std::max(heads, (size_t)L.d.heads);
@@ -382,6 +405,32 @@ int create(Engine* e, const mllmb200_lm_layer* descs) {
     bool ok = make_act_map(&L.a_mix, e->mix, c.max_rows, pad_to(mix_cols(L), 64)) == MLLMB200_OK;
     if (L.d.ff) ok = ok && make_act_map(&L.a_act, e->act, c.max_rows * (L.d.experts ? L.d.top : 1), pad_to(L.d.ff, 64)) == MLLMB200_OK;
     if (!ok) return fail(e, MLLMB200_CUDA_ERROR, "tensor map of the activations");
+  }
+  if (e->paged) {
+    e->max_pages = (c.max_ctx + c.page - 1) / c.page;
+    e->slot_pages.resize(slots);
+    for (int i = c.pages - 1; i >= 0; --i) e->free_pages.push_back(i);
+    size_t ws = 0;
+    for (size_t i = 0; i < e->layers.size(); ++i) {
+      const LayerState& L = e->layers[i];
+      if (!is_attn(L)) continue;
+      Paged a{};
+      a.dim = L.dimp, a.vdim = L.vdimp, a.group = L.d.heads / L.d.kv_heads, a.tokens = 1, a.seqs = c.max_seqs;
+      ws = std::max(ws, paged_decode_bytes(a));
+    }
+    int unbounded = 0;
+    for (const LayerState& L : e->layers) {
+      if (!is_attn(L)) continue;
+      unbounded += L.d.window == 0;
+      e->window = std::max(e->window, L.d.window);
+      e->keep_first = std::max(e->keep_first, L.d.keep);
+    }
+    if (unbounded) e->window = 0;
+    LM_OK(dalloc_bytes(e, &e->page_ws, ws));
+    LM_OK(dalloc(e, &e->d_table, slots * e->max_pages));
+    LM_OK(dalloc(e, &e->d_len, slots));
+    LM_OK(dalloc(e, &e->d_row_page, slots));
+    LM_OK(dalloc(e, &e->zero_sinks, heads));
   }
   LM_OK(dalloc(e, &e->d_pos, slots));
   LM_OK(dalloc(e, &e->d_tail, slots));
@@ -864,6 +913,30 @@ int latent_mixer(Engine* e, const StepCtx& t, LayerState& L) {
   return MLLMB200_OK;
 }
 
+// Attention over pages: sequences that bring one token, and those that bring more.
+int paged_mixer(Engine* e, const StepCtx& t, const LayerState& L, const Weights& w, int ldo) {
+  const auto& d = L.d;
+  Paged a{};
+  a.k = L.kc, a.v = L.vc;
+  a.k_row = L.dimp, a.k_head = (long long)e->c.page * L.dimp, a.k_page = d.kv_heads * a.k_head;
+  a.v_row = L.vdimp, a.v_head = (long long)e->c.page * L.vdimp, a.v_page = d.kv_heads * a.v_head;
+  a.pages = e->c.pages, a.page = e->c.page, a.kv_heads = d.kv_heads, a.dim = L.dimp, a.vdim = L.vdimp;
+  a.ld_table = a.max_pages = e->max_pages, a.rows = t.rows, a.tokens = 1;
+  a.q = e->proj, a.out = e->mix;
+  a.q_row = qk_cols(L), a.q_head = L.dimp, a.out_row = ldo, a.out_head = L.vdimp;
+  a.sink = d.sink ? e->zero_sinks : nullptr;
+  a.bias = d.bias_rows ? w.bias : nullptr;
+  a.heads = d.heads, a.group = d.heads / d.kv_heads, a.bias_max = d.bias_max, a.window = d.window, a.keep = d.keep;
+  a.scale2 = d.score_scale * kPagedLog2e;
+  auto rows = [&](const StepCtx::PagedRows& r) {
+    a.seqs = r.n, a.q_start = r.first, a.q_count = r.count, a.lengths = r.lengths, a.table = r.table;
+    return r.n > 0;
+  };
+  if (rows(t.page_single)) LM_CUDA(launch_paged_decode(a, false, e->page_ws, e->stream));
+  if (rows(t.page_prompt)) LM_CUDA(launch_paged_prompt(a, false, e->stream));
+  return MLLMB200_OK;
+}
+
 int mixer(Engine* e, const StepCtx& t, LayerState& L) {
   if (is_latent(L)) return latent_mixer(e, t, L);
   const Weights& w = e->layers[L.src].w;
@@ -882,9 +955,10 @@ int mixer(Engine* e, const StepCtx& t, LayerState& L) {
     p.dimp = L.dimp;
     p.vdimp = L.vdimp;
     p.kv_heads = d.kv_heads;
-    p.max_ctx = e->c.max_ctx;
-    p.row_sp = t.row_sp;
+    p.max_ctx = e->paged ? e->c.page : e->c.max_ctx;
+    p.row_sp = e->paged ? t.row_page : t.row_sp;
     if (launch_linear(e->stream, e->f32, w.in, e->m_h, e->h, t.rows, p, 1) < 1) return linear_failed(e);
+    if (e->paged) return paged_mixer(e, t, L, w, ldo);
     AttnShape s{};
     s.heads = d.heads;
     s.kv_heads = d.kv_heads;
@@ -1065,11 +1139,49 @@ int upload_meta(Engine* e) {
   return MLLMB200_OK;
 }
 
+// Pages that slot s lacks for its first `length` positions.
+int pages_lacking(const Engine* e, int s, int length) { return std::max(0, (length + e->c.page - 1) / e->c.page - (int)e->slot_pages[s].size()); }
+void take_pages(Engine* e, int s, int length) {
+  for (int n = pages_lacking(e, s, length); n > 0; --n) {
+    e->slot_pages[s].push_back(e->free_pages.back());
+    e->free_pages.pop_back();
+  }
+}
+// Gives back a slot's pages from place `from` on.
+void give_pages(Engine* e, int s, int from) {
+  auto& v = e->slot_pages[s];
+  for (int i = from; i < (int)v.size(); ++i)
+    if (v[i] >= 0) e->free_pages.push_back(v[i]);
+  v.resize(std::min(v.size(), (size_t)from));
+}
+// Gives up the pages that no later token of the slot sees in any layer (what runs on the stream still does, and whoever takes
+// them writes behind it).
+void leave_window(Engine* e, int s) {
+  if (!e->paged || !e->window) return;
+  auto& v = e->slot_pages[s];
+  const int page = e->c.page, first = (e->keep_first + page - 1) / page;
+  for (int i = (e->pos[s] - e->window + 1) / page - 1; i >= first && v[i] >= 0; --i) {
+    e->free_pages.push_back(v[i]);
+    v[i] = -1;
+  }
+}
+void table_row(const Engine* e, int s, int* row) {
+  for (int i = 0; i < e->max_pages; ++i) row[i] = i < (int)e->slot_pages[s].size() ? e->slot_pages[s][i] : -1;
+}
+
+// What a step leaves of the wanted rows: logits on the host, or probabilities on the device.
+struct Wanted {
+  float* logits;
+  float* probabilities;
+  long long ld;
+  float temperature;
+};
+
 int step(Engine* e, int n_entries, const int* slots, const int* counts, const int* tokens, int n_want, const int* want,
-         float* logits_out, int do_sample) {
+         const Wanted& out, int do_sample) {
   const auto& c = e->c;
   LM_OK(check_loaded(e));
-  if (n_entries < 1 || !slots || !counts || !tokens || n_want < 0 || (n_want && (!want || !logits_out))) return fail(e, MLLMB200_INVALID_ARG, "step arguments");
+  if (n_entries < 1 || !slots || !counts || !tokens || n_want < 0 || (n_want && (!want || (!out.logits && !out.probabilities)))) return fail(e, MLLMB200_INVALID_ARG, "step arguments");
   std::vector<Entry> entries(n_entries);
   std::vector<char> seen(c.max_seqs, 0);
   long long total = 0;
@@ -1089,6 +1201,13 @@ int step(Engine* e, int n_entries, const int* slots, const int* counts, const in
     if (tokens[i] < 0 || tokens[i] >= c.vocab) return fail(e, MLLMB200_INVALID_ARG, "token %d", tokens[i]);
   for (int i = 0; i < n_want; ++i)
     if (want[i] < 0 || want[i] >= rows) return fail(e, MLLMB200_INVALID_ARG, "wanted place %d of %d rows", want[i], rows);
+
+  if (e->paged) {
+    long long lacking = 0;
+    for (const Entry& en : entries) lacking += pages_lacking(e, en.slot, en.pos0 + en.count);
+    if (lacking > (long long)e->free_pages.size()) return fail(e, MLLMB200_TOO_LARGE, "%lld pages for the step, %zu are free", lacking, e->free_pages.size());
+    for (const Entry& en : entries) take_pages(e, en.slot, en.pos0 + en.count);
+  }
 
   std::vector<int2> row_sp(rows), chunks, entry_chunks(n_entries);
   std::vector<int> row_entry(rows), single_rows, last_rows(n_entries), last_pos(n_entries), new_tail(n_entries);
@@ -1150,6 +1269,23 @@ int step(Engine* e, int n_entries, const int* slots, const int* counts, const in
     }
   for (auto& ps : passes) longest_first(&ps.tiles);
 
+  struct PagedLists {
+    std::vector<int> first, count, lengths, table;
+  } paged_lists[2];  // sequences that bring one token, and more
+  std::vector<int2> row_page;
+  if (e->paged) {
+    row_page.resize(rows);
+    for (const Entry& en : entries) {
+      for (int j = 0; j < en.count; ++j) row_page[en.row0 + j] = make_int2(e->slot_pages[en.slot][(en.pos0 + j) / c.page], (en.pos0 + j) % c.page);
+      PagedLists& l = paged_lists[en.count > 1];
+      l.first.push_back(en.row0);
+      l.count.push_back(en.count);
+      l.lengths.push_back(en.pos0 + en.count);
+      l.table.resize(l.table.size() + e->max_pages);
+      table_row(e, en.slot, l.table.data() + l.table.size() - e->max_pages);
+    }
+  }
+
   MetaBuilder m(e->meta);
   const size_t o_tok = m.add(tokens, rows), o_sp = m.add(row_sp.data(), 2 * (size_t)rows), o_re = m.add(row_entry.data(), rows);
   const size_t o_en = m.add(entries.data(), 5 * (size_t)n_entries), o_ch = m.add(chunks.data(), 2 * chunks.size());
@@ -1163,6 +1299,12 @@ int step(Engine* e, int n_entries, const int* slots, const int* counts, const in
   for (auto& ps : passes) {
     const size_t o_rows = m.add(ps.rows.data(), 4 * ps.rows.size());
     o_pass.push_back({o_rows, m.add(ps.tiles.data(), 4 * ps.tiles.size())});
+  }
+  size_t o_page = m.add(row_page.data(), 2 * row_page.size()), o_lists[2][4];
+  for (int i = 0; i < 2; ++i) {
+    const PagedLists& l = paged_lists[i];
+    const std::vector<int>* lists[4] = {&l.first, &l.count, &l.lengths, &l.table};
+    for (int k = 0; k < 4; ++k) o_lists[i][k] = m.add(lists[k]->data(), lists[k]->size());
   }
   LM_OK(upload_meta(e));
 
@@ -1191,13 +1333,26 @@ int step(Engine* e, int n_entries, const int* slots, const int* counts, const in
     t.expand.push_back({reinterpret_cast<const int4*>(d + o_pass[i].first), reinterpret_cast<const int4*>(d + o_pass[i].second),
                         (int)passes[i].rows.size(), (int)passes[i].tiles.size(), passes[i].total});
 
+  t.row_page = reinterpret_cast<const int2*>(d + o_page);
+  auto paged_rows_of = [&](int i) {
+    StepCtx::PagedRows p;
+    p.n = (int)paged_lists[i].first.size();
+    p.first = d + o_lists[i][0], p.count = d + o_lists[i][1], p.lengths = d + o_lists[i][2], p.table = d + o_lists[i][3];
+    return p;
+  };
+  t.page_single = paged_rows_of(0);
+  t.page_prompt = paged_rows_of(1);
+
   const long long before = g_launches;
   Stream r{};
   LM_OK(forward(e, t, &r));
   for (int w0 = 0; w0 < n_want; w0 += e->logit_rows) {
     const int n = std::min(e->logit_rows, n_want - w0);
     LM_OK(logits_of(e, t, r, d + o_want + w0, n));
-    LM_CUDA(cudaMemcpyAsync(logits_out + (size_t)w0 * c.vocab, e->logits, (size_t)n * c.vocab * 4, cudaMemcpyDeviceToHost, e->stream));
+    if (out.probabilities)
+      LM_CUDA(launch_probability_rows(e->logits, c.vocab, n, c.vocab, out.temperature, out.probabilities + w0 * out.ld, out.ld, e->stream));
+    else
+      LM_CUDA(cudaMemcpyAsync(out.logits + (size_t)w0 * c.vocab, e->logits, (size_t)n * c.vocab * 4, cudaMemcpyDeviceToHost, e->stream));
   }
   if (do_sample) {
     lm_commit_kernel<<<(n_entries + 127) / 128, 128, 0, e->stream>>>(n_entries, d + o_sl, d + o_lp, d + o_nt, e->d_pos, e->d_tail);
@@ -1206,12 +1361,13 @@ int step(Engine* e, int n_entries, const int* slots, const int* counts, const in
     LM_OK(sample(e, n_entries, d + o_sl, nullptr));
   }
   LM_CUDA(cudaGetLastError());
-  if (n_want) LM_CUDA(cudaStreamSynchronize(e->stream));
+  if (n_want && out.logits) LM_CUDA(cudaStreamSynchronize(e->stream));
   e->launches += g_launches - before;
   for (const Entry& en : entries) {
     e->pos[en.slot] = en.pos0 + en.count;
     e->tail[en.slot] ^= 1;
     e->ready[en.slot] = do_sample != 0;
+    leave_window(e, en.slot);
   }
   return MLLMB200_OK;
 }
@@ -1229,6 +1385,13 @@ int enqueue_decode(Engine* e, int count, int chunk, int splits) {
   t.n_latent = count;
   t.latent_ctx = std::min(chunk * splits, e->c.max_ctx);
   LM_CUDA(launch_decode_prep(e->stream, count, e->d_slots, e->d_pos, e->d_token, e->d_tail, e->d_row_sp, e->d_row_token, e->d_entries, e->d_row_entry));
+  if (e->paged) {
+    LM_CUDA(launch_paged_prep(e->stream, count, e->d_row_sp, e->d_table, e->max_pages, e->c.page, e->d_row_page, e->d_len));
+    t.row_page = e->d_row_page;
+    t.page_single.n = count;
+    t.page_single.lengths = e->d_len;
+    t.page_single.table = e->d_table;
+  }
   Stream r{};
   LM_OK(forward(e, t, &r));
   LM_OK(logits_of(e, t, r, e->d_identity, count));
@@ -1247,6 +1410,17 @@ int decode(Engine* e, int count, const int* slots, int steps) {
     if (e->pos[s] + steps > c.max_ctx) return fail(e, MLLMB200_TOO_LARGE, "slot %d: %d + %d tokens, room for %d", s, e->pos[s], steps, c.max_ctx);
     seen[s] = 1;
     longest = std::max(longest, e->pos[s]);
+  }
+  if (e->paged) {
+    long long lacking = 0;
+    for (int i = 0; i < count; ++i) lacking += pages_lacking(e, slots[i], e->pos[slots[i]] + steps);
+    if (lacking > (long long)e->free_pages.size()) return fail(e, MLLMB200_TOO_LARGE, "%lld pages for the steps, %zu are free", lacking, e->free_pages.size());
+    std::vector<int> table((size_t)count * e->max_pages);
+    for (int i = 0; i < count; ++i) {
+      take_pages(e, slots[i], e->pos[slots[i]] + steps);
+      table_row(e, slots[i], table.data() + (size_t)i * e->max_pages);
+    }
+    LM_CUDA(cudaMemcpyAsync(e->d_table, table.data(), table.size() * 4, cudaMemcpyHostToDevice, e->stream));  // (from pageable memory: copied when this returns)
   }
   std::vector<int> now(slots, slots + count);
   if (now != e->cur_slots) {
@@ -1284,6 +1458,26 @@ int decode(Engine* e, int count, const int* slots, int steps) {
       e->tail[s] ^= 1;
     }
   }
+  for (int s : now) leave_window(e, s);
+  return MLLMB200_OK;
+}
+
+int truncate(Engine* e, int s, int length) {
+  if (s < 0 || s >= e->c.max_seqs || length < 0 || length > e->pos[s]) return fail(e, MLLMB200_INVALID_ARG, "slot %d back to %d tokens", s, length);
+  if (length == e->pos[s]) return MLLMB200_OK;
+  if (length > 0) {  // (an empty slot is a new sequence whatever state it had)
+    if (e->c.conv_taps > 1) return fail(e, MLLMB200_UNSUPPORTED, "an input convolution cannot go back");
+    for (const LayerState& L : e->layers)
+      if (L.d.mixer == MLLMB200_LM_RETENTION) return fail(e, MLLMB200_UNSUPPORTED, "retention cannot go back");
+  }
+  if (e->paged) {
+    const int page = e->c.page, low = e->window ? std::max(0, length - e->window + 1) / page : 0;
+    for (int i = low; i < (length + page - 1) / page; ++i)
+      if (e->slot_pages[s][i] < 0) return fail(e, MLLMB200_INVALID_ARG, "slot %d back to %d tokens: their pages have been given up", s, length);
+    give_pages(e, s, (length + page - 1) / page);
+  }
+  e->pos[s] = length;
+  e->ready[s] = 0;
   return MLLMB200_OK;
 }
 
@@ -1338,7 +1532,20 @@ int mllmb200_lm_set_expert(void* handle, int layer, int expert, int which, const
 }
 int mllmb200_lm_step(void* handle, int entries, const int* slots, const int* counts, const int* tokens, int n_want, const int* want,
                      float* logits_out, int sample) {
-  return handle ? step(from(handle), entries, slots, counts, tokens, n_want, want, logits_out, sample) : MLLMB200_INVALID_ARG;
+  return handle ? step(from(handle), entries, slots, counts, tokens, n_want, want, Wanted{logits_out, nullptr, 0, 0.0f}, sample) : MLLMB200_INVALID_ARG;
+}
+int mllmb200_lm_step_probabilities(void* handle, int entries, const int* slots, const int* counts, const int* tokens, int n_want, const int* want,
+                                   float temperature, float* probabilities, long long ld) {
+  auto* e = from(handle);
+  if (!e) return MLLMB200_INVALID_ARG;
+  if (n_want && (!probabilities || ld < e->c.vocab || !(temperature >= 0.0f) || std::isinf(temperature))) return fail(e, MLLMB200_INVALID_ARG, "probabilities of a step");
+  return step(e, entries, slots, counts, tokens, n_want, want, Wanted{nullptr, probabilities, ld, temperature}, 0);
+}
+int mllmb200_lm_truncate(void* handle, int slot, int length) { return handle ? truncate(from(handle), slot, length) : MLLMB200_INVALID_ARG; }
+int mllmb200_lm_free_pages(void* handle, int* pages) {
+  if (!handle || !pages) return MLLMB200_INVALID_ARG;
+  *pages = (int)from(handle)->free_pages.size();
+  return MLLMB200_OK;
 }
 int mllmb200_lm_decode(void* handle, int count, const int* slots, int steps) {
   return handle ? decode(from(handle), count, slots, steps) : MLLMB200_INVALID_ARG;
@@ -1347,6 +1554,7 @@ int mllmb200_lm_free_slot(void* handle, int slot) {
   auto* e = from(handle);
   if (!e || slot < 0 || slot >= e->c.max_seqs) return MLLMB200_INVALID_ARG;
   e->pos[slot] = e->tail[slot] = e->ready[slot] = 0;
+  if (e->paged) give_pages(e, slot, 0);
   return MLLMB200_OK;
 }
 int mllmb200_lm_read(void* handle, int slot, int first, int count, int* tokens_out, int* length_out) {

@@ -495,7 +495,37 @@ cudaError_t launch_prompt(const Paged& a, cudaStream_t s) {
 }
 int status_of(cudaError_t r) { return r == cudaSuccess ? MLLMB200_OK : MLLMB200_CUDA_ERROR; }
 
+__global__ void lm_paged_prep_kernel(int n, const int2* __restrict__ row_sp, const int* __restrict__ table, int ld_table, int page,
+                                     int2* __restrict__ row_page, int* __restrict__ lengths) {
+  pdl_launch_dependents();
+  pdl_wait_prior();
+  const int b = blockIdx.x * blockDim.x + threadIdx.x;
+  if (b >= n) return;
+  const int p = row_sp[b].y, place = p / page;
+  row_page[b] = make_int2(table[(size_t)b * ld_table + place], p - place * page);
+  lengths[b] = p + 1;
+}
+
 }  // namespace
+
+size_t paged_decode_bytes(const Paged& a) { return decode_space(a, std::min(a.seqs, kDecSeqs)).bytes; }
+cudaError_t launch_paged_decode(const Paged& a, bool f16, void* workspace, cudaStream_t s) {
+  const cudaError_t r = configure_decode();
+  if (r != cudaSuccess) return r;
+  auto* ws = static_cast<uint8_t*>(workspace);
+  return f16 ? launch_decode<__half>(a, ws, s) : launch_decode<__nv_bfloat16>(a, ws, s);
+}
+cudaError_t launch_paged_prompt(const Paged& a, bool f16, cudaStream_t s) {
+  cudaError_t r = cudaSuccess;
+  if (launch_paged_prompt_tc(a, f16, s, &r)) return r;
+  r = configure_prompt();
+  if (r != cudaSuccess) return r;
+  return f16 ? launch_prompt<__half>(a, s) : launch_prompt<__nv_bfloat16>(a, s);
+}
+cudaError_t launch_paged_prep(cudaStream_t s, int n, const int2* row_sp, const int* table, int ld_table, int page, int2* row_page, int* lengths) {
+  return launch_pdl(lm_paged_prep_kernel, dim3((n + 127) / 128), dim3(128), 0, s, n, row_sp, table, ld_table, page, row_page, lengths);
+}
+
 }  // namespace lm
 }  // namespace mllmb200
 
@@ -530,11 +560,7 @@ int mllmb200_lm_attn_decode(const mllmb200_lm_pages* pages, const mllmb200_lm_lo
   if (st != MLLMB200_OK) return st;
   if (!a.seqs || !a.rows) return MLLMB200_OK;
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u)) return MLLMB200_INVALID_ARG;
-  cudaError_t r = configure_decode();
-  if (r != cudaSuccess) return MLLMB200_CUDA_ERROR;
-  auto* ws = static_cast<uint8_t*>(workspace);
-  auto s = static_cast<cudaStream_t>(stream);
-  return status_of(pages->dtype == MLLMB200_LM_F16 ? launch_decode<__half>(a, ws, s) : launch_decode<__nv_bfloat16>(a, ws, s));
+  return status_of(launch_paged_decode(a, pages->dtype == MLLMB200_LM_F16, workspace, static_cast<cudaStream_t>(stream)));
 }
 
 int mllmb200_lm_attn_prompt_workspace(const mllmb200_lm_pages* pages, const mllmb200_lm_look* look, size_t* bytes) {
@@ -551,11 +577,7 @@ int mllmb200_lm_attn_prompt(const mllmb200_lm_pages* pages, const mllmb200_lm_lo
   if (st != MLLMB200_OK) return st;
   if (!a.seqs || !a.rows) return MLLMB200_OK;
   (void)workspace;
-  cudaError_t r = cudaSuccess;
-  if (launch_paged_prompt_tc(a, pages->dtype == MLLMB200_LM_F16, static_cast<cudaStream_t>(stream), &r)) return status_of(r);
-  if (configure_prompt() != cudaSuccess) return MLLMB200_CUDA_ERROR;
-  auto s = static_cast<cudaStream_t>(stream);
-  return status_of(pages->dtype == MLLMB200_LM_F16 ? launch_prompt<__half>(a, s) : launch_prompt<__nv_bfloat16>(a, s));
+  return status_of(launch_paged_prompt(a, pages->dtype == MLLMB200_LM_F16, static_cast<cudaStream_t>(stream)));
 }
 
 int mllmb200_lm_operator_status(void* stream) {

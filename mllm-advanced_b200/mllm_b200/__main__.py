@@ -15,6 +15,12 @@ def parser():
     gen.add_argument("--stop", default="", help="comma-separated token ids that end a sequence")
     gen.add_argument("--dtype", default=None, help="number format (default: the design's own)")
     gen.add_argument("--slots", type=int, default=8, help="sequences held at once")
+    gen.add_argument("--page", type=int, default=0, help="tokens per page of the engine's attention caches (default: a contiguous slot per sequence)")
+    gen.add_argument("--pages", type=int, default=None, help="pages in all (default: as many as the slots can need)")
+    gen.add_argument("--draft", default=None, help="folder of a smaller model of the same vocabulary that proposes tokens")
+    gen.add_argument("--drafts", type=int, default=4, help="tokens that the draft model proposes a round")
+    gen.add_argument("--temperature", type=float, default=0.0, help="with --draft: of the draws; 0 = greedy")
+    gen.add_argument("--seed", type=int, default=0, help="with --draft: of the random numbers")
     gen.add_argument("--portion", type=int, default=None, help="most prompt tokens of one sequence in a step")
     tr = sub.add_parser("trace", help="replay steps of given tokens from standard input and write logits")
     add_trace_arguments(tr)
@@ -54,9 +60,22 @@ def main(argv=None):
     elif args.command == "generate":
         prompts = [ids(t) for t in args.tokens]
         ctx = max(len(p) for p in prompts) + args.max_new
-        model, runtime = registry.load(args.model, args.dtype, max_seqs=min(args.slots, len(prompts)), max_ctx=ctx,
-                                       max_rows=min(4096, sum(len(p) for p in prompts)))
-        for out in registry.generate(model, runtime, prompts, args.max_new, set(ids(args.stop)), args.portion):
+        slots = min(args.slots, len(prompts))
+        pages = (args.pages or slots * -(-ctx // args.page)) if args.page else 0
+        rows = min(4096, sum(len(p) for p in prompts))
+        if args.draft:
+            rows = max(rows, slots * (args.drafts + 1))
+        model, runtime = registry.load(args.model, args.dtype, max_seqs=slots, max_ctx=ctx, max_rows=rows, page=args.page, pages=pages)
+        if args.draft:
+            draft, draft_runtime = registry.load(args.draft, args.dtype, max_seqs=slots, max_ctx=ctx, max_rows=rows)
+            if runtime != "engine" or draft_runtime != "engine":
+                raise SystemExit("only models of the language-model engine generate with drafts")
+            from . import scheduler
+            outs = scheduler.generate_drafted(model, draft, prompts, args.max_new, args.drafts, args.temperature, args.seed, set(ids(args.stop)), args.portion)
+            draft.close()
+        else:
+            outs = registry.generate(model, runtime, prompts, args.max_new, set(ids(args.stop)), args.portion)
+        for out in outs:
             print(",".join(str(t) for t in out))
         model.close()
     else:

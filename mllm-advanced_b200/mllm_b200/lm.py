@@ -22,14 +22,15 @@ _LINEARS = {"q", "k", "v", "g", "o", "gate", "up", "down", "embed", "head", "dkv
 
 class Config(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("vocab", "width", "layers", "dtype", "conv_taps", "max_seqs", "max_ctx", "max_rows")] + \
-               [("eps", C.c_float), ("logit_scale", C.c_float), ("norm_place", C.c_int), ("residual_scale", C.c_float)]
+               [("eps", C.c_float), ("logit_scale", C.c_float), ("norm_place", C.c_int), ("residual_scale", C.c_float), ("page", C.c_int),
+                ("pages", C.c_int)]
 
 
 class Layer(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("mixer", "heads", "kv_heads", "dim", "vdim")] + [("score_scale", C.c_float)] + \
                [(n, C.c_int) for n in ("sink", "bias_rows", "bias_max", "rot_dims")] + [("rot_base", C.c_double), ("ff", C.c_int),
                                                                                       ("ff_limit", C.c_float), ("weights_of", C.c_int)] + \
-               [(n, C.c_int) for n in ("kv_rank", "kv_from", "act", "experts", "top")]
+               [(n, C.c_int) for n in ("kv_rank", "kv_from", "act", "experts", "top", "window", "keep")]
 
 
 class EngineError(RuntimeError):
@@ -61,6 +62,7 @@ def lib():
     sig = {"create": [C.POINTER(Config), C.POINTER(Layer), C.POINTER(vp)], "set_tensor": [vp, ci, ci, vp, ci, ci],
            "set_expert": [vp, ci, ci, ci, vp, ci, ci],
            "step": [vp, ci, vp, vp, vp, ci, vp, vp, ci], "decode": [vp, ci, vp, ci], "free_slot": [vp, ci],
+           "step_probabilities": [vp, ci, vp, vp, vp, ci, vp, C.c_float, vp, ll], "truncate": [vp, ci, ci], "free_pages": [vp, vp],
            "read": [vp, ci, ci, ci, vp, vp], "keep_residual": [vp, ci], "read_residual": [vp, ci, ci, vp],
            "stats": [vp, C.POINTER(C.c_size_t), C.POINTER(C.c_longlong)], "synchronize": [vp], "check_device_status": [vp],
            "distance_buckets": [ci, ci, ci, vp],
@@ -94,14 +96,17 @@ def _ints(a):
 
 
 class LanguageModel:
-    """config: fields of Config without `layers` and `dtype`; layers: one dict of Layer fields per layer."""
+    """config: fields of Config without `layers` and `dtype`; layers: one dict of Layer fields per layer.  page, pages: attention
+    layers keep their cache in pages that slots take as they grow (bf16); layers may then have a window and first tokens that stay."""
 
     def __init__(self, config, layers, dtype=BF16):
-        self.config = dict({"norm_place": NORM_SANDWICH, "residual_scale": 1.0}, **config, layers=len(layers), dtype=dtype)
+        self.config = dict({"norm_place": NORM_SANDWICH, "residual_scale": 1.0, "page": 0, "pages": 0}, **config, layers=len(layers), dtype=dtype)
         self.layers = [dict({"sink": 0, "bias_rows": 0, "bias_max": 0, "rot_dims": 0, "rot_base": 1.0, "ff": 0, "ff_limit": 0.0,
-                             "score_scale": 1.0, "weights_of": -1, "kv_rank": 0, "kv_from": -1, "act": CLAMPED, "experts": 0, "top": 0}, **d) for d in layers]
+                             "score_scale": 1.0, "weights_of": -1, "kv_rank": 0, "kv_from": -1, "act": CLAMPED, "experts": 0, "top": 0,
+                             "window": 0, "keep": 0}, **d) for d in layers]
         self.vocab, self.max_seqs = self.config["vocab"], self.config["max_seqs"]
         self.max_ctx, self.max_rows = self.config["max_ctx"], self.config["max_rows"]
+        self.page, self.pages = self.config["page"], self.config["pages"]
         self._L, self._h = lib(), C.c_void_p()
         descs = (Layer * len(layers))(*[Layer(**d) for d in self.layers])
         st = self._L.mllmb200_lm_create(C.byref(Config(**self.config)), descs, C.byref(self._h))
@@ -174,6 +179,34 @@ class LanguageModel:
         for s, n in zip(slots, counts):
             self.length[s] += int(n)
         return logits
+
+    def step_probabilities(self, entries, want, temperature=1.0, out=None):
+        """A step whose wanted places' probabilities stay on the device: fp32 [len(want), vocab], ready on torch's current stream."""
+        import torch
+        slots, counts = _ints([s for s, _ in entries]), _ints([len(t) for _, t in entries])
+        tokens, want = _ints(np.concatenate([np.asarray(t, np.int32) for _, t in entries])), _ints(want)
+        if out is None:
+            out = torch.empty((len(want), self.vocab), dtype=torch.float32, device="cuda")
+        if out.shape != (len(want), self.vocab) or out.dtype != torch.float32 or out.stride(1) != 1 or not out.is_cuda:
+            raise ValueError("step_probabilities: out [wanted, vocab] in fp32 on the GPU")
+        mine, here = self.stream(), torch.cuda.current_stream()
+        mine.wait_stream(here)  # whoever still uses out's memory
+        self._check(self._L.mllmb200_lm_step_probabilities(self._h, len(slots), slots.ctypes.data, counts.ctypes.data, tokens.ctypes.data, len(want), want.ctypes.data,
+                                                           temperature, out.data_ptr(), max(out.stride(0), self.vocab)), "step_probabilities")
+        here.wait_stream(mine)
+        for s, n in zip(slots, counts):
+            self.length[s] += int(n)
+        return out
+
+    def truncate(self, slot, length):
+        """Takes a slot back to its first `length` tokens (not with retention or an input convolution)."""
+        self._check(self._L.mllmb200_lm_truncate(self._h, slot, length), "truncate")
+        self.length[slot] = length
+
+    def free_pages(self):
+        n = C.c_int()
+        self._check(self._L.mllmb200_lm_free_pages(self._h, C.byref(n)), "free_pages")
+        return n.value
 
     def decode(self, slots, steps):
         """Greedy steps for these slots together; the tokens are read with `read`."""

@@ -14,20 +14,22 @@ from .safetensors import Tensors
 DTYPES = {"bfloat16": lm.BF16, "float32": lm.F32}
 
 
-def _load_vupuzen(cfg, folder, dtype, max_seqs, max_ctx, max_rows):
-    return vupuzen.load(cfg, Tensors(folder), DTYPES[dtype], max_seqs, max_ctx, max_rows)
+def _load_vupuzen(cfg, folder, dtype, max_seqs, max_ctx, max_rows, page, pages):
+    return vupuzen.load(cfg, Tensors(folder), DTYPES[dtype], max_seqs, max_ctx, max_rows, page, pages)
 
 
-def _load_taralix(cfg, folder, dtype, max_seqs, max_ctx, max_rows):
-    return taralix.load(cfg, Tensors(folder), DTYPES[dtype], max_seqs, max_ctx, max_rows)
+def _load_taralix(cfg, folder, dtype, max_seqs, max_ctx, max_rows, page, pages):
+    return taralix.load(cfg, Tensors(folder), DTYPES[dtype], max_seqs, max_ctx, max_rows, page, pages)
 
 
-def _load_qwen2(cfg, folder, dtype, max_seqs, max_ctx, max_rows):
+def _load_qwen2(cfg, folder, dtype, max_seqs, max_ctx, max_rows, page, pages):
     """Weights by their published names, the linears quantized to int4 on the host (W4A32), lm_head in fp16."""
     import torch
 
     from . import binding as B
     from .decoder import LINEAR_NAMES, Qwen2Decoder
+    if page or pages:
+        raise ValueError("the quantized decoder has no pages")
     t = Tensors(folder)
     heads = cfg["num_attention_heads"]
     dec = Qwen2Decoder(dict(layers=cfg["num_hidden_layers"], hidden=cfg["hidden_size"], q_heads=heads, kv_heads=cfg["num_key_value_heads"],
@@ -67,14 +69,15 @@ def architecture(cfg):
     return name
 
 
-def load(folder, dtype=None, max_seqs=8, max_ctx=2048, max_rows=2048):
-    """(model, runtime).  dtype: one of the design's number formats, by default the first."""
+def load(folder, dtype=None, max_seqs=8, max_ctx=2048, max_rows=2048, page=0, pages=0):
+    """(model, runtime).  dtype: one of the design's number formats, by default the first.  page, pages: the engine's attention
+    layers keep their cache in `pages` pages of `page` tokens, shared by all slots."""
     cfg = read_config(folder)
     runtime, dtypes, loader = MODELS[architecture(cfg)]
     dtype = dtype or dtypes[0]
     if dtype not in dtypes:
         raise ValueError(f"{architecture(cfg)} runs in {', '.join(dtypes)}, not in {dtype}")
-    return loader(cfg, folder, dtype, max_seqs, max_ctx, max_rows), runtime
+    return loader(cfg, folder, dtype, max_seqs, max_ctx, max_rows, page, pages), runtime
 
 
 def generate(model, runtime, prompts, max_new, stop=(), portion=None):

@@ -29,8 +29,8 @@ def layers_from_config(cfg):
     return out
 
 
-def model_config(cfg, max_seqs, max_ctx, max_rows):
-    return {"vocab": cfg["vocab"], "width": cfg["width"], "conv_taps": 0, "eps": cfg["norm"]["eps"], "logit_scale": 1.0,
+def model_config(cfg, max_seqs, max_ctx, max_rows, page=0, pages=0):
+    return {"page": page, "pages": pages, "vocab": cfg["vocab"], "width": cfg["width"], "conv_taps": 0, "eps": cfg["norm"]["eps"], "logit_scale": 1.0,
             "norm_place": lm.NORM_POST, "residual_scale": cfg["postln_alpha"], "max_seqs": max_seqs, "max_ctx": max_ctx, "max_rows": max_rows}
 
 
@@ -59,8 +59,8 @@ def load_layer(model, tensors, i, entry):
             model.set_expert(i, x, name, tensors.bf16(f"{p}mlp.e{x}.{name}"))
 
 
-def load(cfg, tensors, dtype, max_seqs, max_ctx, max_rows):
-    model = lm.LanguageModel(model_config(cfg, max_seqs, max_ctx, max_rows), layers_from_config(cfg), dtype)
+def load(cfg, tensors, dtype, max_seqs, max_ctx, max_rows, page=0, pages=0):
+    model = lm.LanguageModel(model_config(cfg, max_seqs, max_ctx, max_rows, page, pages), layers_from_config(cfg), dtype)
     model.set_tensor(-1, "embed", tensors.bf16("embed"))
     model.set_tensor(-1, "head", tensors.bf16("head"))
     model.set_tensor(-1, "final_norm", 1.0 + tensors.f32("final.norm"))

@@ -3,7 +3,8 @@
 Every layer wraps its sublayers in norms on both sides (one gain per norm), reads its mixer's input through a causal
 convolution, and mixes by attention (no rotation; a learned bias by log-bucketed distance; a sink of score 0) or by
 retention (rotated, a fixed decay per head).  The feed-forward is a clamped gated one, or absent.  A layer may use an
-earlier layer's tensors."""
+earlier layer's tensors.  An attention layer may have a window and first tokens that stay visible ("window" and "keep" of its
+mixer); such models run on a cache in pages."""
 import numpy as np
 
 from . import lm
@@ -19,7 +20,8 @@ def layers_from_config(cfg, rel_rows):
         src = e.get("weights_of")
         d = {"heads": m["heads"], "dim": m["dim"], "vdim": m["vdim"], "weights_of": -1 if src is None else src}
         if e["type"] == "attention":
-            d.update(mixer=lm.ATTENTION, kv_heads=m["kv_heads"], score_scale=m["scale"], sink=1, bias_rows=rel_rows(i), bias_max=m["bias_max"])
+            d.update(mixer=lm.ATTENTION, kv_heads=m["kv_heads"], score_scale=m["scale"], sink=1, bias_rows=rel_rows(i), bias_max=m["bias_max"],
+                     window=m.get("window") or 0, keep=m.get("keep") or 0)
         elif e["type"] == "retention":
             rot = m.get("rot") or {"dims": 0, "base": 1.0}
             d.update(mixer=lm.RETENTION, kv_heads=m["heads"], rot_dims=rot["dims"], rot_base=rot["base"])
@@ -35,8 +37,8 @@ def layers_from_config(cfg, rel_rows):
     return out
 
 
-def model_config(cfg, max_seqs, max_ctx, max_rows):
-    return {"vocab": cfg["vocab"], "width": cfg["width"], "conv_taps": cfg["canon"]["taps"], "eps": cfg["norm"]["eps"],
+def model_config(cfg, max_seqs, max_ctx, max_rows, page=0, pages=0):
+    return {"page": page, "pages": pages, "vocab": cfg["vocab"], "width": cfg["width"], "conv_taps": cfg["canon"]["taps"], "eps": cfg["norm"]["eps"],
             "logit_scale": cfg["logit_scale"], "max_seqs": max_seqs, "max_ctx": max_ctx, "max_rows": max_rows}
 
 
@@ -57,8 +59,8 @@ def layer_tensors(entry):
     return names
 
 
-def load(cfg, tensors, dtype, max_seqs, max_ctx, max_rows):
-    model = lm.LanguageModel(model_config(cfg, max_seqs, max_ctx, max_rows),
+def load(cfg, tensors, dtype, max_seqs, max_ctx, max_rows, page=0, pages=0):
+    model = lm.LanguageModel(model_config(cfg, max_seqs, max_ctx, max_rows, page, pages),
                              layers_from_config(cfg, lambda i: tensors.shape(f"l{owner(cfg, i)}.mix.rel")[0]), dtype)
     model.set_tensor(-1, "embed", tensors.bf16("embed"))
     model.set_tensor(-1, "head", tensors.bf16("head"))

@@ -68,7 +68,10 @@ def attention(h, w, cfg):
     for a in range(H):
         g = a // (H // G)
         s = (q[:, a] @ k[:, g].T) * cfg["scale"] + bias[np.maximum(dist, 0), a]
-        s = np.where(dist >= 0, s, -np.inf)
+        seen = dist >= 0
+        if cfg.get("window"):
+            seen &= (dist < cfg["window"]) | (np.arange(T) < (cfg.get("keep") or 0))[None, :]
+        s = np.where(seen, s, -np.inf)
         out[:, a] = softmax_with_sink(s) @ v[:, g]
     return out.reshape(T, H * DV) @ w["o"].T
 
