@@ -205,7 +205,7 @@ MLLMB200_API int mllmb200_lm_probabilities(const void* logits, int dtype, long l
  * comes from max(p - q, 0) (from p where that has no mass), behind the last draft from p: the lowest index whose running sum
  * exceeds pick times the whole.  A token outside [0, vocab) ends a sequence's drafts: the next token comes from p there.
  * Negative numbers and NaN count as 0.  accepted[s]: accepted drafts; out [seqs][drafts + 1]: these, the next token (-1 where
- * p has no mass), and -1 behind it.  drafts may be 0: a plain draw from p. */
+ * p has no mass), and -1 behind it.  drafts may be 0: a plain draw from p.  vocab: at most 2^20. */
 MLLMB200_API int mllmb200_lm_verify(const float* target, long long t_seq, long long t_row, const float* draft, long long d_seq,
                                     long long d_row, const int* tokens, long long ld_tokens, const float* accept,
                                     long long ld_accept, const float* pick, int seqs, int drafts, int vocab, int* accepted,

@@ -1,6 +1,7 @@
 // Logits to probabilities, and drafted tokens against the target's probabilities (include/mllmb200_lm.h).  Both work a row
 // of the vocabulary at a time: a cluster of CTAs per row, each holding its part in shared memory or registers, so that the
 // row is read once; what the parts have to tell one another goes through distributed shared memory.
+#include <algorithm>
 #include <cmath>
 
 #include "../device_common.cuh"
@@ -37,7 +38,146 @@ __device__ __forceinline__ int ld_remote(const int* local, uint32_t rank) {
   return v;
 }
 
+constexpr int kRowThreads = 512, kRowWarps = kRowThreads / 32, kRowItems = 10;  // a CTA's part of a row: up to 10 x 4 numbers a thread
+constexpr int kRowMost = 8 * kRowThreads * 4 * kRowItems;                        // a cluster of 8 CTAs holds rows up to here
+
+// Numbers i .. i + 3 of a row, `fill` from `end` on.  VEC: i is a multiple of 4 and the row lies on 4 numbers; else the four are
+// kRowThreads apart.
+template <bool VEC, class T>
+__device__ __forceinline__ void load4(const T* row, int i, int end, float fill, float (&v)[4]) {
+  if (VEC && i + 3 < end) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 x = *reinterpret_cast<const float4*>(row + i);
+      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    } else {
+      const uint2 x = *reinterpret_cast<const uint2*>(row + i);
+      const T* t = reinterpret_cast<const T*>(&x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = to_f32(t[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int at = i + e * (VEC ? 1 : kRowThreads);
+      v[e] = at < end ? to_f32(row[at]) : fill;
+    }
+  }
+}
+// first number of a thread's item k in a part that starts at v0
+template <bool VEC>
+__device__ __forceinline__ int item_at(int v0, int k, int tid) {
+  return VEC ? v0 + (k * kRowThreads + tid) * 4 : v0 + k * kRowThreads * 4 + tid;
+}
+template <bool VEC>
+__device__ __forceinline__ int element(int i, int e) { return VEC ? i + e : i + e * kRowThreads; }
+
 // ------------------------------------------------------------------------------------------ probabilities
+// grid (cluster, rows): every CTA reads its part of the row once, all loads in flight, and keeps it in registers; weights are taken
+// against the part's own maximum, so that one exchange in the cluster (maximum, sum) settles the row.  Bound by memory: 8
+// bytes a number.  384 rows of 151936: 452 us with three passes of scalar loads over the row.
+template <class T, int ITEMS, bool VEC>
+__global__ void __launch_bounds__(kRowThreads, 2) lm_probability_rows_kernel(const T* __restrict__ logits, long long ld, int vocab, int per, float inv_t, bool greedy,
+                                                                          float* __restrict__ out, long long ld_out) {
+  __shared__ float s_red[kRowWarps], s_max, s_sum;
+  __shared__ int s_at[kRowWarps], s_first;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, ctas = gridDim.x, part = blockIdx.x;
+  pdl_launch_dependents();
+  pdl_wait_prior();
+  const T* z = logits + blockIdx.y * ld;
+  float* y = out + blockIdx.y * ld_out;
+  const int v0 = min(part * per, vocab), v1 = min(v0 + per, vocab);
+  float x[ITEMS][4], mx = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) load4<VEC>(z, item_at<VEC>(v0, k, tid), v1, -INFINITY, x[k]);
+  bool odd = false;  // NaN or +inf
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) odd = odd || !(x[k][e] < INFINITY), mx = fmaxf(mx, x[k][e]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if (lane == 0) s_red[warp] = mx;
+  odd = __syncthreads_or(odd);
+#pragma unroll
+  for (int w = 0; w < kRowWarps; ++w) mx = fmaxf(mx, s_red[w]);
+  if (greedy) {
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int k = ITEMS - 1; k >= 0; --k)
+#pragma unroll
+      for (int e = 3; e >= 0; --e)
+        if (x[k][e] == mx && mx > -INFINITY) at = min(at, element<VEC>(item_at<VEC>(v0, k, tid), e));
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (lane == 0) s_at[warp] = at;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 0; w < kRowWarps; ++w) at = min(at, s_at[w]);
+      s_first = at, s_max = mx;
+    }
+    cluster_sync_all();
+    float best = -INFINITY;
+    for (int r = 0; r < ctas; ++r) {
+      const float m = ld_remote(&s_max, r);
+      if (m > best) best = m, at = ld_remote(&s_first, r);  // (parts in order: the first of equals stays)
+    }
+    if (!(best > -INFINITY)) at = -1;
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[k][e] = element<VEC>(item_at<VEC>(v0, k, tid), e) == at ? 1.0f : 0.0f;
+  } else {
+    const float base = mx > -INFINITY ? mx : 0.0f;
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[k][e] = expf((x[k][e] - base) * inv_t);
+        sum += x[k][e];
+      }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    __syncthreads();
+    if (lane == 0) s_red[warp] = sum;
+    __syncthreads();
+    if (tid == 0) {
+      sum = 0.0f;
+      for (int w = 0; w < kRowWarps; ++w) sum += s_red[w];
+      s_max = mx, s_sum = odd ? __int_as_float(0x7fffffff) : sum;  // (a NaN here is one everywhere)
+    }
+    cluster_sync_all();
+    float m_r[8], s_r[8], top = -INFINITY, total = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      m_r[r] = r < ctas ? ld_remote(&s_max, r) : -INFINITY;
+      s_r[r] = r < ctas ? ld_remote(&s_sum, r) : 0.0f;
+      top = fmaxf(top, m_r[r]);
+    }
+    const float at = top > -INFINITY ? top : 0.0f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) total += expf((m_r[r] - at) * inv_t) * s_r[r];
+    const float f = total == 0.0f ? 0.0f : expf((base - at) * inv_t) / total;  // (0: nothing but -inf)
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[k][e] *= f;
+  }
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA has read the others
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int i = item_at<VEC>(v0, k, tid);
+    if (VEC && i + 3 < v1) {
+      *reinterpret_cast<float4*>(y + i) = make_float4(x[k][0], x[k][1], x[k][2], x[k][3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (element<VEC>(i, e) < v1) y[element<VEC>(i, e)] = x[k][e];
+    }
+  }
+  cluster_wait();
+}
+
+// Longer rows: three passes.
 // grid (cluster, rows).  TEMP0: one at the first largest.
 template <class T>
 __global__ void __launch_bounds__(kDrThreads) lm_probabilities_kernel(const T* __restrict__ logits, long long ld, int vocab, float inv_t,
@@ -110,124 +250,225 @@ struct VerifyArgs {
 };
 __device__ __forceinline__ double mass_of(float p) { return p > 0.0f ? (double)p : 0.0; }
 
-// grid (cluster, sequences)
-__global__ void __launch_bounds__(kDrThreads) lm_verify_kernel(VerifyArgs a) {
-  __shared__ double s_rest[kDrWarps], s_all[kDrWarps], s_sum[2], s_scan[kDrWarps];
-  __shared__ int s_n, s_kind, s_found, s_last;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, ctas = gridDim.x, part = blockIdx.x, seq = blockIdx.y, k = a.drafts;
-  pdl_launch_dependents();
-  pdl_wait_prior();
+// First place of a sequence that is refused (.y 1) or has no drafted token (.y 0); one warp.
+__device__ __forceinline__ int2 first_refused(const VerifyArgs& a, int seq, int lane) {
   const float* target = a.target + seq * a.t_seq;
   const float* draft = a.draft + seq * a.d_seq;
   const int* tokens = a.tokens + seq * a.ld_tokens;
-  if (warp == 0) {  // first place that is refused (kind 1) or without a drafted token (kind 0)
-    int n = k, kind = 0;
-    for (int i0 = 0; i0 < k; i0 += 32) {
-      const int i = i0 + lane;
-      bool ends = false, refused = false;
-      if (i < k) {
-        const int x = tokens[i];
-        ends = x < 0 || x >= a.vocab;
-        if (!ends) {
-          const double p = mass_of(target[i * a.t_row + x]), q = mass_of(draft[i * a.d_row + x]);
-          refused = !((double)a.accept[seq * a.ld_accept + i] * q < p);
-        }
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, ends || refused);
-      if (hit) {
-        const int who = __ffs(hit) - 1;
-        n = i0 + who;
-        kind = __shfl_sync(0xffffffffu, (int)refused, who);
-        break;
-      }
+  for (int i0 = 0; i0 < a.drafts; i0 += 32) {
+    const int i = i0 + lane;
+    bool ends = false, refused = false;
+    if (i < a.drafts) {
+      const float u = a.accept[seq * a.ld_accept + i];
+      const int x = tokens[i];
+      ends = x < 0 || x >= a.vocab;
+      if (!ends) refused = !((double)u * mass_of(draft[i * a.d_row + x]) < mass_of(target[i * a.t_row + x]));
     }
-    if (lane == 0) s_n = n, s_kind = kind;
+    const unsigned hit = __ballot_sync(0xffffffffu, ends || refused);
+    if (hit) {
+      const int who = __ffs(hit) - 1;
+      return make_int2(i0 + who, __shfl_sync(0xffffffffu, (int)refused, who));
+    }
   }
+  return make_int2(a.drafts, 0);
+}
+
+// grid (cluster, sequences): one pass over the row (or the two rows) of the first refused place leaves a sum in 64 bits per 128
+// numbers in shared memory; these settle on which CTA and which 128 numbers the draw falls, and one warp reads those again.
+// What bounds it: latency for a few sequences (tokens, their probabilities, the rows, one after the other), memory for many.
+// 64 sequences of 151936 tokens: 66 us where every thread read consecutive numbers, twice.
+template <bool VEC>
+__global__ void __launch_bounds__(kRowThreads, 2) lm_verify_kernel(VerifyArgs a, int per) {
+  extern __shared__ double s_part[];  // in the order of the row
+  __shared__ double s_sum, s_before;
+  __shared__ int s_which, s_place[2];
+  constexpr int kItem = kRowThreads * 4, kSums = VEC ? kRowWarps : 4 * kRowWarps;  // numbers and sums of a turn
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, ctas = gridDim.x, part = blockIdx.x, seq = blockIdx.y, k = a.drafts;
+  pdl_launch_dependents();
+  pdl_wait_prior();
+  if (warp == 0) {
+    const int2 f = first_refused(a, seq, lane);
+    if (lane == 0) s_place[0] = f.x, s_place[1] = f.y;
+  }
+  const double pick = mass_of(a.pick[seq]);
   __syncthreads();
-  const int n = s_n;
-  const bool refused = s_kind;
-  const float* p = target + n * a.t_row;
-  const float* q = draft + (refused ? n * a.d_row : 0);
-  const int per = ((a.vocab + ctas - 1) / ctas + 3) / 4 * 4, v0 = min(part * per, a.vocab), v1 = min(v0 + per, a.vocab);
-  // a thread's share: consecutive numbers
-  const int each = (v1 - v0 + kDrThreads - 1) / kDrThreads, t0 = min(v0 + tid * each, v1), t1 = min(t0 + each, v1);
-  double rest = 0.0, all = 0.0;
-  for (int i = t0; i < t1; ++i) {
-    const double x = mass_of(p[i]);
-    all += x;
-    if (refused) rest += fmax(x - mass_of(q[i]), 0.0);
-  }
+  const int n = s_place[0];
+  bool rest = s_place[1];
+  const float* p = a.target + seq * a.t_seq + n * a.t_row;
+  const float* q = a.draft + seq * a.d_seq + (rest ? n * a.d_row : 0);
+  const int v0 = min(part * per, a.vocab), v1 = min(v0 + per, a.vocab), turns = (v1 - v0 + kItem - 1) / kItem, n_sums = turns * kSums;
   auto warp_sum = [](double v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
   };
-  const double wr = warp_sum(rest), wa = warp_sum(all);
-  if (lane == 0) s_rest[warp] = wr, s_all[warp] = wa;
-  __syncthreads();
-  if (tid == 0) {
-    double r = 0.0, l = 0.0;
-    for (int w = 0; w < kDrWarps; ++w) r += s_rest[w], l += s_all[w];
-    s_sum[0] = r, s_sum[1] = l;
-    s_found = 0x7fffffff, s_last = -1;
-  }
-  cluster_sync_all();
-  double total_rest = 0.0, total_all = 0.0, before[2] = {0.0, 0.0};
-  for (int r = 0; r < ctas; ++r) {
-    const double x = ld_remote(&s_sum[0], r), y = ld_remote(&s_sum[1], r);
-    if (r < part) before[0] += x, before[1] += y;
-    total_rest += x, total_all += y;
-  }
-  const bool from_rest = refused && total_rest > 0.0;
-  const double total = from_rest ? total_rest : total_all, goal = mass_of(a.pick[seq]) * total;
-  // running sums of the threads
-  double up = from_rest ? rest : all;
-  const double own = up;
+  auto mass = [&](float x, float y) { return rest ? fmax(mass_of(x) - mass_of(y), 0.0) : mass_of(x); };
+  double total = 0.0, before = 0.0, own = 0.0;
+  while (true) {
+    constexpr int kAhead = 4;  // turns requested together
+    for (int t0 = 0; t0 < turns; t0 += kAhead) {
+      float x[kAhead][4], y[kAhead][4] = {};
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const double v = __shfl_up_sync(0xffffffffu, up, o);
-    if (lane >= o) up += v;
-  }
-  if (lane == 31) s_scan[warp] = up;
-  __syncthreads();
-  double run = before[from_rest ? 0 : 1] + (up - own);
-  for (int w = 0; w < warp; ++w) run += s_scan[w];
-  int found = 0x7fffffff, last = -1;
-  for (int i = t0; i < t1; ++i) {
-    double x = mass_of(p[i]);
-    if (from_rest) x = fmax(x - mass_of(q[i]), 0.0);
-    run += x;
-    if (x > 0.0) last = i;
-    if (x > 0.0 && run > goal && i < found) found = i;
-  }
-  if (found != 0x7fffffff) atomicMin(&s_found, found);
-  if (last >= 0) atomicMax(&s_last, last);
-  cluster_sync_all();
-  if (part == 0 && tid == 0) {
-    for (int r = 0; r < ctas; ++r) {
-      found = min(found, ld_remote(&s_found, r));
-      last = max(last, ld_remote(&s_last, r));
+      for (int u = 0; u < kAhead; ++u) {
+        load4<VEC>(p, item_at<VEC>(v0, t0 + u, tid), v1, 0.0f, x[u]);
+        if (rest) load4<VEC>(q, item_at<VEC>(v0, t0 + u, tid), v1, 0.0f, y[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (t0 + u >= turns) break;
+        if constexpr (VEC) {
+          const double v = warp_sum((mass(x[u][0], y[u][0]) + mass(x[u][1], y[u][1])) + (mass(x[u][2], y[u][2]) + mass(x[u][3], y[u][3])));
+          if (lane == 0) s_part[(t0 + u) * kSums + warp] = v;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const double v = warp_sum(mass(x[u][e], y[u][e]));
+            if (lane == 0) s_part[(t0 + u) * kSums + e * kRowWarps + warp] = v;
+          }
+        }
+      }
     }
-    int* out = a.out + seq * a.ld_out;
-    for (int i = 0; i <= k; ++i) out[i] = i < n ? tokens[i] : i == n ? (found != 0x7fffffff ? found : last) : -1;
-    a.accepted[seq] = n;
+    __syncthreads();
+    if (warp == 0) {
+      double v = 0.0;
+      for (int i = lane; i < n_sums; i += 32) v += s_part[i];
+      v = warp_sum(v);
+      if (lane == 0) s_sum = v;
+    }
+    cluster_sync_all();
+    total = before = 0.0;
+    for (int r = 0; r < ctas; ++r) {
+      const double v = ld_remote(&s_sum, r);
+      if (r == part) before = total, own = v;
+      total += v;
+    }
+    if (total > 0.0 || !rest) break;
+    rest = false;  // refused, and nothing is left of the target's numbers: from the target
+    cluster_sync_all();
   }
-  cluster_sync_all();
+  const double goal = fmin(pick * total, total);
+  // the CTA that the draw falls on (pick of 1 and beyond: the last that has mass)
+  bool mine = own > 0.0 && before <= goal && goal < before + own;
+  if (total > 0.0 && goal >= total) {
+    int last = -1;
+    for (int r = 0; r < ctas; ++r)
+      if (ld_remote(&s_sum, r) > 0.0) last = r;
+    mine = last == part;
+  }
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA has read the others
+  int* out = a.out + seq * a.ld_out;
+  if (part == 0) {
+    const int* tokens = a.tokens + seq * a.ld_tokens;
+    for (int i = tid; i <= k; i += kRowThreads)
+      if (i != n || !(total > 0.0)) out[i] = i < n ? tokens[i] : -1;
+    if (tid == 0) a.accepted[seq] = n;
+  }
+  if (mine) {  // (the same for all threads)
+    if (warp == 0) {  // which of the sums: running sums of 32 at a time
+      int which = -1, last = -1;
+      double run = before, at_which = before, at_last = before;
+      for (int i0 = 0; i0 < n_sums && which < 0; i0 += 32) {
+        const double v = i0 + lane < n_sums ? s_part[i0 + lane] : 0.0;
+        double up = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double t = __shfl_up_sync(0xffffffffu, up, o);
+          if (lane >= o) up += t;
+        }
+        const unsigned some = __ballot_sync(0xffffffffu, v > 0.0), over = __ballot_sync(0xffffffffu, v > 0.0 && run + up > goal);
+        if (some) {
+          last = i0 + 31 - __clz(some);
+          at_last = run + __shfl_sync(0xffffffffu, up - v, 31 - __clz(some));
+        }
+        if (over) {
+          which = i0 + __ffs(over) - 1;
+          at_which = run + __shfl_sync(0xffffffffu, up - v, __ffs(over) - 1);
+        }
+        run += __shfl_sync(0xffffffffu, up, 31);
+      }
+      if (lane == 0) s_which = which < 0 ? last : which, s_before = which < 0 ? at_last : at_which;
+    }
+    __syncthreads();
+    const int which = s_which;
+    if (which % kRowWarps == warp) {
+      const int i = item_at<VEC>(v0, which / kSums, tid), only = which / kRowWarps % 4;
+      float x[4], y[4] = {};
+      load4<VEC>(p, i, v1, 0.0f, x);
+      if (rest) load4<VEC>(q, i, v1, 0.0f, y);
+      double m[4], up = 0.0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        m[e] = VEC || e == only ? mass(x[e], y[e]) : 0.0;
+        up += m[e];
+      }
+      const double whole = up;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double t = __shfl_up_sync(0xffffffffu, up, o);
+        if (lane >= o) up += t;
+      }
+      double run = s_before + (up - whole);
+      int found = 0x7fffffff, last = -1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        run += m[e];
+        if (m[e] > 0.0) {
+          last = element<VEC>(i, e);
+          if (run > goal) found = min(found, last);
+        }
+      }
+      found = __reduce_min_sync(0xffffffffu, found);
+      last = __reduce_max_sync(0xffffffffu, last);
+      if (lane == 0) out[n] = found != 0x7fffffff ? found : last;
+    }
+  }
+  cluster_wait();
 }
 
-int cluster_for(int rows, int vocab) {
-  int c = 1;
-  while (c < 8 && rows * c < 2 * kSms && vocab / (2 * c) >= 1024) c *= 2;
-  return c;
+// Cluster and items per thread for rows held in registers: as few CTAs as hold the row, more while they do not fill the GPU.
+struct RowPlan {
+  int ctas, per, items;
+};
+RowPlan row_plan(int rows, int vocab) {
+  constexpr int item = kRowThreads * 4;
+  RowPlan p{1, 0, 0};
+  auto size = [&] { p.per = ((vocab + p.ctas - 1) / p.ctas + 3) / 4 * 4, p.items = (p.per + item - 1) / item; };
+  size();
+  while (p.ctas < 8 && (p.items > kRowItems || (p.items > 1 && (long long)rows * p.ctas * 2 <= 2 * kSms))) p.ctas *= 2, size();
+  return p;
+}
+// f(instance) for 1, 2, 4, 6, 8 or 10 items
+template <class F>
+cudaError_t with_items(int items, F f) {
+  if (items <= 1) return f(std::integral_constant<int, 1>());
+  if (items <= 2) return f(std::integral_constant<int, 2>());
+  if (items <= 4) return f(std::integral_constant<int, 4>());
+  if (items <= 6) return f(std::integral_constant<int, 6>());
+  if (items <= 8) return f(std::integral_constant<int, 8>());
+  return f(std::integral_constant<int, 10>());
+}
+bool on(const void* p, size_t bytes, long long stride = 0, long long stride2 = 0) {
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride % 4 == 0 && stride2 % 4 == 0;
 }
 
 template <class T>
 cudaError_t launch_probabilities(const void* logits, long long ld, int rows, int vocab, float t, float* out, long long ld_out, cudaStream_t s) {
-  const int c = cluster_for(rows, vocab);
+  const float inv_t = t > 0.0f ? std::fmin(1.0f / t, 3.402823466e+38f) : 0.0f;
+  const bool vec = on(logits, 4 * sizeof(T), ld) && on(out, 16, ld_out);
   for (int r0 = 0; r0 < rows; r0 += 65535) {
-    const int n = rows - r0 < 65535 ? rows - r0 : 65535;
-    const cudaError_t r = launch_pdl_cluster(lm_probabilities_kernel<T>, dim3(c, n), dim3(kDrThreads), dim3(c, 1, 1), 0, s,
-                                             static_cast<const T*>(logits) + r0 * ld, ld, vocab, t > 0.0f ? std::fmin(1.0f / t, 3.402823466e+38f) : 0.0f, t == 0.0f, out + r0 * ld_out, ld_out);
+    const int n = std::min(rows - r0, 65535);
+    const T* z = static_cast<const T*>(logits) + r0 * ld;
+    float* y = out + r0 * ld_out;
+    cudaError_t r;
+    if (vocab <= kRowMost) {
+      const RowPlan p = row_plan(n, vocab);
+      r = with_items(p.items, [&](auto items) {
+        auto go = [&](auto kernel) { return launch_pdl_cluster(kernel, dim3(p.ctas, n), dim3(kRowThreads), dim3(p.ctas, 1, 1), 0, s, z, ld, vocab, p.per, inv_t, t == 0.0f, y, ld_out); };
+        return vec ? go(lm_probability_rows_kernel<T, decltype(items)::value, true>) : go(lm_probability_rows_kernel<T, decltype(items)::value, false>);
+      });
+    } else {
+      r = launch_pdl_cluster(lm_probabilities_kernel<T>, dim3(8, n), dim3(kDrThreads), dim3(8, 1, 1), 0, s, z, ld, vocab, inv_t, t == 0.0f, y, ld_out);
+    }
     if (r != cudaSuccess) return r;
   }
   return cudaSuccess;
@@ -265,16 +506,27 @@ int mllmb200_lm_verify(const float* target, long long t_seq, long long t_row, co
                        int* accepted, int* out, long long ld_out, void* stream) {
   if (seqs < 0 || drafts < 0 || vocab < 1 || ld_out < drafts + 1 || t_seq < 0 || t_row < 0 || d_seq < 0 || d_row < 0 || ld_tokens < 0 || ld_accept < 0)
     return MLLMB200_INVALID_ARG;
+  if (vocab > 1 << 20) return MLLMB200_UNSUPPORTED;
   if (!seqs) return MLLMB200_OK;
   if (!target || !pick || !accepted || !out || (drafts && (!draft || !tokens || !accept))) return MLLMB200_INVALID_ARG;
   VerifyArgs a{target, draft, accept, pick, tokens, t_seq, t_row, d_seq, d_row, ld_tokens, ld_accept, ld_out, 0, drafts, vocab, accepted, out};
-  const int c = cluster_for(seqs, vocab);
+  const bool vec = on(target, 16, t_seq, t_row) && (!drafts || on(draft, 16, d_seq, d_row));
+  auto st = static_cast<cudaStream_t>(stream);
   for (int s0 = 0; s0 < seqs; s0 += 65535) {
     VerifyArgs b = a;
-    b.seqs = seqs - s0 < 65535 ? seqs - s0 : 65535;
+    b.seqs = std::min(seqs - s0, 65535);
     b.target += s0 * t_seq, b.pick += s0, b.accepted += s0, b.out += s0 * ld_out;
     if (drafts) b.draft += s0 * d_seq, b.tokens += s0 * ld_tokens, b.accept += s0 * ld_accept;
-    const cudaError_t r = launch_pdl_cluster(lm_verify_kernel, dim3(c, b.seqs), dim3(kDrThreads), dim3(c, 1, 1), 0, static_cast<cudaStream_t>(stream), b);
+    int ctas = 1, per;
+    size_t smem;
+    auto size = [&] {
+      per = ((vocab + ctas - 1) / ctas + 3) / 4 * 4;
+      smem = (size_t)((per + kRowThreads * 4 - 1) / (kRowThreads * 4)) * kRowWarps * (vec ? 1 : 4) * sizeof(double);
+    };
+    size();
+    while (ctas < 8 && (smem > 40 * 1024 || ((long long)b.seqs * ctas <= 2 * kSms && vocab > ctas * kRowThreads * 4))) ctas *= 2, size();
+    auto go = [&](auto kernel) { return launch_pdl_cluster(kernel, dim3(ctas, b.seqs), dim3(kRowThreads), dim3(ctas, 1, 1), smem, st, b, per); };
+    const cudaError_t r = vec ? go(lm_verify_kernel<true>) : go(lm_verify_kernel<false>);
     if (r != cudaSuccess) return MLLMB200_CUDA_ERROR;
   }
   return MLLMB200_OK;

@@ -4,7 +4,7 @@ against the target's probabilities from given random numbers.  Calls run on the 
 import torch
 
 from . import lm
-from .paged import _fail, _need, _on
+from .paged import _fail, _on, _refuse
 
 _DTYPES = {torch.float32: lm.F32, torch.bfloat16: lm.BF16, torch.float16: lm.F16}
 
@@ -12,15 +12,17 @@ _DTYPES = {torch.float32: lm.F32, torch.bfloat16: lm.BF16, torch.float16: lm.F16
 def probabilities(logits, temperature=1.0, out=None, stream=None):
     """Rows of logits [rows, vocab] (fp32, bf16 or fp16) to probabilities in fp32: exp((z - max z) / temperature) over their sum;
     temperature 0: 1 at the first largest.  -inf gives 0, a row of nothing else zeros; NaN or +inf make their row NaN."""
-    _need(logits.dim() == 2 and logits.stride(1) == 1 and logits.dtype in _DTYPES and logits.is_cuda, "probabilities: logits [rows, vocab] on the GPU, rows contiguous")
+    dtype = _DTYPES.get(logits.dtype)
+    if not (logits.dim() == 2 and logits.stride(1) == 1 and dtype is not None and logits.is_cuda):
+        _refuse("probabilities", (lambda: False, "logits [rows, vocab] in fp32, bf16 or fp16 on the GPU, rows contiguous"))
     rows, vocab = logits.shape
-    if out is not None:
-        _need(out.shape == logits.shape and out.dtype == torch.float32 and out.device == logits.device and out.stride(1) == 1, "probabilities: out like the logits, fp32")
+    if out is not None and not (out.shape == (rows, vocab) and out.dtype == torch.float32 and out.get_device() == logits.get_device() and out.stride(1) == 1):
+        _refuse("probabilities", (lambda: False, "out like the logits, in fp32"))
 
     def call(s):
-        o = out if out is not None else torch.empty((rows, vocab), dtype=torch.float32, device=logits.device)
-        return lm.lib().mllmb200_lm_probabilities(logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), rows, vocab, temperature, o.data_ptr(), max(o.stride(0), vocab), s), o
-    st, o = _on(logits.device, stream, call)
+        o = out if out is not None else logits.new_empty((rows, vocab), dtype=torch.float32)
+        return lm.lib().mllmb200_lm_probabilities(logits.data_ptr(), dtype, logits.stride(0), rows, vocab, temperature, o.data_ptr(), max(o.stride(0), vocab), s), o
+    st, o = _on(logits.get_device(), stream, call)
     if st:
         _fail("probabilities", st)
     return o
@@ -37,19 +39,24 @@ def verify(target, draft, tokens, accept, pick, stream=None):
 
     Returns accepted (int32 [sequences]) and the new tokens (int32 [sequences, drafts + 1]): the accepted ones, the next
     one, -1 behind it."""
-    _need(target.dim() == 3 and draft.dim() == 3 and target.dtype == draft.dtype == torch.float32, "verify: probabilities [sequences, places, vocab] in fp32")
+    if target.dim() != 3 or draft.dim() != 3 or tokens.dim() != 2 or accept.dim() != 2:
+        _refuse("verify", (lambda: False, "probabilities [sequences, places, vocab], tokens and random numbers [sequences, drafts]"))
     seqs, places, vocab = target.shape
-    k = places - 1
-    _need(k >= 0 and draft.shape == (seqs, k, vocab) and tokens.shape == (seqs, k) and accept.shape == (seqs, k) and pick.shape == (seqs,), "verify: one place more in the target's probabilities than drafts")
-    _need(tokens.dtype == torch.int32 and accept.dtype == pick.dtype == torch.float32, "verify: tokens in int32, random numbers in fp32")
-    _need(target.stride(2) == 1 and (not k or (draft.stride(2) == 1 and (k == 1 or (tokens.stride(1) == 1 and accept.stride(1) == 1)))) and (seqs < 2 or pick.stride(0) == 1), "verify: rows are contiguous")
-    device = target.device
-    _need(device.type == "cuda" and all(t.device == device for t in (draft, tokens, accept, pick)), "verify: tensors on one GPU")
+    k, device = places - 1, target.get_device()
+    t_seq, t_row, t_one = target.stride()
+    d_seq, d_row, d_one = draft.stride()
+    if not (k >= 0 and draft.shape == (seqs, k, vocab) and tokens.shape == (seqs, k) and accept.shape == (seqs, k) and pick.shape == (seqs,) and
+            target.dtype == draft.dtype == accept.dtype == pick.dtype == torch.float32 and tokens.dtype == torch.int32 and t_one == 1 and (k == 0 or d_one == 1) and
+            (k < 2 or (tokens.stride(1) == 1 and accept.stride(1) == 1)) and (seqs < 2 or pick.stride(0) == 1) and device >= 0 and
+            draft.get_device() == tokens.get_device() == accept.get_device() == pick.get_device() == device):
+        _refuse("verify", (lambda: k >= 0 and draft.shape == (seqs, k, vocab) and tokens.shape == accept.shape == (seqs, k) and pick.shape == (seqs,), "one place more in the target's probabilities than drafts"),
+                (lambda: target.dtype == draft.dtype == accept.dtype == pick.dtype == torch.float32 and tokens.dtype == torch.int32, "tokens in int32, all else in fp32"),
+                (lambda: device >= 0 and all(t.get_device() == device for t in (draft, tokens, accept, pick)), "tensors on one GPU"), (lambda: False, "rows are contiguous"))
 
     def call(s):
-        accepted, out = torch.empty(seqs, dtype=torch.int32, device=device), torch.empty((seqs, places), dtype=torch.int32, device=device)
-        st = lm.lib().mllmb200_lm_verify(target.data_ptr(), target.stride(0), target.stride(1), draft.data_ptr(), draft.stride(0), draft.stride(1), tokens.data_ptr(),
-                                         tokens.stride(0), accept.data_ptr(), accept.stride(0), pick.data_ptr(), seqs, k, vocab, accepted.data_ptr(), out.data_ptr(), places, s)
+        accepted, out = tokens.new_empty((seqs,)), tokens.new_empty((seqs, places))
+        st = lm.lib().mllmb200_lm_verify(target.data_ptr(), t_seq, t_row, draft.data_ptr(), d_seq, d_row, tokens.data_ptr(), tokens.stride(0), accept.data_ptr(), accept.stride(0),
+                                         pick.data_ptr(), seqs, k, vocab, accepted.data_ptr(), out.data_ptr(), places, s)
         return st, (accepted, out)
     st, o = _on(device, stream, call)
     if st:

@@ -21,96 +21,111 @@ from .binding import scratch
 _PAGES = struct.Struct("@PP6q3P10i")
 _LOOK = struct.Struct("@PP4qPP4if4x")
 _DTYPES = {torch.bfloat16: lm.BF16, torch.float16: lm.F16}
-_sizes = {}
+_INT, _F32 = torch.int32, torch.float32
+_sizes = {}  # bytes of workspace by sizes
 
 
 def _fail(where, status):
     raise lm.EngineError(status, where, lm.STATUS.get(status))
 
 
-def _on(device, stream, call):
+def _refuse(where, *checks):
+    """The first check that does not hold, as an error."""
+    for ok, what in checks:
+        if not ok():
+            raise ValueError(f"{where}: {what}")
+    raise ValueError(f"{where}: arguments")
+
+
+try:  # the current device and its stream without the Python objects around them (4 us of a call that takes 10)
+    _device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+except AttributeError:  # (names that torch does not promise)
+    _device, _raw_stream = torch.cuda.current_device, lambda index: torch.cuda.current_stream(index).cuda_stream
+
+
+def _on(index, stream, call):
     """call(raw stream) with the tensors' device as the current one."""
-    if stream is not None:
-        with torch.cuda.stream(stream):
-            return call(stream.cuda_stream)
-    if device.index == torch.cuda.current_device():
-        return call(torch.cuda.current_stream().cuda_stream)
-    with torch.cuda.device(device):
-        return call(torch.cuda.current_stream().cuda_stream)
+    if stream is None and index == _device():
+        return call(_raw_stream(index))
+    with torch.cuda.device(index) if stream is None else torch.cuda.stream(stream):
+        return call(_raw_stream(index) if stream is None else stream.cuda_stream)
 
 
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
-
-
-def _pages(k, v, table, lengths, q_start, rows, where):
-    kd, ks, vs = k.shape, k.stride(), v.stride()
-    _need(len(kd) == 4 and v.dim() == 4 and kd[:3] == v.shape[:3], f"{where}: keys and values are [pages, kv_heads, page, size]")
-    dtype = _DTYPES.get(k.dtype)
-    _need(dtype is not None and v.dtype == k.dtype, f"{where}: keys and values in bf16 or fp16")
-    _need(ks[3] == 1 and vs[3] == 1, f"{where}: rows of keys and values are contiguous")
-    _need(table.dtype == lengths.dtype == torch.int32 and table.dim() == 2 and lengths.dim() == 1, f"{where}: table [sequences, pages] and lengths [sequences] in int32")
+def _pages(where, k, v, table, lengths, q_start, rows):
+    dtype, device = _DTYPES.get(k.dtype), k.get_device()
+    if k.dim() != 4 or v.dim() != 4 or table.dim() != 2 or lengths.dim() != 1:
+        _refuse(where, (lambda: k.dim() == v.dim() == 4, "keys and values are [pages, kv_heads, page, size]"), (lambda: False, "table is [sequences, pages], lengths [sequences]"))
+    pages, heads, page, dim = k.shape
     seqs, width = table.shape
-    _need(lengths.shape[0] == seqs and lengths.stride(0) == 1 and (width < 2 or table.stride(1) == 1), f"{where}: a length and a contiguous row of the table per sequence")
-    start = 0
-    if q_start is not None:
-        _need(q_start.dtype == torch.int32 and q_start.dim() == 1 and q_start.shape[0] == seqs + 1 and q_start.is_contiguous(), f"{where}: q_start [sequences + 1] in int32")
-        start = q_start.data_ptr()
-    device = k.device
-    _need(device.type == "cuda" and all(t is None or t.device == device for t in (v, table, lengths, q_start)), f"{where}: tensors on one GPU")
-    return _PAGES.pack(k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], table.data_ptr(), lengths.data_ptr(), start, dtype, kd[0], kd[2],
-                       kd[1], kd[3], v.shape[3], table.stride(0), width, seqs, rows)
+    k_page, k_head, k_row, k_one = k.stride()
+    v_page, v_head, v_row, v_one = v.stride()
+    vs = v.shape
+    if not (dtype is not None and v.dtype == k.dtype and vs[0] == pages and vs[1] == heads and vs[2] == page and k_one == 1 and v_one == 1 and
+            table.dtype == _INT and lengths.dtype == _INT and lengths.shape[0] == seqs and (seqs < 2 or lengths.stride(0) == 1) and (width < 2 or table.stride(1) == 1) and
+            device >= 0 and v.get_device() == device and table.get_device() == device and lengths.get_device() == device and
+            (q_start is None or (q_start.dtype == _INT and q_start.dim() == 1 and q_start.shape[0] == seqs + 1 and q_start.stride(0) == 1 and q_start.get_device() == device))):
+        _refuse(where, (lambda: dtype is not None and v.dtype == k.dtype, "keys and values in bf16 or fp16"), (lambda: vs[:3] == k.shape[:3], "keys and values of the same pages"),
+                (lambda: k_one == v_one == 1, "rows of keys and values are contiguous"), (lambda: table.dtype == lengths.dtype == _INT, "table and lengths in int32"),
+                (lambda: lengths.shape[0] == seqs and (seqs < 2 or lengths.stride(0) == 1) and (width < 2 or table.stride(1) == 1), "a length and a contiguous row of the table per sequence"),
+                (lambda: q_start is None or (q_start.dtype == _INT and q_start.shape == (seqs + 1,) and q_start.is_contiguous()), "q_start [sequences + 1] in int32"),
+                (lambda: False, "tensors on one GPU"))
+    return _PAGES.pack(k.data_ptr(), v.data_ptr(), k_page, k_head, k_row, v_page, v_head, v_row, table.data_ptr(), lengths.data_ptr(), 0 if q_start is None else q_start.data_ptr(),
+                       dtype, pages, page, heads, dim, vs[3], table.stride(0), width, seqs, rows)
 
 
 def append(k_pages, v_pages, k, v, table, lengths, q_start=None, stream=None):
     """Rows of new keys [rows, kv_heads, dim] and values [rows, kv_heads, vdim] into their pages.  Sequence s brings the rows
     q_start[s] .. q_start[s + 1] - 1 (without q_start: as many as every other); rows behind the last sequence are not stored."""
-    _need(k.dim() == 3 and v.dim() == 3 and k.dtype == v.dtype == k_pages.dtype and k.device == v.device == k_pages.device, "append: new keys and values [rows, kv_heads, size] of the cache's type")
-    _need(k.shape[:2] == v.shape[:2] and (k.shape[1], k.shape[2]) == (k_pages.shape[1], k_pages.shape[3]) and v.shape[2] == v_pages.shape[3], "append: sizes of keys and values")
-    _need(k.stride(2) == 1 and v.stride(2) == 1, "append: rows of keys and values are contiguous")
-    pages = _pages(k_pages, v_pages, table, lengths, q_start, k.shape[0], "append")
-
-    def call(s):
-        return lm.lib().mllmb200_lm_pages_append(pages, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), s)
-    st = _on(k.device, stream, call)
+    if not (k.dim() == 3 and v.dim() == 3 and k_pages.dim() == 4 and v_pages.dim() == 4 and k.dtype == v.dtype == k_pages.dtype and k.get_device() == v.get_device() == k_pages.get_device() and
+            k.shape[0] == v.shape[0] and k.shape[1] == v.shape[1] == k_pages.shape[1] and k.shape[2] == k_pages.shape[3] and v.shape[2] == v_pages.shape[3] and k.stride(2) == 1 and v.stride(2) == 1):
+        _refuse("append", (lambda: k.dim() == v.dim() == 3 and k.dtype == v.dtype == k_pages.dtype and k.device == v.device == k_pages.device, "new keys and values [rows, kv_heads, size] of the cache's type"),
+                (lambda: k.stride(2) == v.stride(2) == 1, "rows of keys and values are contiguous"), (lambda: False, "sizes of keys and values"))
+    pages = _pages("append", k_pages, v_pages, table, lengths, q_start, k.shape[0])
+    st = _on(k.get_device(), stream, lambda s: lm.lib().mllmb200_lm_pages_append(pages, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), s))
     if st:
         _fail("append", st)
 
 
 def _attention(where, q, k_pages, v_pages, table, lengths, q_start, scale, window, keep, sink, bias, out, stream):
-    _need(q.dim() == 3 and q.dtype == k_pages.dtype and q.device == k_pages.device and q.stride(2) == 1, f"{where}: queries [rows, heads, dim] of the cache's type, rows contiguous")
+    if q.dim() != 3:
+        _refuse(where, (lambda: False, "queries [rows, heads, dim]"))
     rows, heads, dim = q.shape
-    _need(dim == k_pages.shape[3], f"{where}: size of queries and keys")
-    pages = _pages(k_pages, v_pages, table, lengths, q_start, rows, where)
-    vdim, bias_max = v_pages.shape[3], 0
-    if sink is not None:
-        _need(sink.dtype == torch.float32 and sink.shape == (heads,) and sink.is_contiguous() and sink.device == q.device, f"{where}: sink [heads] in fp32")
-    if bias is not None:
-        _need(bias.dtype == torch.float32 and bias.dim() == 2 and bias.shape[0] == heads and bias.shape[1] > 0 and bias.is_contiguous() and bias.device == q.device, f"{where}: bias [heads, distances] in fp32")
-        bias_max = bias.shape[1] - 1
-    if out is not None:
-        _need(out.shape == (rows, heads, vdim) and out.dtype == q.dtype and out.device == q.device and out.stride(2) == 1, f"{where}: out [rows, heads, vdim] of the queries' type")
+    q_row, q_head, q_one = q.stride()
+    index = q.get_device()
+    pages = _pages(where, k_pages, v_pages, table, lengths, q_start, rows)
+    kv_heads, vdim = k_pages.shape[1], v_pages.shape[3]
+    if not (q.dtype == k_pages.dtype and index == k_pages.get_device() and q_one == 1 and dim == k_pages.shape[3] and
+            (sink is None or (sink.dtype == _F32 and sink.shape == (heads,) and sink.is_contiguous() and sink.get_device() == index)) and
+            (bias is None or (bias.dtype == _F32 and bias.dim() == 2 and bias.shape[0] == heads and bias.shape[1] > 0 and bias.is_contiguous() and bias.get_device() == index)) and
+            (out is None or (out.shape == (rows, heads, vdim) and out.dtype == q.dtype and out.get_device() == index and out.stride(2) == 1))):
+        _refuse(where, (lambda: q.dtype == k_pages.dtype and index == k_pages.get_device() and q_one == 1, "queries of the cache's type and device, rows contiguous"),
+                (lambda: dim == k_pages.shape[3], "size of queries and keys"), (lambda: sink is None or (sink.dtype == _F32 and sink.shape == (heads,) and sink.is_contiguous() and sink.get_device() == index), "sink [heads] in fp32"),
+                (lambda: bias is None or (bias.dtype == _F32 and bias.dim() == 2 and bias.shape[0] == heads and bias.shape[1] > 0 and bias.is_contiguous() and bias.get_device() == index), "bias [heads, distances] in fp32"),
+                (lambda: False, "out [rows, heads, vdim] of the queries' type, rows contiguous"))
     L = lm.lib()
-    run, size = (L.mllmb200_lm_attn_decode, L.mllmb200_lm_attn_decode_workspace) if q_start is None else (L.mllmb200_lm_attn_prompt, L.mllmb200_lm_attn_prompt_workspace)
+    decode = q_start is None
+    key = (decode, rows, heads, kv_heads, dim, vdim, table.shape)
 
     def call(s):
-        o = out if out is not None else torch.empty((rows, heads, vdim), dtype=q.dtype, device=q.device)
-        look = _LOOK.pack(q.data_ptr(), o.data_ptr(), q.stride(0), q.stride(1), o.stride(0), o.stride(1), 0 if sink is None else sink.data_ptr(),
-                          0 if bias is None else bias.data_ptr(), heads, bias_max, window, keep, dim ** -0.5 if scale is None else scale)
-        key = (q_start is None, rows, heads, k_pages.shape[1], dim, vdim, table.shape)
+        o = out if out is not None else q.new_empty((rows, heads, vdim))
+        o_row, o_head, _ = o.stride()
+        look = _LOOK.pack(q.data_ptr(), o.data_ptr(), q_row, q_head, o_row, o_head, 0 if sink is None else sink.data_ptr(), 0 if bias is None else bias.data_ptr(), heads,
+                          0 if bias is None else bias.shape[1] - 1, window, keep, dim ** -0.5 if scale is None else scale)
         need = _sizes.get(key)
         if need is None:  # (a function of the sizes)
             n = C.c_size_t()
-            st = size(pages, look, C.byref(n))
+            st = (L.mllmb200_lm_attn_decode_workspace if decode else L.mllmb200_lm_attn_prompt_workspace)(pages, look, C.byref(n))
             if st:
                 return st, o
             if len(_sizes) > 4096:
                 _sizes.clear()
             need = _sizes[key] = n.value
+        run = L.mllmb200_lm_attn_decode if decode else L.mllmb200_lm_attn_prompt
+        if not need:
+            return run(pages, look, None, s), o
         with scratch(need, s) as ws:
             return run(pages, look, ws, s), o
-    st, o = _on(q.device, stream, call)
+    st, o = _on(index, stream, call)
     if st:
         _fail(where, st)
     return o
@@ -129,7 +144,8 @@ def decode_attention(q, k_pages, v_pages, table, lengths, scale=None, window=0, 
 def prompt_attention(q, k_pages, v_pages, table, lengths, q_start, scale=None, window=0, keep=0, sink=None, bias=None, out=None, stream=None):
     """The same for any number of tokens per sequence: sequence s has the rows q_start[s] .. q_start[s + 1] - 1 of q.  Rows behind
     the last sequence are left as they are in `out`."""
-    _need(q_start is not None, "prompt_attention: q_start")
+    if q_start is None:
+        raise ValueError("prompt_attention: q_start")
     return _attention("prompt_attention", q, k_pages, v_pages, table, lengths, q_start, scale, window, keep, sink, bias, out, stream)
 
 
