@@ -50,26 +50,11 @@ __global__ void __launch_bounds__(128) lm_pages_append_kernel(Paged a, const voi
 }
 
 // ------------------------------------------------------------------------------------------ decode
-constexpr int kDecSeqs = 512;  // sequences of a launch
-constexpr int kDecCtas = kSms;
-
-// An item is (sequence, kv head, block of 16 MT rows); its keys are walked in blocks of 16 per warp.  The blocks of all
-// items, one after the other, are dealt out evenly: CTA c takes [c T / G, (c + 1) T / G).  An item that lies in one CTA is
-// finished there; of the others every CTA leaves the maximum, the sum and the unnormalized output of its share: in place 2 c + 1 where
-// the item begins in it, else in place 2 c.
-struct DecodeWork {
-  float* part_o;    // [2 G][16 MT][vdim]
-  float2* part_ml;  // [2 G][16 MT]
-  long long* base;  // [seqs + 1] blocks of a kv head and row block before every sequence
-  int row_blocks;
-};
-__device__ __forceinline__ int owner_of(long long b, long long total, int ctas) { return (int)(((b + 1) * ctas - 1) / total); }
-
 template <class T, int DV, int MT, int STAGES, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS, 1) lm_paged_decode_kernel(Paged a, DecodeWork w) {
   constexpr int kDecWarps = WARPS, kDecThreads = 32 * WARPS, kDecB = 16 * WARPS;
   extern __shared__ __align__(16) uint8_t pd_smem[];
-  __shared__ long long s_base[kDecSeqs + 1], s_warp[kDecWarps];
+  __shared__ long long s_base[kDecSeqs + 1];
   __shared__ float s_m[kDecWarps][16 * MT], s_l[kDecWarps][16 * MT];
   constexpr int kRows = 16 * MT;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -81,36 +66,14 @@ __global__ void __launch_bounds__(32 * WARPS, 1) lm_paged_decode_kernel(Paged a,
   T* mine = ring + (size_t)warp * STAGES * stage_elems;
   pdl_launch_dependents();
   pdl_wait_prior();
-  {  // blocks of every sequence, summed up
-    constexpr int kEach = kDecSeqs / kDecThreads;
-    long long sum[kEach], run = 0;
-    const int s0 = tid * kEach;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      if (s0 + i < a.seqs) {
-        const int len = paged_length(a, s0 + i);
-        run += paged_seen<kDecB>(a, len - a.tokens, len - 1).blocks;
-      }
-      sum[i] = run;
-    }
-    long long up = run;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, up, o);
-      if (lane >= o) up += v;
-    }
-    if (lane == 31) s_warp[warp] = up;
-    __syncthreads();
-    up -= run;
-    for (int i = 0; i < warp; ++i) up += s_warp[i];
-    if (tid == 0) s_base[0] = 0;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i)
-      if (s0 + i < a.seqs) s_base[s0 + i + 1] = up + sum[i];
-    __syncthreads();
-    if (blockIdx.x == 0)
-      for (int i = tid; i <= a.seqs; i += kDecThreads) w.base[i] = s_base[i];
+  if (w.redo) {  // again, and only if some CTA of the kernel before asks for it
+    bool asked = false;
+    for (int i = tid; i < kSms; i += kDecThreads) asked = asked || w.redo[i] != 0;
+    if (!__syncthreads_or(asked)) return;
   }
+  sum_blocks<kDecB, kDecThreads>(a, s_base);
+  if (blockIdx.x == 0)
+    for (int i = tid; i <= a.seqs; i += kDecThreads) w.base[i] = s_base[i];
   const int items = a.kv_heads * w.row_blocks, rows = a.group * a.tokens;  // per sequence; per kv head
   const long long total = s_base[a.seqs] * items;
   const int ctas = (int)min((long long)gridDim.x, total);  // (every one of them has something)
@@ -121,10 +84,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) lm_paged_decode_kernel(Paged a,
   const uint32_t q_addr = smem_u32(sQ + ((mat & 1) * 8 + ml) * ldk + (mat >> 1) * 8);
 
   while (b < end) {
-    int s = 0;
-    for (int step = kDecSeqs / 2; step; step /= 2)
-      if (s + step < a.seqs && s_base[s + step] * items <= b) s += step;
-    const int len = paged_length(a, s), p_first = len - a.tokens, p_last = len - 1;
+    const int s = sequence_of(a, s_base, items, b), len = paged_length(a, s), p_first = len - a.tokens, p_last = len - 1;
     const Seen seen = paged_seen<kDecB>(a, p_first, p_last);
     const long long in_seq = b - s_base[s] * items;
     const int item = (int)(in_seq / seen.blocks), blk0 = (int)(in_seq - (long long)item * seen.blocks);
@@ -281,6 +241,11 @@ __global__ void __launch_bounds__(128) lm_paged_join_kernel(Paged a, DecodeWork 
   __shared__ float s_f[kDecCtas], s_inv;
   pdl_launch_dependents();
   pdl_wait_prior();
+  if (w.redo) {
+    bool asked = false;
+    for (int i = threadIdx.x; i < kSms; i += 128) asked = asked || w.redo[i] != 0;
+    if (!__syncthreads_or(asked)) return;
+  }
   const int items = a.kv_heads * w.row_blocks, s = blockIdx.x / items, item = blockIdx.x - s * items;
   const int kvh = item / w.row_blocks, r = blockIdx.y, row = (item - kvh * w.row_blocks) * item_rows + r, tid = threadIdx.x;
   if (row >= a.group * a.tokens) return;
@@ -408,14 +373,15 @@ cudaError_t configure_decode() {
 
 // Layout of the decode workspace for `seqs` sequences of a launch.
 struct DecodeSpace {
-  size_t ml, base, bytes;
+  size_t ml, base, flags, bytes;
 };
 DecodeSpace decode_space(const Paged& a, int seqs) {
   DecodeSpace d;
-  const size_t rows = (size_t)2 * kDecCtas * dec_rows(a);
+  const size_t rows = (size_t)2 * kDecCtas * std::max(dec_rows(a), paged_decode_tc_takes(a) ? paged_decode_tc_rows(a) : 0);
   d.ml = up16(rows * a.vdim * 4);
   d.base = d.ml + up16(rows * sizeof(float2));
-  d.bytes = d.base + up16((size_t)(seqs + 1) * sizeof(long long));
+  d.flags = d.base + up16((size_t)(seqs + 1) * sizeof(long long));
+  d.bytes = d.flags + kSms * sizeof(int);
   return d;
 }
 
@@ -464,11 +430,14 @@ int check_decode(const mllmb200_lm_pages* p, const mllmb200_lm_look* l, Paged* a
 }
 
 template <class T>
+cudaError_t join_decode(const Paged& a, const DecodeWork& w, int item_rows, int shares, cudaStream_t s) {
+  return launch_pdl(lm_paged_join_kernel<T>, dim3(a.seqs * a.kv_heads * w.row_blocks, std::min(item_rows, a.group * a.tokens)), dim3(128), 0, s, a, w, item_rows,
+                    shares);
+}
+template <class T>
 cudaError_t launch_decode(Paged a, uint8_t* ws, cudaStream_t s) {
   const int all = a.seqs, item_rows = dec_rows(a);
   const DecodeSpace d = decode_space(a, std::min(all, kDecSeqs));
-  DecodeWork w{reinterpret_cast<float*>(ws), reinterpret_cast<float2*>(ws + d.ml), reinterpret_cast<long long*>(ws + d.base),
-               (a.group * a.tokens + item_rows - 1) / item_rows};
   const size_t smem = decode_smem(a);
   for (int s0 = 0; s0 < all; s0 += kDecSeqs) {
     Paged b = a;
@@ -477,10 +446,23 @@ cudaError_t launch_decode(Paged a, uint8_t* ws, cudaStream_t s) {
     b.table += (size_t)s0 * a.ld_table;
     if (b.q_start) b.q_start += s0, b.q_count += s0;
     else b.q = static_cast<const T*>(a.q) + (long long)s0 * a.tokens * a.q_row, b.out = static_cast<T*>(a.out) + (long long)s0 * a.tokens * a.out_row;
-    cudaError_t r = with_decode<T>(b, [&](auto f) { return launch_pdl(f, dim3(kDecCtas), dim3(32 * dec_warps(b)), smem, s, b, w); });
-    if (r != cudaSuccess) return r;
-    r = launch_pdl(lm_paged_join_kernel<T>, dim3(b.seqs * b.kv_heads * w.row_blocks, std::min(item_rows, b.group * b.tokens)), dim3(128), 0, s, b, w,
-                   item_rows, kDecCtas);
+    DecodeWork w{reinterpret_cast<float*>(ws), reinterpret_cast<float2*>(ws + d.ml), reinterpret_cast<long long*>(ws + d.base), 0, nullptr};
+    int* flags = reinterpret_cast<int*>(ws + d.flags);
+    cudaError_t r = cudaSuccess;
+    if (paged_decode_tc_takes(b)) {
+      const int tokens = paged_decode_tc_rows(b) / b.group;
+      w.row_blocks = (b.tokens + tokens - 1) / tokens;
+      if (launch_paged_decode_tc(b, std::is_same<T, __half>::value, w, flags, s, &r)) {
+        // (a table that names one block of keys: every item lies in one CTA)
+        if (r == cudaSuccess && b.max_pages * b.page > 128) r = join_decode<T>(b, w, tokens * b.group, kDecCtas, s);
+        if (r != cudaSuccess) return r;
+        if (b.tokens == 1) continue;  // (what one token sees, all of it sees)
+        w.redo = flags;
+      }
+    }
+    w.row_blocks = (a.group * a.tokens + item_rows - 1) / item_rows;
+    r = with_decode<T>(b, [&](auto f) { return launch_pdl(f, dim3(kSms), dim3(32 * dec_warps(b)), smem, s, b, w); });
+    if (r == cudaSuccess) r = join_decode<T>(b, w, item_rows, kSms, s);
     if (r != cudaSuccess) return r;
   }
   return cudaSuccess;

@@ -81,6 +81,60 @@ __device__ __forceinline__ bool seen_by_all(const Paged& a, int first, int last,
   return j1 <= first && (a.window == 0 || j0 > last - a.window || j1 < a.keep);
 }
 
+constexpr int kDecSeqs = 512;  // sequences of a launch
+constexpr int kDecCtas = 2 * kSms;  // shares of the work: CTAs, or streams of half as many
+
+// Attention of a few tokens per sequence.  An item is (sequence, kv head, block of rows); its keys are walked in blocks of B.  The blocks of all
+// items, one after the other, are dealt out evenly: share c is [c T / G, (c + 1) T / G).  An item that lies in one share is
+// finished there; of the others every share leaves the maximum, the sum and the unnormalized output of its share: in place 2 c + 1 where
+// the item begins in it, else in place 2 c.
+struct DecodeWork {
+  float* part_o;    // [2 G][rows of an item][vdim]
+  float2* part_ml;  // [2 G][rows of an item]
+  long long* base;  // [seqs + 1] blocks of a kv head and row block before every sequence
+  int row_blocks;
+  const int* redo;  // nullptr: always; else only if one of the CTAs' numbers is not 0
+};
+// (for all threads of a CTA) blocks of every sequence summed up, base[0 .. seqs]
+template <int B, int THREADS, class N>
+__device__ __forceinline__ void sum_blocks(const Paged& a, N* base) {
+  __shared__ N s_warp[THREADS / 32];
+  constexpr int kEach = (kDecSeqs + THREADS - 1) / THREADS;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, s0 = tid * kEach;
+  N sum[kEach], run = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    if (s0 + i < a.seqs) {
+      const int len = paged_length(a, s0 + i);
+      run += paged_seen<B>(a, len - a.tokens, len - 1).blocks;
+    }
+    sum[i] = run;
+  }
+  N up = run;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const N v = __shfl_up_sync(0xffffffffu, up, o);
+    if (lane >= o) up += v;
+  }
+  if (lane == 31) s_warp[warp] = up;
+  __syncthreads();
+  up -= run;
+  for (int i = 0; i < warp; ++i) up += s_warp[i];
+  if (tid == 0) base[0] = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    if (s0 + i < a.seqs) base[s0 + i + 1] = up + sum[i];
+  __syncthreads();
+}
+// the sequence that block b lies in
+__device__ __forceinline__ int sequence_of(const Paged& a, const long long* base, int items, long long b) {
+  int s = 0;
+  for (int step = kDecSeqs / 2; step; step /= 2)
+    if (s + step < a.seqs && base[s + step] * items <= b) s += step;
+  return s;
+}
+__device__ __forceinline__ int owner_of(long long b, long long total, int ctas) { return (int)(((b + 1) * ctas - 1) / total); }
+
 // Numbers of 16 bits on the tensor cores of a warp.
 template <class T>
 struct Num;
@@ -167,6 +221,11 @@ cudaError_t launch_paged_prep(cudaStream_t s, int n, const int2* row_sp, const i
 // out fp32 [rows][ld_out] (the checks are those of mllmb200_lm_probabilities)
 cudaError_t launch_probability_rows(const float* logits, long long ld, int rows, int vocab, float temperature, float* out, long long ld_out, cudaStream_t s);
 
+// The same on tcgen05, one block of rows per 128 / group tokens; false: not these sizes.  flags [CTAs]: 1 where values that only some
+// tokens see were not finite, and the call has to be done on mma.sync.
+bool paged_decode_tc_takes(const Paged& a);
+int paged_decode_tc_rows(const Paged& a);  // rows of an item
+bool launch_paged_decode_tc(const Paged& a, bool f16, const DecodeWork& w, int* flags, cudaStream_t s, cudaError_t* launched);
 bool launch_paged_prompt_tc(const Paged& a, bool f16, cudaStream_t s, cudaError_t* launched);
 
 }  // namespace lm

@@ -60,6 +60,73 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]
       : "memory");
 }
 
+// One row's scores of a block (128 columns of tensor memory in registers): bias and mask.  first, last: positions of the rows that
+// are worked on together.
+template <bool BIAS>
+__device__ __forceinline__ void weigh_block(const Paged& a, uint32_t (&v)[4][32], const float* bias, int pos, int first, int last, int j0) {
+  if (BIAS) {
+    const float far = bias ? bias[a.bias_max] * kPagedLog2e : 0.0f;
+    const bool near = first - (j0 + kTcKeys - 1) < a.bias_max;  // some distance has a bias of its own
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float b = near && bias ? __ldg(bias + max(0, min(pos - (j0 + c * 32 + i), a.bias_max))) * kPagedLog2e : far;
+        v[c][i] = __float_as_uint(fmaf(__uint_as_float(v[c][i]), a.scale2, b));
+      }
+  }
+  if (first < 0 || !seen_by_all(a, first, last, j0, j0 + kTcKeys - 1)) {
+    const int hi = pos - j0, lo = a.window ? hi - a.window : -1, kp = a.window ? a.keep - j0 : 0;  // column i: i <= hi and (i > lo or i < kp)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const int col = c * 32 + i;
+        if (!(col <= hi && (col > lo || col < kp))) v[c][i] = 0xff800000u;
+      }
+  }
+}
+__device__ __forceinline__ float row_top(const uint32_t (&v)[4][32]) {
+  float mx[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    mx[c] = __uint_as_float(v[c][0]);
+#pragma unroll
+    for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(v[c][i]));
+  }
+  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+}
+// O of the row times alpha, in tensor memory
+template <int D>
+__device__ __forceinline__ void rescale(uint32_t o_col, float alpha) {
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t o[32];
+    tmem_ld32(o_col + c * 32, o);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+    tmem_st32(o_col + c * 32, o);
+  }
+}
+// weights 2^(score scale + base) in 16 bits over the scores' columns; their sum
+template <class T>
+__device__ __forceinline__ float put_weights(const uint32_t (&v)[4][32], uint32_t s_col, float scale, float base) {
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float p0 = paged_exp2(fmaf(__uint_as_float(v[c][2 * i]), scale, base)), p1 = paged_exp2(fmaf(__uint_as_float(v[c][2 * i + 1]), scale, base));
+      sum[i & 3] += p0 + p1;
+      w[i] = Num<T>::pack(p0, p1);
+    }
+    tmem_st16(s_col + c * 16, w);
+  }
+  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
 struct TcBarriers {
   uint64_t q_full, k_full[4], k_free[4], v_full[4], v_free[4], v_fixed[4], s_full[2], p_ready[2], o_done[2];
 };
@@ -277,66 +344,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld32(s_col + c * 32, v[c]);
       tmem_ld_wait();
-      const int j0 = block_key<kTcKeys>(seen, j);
-      if (BIAS) {
-        const float far = bias ? bias[a.bias_max] * kPagedLog2e : 0.0f;
-        const bool near = first - (j0 + kTcKeys - 1) < a.bias_max;  // some distance has a bias of its own
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float b = near && bias ? __ldg(bias + max(0, min(pos - (j0 + c * 32 + i), a.bias_max))) * kPagedLog2e : far;
-            v[c][i] = __float_as_uint(fmaf(__uint_as_float(v[c][i]), a.scale2, b));
-          }
-      }
-      if (first < 0 || !seen_by_all(a, first, last, j0, j0 + kTcKeys - 1)) {
-        const int hi = pos - j0, lo = a.window ? hi - a.window : -1, kp = a.window ? a.keep - j0 : 0;  // column i: i <= hi and (i > lo or i < kp)
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int col = c * 32 + i;
-            if (!(col <= hi && (col > lo || col < kp))) v[c][i] = 0xff800000u;
-          }
-      }
-      float mx[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        mx[c] = __uint_as_float(v[c][0]);
-#pragma unroll
-        for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(v[c][i]));
-      }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      if (__any_sync(0xffffffffu, top > m + grown)) {
+      weigh_block<BIAS>(a, v, bias, pos, first, last, block_key<kTcKeys>(seen, j));
+      const float top = row_top(v);
+      if (__any_sync(0xffffffffu, live && top > m + grown)) {
         const float m_new = fmaxf(m, top), alpha = m_new == -INFINITY ? 1.0f : paged_exp2((m - m_new) * scale);
         m = m_new;
-        if (j > 0) {
+        if (j > 0) {  // (the products before S of this block are done)
           l *= alpha;
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {  // (the products before S of this block are done)
-            uint32_t o[32];
-            tmem_ld32(o_col + c * 32, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            tmem_st32(o_col + c * 32, o);
-          }
+          rescale<D>(o_col, alpha);
         }
       }
-      const float base = m == -INFINITY ? 0.0f : -m * scale;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t w[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p0 = paged_exp2(fmaf(__uint_as_float(v[c][2 * i]), scale, base)), p1 = paged_exp2(fmaf(__uint_as_float(v[c][2 * i + 1]), scale, base));
-          sum[i & 3] += p0 + p1;
-          w[i] = Num<T>::pack(p0, p1);
-        }
-        tmem_st16(s_col + c * 16, w);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      l += put_weights<T>(v, s_col, scale, m == -INFINITY ? 0.0f : -m * scale);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -386,6 +404,414 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
   }
 }
 
+// ------------------------------------------------------------------------------------------ a few tokens per sequence
+// The rows of an item (all heads of a kv head, of up to 64 / group tokens) fill the first lanes of a tile; what bounds the kernel is
+// the stream of keys and values (64 KB a block of 128 keys for heads of 128).  A CTA runs two streams, each with S, O and queries of
+// its own and an even share of all blocks (two of the kDecCtas shares), so that the products of one run beside the weights of the
+// other; copies run ahead over the ends of items.  The tensor pipe has time to spare, so the weights enter as two halves of 16
+// bits (2^-17 of a weight and better).  Loops over columns are short on purpose: a launch starts with a cold instruction cache.
+//   warps 0-3, 4-7  weights of stream 0 and 1, only those whose rows exist
+//   warp 8, 9, 10-11  copies, MMA issue, values that not every row sees: as above
+struct Share {  // a stream's part of an item
+  int seq, kvh, row0, ntok, blk0, n, p_first, p_last;
+  bool begins, whole;
+  Seen all;  // what the sequence's rows see: the blocks; the item's own rows are at p_first .. p_last
+};
+__device__ __forceinline__ Share share_at(const Paged& a, const int* base, int row_blocks, int tpi, int b, int end) {
+  Share g;
+  const int items = a.kv_heads * row_blocks;
+  int s = 0;
+  for (int step = kDecSeqs / 2; step; step /= 2)
+    if (s + step < a.seqs && base[s + step] * items <= b) s += step;
+  g.seq = s;
+  const int len = paged_length(a, s);
+  g.all = paged_seen<kTcKeys>(a, len - a.tokens, len - 1);
+  const int in_seq = b - base[s] * items, item = in_seq / g.all.blocks, rb = item % row_blocks;
+  g.blk0 = in_seq - item * g.all.blocks;
+  g.n = min(end - b, g.all.blocks - g.blk0);
+  g.kvh = item / row_blocks;
+  const int2 rows = paged_rows(a, s);
+  g.row0 = rows.x + rb * tpi;
+  g.ntok = min(min(tpi, a.tokens - rb * tpi), max(0, rows.y - rb * tpi));
+  g.p_first = len - a.tokens + rb * tpi;
+  g.p_last = g.p_first + g.ntok - 1;
+  g.begins = g.blk0 == 0;
+  g.whole = g.begins && g.n == g.all.blocks;
+  return g;
+}
+// Place in a ring of n: slot and the parity of its pass.
+struct Ring {
+  int slot = 0, count = 0;
+  uint32_t pass = 0;
+  __device__ __forceinline__ void next(int n) {
+    ++count;
+    if (++slot == n) slot = 0, pass ^= 1u;
+  }
+};
+struct DecBarriers {
+  uint64_t q_full[2][2], q_free[2][2], k_full[8], k_free[8], v_full[8], v_free[8], v_fixed[8], s_full[2], p_ready[2], o_done[2], o_free[2];
+};
+
+template <class T, int D, bool BIAS>
+__global__ void __launch_bounds__(kTcThreads, 1) lm_paged_decode_tc_kernel(const __grid_constant__ Paged a, const __grid_constant__ CUtensorMap qmap,
+                                                                           const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                                                                           DecodeWork w, int* flags, int piece, int tpi, int q_rows, int nk, int nv) {
+  using L = TcLayout<D>;
+  extern __shared__ uint8_t tc_smem_raw[];
+  __shared__ DecBarriers bars;
+  __shared__ int s_base[kDecSeqs + 1];
+  __shared__ uint32_t s_tmem;
+  __shared__ volatile int s_bad, s_gave_up;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  // queries, two of each stream [D / 64][q_rows][64] (the products read 128 rows: what lies behind makes rows that nobody reads), keys, values
+  const uint32_t smem0 = (smem_u32(tc_smem_raw) + 1023u) & ~1023u, q_bytes = (uint32_t)(D / 64 * q_rows * 128);
+  const uint32_t keys0 = smem0 + 4 * q_bytes, values0 = keys0 + (uint32_t)nk * L::kTile;
+  const int item_rows = tpi * a.group, row_warps = (item_rows + 31) / 32;
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      for (int k = 0; k < 2; ++k) mbar_init(&bars.q_full[i][k], 1), mbar_init(&bars.q_free[i][k], 1);
+      mbar_init(&bars.s_full[i], 1), mbar_init(&bars.o_done[i], 1), mbar_init(&bars.p_ready[i], row_warps), mbar_init(&bars.o_free[i], row_warps);
+    }
+    for (int i = 0; i < nk; ++i) mbar_init(&bars.k_full[i], 1), mbar_init(&bars.k_free[i], 1);
+    for (int i = 0; i < nv; ++i) mbar_init(&bars.v_full[i], 1), mbar_init(&bars.v_free[i], 1), mbar_init(&bars.v_fixed[i], 2);
+    s_bad = s_gave_up = 0;
+    mbar_fence_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(&s_tmem, 512);
+    tmem_relinquish();
+  }
+  pdl_launch_dependents();
+  pdl_wait_prior();
+  sum_blocks<kTcKeys, kTcThreads>(a, s_base);
+  if (blockIdx.x == 0)
+    for (int i = tid; i <= a.seqs; i += kTcThreads) w.base[i] = s_base[i];
+  for (int s = blockIdx.x; s < a.seqs; s += gridDim.x) {  // sequences without keys
+    if (s_base[s + 1] != s_base[s]) continue;
+    const int2 rows = paged_rows(a, s);
+    for (int i = tid; i < min(rows.y, a.tokens) * a.heads * (D / 8); i += kTcThreads) {
+      const int c = i % (D / 8), h = i / (D / 8) % a.heads, t = i / (D / 8) / a.heads;
+      *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (rows.x + t) * a.out_row + h * a.out_head + c * 8) = make_uint4(0, 0, 0, 0);
+    }
+  }
+  const int total = s_base[a.seqs] * a.kv_heads * w.row_blocks, shares = min(kDecCtas, total);  // (every one of them has something)
+  int start[2], end[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int c = t * kSms + blockIdx.x;
+    start[t] = c < shares ? (int)((long long)total * c / shares) : 0;
+    end[t] = c < shares ? (int)((long long)total * (c + 1) / shares) : 0;
+  }
+  const int rounds = max(end[0] - start[0], end[1] - start[1]);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (s_gave_up) return false;
+    if (mbar_wait_bounded(bar, parity)) return true;
+    s_gave_up = 1;
+    return false;
+  };
+  auto all_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+  struct Place {  // of a role in a stream's list of blocks
+    int b, end, i, sg;
+    Share g;
+  };
+  auto enter = [&](Place& p) {  // before block p.b: its share
+    if (p.i == 0) p.g = share_at(a, s_base, w.row_blocks, tpi, p.b, p.end);
+  };
+  auto leave = [&](Place& p) {
+    ++p.b;
+    if (++p.i == p.g.n) p.i = 0, ++p.sg;
+  };
+  Place place[2] = {{start[0], end[0], 0, 0, {}}, {start[1], end[1], 0, 0, {}}};
+
+  if (warp == 8) {
+    // ------------------------------------------------------------ copies: the streams' blocks in turn
+    const int pieces = kTcKeys / piece;
+    bool ok = true;
+    Ring kr, vr;
+    for (int r = 0; r < rounds && ok; ++r)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        Place& p = place[t];
+        if (p.b >= p.end || !ok) continue;
+        enter(p);
+        if (p.i == 0) {
+          uint64_t* full = &bars.q_full[t][p.sg & 1];
+          if (p.sg >= 2) ok = all_wait(&bars.q_free[t][p.sg & 1], (uint32_t)((p.sg >> 1) - 1) & 1u);
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(full, (uint32_t)(item_rows * D * 2));
+            for (int c = 0; c < D / 64; ++c)
+              tma_load_3d(smem0 + (2 * t + (p.sg & 1)) * q_bytes + c * q_rows * 128, &qmap, c * 64, p.g.kvh * a.group, p.g.row0, full);
+          }
+          __syncwarp();
+        }
+        // lane i: page of piece i, a.pages (zeros) where nothing of it is seen
+        const int key = block_key<kTcKeys>(p.g.all, p.g.blk0 + p.i) + lane * piece, place_in = key / a.page, inside = key - place_in * a.page;
+        int page = a.pages;
+        if (lane < pieces && key <= p.g.all.last && (key + piece > p.g.all.lo || key < p.g.all.head)) {
+          const int q = paged_page(a, p.g.seq, place_in);
+          if (q >= 0) page = q;
+        }
+        auto copy = [&](const CUtensorMap* map, uint32_t block, uint64_t* full) {
+          if (lane == 0) mbar_arrive_expect_tx(full, L::kTile);
+          __syncwarp();
+          if (lane < pieces) {
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) tma_load_4d(block + lane * piece * 128 + c * 16384, map, c * 64, inside, p.g.kvh, page, full);
+          }
+          __syncwarp();
+        };
+        if (kr.count >= nk) ok = all_wait(&bars.k_free[kr.slot], kr.pass ^ 1u);
+        if (!ok) break;
+        copy(&kmap, keys0 + kr.slot * L::kTile, &bars.k_full[kr.slot]);
+        kr.next(nk);
+        if (vr.count >= nv) ok = all_wait(&bars.v_free[vr.slot], vr.pass ^ 1u);
+        if (!ok) break;
+        copy(&vmap, values0 + vr.slot * L::kTile, &bars.v_full[vr.slot]);
+        vr.next(nv);
+        leave(p);
+      }
+    if (!ok) {  // nothing in flight when the CTA leaves
+      for (int i = max(0, kr.count - nk); i < kr.count; ++i) mbar_wait_bounded(&bars.k_full[i % nk], (uint32_t)(i / nk) & 1u);
+      for (int i = max(0, vr.count - nv); i < vr.count; ++i) mbar_wait_bounded(&bars.v_full[i % nv], (uint32_t)(i / nv) & 1u);
+      for (int t = 0; t < 2; ++t)
+        for (int i = max(0, place[t].sg - 1); i <= place[t].sg; ++i) mbar_wait_bounded(&bars.q_full[t][i & 1], (uint32_t)(i >> 1) & 1u);
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ MMA issue: scores of a stream's next block behind its values
+    const bool issuer = elect_one_sync();
+    const uint32_t idesc_s = tc_idesc<T>(kTcKeys, false), idesc_o = tc_idesc<T>(D, true);
+    bool ok = true;
+    Place next[2] = {place[0], place[1]};  // of the scores
+    Ring kr, vr;
+    auto scores = [&](int t) {
+      Place& p = next[t];
+      if (p.b >= p.end || !ok) return;
+      enter(p);
+      if (p.i == 0) ok = all_wait(&bars.q_full[t][p.sg & 1], (uint32_t)(p.sg >> 1) & 1u);
+      ok = ok && all_wait(&bars.k_full[kr.slot], kr.pass);
+      if (!ok) return;
+      tc_fence_after();
+      if (issuer) {
+        const uint64_t q = tc_desc(smem0 + (2 * t + (p.sg & 1)) * q_bytes, 16), k = tc_desc(keys0 + kr.slot * L::kTile, 16);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks)
+          tc_mma_f16(tmem + t * 128, q + (uint64_t)((ks / 4) * q_rows * 8 + (ks % 4) * 2), k + (uint64_t)((ks / 4) * 1024 + (ks % 4) * 2), idesc_s, ks > 0);
+        tc_commit(&bars.s_full[t]);
+        tc_commit(&bars.k_free[kr.slot]);
+        if (p.i == p.g.n - 1) tc_commit(&bars.q_free[t][p.sg & 1]);
+      }
+      __syncwarp();
+      kr.next(nk);
+      leave(p);
+    };
+    scores(0);
+    scores(1);
+    for (int r = 0; r < rounds && ok; ++r)
+      for (int t = 0; t < 2 && ok; ++t) {
+        Place& p = place[t];
+        if (p.b >= p.end) continue;
+        enter(p);
+        ok = all_wait(&bars.p_ready[t], (uint32_t)r & 1u) && all_wait(&bars.v_full[vr.slot], vr.pass) && all_wait(&bars.v_fixed[vr.slot], vr.pass);
+        if (ok && p.i == 0 && p.sg > 0) ok = all_wait(&bars.o_free[t], (uint32_t)(p.sg - 1) & 1u);  // the last share's output has been read
+        if (!ok) break;
+        tc_fence_after();
+        if (issuer) {
+          const uint64_t v = tc_desc(values0 + vr.slot * L::kTile, 16384);
+#pragma unroll
+          for (int ks = 0; ks < kTcKeys / 8; ++ks)  // 32 columns of tensor memory per 32 keys: 16 of the upper halves, 16 of the lower
+            tc_mma_f16_ts(tmem + 256 + t * D, tmem + t * 128 + (ks & 7) / 2 * 32 + (ks & 1) * 8 + (ks >> 3) * 16, v + (uint64_t)((ks & 7) * 128), idesc_o,
+                          p.i > 0 || ks > 0);
+          tc_commit(&bars.v_free[vr.slot]);
+          if (p.i == p.g.n - 1) tc_commit(&bars.o_done[t]);
+        }
+        __syncwarp();
+        vr.next(nv);
+        leave(p);
+        scores(t);
+      }
+  } else if (warp >= 10) {
+    // ------------------------------------------------------------ values that not every row sees
+    bool ok = true;
+    Ring vr;
+    for (int r = 0; r < rounds && ok; ++r)
+      for (int t = 0; t < 2 && ok; ++t) {
+        Place& p = place[t];
+        if (p.b >= p.end) continue;
+        enter(p);
+        ok = wait(&bars.v_full[vr.slot], vr.pass);
+        if (!ok) break;
+        const Share& g = p.g;
+        const int j0 = block_key<kTcKeys>(g.all, g.blk0 + p.i);
+        if (g.p_first < 0 || !seen_by_all(a, g.p_first, g.p_last, j0, j0 + kTcKeys - 1)) {
+          const Seen own = paged_seen<kTcKeys>(a, g.p_first, g.p_last);
+          const uint32_t block = values0 + vr.slot * L::kTile;
+          bool bad = false;
+          for (int row = tid - 320; row < kTcKeys; row += 64) {
+            const bool seen = seen_by_some(own, j0 + row);
+            if (seen && g.p_first >= 0 && seen_by_all(a, g.p_first, g.p_last, j0 + row, j0 + row)) continue;
+            for (int c = 0; c < D / 8; ++c) {
+              const uint32_t at = block + (c / 8) * 16384 + row * 128 + (c % 8) * 16;
+              if (seen) {
+                uint4 x;
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory");
+                bad = bad || not_finite2<T>(x.x) || not_finite2<T>(x.y) || not_finite2<T>(x.z) || not_finite2<T>(x.w);
+              } else {
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
+              }
+            }
+          }
+          if (bad) s_bad = 1;
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.v_fixed[vr.slot]);
+        vr.next(nv);
+        leave(p);
+      }
+  } else {
+    // ------------------------------------------------------------ weights: one row per thread
+    const int t = warp >> 2, rw = warp & 3, r = rw * 32 + lane, tok = r / a.group, hg = r - tok * a.group;
+    if (rw < row_warps) {
+      const uint32_t lanes = (uint32_t)(rw * 32) << 16, s_col = tmem + t * 128 + lanes, o_col = tmem + 256 + t * D + lanes;
+      const float scale = BIAS ? 1.0f : a.scale2, grown = 8.0f / scale;
+      bool ok = true, live = false;
+      float m = -INFINITY, l = 0.0f;
+      int pos = -1, head = 0;
+      const float* bias = nullptr;
+      Place p = t ? place[1] : place[0];
+      for (int n = 0; p.b < p.end; ++n) {
+        enter(p);
+        const Share& g = p.g;
+        if (p.i == 0) {
+          live = tok < g.ntok;
+          head = g.kvh * a.group + hg;
+          pos = live ? g.p_first + tok : -1;
+          bias = BIAS && live ? a.bias + (size_t)head * (a.bias_max + 1) : nullptr;
+          m = -INFINITY, l = 0.0f;
+        }
+        ok = ok && all_wait(&bars.s_full[t], (uint32_t)n & 1u);
+        tc_fence_after();
+        const int j0 = block_key<kTcKeys>(g.all, g.blk0 + p.i);
+        const bool masked = g.p_first < 0 || !seen_by_all(a, g.p_first, g.p_last, j0, j0 + kTcKeys - 1);
+        const int hi = pos - j0, lo = a.window ? hi - a.window : -1, kp = a.window ? a.keep - j0 : 0;  // column i: i <= hi and (i > lo or i < kp)
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32];
+          tmem_ld32(s_col + c * 32, v);
+          tmem_ld_wait();
+          if (BIAS || masked) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const int col = c * 32 + i;
+              if (BIAS) {
+                const float b = bias ? __ldg(bias + max(0, min(hi - col, a.bias_max))) * kPagedLog2e : 0.0f;
+                v[i] = __float_as_uint(fmaf(__uint_as_float(v[i]), a.scale2, b));
+              }
+              if (masked && !(col <= hi && (col > lo || col < kp))) v[i] = 0xff800000u;
+            }
+            tmem_st32(s_col + c * 32, v);
+          }
+          float mx[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(v[i]);
+#pragma unroll
+          for (int i = 4; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[i]));
+          top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+        }
+        if (BIAS || masked) tmem_st_wait();
+        if (__any_sync(0xffffffffu, live && top > m + grown)) {
+          const float m_new = fmaxf(m, top), alpha = m_new == -INFINITY ? 1.0f : paged_exp2((m - m_new) * scale);
+          m = m_new;
+          if (p.i > 0) {  // (the products before S of this block are done)
+            l *= alpha;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(o_col + c * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st32(o_col + c * 32, o);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.0f : -m * scale;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32], w_hi[16], w_lo[16];
+          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          tmem_ld32(s_col + c * 32, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float p0 = paged_exp2(fmaf(__uint_as_float(v[2 * i]), scale, base)), p1 = paged_exp2(fmaf(__uint_as_float(v[2 * i + 1]), scale, base));
+            sum[i & 3] += p0 + p1;
+            w_hi[i] = Num<T>::pack(p0, p1);
+            const float2 h = Num<T>::unpack(w_hi[i]);
+            w_lo[i] = Num<T>::pack(p0 - h.x, p1 - h.y);
+          }
+          tmem_st16(s_col + c * 32, w_hi);
+          tmem_st16(s_col + c * 32 + 16, w_lo);
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.p_ready[t]);
+        if (p.i == g.n - 1) {  // the share's end
+          ok = ok && all_wait(&bars.o_done[t], (uint32_t)p.sg & 1u);
+          tc_fence_after();
+          const float ms = m * scale, sink = g.whole && a.sink && live ? a.sink[head] * kPagedLog2e : -INFINITY, most = fmaxf(ms, sink);  // base 2
+          const float at = most == -INFINITY ? 0.0f : most, f = exp2f(ms - at), sum = l * f + exp2f(sink - at), inv = !g.whole ? f : pos < 0 ? 0.0f : f / sum;
+          const size_t row = (size_t)(2 * (t * kSms + blockIdx.x) + g.begins) * item_rows + r;
+          if (!g.whole && live) w.part_ml[row] = make_float2(most, sum);
+          T* out = static_cast<T*>(a.out) + (g.row0 + tok) * a.out_row + head * a.out_head;
+          float* part = w.part_o + row * D;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(o_col + c * 32, o);
+            tmem_ld_wait();
+            if (!live || !ok) continue;
+            if (g.whole) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                uint32_t y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  y[i] = pos < 0 ? 0u : Num<T>::pack(__uint_as_float(o[8 * k + 2 * i]) * inv, __uint_as_float(o[8 * k + 2 * i + 1]) * inv);
+                *reinterpret_cast<uint4*>(out + c * 32 + k * 8) = make_uint4(y[0], y[1], y[2], y[3]);
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                *reinterpret_cast<float4*>(part + c * 32 + k * 4) = make_float4(__uint_as_float(o[4 * k]) * inv, __uint_as_float(o[4 * k + 1]) * inv,
+                                                                               __uint_as_float(o[4 * k + 2]) * inv, __uint_as_float(o[4 * k + 3]) * inv);
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.o_free[t]);
+        }
+        leave(p);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0) flags[blockIdx.x] = s_bad;
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                               CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeFn encode_fn() {
@@ -424,6 +850,40 @@ cudaError_t launch(const Paged& a, const CUtensorMap& q, const CUtensorMap& k, c
   return a.bias ? go(lm_paged_prompt_tc_kernel<T, D, true>, configure<T, D, true>()) : go(lm_paged_prompt_tc_kernel<T, D, false>, configure<T, D, false>());
 }
 
+constexpr int kDecodeSmem = 232448 - 4096;  // what a CTA may have, less the static part
+
+template <class T, int D, bool BIAS>
+cudaError_t configure_decode() {
+  static std::atomic<unsigned long long> done{0};
+  return once_per_device(&done, [] { return cudaFuncSetAttribute(lm_paged_decode_tc_kernel<T, D, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kDecodeSmem); });
+}
+template <class T, int D>
+cudaError_t launch_decode(const Paged& a, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const DecodeWork& w, int* flags, int piece, cudaStream_t s) {
+  const int rows = paged_decode_tc_rows(a), tpi = rows / a.group, q_rows = (rows + 7) / 8 * 8, fixed = 1024 + 4 * (D / 64) * q_rows * 128;
+  const int blocks = std::min(12, (kDecodeSmem - fixed) / TcLayout<D>::kTile), nv = blocks / 2, nk = blocks - nv;
+  const size_t smem = fixed + (size_t)blocks * TcLayout<D>::kTile;
+  auto go = [&](auto kernel, cudaError_t r) {
+    return r != cudaSuccess ? r : launch_pdl(kernel, dim3(kSms), dim3(kTcThreads), smem, s, a, q, k, v, w, flags, piece, tpi, q_rows, nk, nv);
+  };
+  return a.bias ? go(lm_paged_decode_tc_kernel<T, D, true>, configure_decode<T, D, true>()) : go(lm_paged_decode_tc_kernel<T, D, false>, configure_decode<T, D, false>());
+}
+
+// Tensor maps of a call; false: addresses or strides that they do not take.
+struct Maps {
+  CUtensorMap q, k, v;
+  int piece;
+};
+bool make_maps(const Paged& a, bool f16, int toks, Maps* m) {
+  m->piece = 16;
+  while (m->piece < kTcKeys && a.page % (2 * m->piece) == 0) m->piece *= 2;
+  const auto type = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const cuuint32_t q_box[3] = {64, (cuuint32_t)a.group, (cuuint32_t)toks}, box[4] = {64, (cuuint32_t)m->piece, 1, 1};
+  const cuuint64_t D = a.dim, dims[4] = {D, (cuuint64_t)a.page, (cuuint64_t)a.kv_heads, (cuuint64_t)a.pages};
+  return encode<3>(&m->q, type, a.q, {D, (cuuint64_t)a.heads, (cuuint64_t)a.rows}, {(cuuint64_t)a.q_head * 2, (cuuint64_t)a.q_row * 2}, q_box) &&
+         encode<4>(&m->k, type, a.k, dims, {(cuuint64_t)a.k_row * 2, (cuuint64_t)a.k_head * 2, (cuuint64_t)a.k_page * 2}, box) &&
+         encode<4>(&m->v, type, a.v, dims, {(cuuint64_t)a.v_row * 2, (cuuint64_t)a.v_head * 2, (cuuint64_t)a.v_page * 2}, box);
+}
+
 }  // namespace
 
 // Whether the kernel takes these sizes (and the tensor maps, these addresses and strides); `launched` says what became of it.
@@ -431,18 +891,23 @@ bool launch_paged_prompt_tc(const Paged& a, bool f16, cudaStream_t s, cudaError_
   if (a.dim != a.vdim || (a.dim != 64 && a.dim != 128) || !(a.scale2 > 1e-30f) || !(a.scale2 < 1e30f)) return false;
   const int toks = 128 / a.group;
   if (((long long)a.rows / (2 * toks) + a.seqs) * a.kv_heads > 0x7fffffffll) return false;
-  int piece = 16;
-  while (piece < kTcKeys && a.page % (2 * piece) == 0) piece *= 2;
-  const auto type = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  CUtensorMap q, k, v;
-  const cuuint32_t q_box[3] = {64, (cuuint32_t)a.group, (cuuint32_t)toks}, box[4] = {64, (cuuint32_t)piece, 1, 1};
-  const cuuint64_t D = a.dim, dims[4] = {D, (cuuint64_t)a.page, (cuuint64_t)a.kv_heads, (cuuint64_t)a.pages};
-  if (!encode<3>(&q, type, a.q, {D, (cuuint64_t)a.heads, (cuuint64_t)a.rows}, {(cuuint64_t)a.q_head * 2, (cuuint64_t)a.q_row * 2}, q_box) ||
-      !encode<4>(&k, type, a.k, dims, {(cuuint64_t)a.k_row * 2, (cuuint64_t)a.k_head * 2, (cuuint64_t)a.k_page * 2}, box) ||
-      !encode<4>(&v, type, a.v, dims, {(cuuint64_t)a.v_row * 2, (cuuint64_t)a.v_head * 2, (cuuint64_t)a.v_page * 2}, box))
-    return false;
-  *launched = f16 ? (a.dim == 64 ? launch<__half, 64>(a, q, k, v, piece, s) : launch<__half, 128>(a, q, k, v, piece, s))
-                  : (a.dim == 64 ? launch<__nv_bfloat16, 64>(a, q, k, v, piece, s) : launch<__nv_bfloat16, 128>(a, q, k, v, piece, s));
+  Maps m;
+  if (!make_maps(a, f16, toks, &m)) return false;
+  *launched = f16 ? (a.dim == 64 ? launch<__half, 64>(a, m.q, m.k, m.v, m.piece, s) : launch<__half, 128>(a, m.q, m.k, m.v, m.piece, s))
+                  : (a.dim == 64 ? launch<__nv_bfloat16, 64>(a, m.q, m.k, m.v, m.piece, s) : launch<__nv_bfloat16, 128>(a, m.q, m.k, m.v, m.piece, s));
+  return true;
+}
+
+bool paged_decode_tc_takes(const Paged& a) { return a.dim == a.vdim && (a.dim == 64 || a.dim == 128) && a.group <= 64; }
+int paged_decode_tc_rows(const Paged& a) { return std::max(1, std::min(a.tokens, 64 / a.group)) * a.group; }
+bool launch_paged_decode_tc(const Paged& a, bool f16, const DecodeWork& w, int* flags, cudaStream_t s, cudaError_t* launched) {
+  if (!paged_decode_tc_takes(a) || !(a.scale2 > 1e-30f) || !(a.scale2 < 1e30f)) return false;
+  if (((long long)a.max_pages * a.page / kTcKeys + 2) * a.seqs * a.kv_heads * w.row_blocks > 0x7fffffffll) return false;  // (blocks are counted in 32 bits)
+  Maps m;
+  if (!make_maps(a, f16, paged_decode_tc_rows(a) / a.group, &m)) return false;
+  *launched = f16 ? (a.dim == 64 ? launch_decode<__half, 64>(a, m.q, m.k, m.v, w, flags, m.piece, s) : launch_decode<__half, 128>(a, m.q, m.k, m.v, w, flags, m.piece, s))
+                  : (a.dim == 64 ? launch_decode<__nv_bfloat16, 64>(a, m.q, m.k, m.v, w, flags, m.piece, s)
+                                 : launch_decode<__nv_bfloat16, 128>(a, m.q, m.k, m.v, w, flags, m.piece, s));
   return true;
 }
 
