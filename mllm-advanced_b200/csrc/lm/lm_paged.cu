@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) lm_paged_decode_kernel(Paged a,
   pdl_wait_prior();
   if (w.redo) {  // again, and only if some CTA of the kernel before asks for it
     bool asked = false;
-    for (int i = tid; i < kSms; i += kDecThreads) asked = asked || w.redo[i] != 0;
+    for (int i = tid; i < kDecCtas; i += kDecThreads) asked = asked || w.redo[i] != 0;
     if (!__syncthreads_or(asked)) return;
   }
   sum_blocks<kDecB, kDecThreads>(a, s_base);
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(128) lm_paged_join_kernel(Paged a, DecodeWork 
   pdl_wait_prior();
   if (w.redo) {
     bool asked = false;
-    for (int i = threadIdx.x; i < kSms; i += 128) asked = asked || w.redo[i] != 0;
+    for (int i = threadIdx.x; i < kDecCtas; i += 128) asked = asked || w.redo[i] != 0;
     if (!__syncthreads_or(asked)) return;
   }
   const int items = a.kv_heads * w.row_blocks, s = blockIdx.x / items, item = blockIdx.x - s * items;
@@ -381,7 +381,7 @@ DecodeSpace decode_space(const Paged& a, int seqs) {
   d.ml = up16(rows * a.vdim * 4);
   d.base = d.ml + up16(rows * sizeof(float2));
   d.flags = d.base + up16((size_t)(seqs + 1) * sizeof(long long));
-  d.bytes = d.flags + kSms * sizeof(int);
+  d.bytes = d.flags + kDecCtas * sizeof(int);
   return d;
 }
 
@@ -461,8 +461,8 @@ cudaError_t launch_decode(Paged a, uint8_t* ws, cudaStream_t s) {
       }
     }
     w.row_blocks = (a.group * a.tokens + item_rows - 1) / item_rows;
-    r = with_decode<T>(b, [&](auto f) { return launch_pdl(f, dim3(kSms), dim3(32 * dec_warps(b)), smem, s, b, w); });
-    if (r == cudaSuccess) r = join_decode<T>(b, w, item_rows, kSms, s);
+    r = with_decode<T>(b, [&](auto f) { return launch_pdl(f, dim3(kDecCtas), dim3(32 * dec_warps(b)), smem, s, b, w); });
+    if (r == cudaSuccess) r = join_decode<T>(b, w, item_rows, kDecCtas, s);
     if (r != cudaSuccess) return r;
   }
   return cudaSuccess;

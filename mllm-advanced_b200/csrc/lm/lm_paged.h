@@ -82,7 +82,7 @@ __device__ __forceinline__ bool seen_by_all(const Paged& a, int first, int last,
 }
 
 constexpr int kDecSeqs = 512;  // sequences of a launch
-constexpr int kDecCtas = 2 * kSms;  // shares of the work: CTAs, or streams of half as many
+constexpr int kDecCtas = kSms;  // shares of the work, at most
 
 // Attention of a few tokens per sequence.  An item is (sequence, kv head, block of rows); its keys are walked in blocks of B.  The blocks of all
 // items, one after the other, are dealt out evenly: share c is [c T / G, (c + 1) T / G).  An item that lies in one share is

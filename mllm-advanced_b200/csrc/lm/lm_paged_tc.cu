@@ -405,14 +405,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
 }
 
 // ------------------------------------------------------------------------------------------ a few tokens per sequence
-// The rows of an item (all heads of a kv head, of up to 64 / group tokens) fill the first lanes of a tile; what bounds the kernel is
-// the stream of keys and values (64 KB a block of 128 keys for heads of 128).  A CTA runs two streams, each with S, O and queries of
-// its own and an even share of all blocks (two of the kDecCtas shares), so that the products of one run beside the weights of the
-// other; copies run ahead over the ends of items.  The tensor pipe has time to spare, so the weights enter as two halves of 16
-// bits (2^-17 of a weight and better).  Loops over columns are short on purpose: a launch starts with a cold instruction cache.
-//   warps 0-3, 4-7  weights of stream 0 and 1, only those whose rows exist
-//   warp 8, 9, 10-11  copies, MMA issue, values that not every row sees: as above
-struct Share {  // a stream's part of an item
+// What bounds this is the stream of keys and values (64 KB a block of 128 keys for heads of 128), as long as a block's work stays
+// shorter than its way from memory.  So the keys are the wide side of both products: S^T = K Q^T has a key per lane and an item's rows
+// (all heads of a kv head, of up to 64 / group tokens) as its 16, 32 or 64 columns, and O^T += V^T P^T a value's number per lane.
+// Every thread of the four warps has its own key; a row's maximum is looked for across threads only when some score has
+// outgrown the one in use by more than 2^8, and sums are added up across threads at an item's end.  Weights enter as two halves of
+// 16 bits (2^-17 of a weight and better).  A CTA walks an even share of all blocks, copies running ahead over the ends of items:
+//   warps 0-3        weights
+//   warp 4, 5, 6     copies; MMA issue (scores a block ahead); values that not every row sees
+struct Share {  // a CTA's part of an item
   int seq, kvh, row0, ntok, blk0, n, p_first, p_last;
   bool begins, whole;
   Seen all;  // what the sequence's rows see: the blocks; the item's own rows are at p_first .. p_last
@@ -448,367 +449,399 @@ struct Ring {
     if (++slot == n) slot = 0, pass ^= 1u;
   }
 };
+constexpr int kDecThreads = 256;
+
+template <int D, int NP>
+struct DecLayout {
+  static constexpr int kTile = 128 * D * 2;     // a block of keys or values
+  static constexpr int kQ = NP * D * 2;         // an item's queries
+  static constexpr int kP = 128 * NP * 2;       // weights of a block, one half
+  static constexpr int kFixed = 1024 + 2 * kQ + 4 * kP;
+  static constexpr int kBlocks = (232448 - 5120 - kFixed) / kTile < 12 ? (232448 - 5120 - kFixed) / kTile : 12;  // (5120: the static part)
+  static constexpr int kV = kBlocks / 2, kK = kBlocks - kV;
+  static constexpr int kBytes = kFixed + kBlocks * kTile;
+  static constexpr int kColumns = NP <= 16 ? 64 : NP <= 32 ? 128 : 256;  // of tensor memory: S twice, O
+  static constexpr uint64_t kSwizzle = NP == 16 ? 6 : NP == 32 ? 4 : 2;  // rows of 32, 64, 128 bytes
+};
+template <int D, int NP>
 struct DecBarriers {
-  uint64_t q_full[2][2], q_free[2][2], k_full[8], k_free[8], v_full[8], v_free[8], v_fixed[8], s_full[2], p_ready[2], o_done[2], o_free[2];
+  using L = DecLayout<D, NP>;
+  uint64_t q_full[2], q_free[2], k_full[L::kK], k_free[L::kK], v_full[L::kV], v_free[L::kV], v_fixed[L::kV], s_full[2], p_ready[2], p_free[2], o_free;
 };
 
-template <class T, int D, bool BIAS>
-__global__ void __launch_bounds__(kTcThreads, 1) lm_paged_decode_tc_kernel(const __grid_constant__ Paged a, const __grid_constant__ CUtensorMap qmap,
-                                                                           const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                                                                           DecodeWork w, int* flags, int piece, int tpi, int q_rows, int nk, int nv) {
-  using L = TcLayout<D>;
+template <class T, int D, int NP, bool BIAS>
+__global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(const __grid_constant__ Paged a, const __grid_constant__ CUtensorMap qmap,
+                                                                            const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                                                                            DecodeWork w, int* flags, int piece, int tpi) {
+  using L = DecLayout<D, NP>;
+  constexpr int kC = NP < 32 ? NP : 32;  // columns handled at a time
   extern __shared__ uint8_t tc_smem_raw[];
-  __shared__ DecBarriers bars;
+  __shared__ DecBarriers<D, NP> bars;
   __shared__ int s_base[kDecSeqs + 1];
+  __shared__ float s_max[4][NP], s_ref[NP], s_alpha[NP];  // the rows' maxima by warp; the one in use, times scale (base 2)
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_bad, s_gave_up;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-  // queries, two of each stream [D / 64][q_rows][64] (the products read 128 rows: what lies behind makes rows that nobody reads), keys, values
-  const uint32_t smem0 = (smem_u32(tc_smem_raw) + 1023u) & ~1023u, q_bytes = (uint32_t)(D / 64 * q_rows * 128);
-  const uint32_t keys0 = smem0 + 4 * q_bytes, values0 = keys0 + (uint32_t)nk * L::kTile;
-  const int item_rows = tpi * a.group, row_warps = (item_rows + 31) / 32;
+  // keys, values, weights [2][halves][128 keys][NP], queries [2][D / 64][NP][64]
+  const uint32_t keys0 = (smem_u32(tc_smem_raw) + 1023u) & ~1023u, values0 = keys0 + L::kK * L::kTile, p0 = values0 + L::kV * L::kTile, q0 = p0 + 4 * L::kP;
+  const int item_rows = tpi * a.group;
   if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
-      for (int k = 0; k < 2; ++k) mbar_init(&bars.q_full[i][k], 1), mbar_init(&bars.q_free[i][k], 1);
-      mbar_init(&bars.s_full[i], 1), mbar_init(&bars.o_done[i], 1), mbar_init(&bars.p_ready[i], row_warps), mbar_init(&bars.o_free[i], row_warps);
-    }
-    for (int i = 0; i < nk; ++i) mbar_init(&bars.k_full[i], 1), mbar_init(&bars.k_free[i], 1);
-    for (int i = 0; i < nv; ++i) mbar_init(&bars.v_full[i], 1), mbar_init(&bars.v_free[i], 1), mbar_init(&bars.v_fixed[i], 2);
+    for (int i = 0; i < 2; ++i)
+      mbar_init(&bars.q_full[i], 1), mbar_init(&bars.q_free[i], 1), mbar_init(&bars.s_full[i], 1), mbar_init(&bars.p_ready[i], 4), mbar_init(&bars.p_free[i], 1);
+    for (int i = 0; i < L::kK; ++i) mbar_init(&bars.k_full[i], 1), mbar_init(&bars.k_free[i], 1);
+    for (int i = 0; i < L::kV; ++i) mbar_init(&bars.v_full[i], 1), mbar_init(&bars.v_free[i], 1), mbar_init(&bars.v_fixed[i], 1);
+    mbar_init(&bars.o_free, 4);
     s_bad = s_gave_up = 0;
     mbar_fence_init();
   }
-  if (warp == 9) {
-    tmem_alloc(&s_tmem, 512);
+  if (warp == 5) {
+    tmem_alloc(&s_tmem, L::kColumns);
     tmem_relinquish();
   }
   pdl_launch_dependents();
   pdl_wait_prior();
-  sum_blocks<kTcKeys, kTcThreads>(a, s_base);
+  sum_blocks<kTcKeys, kDecThreads>(a, s_base);
   if (blockIdx.x == 0)
-    for (int i = tid; i <= a.seqs; i += kTcThreads) w.base[i] = s_base[i];
+    for (int i = tid; i <= a.seqs; i += kDecThreads) w.base[i] = s_base[i];
   for (int s = blockIdx.x; s < a.seqs; s += gridDim.x) {  // sequences without keys
     if (s_base[s + 1] != s_base[s]) continue;
     const int2 rows = paged_rows(a, s);
-    for (int i = tid; i < min(rows.y, a.tokens) * a.heads * (D / 8); i += kTcThreads) {
+    for (int i = tid; i < min(rows.y, a.tokens) * a.heads * (D / 8); i += kDecThreads) {
       const int c = i % (D / 8), h = i / (D / 8) % a.heads, t = i / (D / 8) / a.heads;
       *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (rows.x + t) * a.out_row + h * a.out_head + c * 8) = make_uint4(0, 0, 0, 0);
     }
   }
-  const int total = s_base[a.seqs] * a.kv_heads * w.row_blocks, shares = min(kDecCtas, total);  // (every one of them has something)
-  int start[2], end[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int c = t * kSms + blockIdx.x;
-    start[t] = c < shares ? (int)((long long)total * c / shares) : 0;
-    end[t] = c < shares ? (int)((long long)total * (c + 1) / shares) : 0;
-  }
-  const int rounds = max(end[0] - start[0], end[1] - start[1]);
+  const int total = s_base[a.seqs] * a.kv_heads * w.row_blocks, shares = min((int)gridDim.x, total);  // (every one of them has something)
+  const bool some = (int)blockIdx.x < shares;
+  const int start = some ? (int)((long long)total * blockIdx.x / shares) : 0, end = some ? (int)((long long)total * (blockIdx.x + 1) / shares) : 0;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
   auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity)) return true;
     if (s_gave_up) return false;
     if (mbar_wait_bounded(bar, parity)) return true;
     s_gave_up = 1;
     return false;
   };
   auto all_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
-  struct Place {  // of a role in a stream's list of blocks
-    int b, end, i, sg;
+  struct Place {  // of a role in the list of blocks
+    int b, i, sg;
     Share g;
+  } p{start, 0, 0, {}};
+  auto enter = [&](Place& q) {  // block q.b: its share
+    if (q.i == 0) q.g = share_at(a, s_base, w.row_blocks, tpi, q.b, end);
   };
-  auto enter = [&](Place& p) {  // before block p.b: its share
-    if (p.i == 0) p.g = share_at(a, s_base, w.row_blocks, tpi, p.b, p.end);
+  auto leave = [&](Place& q) {
+    ++q.b;
+    if (++q.i == q.g.n) q.i = 0, ++q.sg;
   };
-  auto leave = [&](Place& p) {
-    ++p.b;
-    if (++p.i == p.g.n) p.i = 0, ++p.sg;
-  };
-  Place place[2] = {{start[0], end[0], 0, 0, {}}, {start[1], end[1], 0, 0, {}}};
 
-  if (warp == 8) {
-    // ------------------------------------------------------------ copies: the streams' blocks in turn
+  if (warp == 4) {
+    // ------------------------------------------------------------ copies
     const int pieces = kTcKeys / piece;
     bool ok = true;
     Ring kr, vr;
-    for (int r = 0; r < rounds && ok; ++r)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        Place& p = place[t];
-        if (p.b >= p.end || !ok) continue;
-        enter(p);
-        if (p.i == 0) {
-          uint64_t* full = &bars.q_full[t][p.sg & 1];
-          if (p.sg >= 2) ok = all_wait(&bars.q_free[t][p.sg & 1], (uint32_t)((p.sg >> 1) - 1) & 1u);
-          if (!ok) break;
-          if (lane == 0) {
-            mbar_arrive_expect_tx(full, (uint32_t)(item_rows * D * 2));
-            for (int c = 0; c < D / 64; ++c)
-              tma_load_3d(smem0 + (2 * t + (p.sg & 1)) * q_bytes + c * q_rows * 128, &qmap, c * 64, p.g.kvh * a.group, p.g.row0, full);
-          }
-          __syncwarp();
-        }
-        // lane i: page of piece i, a.pages (zeros) where nothing of it is seen
-        const int key = block_key<kTcKeys>(p.g.all, p.g.blk0 + p.i) + lane * piece, place_in = key / a.page, inside = key - place_in * a.page;
-        int page = a.pages;
-        if (lane < pieces && key <= p.g.all.last && (key + piece > p.g.all.lo || key < p.g.all.head)) {
-          const int q = paged_page(a, p.g.seq, place_in);
-          if (q >= 0) page = q;
-        }
-        auto copy = [&](const CUtensorMap* map, uint32_t block, uint64_t* full) {
-          if (lane == 0) mbar_arrive_expect_tx(full, L::kTile);
-          __syncwarp();
-          if (lane < pieces) {
-#pragma unroll
-            for (int c = 0; c < D / 64; ++c) tma_load_4d(block + lane * piece * 128 + c * 16384, map, c * 64, inside, p.g.kvh, page, full);
-          }
-          __syncwarp();
-        };
-        if (kr.count >= nk) ok = all_wait(&bars.k_free[kr.slot], kr.pass ^ 1u);
-        if (!ok) break;
-        copy(&kmap, keys0 + kr.slot * L::kTile, &bars.k_full[kr.slot]);
-        kr.next(nk);
-        if (vr.count >= nv) ok = all_wait(&bars.v_free[vr.slot], vr.pass ^ 1u);
-        if (!ok) break;
-        copy(&vmap, values0 + vr.slot * L::kTile, &bars.v_full[vr.slot]);
-        vr.next(nv);
-        leave(p);
-      }
-    if (!ok) {  // nothing in flight when the CTA leaves
-      for (int i = max(0, kr.count - nk); i < kr.count; ++i) mbar_wait_bounded(&bars.k_full[i % nk], (uint32_t)(i / nk) & 1u);
-      for (int i = max(0, vr.count - nv); i < vr.count; ++i) mbar_wait_bounded(&bars.v_full[i % nv], (uint32_t)(i / nv) & 1u);
-      for (int t = 0; t < 2; ++t)
-        for (int i = max(0, place[t].sg - 1); i <= place[t].sg; ++i) mbar_wait_bounded(&bars.q_full[t][i & 1], (uint32_t)(i >> 1) & 1u);
-    }
-  } else if (warp == 9) {
-    // ------------------------------------------------------------ MMA issue: scores of a stream's next block behind its values
-    const bool issuer = elect_one_sync();
-    const uint32_t idesc_s = tc_idesc<T>(kTcKeys, false), idesc_o = tc_idesc<T>(D, true);
-    bool ok = true;
-    Place next[2] = {place[0], place[1]};  // of the scores
-    Ring kr, vr;
-    auto scores = [&](int t) {
-      Place& p = next[t];
-      if (p.b >= p.end || !ok) return;
+    while (p.b < end && ok) {
       enter(p);
-      if (p.i == 0) ok = all_wait(&bars.q_full[t][p.sg & 1], (uint32_t)(p.sg >> 1) & 1u);
+      if (p.i == 0) {
+        const int qb = p.sg & 1;
+        if (p.sg >= 2) ok = all_wait(&bars.q_free[qb], (uint32_t)((p.sg >> 1) - 1) & 1u);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&bars.q_full[qb], (uint32_t)(item_rows * D * 2));
+          for (int c = 0; c < D / 64; ++c) tma_load_3d(q0 + qb * L::kQ + c * NP * 128, &qmap, c * 64, p.g.kvh * a.group, p.g.row0, &bars.q_full[qb]);
+        }
+        __syncwarp();
+      }
+      // lane i: page of piece i, a.pages (zeros) where nothing of it is seen
+      const int key = block_key<kTcKeys>(p.g.all, p.g.blk0 + p.i) + lane * piece, place = key / a.page, inside = key - place * a.page;
+      int page = a.pages;
+      if (lane < pieces && key <= p.g.all.last && (key + piece > p.g.all.lo || key < p.g.all.head)) {
+        const int q = paged_page(a, p.g.seq, place);
+        if (q >= 0) page = q;
+      }
+      auto copy = [&](const CUtensorMap* map, uint32_t block, uint64_t* full) {
+        if (lane == 0) mbar_arrive_expect_tx(full, L::kTile);
+        __syncwarp();
+        if (lane < pieces) {
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) tma_load_4d(block + lane * piece * 128 + c * 16384, map, c * 64, inside, p.g.kvh, page, full);
+        }
+        __syncwarp();
+      };
+      if (kr.count >= L::kK) ok = all_wait(&bars.k_free[kr.slot], kr.pass ^ 1u);
+      if (!ok) break;
+      copy(&kmap, keys0 + kr.slot * L::kTile, &bars.k_full[kr.slot]);
+      kr.next(L::kK);
+      if (vr.count >= L::kV) ok = all_wait(&bars.v_free[vr.slot], vr.pass ^ 1u);
+      if (!ok) break;
+      copy(&vmap, values0 + vr.slot * L::kTile, &bars.v_full[vr.slot]);
+      vr.next(L::kV);
+      leave(p);
+    }
+    if (!ok) {  // nothing in flight when the CTA leaves
+      for (int i = max(0, kr.count - L::kK); i < kr.count; ++i) mbar_wait_bounded(&bars.k_full[i % L::kK], (uint32_t)(i / L::kK) & 1u);
+      for (int i = max(0, vr.count - L::kV); i < vr.count; ++i) mbar_wait_bounded(&bars.v_full[i % L::kV], (uint32_t)(i / L::kV) & 1u);
+      for (int i = max(0, p.sg - 1); i <= p.sg; ++i) mbar_wait_bounded(&bars.q_full[i & 1], (uint32_t)(i >> 1) & 1u);
+    }
+  } else if (warp == 5) {
+    // ------------------------------------------------------------ MMA issue
+    const bool issuer = elect_one_sync();
+    const uint32_t idesc_s = tc_idesc<T>(NP, false), idesc_o = tc_idesc<T>(NP, true) | (1u << 15);  // both operands of O^T run along M, N
+    bool ok = true;
+    Place ps = p;
+    Ring kr, vr;
+    auto scores = [&]() {  // of block kr.count
+      if (ps.b >= end || !ok) return;
+      enter(ps);
+      if (ps.i == 0) ok = all_wait(&bars.q_full[ps.sg & 1], (uint32_t)(ps.sg >> 1) & 1u);
       ok = ok && all_wait(&bars.k_full[kr.slot], kr.pass);
       if (!ok) return;
       tc_fence_after();
       if (issuer) {
-        const uint64_t q = tc_desc(smem0 + (2 * t + (p.sg & 1)) * q_bytes, 16), k = tc_desc(keys0 + kr.slot * L::kTile, 16);
+        const uint64_t k = tc_desc(keys0 + kr.slot * L::kTile, 16), q = tc_desc(q0 + (ps.sg & 1) * L::kQ, 16);
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks)
-          tc_mma_f16(tmem + t * 128, q + (uint64_t)((ks / 4) * q_rows * 8 + (ks % 4) * 2), k + (uint64_t)((ks / 4) * 1024 + (ks % 4) * 2), idesc_s, ks > 0);
-        tc_commit(&bars.s_full[t]);
+          tc_mma_f16(tmem + (kr.count & 1) * NP, k + (uint64_t)((ks / 4) * 1024 + (ks % 4) * 2), q + (uint64_t)((ks / 4) * NP * 8 + (ks % 4) * 2), idesc_s, ks > 0);
+        tc_commit(&bars.s_full[kr.count & 1]);
         tc_commit(&bars.k_free[kr.slot]);
-        if (p.i == p.g.n - 1) tc_commit(&bars.q_free[t][p.sg & 1]);
+        if (ps.i == ps.g.n - 1) tc_commit(&bars.q_free[ps.sg & 1]);
       }
       __syncwarp();
-      kr.next(nk);
-      leave(p);
+      kr.next(L::kK);
+      leave(ps);
     };
-    scores(0);
-    scores(1);
-    for (int r = 0; r < rounds && ok; ++r)
-      for (int t = 0; t < 2 && ok; ++t) {
-        Place& p = place[t];
-        if (p.b >= p.end) continue;
-        enter(p);
-        ok = all_wait(&bars.p_ready[t], (uint32_t)r & 1u) && all_wait(&bars.v_full[vr.slot], vr.pass) && all_wait(&bars.v_fixed[vr.slot], vr.pass);
-        if (ok && p.i == 0 && p.sg > 0) ok = all_wait(&bars.o_free[t], (uint32_t)(p.sg - 1) & 1u);  // the last share's output has been read
-        if (!ok) break;
-        tc_fence_after();
-        if (issuer) {
-          const uint64_t v = tc_desc(values0 + vr.slot * L::kTile, 16384);
+    scores();
+    scores();
+    while (p.b < end && ok) {
+      enter(p);
+      const int r = vr.count;
+      ok = all_wait(&bars.v_full[vr.slot], vr.pass) && all_wait(&bars.v_fixed[vr.slot], vr.pass);
+      if (ok && p.i == 0 && p.sg > 0) ok = all_wait(&bars.o_free, (uint32_t)(p.sg - 1) & 1u);  // the last share's output has been read
+      ok = ok && all_wait(&bars.p_ready[r & 1], (uint32_t)(r >> 1) & 1u);
+      if (!ok) break;
+      tc_fence_after();
+      if (issuer) {
+        constexpr uint32_t kStep = NP * 2 * 16 / 16;  // 16 keys of weights, in 16 bytes
+        const uint64_t v = tc_desc(values0 + vr.slot * L::kTile, 16384);
+        const uint64_t hi = (uint64_t)(((p0 + (r & 1) * 2 * L::kP) >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(NP * 16 >> 4) << 32) | (1ull << 46) | (L::kSwizzle << 61);
 #pragma unroll
-          for (int ks = 0; ks < kTcKeys / 8; ++ks)  // 32 columns of tensor memory per 32 keys: 16 of the upper halves, 16 of the lower
-            tc_mma_f16_ts(tmem + 256 + t * D, tmem + t * 128 + (ks & 7) / 2 * 32 + (ks & 1) * 8 + (ks >> 3) * 16, v + (uint64_t)((ks & 7) * 128), idesc_o,
-                          p.i > 0 || ks > 0);
-          tc_commit(&bars.v_free[vr.slot]);
-          if (p.i == p.g.n - 1) tc_commit(&bars.o_done[t]);
-        }
-        __syncwarp();
-        vr.next(nv);
-        leave(p);
-        scores(t);
+        for (int ks = 0; ks < kTcKeys / 8; ++ks)  // the upper halves, then the lower
+          tc_mma_f16(tmem + 2 * NP, v + (uint64_t)((ks & 7) * 128), hi + (uint64_t)((ks & 7) * kStep + (ks >> 3) * (L::kP >> 4)), idesc_o, p.i > 0 || ks > 0);
+        tc_commit(&bars.p_free[r & 1]);
+        tc_commit(&bars.v_free[vr.slot]);
       }
-  } else if (warp >= 10) {
+      __syncwarp();
+      vr.next(L::kV);
+      leave(p);
+      scores();
+    }
+  } else if (warp == 6) {
     // ------------------------------------------------------------ values that not every row sees
     bool ok = true;
     Ring vr;
-    for (int r = 0; r < rounds && ok; ++r)
-      for (int t = 0; t < 2 && ok; ++t) {
-        Place& p = place[t];
-        if (p.b >= p.end) continue;
-        enter(p);
-        ok = wait(&bars.v_full[vr.slot], vr.pass);
-        if (!ok) break;
-        const Share& g = p.g;
-        const int j0 = block_key<kTcKeys>(g.all, g.blk0 + p.i);
-        if (g.p_first < 0 || !seen_by_all(a, g.p_first, g.p_last, j0, j0 + kTcKeys - 1)) {
-          const Seen own = paged_seen<kTcKeys>(a, g.p_first, g.p_last);
-          const uint32_t block = values0 + vr.slot * L::kTile;
-          bool bad = false;
-          for (int row = tid - 320; row < kTcKeys; row += 64) {
-            const bool seen = seen_by_some(own, j0 + row);
-            if (seen && g.p_first >= 0 && seen_by_all(a, g.p_first, g.p_last, j0 + row, j0 + row)) continue;
-            for (int c = 0; c < D / 8; ++c) {
-              const uint32_t at = block + (c / 8) * 16384 + row * 128 + (c % 8) * 16;
-              if (seen) {
-                uint4 x;
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory");
-                bad = bad || not_finite2<T>(x.x) || not_finite2<T>(x.y) || not_finite2<T>(x.z) || not_finite2<T>(x.w);
-              } else {
-                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
-              }
+    while (p.b < end) {
+      enter(p);
+      ok = wait(&bars.v_full[vr.slot], vr.pass);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      const Share& g = p.g;
+      const int j0 = block_key<kTcKeys>(g.all, g.blk0 + p.i);
+      if (g.p_first < 0 || !seen_by_all(a, g.p_first, g.p_last, j0, j0 + kTcKeys - 1)) {
+        const Seen own = paged_seen<kTcKeys>(a, g.p_first, g.p_last);
+        const uint32_t block = values0 + vr.slot * L::kTile;
+        bool bad = false;
+        for (int row = lane; row < kTcKeys; row += 32) {
+          const bool seen = seen_by_some(own, j0 + row);
+          if (seen && g.p_first >= 0 && seen_by_all(a, g.p_first, g.p_last, j0 + row, j0 + row)) continue;
+          for (int c = 0; c < D / 8; ++c) {
+            const uint32_t at = block + (c / 8) * 16384 + row * 128 + (((c % 8) ^ (row & 7)) * 16);
+            if (seen) {
+              uint4 x;
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory");
+              bad = bad || not_finite2<T>(x.x) || not_finite2<T>(x.y) || not_finite2<T>(x.z) || not_finite2<T>(x.w);
+            } else {
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
             }
           }
-          if (bad) s_bad = 1;
-          fence_proxy_async_smem();
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.v_fixed[vr.slot]);
-        vr.next(nv);
-        leave(p);
+        if (bad) s_bad = 1;
+        fence_proxy_async_smem();
       }
-  } else {
-    // ------------------------------------------------------------ weights: one row per thread
-    const int t = warp >> 2, rw = warp & 3, r = rw * 32 + lane, tok = r / a.group, hg = r - tok * a.group;
-    if (rw < row_warps) {
-      const uint32_t lanes = (uint32_t)(rw * 32) << 16, s_col = tmem + t * 128 + lanes, o_col = tmem + 256 + t * D + lanes;
-      const float scale = BIAS ? 1.0f : a.scale2, grown = 8.0f / scale;
-      bool ok = true, live = false;
-      float m = -INFINITY, l = 0.0f;
-      int pos = -1, head = 0;
-      const float* bias = nullptr;
-      Place p = t ? place[1] : place[0];
-      for (int n = 0; p.b < p.end; ++n) {
-        enter(p);
-        const Share& g = p.g;
-        if (p.i == 0) {
-          live = tok < g.ntok;
-          head = g.kvh * a.group + hg;
-          pos = live ? g.p_first + tok : -1;
-          bias = BIAS && live ? a.bias + (size_t)head * (a.bias_max + 1) : nullptr;
-          m = -INFINITY, l = 0.0f;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.v_fixed[vr.slot]);
+      vr.next(L::kV);
+      leave(p);
+    }
+  } else if (warp < 4) {
+    // ------------------------------------------------------------ weights: one key per thread
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    const float scale = BIAS ? 1.0f : a.scale2;  // BIAS: scores are scaled when it is added
+    auto sync = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+    auto any = [](bool v) {
+      int r;
+      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.b32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"((int)v) : "memory");
+      return r != 0;
+    };
+    bool ok = true;
+    float l[NP];
+    for (int r = 0; p.b < end; ++r) {
+      enter(p);
+      const Share& g = p.g;
+      const int j = block_key<kTcKeys>(g.all, g.blk0 + p.i) + tid, rows = g.ntok * a.group;
+      const bool masked = g.p_first < 0 || !seen_by_all(a, g.p_first, g.p_last, j - tid, j - tid + kTcKeys - 1);
+      const uint32_t s_col = tmem + (r & 1) * NP + lanes, o_col = tmem + 2 * NP + lanes;
+      if (p.i == 0) {
+#pragma unroll
+        for (int c = 0; c < NP; ++c) l[c] = 0.0f;
+        sync();  // (the last share's numbers have been read)
+        if (tid < NP) s_ref[tid] = tid < rows ? -INFINITY : INFINITY;  // (columns without a row: weights of 0)
+        sync();
+      }
+      ok = ok && all_wait(&bars.s_full[r & 1], (uint32_t)(r >> 1) & 1u);
+      tc_fence_after();
+      bool over = false;
+      uint32_t v[kC];
+      auto load = [&](int c0) {  // columns c0 .. c0 + kC - 1: scores, with bias and mask
+        if constexpr (kC == 16) tmem_ld16(s_col + c0, v);
+        else tmem_ld32(s_col + c0, v);
+        tmem_ld_wait();
+        if (BIAS || masked) {
+          int tok = c0 / a.group, hg = c0 - tok * a.group;
+#pragma unroll
+          for (int i = 0; i < kC; ++i) {
+            const int pos = g.p_first + tok;
+            float x = __uint_as_float(v[i]);
+            if (BIAS && c0 + i < rows) x = fmaf(x, a.scale2, __ldg(a.bias + (size_t)(g.kvh * a.group + hg) * (a.bias_max + 1) + max(0, min(pos - j, a.bias_max))) * kPagedLog2e);
+            v[i] = masked && !seen_by(a, pos, j) ? 0xff800000u : __float_as_uint(x);
+            if (++hg == a.group) hg = 0, ++tok;
+          }
         }
-        ok = ok && all_wait(&bars.s_full[t], (uint32_t)n & 1u);
+      };
+#pragma unroll
+      for (int c0 = 0; c0 < NP; c0 += kC) {
+        load(c0);
+#pragma unroll
+        for (int i = 0; i < kC; ++i) over = over || fmaf(__uint_as_float(v[i]), scale, -8.0f) > s_ref[c0 + i];
+      }
+      if (any(over)) {  // some row's maximum has outgrown its reference (always in an item's first block, unless nothing is seen)
+#pragma unroll
+        for (int c0 = 0; c0 < NP; c0 += kC) {
+          if (NP > kC) load(c0);
+#pragma unroll
+          for (int i = 0; i < kC; ++i) {
+            float x = __uint_as_float(v[i]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+            if (lane == 0) s_max[warp][c0 + i] = x;
+          }
+        }
+        sync();
+        if (tid < rows) {
+          const float old = s_ref[tid], top = fmaxf(fmaxf(s_max[0][tid], s_max[1][tid]), fmaxf(s_max[2][tid], s_max[3][tid])) * scale, now = fmaxf(old, top);
+          s_alpha[tid] = now == -INFINITY ? 1.0f : exp2f(old - now);
+          s_ref[tid] = now;
+        } else if (tid < NP) {
+          s_alpha[tid] = 1.0f;
+        }
+        sync();
+#pragma unroll
+        for (int c = 0; c < NP; ++c) l[c] *= s_alpha[c];
+        if (p.i > 0) {  // behind the products of the block before
+          ok = ok && all_wait(&bars.p_free[(r - 1) & 1], (uint32_t)((r - 1) >> 1) & 1u);
+          tc_fence_after();
+#pragma unroll
+          for (int c0 = 0; c0 < NP; c0 += 16) {
+            uint32_t o[16];
+            tmem_ld16(o_col + c0, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * s_alpha[c0 + i]);
+            tmem_st16(o_col + c0, o);
+          }
+          tmem_st_wait();
+        }
+      }
+      if (r >= 2) ok = ok && all_wait(&bars.p_free[r & 1], (uint32_t)((r >> 1) - 1) & 1u);  // the products of two blocks before: their weights' place
+      const uint32_t row = p0 + (r & 1) * 2 * L::kP + tid * NP * 2;
+#pragma unroll
+      for (int c0 = 0; c0 < NP; c0 += kC) {
+        if (NP > kC) load(c0);
+#pragma unroll
+        for (int c = 0; c < kC; c += 8) {
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = c + 2 * i;
+            const float r0 = s_ref[c0 + k], r1 = s_ref[c0 + k + 1];
+            const float w0 = paged_exp2(fmaf(__uint_as_float(v[k]), scale, r0 == -INFINITY ? 0.0f : -r0)), w1 = paged_exp2(fmaf(__uint_as_float(v[k + 1]), scale, r1 == -INFINITY ? 0.0f : -r1));
+            l[c0 + k] += w0, l[c0 + k + 1] += w1;
+            hi[i] = Num<T>::pack(w0, w1);
+            const float2 h = Num<T>::unpack(hi[i]);
+            lo[i] = Num<T>::pack(w0 - h.x, w1 - h.y);
+          }
+          const int chunk = (c0 + c) / 8, sw = NP == 16 ? (tid >> 2) & 1 : NP == 32 ? (tid >> 1) & 3 : tid & 7;
+          const uint32_t at = row + ((chunk ^ sw) * 16);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + L::kP), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
+        }
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.p_ready[r & 1]);
+      if (p.i == g.n - 1) {  // the share's end: the rows' sums, then a number of the value per thread
+#pragma unroll
+        for (int c = 0; c < NP; ++c) {
+          float x = l[c];
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+          if (lane == 0) s_max[warp][c] = x;
+        }
+        sync();
+        const size_t slot = (size_t)(2 * blockIdx.x + g.begins) * item_rows;
+        if (tid < rows) {
+          const int tok = tid / a.group, head = g.kvh * a.group + tid - tok * a.group;
+          const float ref = s_ref[tid], sink = g.whole && a.sink ? a.sink[head] * kPagedLog2e : -INFINITY, most = fmaxf(ref, sink), at = most == -INFINITY ? 0.0f : most;
+          const float f = exp2f(ref - at), sum = ((s_max[0][tid] + s_max[1][tid]) + (s_max[2][tid] + s_max[3][tid])) * f + exp2f(sink - at);
+          s_alpha[tid] = !g.whole ? f : g.p_first + tok < 0 ? 0.0f : f / sum;
+          if (!g.whole) w.part_ml[slot + tid] = make_float2(most, sum);
+        }
+        ok = ok && all_wait(&bars.p_free[r & 1], (uint32_t)(r >> 1) & 1u);
         tc_fence_after();
-        const int j0 = block_key<kTcKeys>(g.all, g.blk0 + p.i);
-        const bool masked = g.p_first < 0 || !seen_by_all(a, g.p_first, g.p_last, j0, j0 + kTcKeys - 1);
-        const int hi = pos - j0, lo = a.window ? hi - a.window : -1, kp = a.window ? a.keep - j0 : 0;  // column i: i <= hi and (i > lo or i < kp)
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[32];
-          tmem_ld32(s_col + c * 32, v);
-          tmem_ld_wait();
-          if (BIAS || masked) {
+        sync();
+        if (tid < D && ok) {
+          T* out = static_cast<T*>(a.out) + (long long)g.row0 * a.out_row + (long long)g.kvh * a.group * a.out_head + tid;
+          float* part = w.part_o + slot * D + tid;
+          int tok = 0, hg = 0;
+          for (int c0 = 0; c0 < NP; c0 += 16) {
+            uint32_t o[16];
+            tmem_ld16(o_col + c0, o);
+            tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int col = c * 32 + i;
-              if (BIAS) {
-                const float b = bias ? __ldg(bias + max(0, min(hi - col, a.bias_max))) * kPagedLog2e : 0.0f;
-                v[i] = __float_as_uint(fmaf(__uint_as_float(v[i]), a.scale2, b));
-              }
-              if (masked && !(col <= hi && (col > lo || col < kp))) v[i] = 0xff800000u;
-            }
-            tmem_st32(s_col + c * 32, v);
-          }
-          float mx[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(v[i]);
-#pragma unroll
-          for (int i = 4; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[i]));
-          top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-        }
-        if (BIAS || masked) tmem_st_wait();
-        if (__any_sync(0xffffffffu, live && top > m + grown)) {
-          const float m_new = fmaxf(m, top), alpha = m_new == -INFINITY ? 1.0f : paged_exp2((m - m_new) * scale);
-          m = m_new;
-          if (p.i > 0) {  // (the products before S of this block are done)
-            l *= alpha;
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32(o_col + c * 32, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tmem_st32(o_col + c * 32, o);
+            for (int i = 0; i < 16; ++i) {
+              if (c0 + i >= rows) break;
+              const float x = g.p_first + tok < 0 ? 0.0f : __uint_as_float(o[i]) * s_alpha[c0 + i];
+              if (g.whole) out[tok * a.out_row + hg * a.out_head] = T(x);
+              else part[(size_t)(c0 + i) * D] = x;
+              if (++hg == a.group) hg = 0, ++tok;
             }
           }
         }
-        const float base = m == -INFINITY ? 0.0f : -m * scale;
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[32], w_hi[16], w_lo[16];
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          tmem_ld32(s_col + c * 32, v);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float p0 = paged_exp2(fmaf(__uint_as_float(v[2 * i]), scale, base)), p1 = paged_exp2(fmaf(__uint_as_float(v[2 * i + 1]), scale, base));
-            sum[i & 3] += p0 + p1;
-            w_hi[i] = Num<T>::pack(p0, p1);
-            const float2 h = Num<T>::unpack(w_hi[i]);
-            w_lo[i] = Num<T>::pack(p0 - h.x, p1 - h.y);
-          }
-          tmem_st16(s_col + c * 32, w_hi);
-          tmem_st16(s_col + c * 32 + 16, w_lo);
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        }
-        tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.p_ready[t]);
-        if (p.i == g.n - 1) {  // the share's end
-          ok = ok && all_wait(&bars.o_done[t], (uint32_t)p.sg & 1u);
-          tc_fence_after();
-          const float ms = m * scale, sink = g.whole && a.sink && live ? a.sink[head] * kPagedLog2e : -INFINITY, most = fmaxf(ms, sink);  // base 2
-          const float at = most == -INFINITY ? 0.0f : most, f = exp2f(ms - at), sum = l * f + exp2f(sink - at), inv = !g.whole ? f : pos < 0 ? 0.0f : f / sum;
-          const size_t row = (size_t)(2 * (t * kSms + blockIdx.x) + g.begins) * item_rows + r;
-          if (!g.whole && live) w.part_ml[row] = make_float2(most, sum);
-          T* out = static_cast<T*>(a.out) + (g.row0 + tok) * a.out_row + head * a.out_head;
-          float* part = w.part_o + row * D;
-#pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(o_col + c * 32, o);
-            tmem_ld_wait();
-            if (!live || !ok) continue;
-            if (g.whole) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                uint32_t y[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  y[i] = pos < 0 ? 0u : Num<T>::pack(__uint_as_float(o[8 * k + 2 * i]) * inv, __uint_as_float(o[8 * k + 2 * i + 1]) * inv);
-                *reinterpret_cast<uint4*>(out + c * 32 + k * 8) = make_uint4(y[0], y[1], y[2], y[3]);
-              }
-            } else {
-#pragma unroll
-              for (int k = 0; k < 8; ++k)
-                *reinterpret_cast<float4*>(part + c * 32 + k * 4) = make_float4(__uint_as_float(o[4 * k]) * inv, __uint_as_float(o[4 * k + 1]) * inv,
-                                                                               __uint_as_float(o[4 * k + 2]) * inv, __uint_as_float(o[4 * k + 3]) * inv);
-            }
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars.o_free[t]);
-        }
-        leave(p);
+        if (lane == 0) mbar_arrive(&bars.o_free);
       }
+      leave(p);
     }
   }
   tc_fence_before();
   __syncthreads();
   if (tid == 0) flags[blockIdx.x] = s_bad;
-  if (warp == 9) {
+  if (warp == 5) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, L::kColumns);
   }
 }
 
@@ -850,22 +883,23 @@ cudaError_t launch(const Paged& a, const CUtensorMap& q, const CUtensorMap& k, c
   return a.bias ? go(lm_paged_prompt_tc_kernel<T, D, true>, configure<T, D, true>()) : go(lm_paged_prompt_tc_kernel<T, D, false>, configure<T, D, false>());
 }
 
-constexpr int kDecodeSmem = 232448 - 4096;  // what a CTA may have, less the static part
-
-template <class T, int D, bool BIAS>
-cudaError_t configure_decode() {
+template <class T, int D, int NP, bool BIAS>
+cudaError_t launch_decode_form(const Paged& a, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const DecodeWork& w, int* flags, int piece,
+                               cudaStream_t s) {
   static std::atomic<unsigned long long> done{0};
-  return once_per_device(&done, [] { return cudaFuncSetAttribute(lm_paged_decode_tc_kernel<T, D, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kDecodeSmem); });
+  const auto kernel = lm_paged_decode_tc_kernel<T, D, NP, BIAS>;
+  const cudaError_t r = once_per_device(&done, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DecLayout<D, NP>::kBytes); });
+  if (r != cudaSuccess) return r;
+  return launch_pdl(kernel, dim3(kDecCtas), dim3(kDecThreads), DecLayout<D, NP>::kBytes, s, a, q, k, v, w, flags, piece, paged_decode_tc_rows(a) / a.group);
 }
 template <class T, int D>
 cudaError_t launch_decode(const Paged& a, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const DecodeWork& w, int* flags, int piece, cudaStream_t s) {
-  const int rows = paged_decode_tc_rows(a), tpi = rows / a.group, q_rows = (rows + 7) / 8 * 8, fixed = 1024 + 4 * (D / 64) * q_rows * 128;
-  const int blocks = std::min(12, (kDecodeSmem - fixed) / TcLayout<D>::kTile), nv = blocks / 2, nk = blocks - nv;
-  const size_t smem = fixed + (size_t)blocks * TcLayout<D>::kTile;
-  auto go = [&](auto kernel, cudaError_t r) {
-    return r != cudaSuccess ? r : launch_pdl(kernel, dim3(kSms), dim3(kTcThreads), smem, s, a, q, k, v, w, flags, piece, tpi, q_rows, nk, nv);
+  const int rows = paged_decode_tc_rows(a);
+  auto go = [&](auto np) {
+    constexpr int NP = decltype(np)::value;
+    return a.bias ? launch_decode_form<T, D, NP, true>(a, q, k, v, w, flags, piece, s) : launch_decode_form<T, D, NP, false>(a, q, k, v, w, flags, piece, s);
   };
-  return a.bias ? go(lm_paged_decode_tc_kernel<T, D, true>, configure_decode<T, D, true>()) : go(lm_paged_decode_tc_kernel<T, D, false>, configure_decode<T, D, false>());
+  return rows <= 16 ? go(std::integral_constant<int, 16>()) : rows <= 32 ? go(std::integral_constant<int, 32>()) : go(std::integral_constant<int, 64>());
 }
 
 // Tensor maps of a call; false: addresses or strides that they do not take.
