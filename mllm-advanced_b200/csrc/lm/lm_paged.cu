@@ -78,8 +78,12 @@ __global__ void __launch_bounds__(32 * WARPS, 1) lm_paged_decode_kernel(Paged a,
   const long long total = s_base[a.seqs] * items;
   const int ctas = (int)min((long long)gridDim.x, total);  // (every one of them has something)
   if ((int)blockIdx.x >= ctas) return;
-  long long b = total * blockIdx.x / ctas;
-  const long long end = total * (blockIdx.x + 1) / ctas;
+  long long b = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
+  if (w.redo) {  // whole items, so that nothing is left to join
+    auto item_start = [&](long long i) { return s_base[i / items] * items + i % items * (s_base[min((int)(i / items) + 1, a.seqs)] - s_base[i / items]); };
+    const long long n = (long long)a.seqs * items;
+    b = item_start(n * blockIdx.x / ctas), end = item_start(n * (blockIdx.x + 1) / ctas);
+  }
   const int mat = lane >> 3, ml = lane & 7, cr = lane >> 3, cc = lane & 7;
   const uint32_t q_addr = smem_u32(sQ + ((mat & 1) * 8 + ml) * ldk + (mat >> 1) * 8);
 
@@ -234,65 +238,60 @@ __global__ void __launch_bounds__(32 * WARPS, 1) lm_paged_decode_kernel(Paged a,
   }
 }
 
-// grid (items of all sequences, rows of an item): joins the shares of items that lie in several CTAs; zeros for those
-// without keys.
+// grid (items of all sequences, rows of an item / 4): a warp joins the shares of a row of an item that lies in several CTAs; zeros
+// for those without keys.
+constexpr int kJoinWarps = 4;
 template <class T>
-__global__ void __launch_bounds__(128) lm_paged_join_kernel(Paged a, DecodeWork w, int item_rows, int grid) {
-  __shared__ float s_f[kDecCtas], s_inv;
+__global__ void __launch_bounds__(32 * kJoinWarps) lm_paged_join_kernel(Paged a, DecodeWork w, int item_rows) {
   pdl_launch_dependents();
-  pdl_wait_prior();
-  if (w.redo) {
-    bool asked = false;
-    for (int i = threadIdx.x; i < kDecCtas; i += 128) asked = asked || w.redo[i] != 0;
-    if (!__syncthreads_or(asked)) return;
-  }
-  const int items = a.kv_heads * w.row_blocks, s = blockIdx.x / items, item = blockIdx.x - s * items;
-  const int kvh = item / w.row_blocks, r = blockIdx.y, row = (item - kvh * w.row_blocks) * item_rows + r, tid = threadIdx.x;
-  if (row >= a.group * a.tokens) return;
-  const long long b0 = w.base[s] * items, nb = w.base[s + 1] - w.base[s], first = b0 + item * nb, total = w.base[a.seqs] * items;
+  const int items = a.kv_heads * w.row_blocks, s = blockIdx.x / items, item = blockIdx.x - s * items, lane = threadIdx.x & 31;
+  const int kvh = item / w.row_blocks, r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5), row = (item - kvh * w.row_blocks) * item_rows + r;
   const int tok = row / a.group, h = kvh * a.group + row - tok * a.group;
+  pdl_wait_prior();
+  if (r >= item_rows || row >= a.group * a.tokens) return;
+  const long long b0 = w.base[s] * items, nb = w.base[s + 1] - w.base[s], first = b0 + item * nb, total = w.base[a.seqs] * items;
+  const int ctas = (int)min((long long)kDecCtas, total), c0 = nb ? owner_of(first, total, ctas) : 0, n = nb ? owner_of(first + nb - 1, total, ctas) - c0 + 1 : 0;
+  if (n == 1) return;  // finished there
   const int2 q_rows = paged_rows(a, s);
   if (tok >= q_rows.y) return;
   T* out = static_cast<T*>(a.out) + (q_rows.x + tok) * a.out_row + h * a.out_head;
-  if (nb == 0) {
-    for (int d = tid; d < a.vdim; d += 128) out[d] = T(0.0f);
-    return;
-  }
-  const int ctas = (int)min((long long)grid, total);
-  const int c0 = owner_of(first, total, ctas), c1 = owner_of(first + nb - 1, total, ctas), n = c1 - c0 + 1;
-  if (n == 1) return;  // finished there
-  const bool nothing = paged_length(a, s) - a.tokens + tok < 0;
+  const bool nothing = n == 0 || paged_length(a, s) - a.tokens + tok < 0;
   auto slot = [&](int i) { return (size_t)(2 * (c0 + i) + (i == 0)) * item_rows + r; };
-  if (tid < 32) {
-    const float sink = a.sink ? a.sink[h] * kPagedLog2e : -INFINITY;
-    float mx = sink;
-    for (int i = tid; i < n; i += 32) mx = fmaxf(mx, w.part_ml[slot(i)].x);
+  const float sink = a.sink ? a.sink[h] * kPagedLog2e : -INFINITY;
+  float mx = sink;
+  for (int i = lane; i < n; i += 32) mx = fmaxf(mx, w.part_ml[slot(i)].x);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const float base = mx == -INFINITY ? 0.0f : mx;
-    float sum = 0.0f;
-    for (int i = tid; i < n; i += 32) {
-      const float2 v = w.part_ml[slot(i)];
-      const float f = exp2f(v.x - base);
-      s_f[i] = f;
-      sum = fmaf(f, v.y, sum);
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  const float base = mx == -INFINITY ? 0.0f : mx;
+  float sum = 0.0f, v[8] = {};  // columns 4 lane .. and 128 + 4 lane ..
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    float f = 0.0f;
+    if (i0 + lane < n) {
+      const float2 ml = w.part_ml[slot(i0 + lane)];
+      f = exp2f(ml.x - base);
+      sum = fmaf(f, ml.y, sum);
     }
+#pragma unroll 4
+    for (int i = 0; i < min(32, n - i0); ++i) {
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      const float* part = w.part_o + slot(i0 + i) * a.vdim;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (tid == 0) s_inv = 1.0f / (sum + (a.sink ? exp2f(sink - base) : 0.0f));
-  }
-  __syncthreads();
-  for (int d = tid; d < a.vdim; d += 128) {
-    float v = 0.0f;
-    for (int i0 = 0; i0 < n; i0 += 8) {
-      float x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = w.part_o[slot(min(i0 + j, n - 1)) * a.vdim + d];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v = fmaf(i0 + j < n ? s_f[i0 + j] : 0.0f, x[j], v);
+      for (int c = 0; c < 2; ++c)
+        if (c * 128 + lane * 4 < a.vdim) {
+          const float4 x = *reinterpret_cast<const float4*>(part + c * 128 + lane * 4);
+          v[c * 4] = fmaf(fi, x.x, v[c * 4]), v[c * 4 + 1] = fmaf(fi, x.y, v[c * 4 + 1]);
+          v[c * 4 + 2] = fmaf(fi, x.z, v[c * 4 + 2]), v[c * 4 + 3] = fmaf(fi, x.w, v[c * 4 + 3]);
+        }
     }
-    out[d] = T(nothing ? 0.0f : v * s_inv);
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const float inv = 1.0f / (sum + exp2f(sink - base));
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+    if (c * 128 + lane * 4 < a.vdim)
+      *reinterpret_cast<uint2*>(out + c * 128 + lane * 4) =
+          nothing ? make_uint2(0, 0) : make_uint2(Num<T>::pack(v[c * 4] * inv, v[c * 4 + 1] * inv), Num<T>::pack(v[c * 4 + 2] * inv, v[c * 4 + 3] * inv));
 }
 
 // ------------------------------------------------------------------------------------------ prompts, any head size
@@ -430,9 +429,9 @@ int check_decode(const mllmb200_lm_pages* p, const mllmb200_lm_look* l, Paged* a
 }
 
 template <class T>
-cudaError_t join_decode(const Paged& a, const DecodeWork& w, int item_rows, int shares, cudaStream_t s) {
-  return launch_pdl(lm_paged_join_kernel<T>, dim3(a.seqs * a.kv_heads * w.row_blocks, std::min(item_rows, a.group * a.tokens)), dim3(128), 0, s, a, w, item_rows,
-                    shares);
+cudaError_t join_decode(const Paged& a, const DecodeWork& w, int item_rows, cudaStream_t s) {
+  const int rows = std::min(item_rows, a.group * a.tokens);
+  return launch_pdl(lm_paged_join_kernel<T>, dim3(a.seqs * a.kv_heads * w.row_blocks, (rows + kJoinWarps - 1) / kJoinWarps), dim3(32 * kJoinWarps), 0, s, a, w, item_rows);
 }
 template <class T>
 cudaError_t launch_decode(Paged a, uint8_t* ws, cudaStream_t s) {
@@ -454,7 +453,7 @@ cudaError_t launch_decode(Paged a, uint8_t* ws, cudaStream_t s) {
       w.row_blocks = (b.tokens + tokens - 1) / tokens;
       if (launch_paged_decode_tc(b, std::is_same<T, __half>::value, w, flags, s, &r)) {
         // (a table that names one block of keys: every item lies in one CTA)
-        if (r == cudaSuccess && b.max_pages * b.page > 128) r = join_decode<T>(b, w, tokens * b.group, kDecCtas, s);
+        if (r == cudaSuccess && b.max_pages * b.page > 128) r = join_decode<T>(b, w, tokens * b.group, s);
         if (r != cudaSuccess) return r;
         if (b.tokens == 1) continue;  // (what one token sees, all of it sees)
         w.redo = flags;
@@ -462,7 +461,7 @@ cudaError_t launch_decode(Paged a, uint8_t* ws, cudaStream_t s) {
     }
     w.row_blocks = (a.group * a.tokens + item_rows - 1) / item_rows;
     r = with_decode<T>(b, [&](auto f) { return launch_pdl(f, dim3(kDecCtas), dim3(32 * dec_warps(b)), smem, s, b, w); });
-    if (r == cudaSuccess) r = join_decode<T>(b, w, item_rows, kDecCtas, s);
+    if (r == cudaSuccess && !w.redo) r = join_decode<T>(b, w, item_rows, s);
     if (r != cudaSuccess) return r;
   }
   return cudaSuccess;

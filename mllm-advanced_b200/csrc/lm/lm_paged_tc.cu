@@ -456,7 +456,8 @@ struct DecLayout {
   static constexpr int kTile = 128 * D * 2;     // a block of keys or values
   static constexpr int kQ = NP * D * 2;         // an item's queries
   static constexpr int kP = 128 * NP * 2;       // weights of a block, one half
-  static constexpr int kFixed = 1024 + 2 * kQ + 4 * kP;
+  static constexpr int kBufs = NP == 16 ? 2 : 1;  // places for queries and for weights: with more rows keys and values need the room more
+  static constexpr int kFixed = 1024 + kBufs * (kQ + 2 * kP);
   static constexpr int kBlocks = (232448 - 5120 - kFixed) / kTile < 12 ? (232448 - 5120 - kFixed) / kTile : 12;  // (5120: the static part)
   static constexpr int kV = kBlocks / 2, kK = kBlocks - kV;
   static constexpr int kBytes = kFixed + kBlocks * kTile;
@@ -478,12 +479,14 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
   extern __shared__ uint8_t tc_smem_raw[];
   __shared__ DecBarriers<D, NP> bars;
   __shared__ int s_base[kDecSeqs + 1];
-  __shared__ float s_max[4][NP], s_ref[NP], s_alpha[NP];  // the rows' maxima by warp; the one in use, times scale (base 2)
+  __shared__ float s_max[4][NP];
+  __shared__ __align__(16) float s_ref[NP], s_alpha[NP], s_base2[NP];  // the rows' maxima by warp; the one in use, times scale (base 2); what is added to scores
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_bad, s_gave_up;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-  // keys, values, weights [2][halves][128 keys][NP], queries [2][D / 64][NP][64]
-  const uint32_t keys0 = (smem_u32(tc_smem_raw) + 1023u) & ~1023u, values0 = keys0 + L::kK * L::kTile, p0 = values0 + L::kV * L::kTile, q0 = p0 + 4 * L::kP;
+  // keys, values, weights [kBufs][halves][128 keys][NP], queries [kBufs][D / 64][NP][64]
+  const uint32_t keys0 = (smem_u32(tc_smem_raw) + 1023u) & ~1023u, values0 = keys0 + L::kK * L::kTile, p0 = values0 + L::kV * L::kTile, q0 = p0 + L::kBufs * 2 * L::kP;
+  constexpr int kB = L::kBufs;
   const int item_rows = tpi * a.group;
   if (tid == 0) {
     for (int i = 0; i < 2; ++i)
@@ -546,8 +549,8 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
     while (p.b < end && ok) {
       enter(p);
       if (p.i == 0) {
-        const int qb = p.sg & 1;
-        if (p.sg >= 2) ok = all_wait(&bars.q_free[qb], (uint32_t)((p.sg >> 1) - 1) & 1u);
+        const int qb = p.sg % kB;
+        if (p.sg >= kB) ok = all_wait(&bars.q_free[qb], (uint32_t)(p.sg / kB - 1) & 1u);
         if (!ok) break;
         if (lane == 0) {
           mbar_arrive_expect_tx(&bars.q_full[qb], (uint32_t)(item_rows * D * 2));
@@ -555,13 +558,18 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
         }
         __syncwarp();
       }
-      // lane i: page of piece i, a.pages (zeros) where nothing of it is seen
-      const int key = block_key<kTcKeys>(p.g.all, p.g.blk0 + p.i) + lane * piece, place = key / a.page, inside = key - place * a.page;
-      int page = a.pages;
-      if (lane < pieces && key <= p.g.all.last && (key + piece > p.g.all.lo || key < p.g.all.head)) {
-        const int q = paged_page(a, p.g.seq, place);
-        if (q >= 0) page = q;
-      }
+      // lane l: row inside its page and page of piece l of the share's block i, a.pages (zeros) where nothing of it is seen
+      auto piece_of = [&](int i) {
+        const int key = block_key<kTcKeys>(p.g.all, p.g.blk0 + i) + lane * piece, place = key / a.page;
+        int page = a.pages;
+        if (i < p.g.n && lane < pieces && key <= p.g.all.last && (key + piece > p.g.all.lo || key < p.g.all.head)) {
+          const int q = paged_page(a, p.g.seq, place);
+          if (q >= 0) page = q;
+        }
+        return make_int2(key - place * a.page, page);
+      };
+      const int2 there = piece_of(p.i);
+      const int inside = there.x, page = there.y;
       auto copy = [&](const CUtensorMap* map, uint32_t block, uint64_t* full) {
         if (lane == 0) mbar_arrive_expect_tx(full, L::kTile);
         __syncwarp();
@@ -584,7 +592,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
     if (!ok) {  // nothing in flight when the CTA leaves
       for (int i = max(0, kr.count - L::kK); i < kr.count; ++i) mbar_wait_bounded(&bars.k_full[i % L::kK], (uint32_t)(i / L::kK) & 1u);
       for (int i = max(0, vr.count - L::kV); i < vr.count; ++i) mbar_wait_bounded(&bars.v_full[i % L::kV], (uint32_t)(i / L::kV) & 1u);
-      for (int i = max(0, p.sg - 1); i <= p.sg; ++i) mbar_wait_bounded(&bars.q_full[i & 1], (uint32_t)(i >> 1) & 1u);
+      for (int i = max(0, p.sg + 1 - kB); i <= p.sg; ++i) mbar_wait_bounded(&bars.q_full[i % kB], (uint32_t)(i / kB) & 1u);
     }
   } else if (warp == 5) {
     // ------------------------------------------------------------ MMA issue
@@ -596,18 +604,18 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
     auto scores = [&]() {  // of block kr.count
       if (ps.b >= end || !ok) return;
       enter(ps);
-      if (ps.i == 0) ok = all_wait(&bars.q_full[ps.sg & 1], (uint32_t)(ps.sg >> 1) & 1u);
+      if (ps.i == 0) ok = all_wait(&bars.q_full[ps.sg % kB], (uint32_t)(ps.sg / kB) & 1u);
       ok = ok && all_wait(&bars.k_full[kr.slot], kr.pass);
       if (!ok) return;
       tc_fence_after();
       if (issuer) {
-        const uint64_t k = tc_desc(keys0 + kr.slot * L::kTile, 16), q = tc_desc(q0 + (ps.sg & 1) * L::kQ, 16);
+        const uint64_t k = tc_desc(keys0 + kr.slot * L::kTile, 16), q = tc_desc(q0 + ps.sg % kB * L::kQ, 16);
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks)
           tc_mma_f16(tmem + (kr.count & 1) * NP, k + (uint64_t)((ks / 4) * 1024 + (ks % 4) * 2), q + (uint64_t)((ks / 4) * NP * 8 + (ks % 4) * 2), idesc_s, ks > 0);
         tc_commit(&bars.s_full[kr.count & 1]);
         tc_commit(&bars.k_free[kr.slot]);
-        if (ps.i == ps.g.n - 1) tc_commit(&bars.q_free[ps.sg & 1]);
+        if (ps.i == ps.g.n - 1) tc_commit(&bars.q_free[ps.sg % kB]);
       }
       __syncwarp();
       kr.next(L::kK);
@@ -626,11 +634,11 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
       if (issuer) {
         constexpr uint32_t kStep = NP * 2 * 16 / 16;  // 16 keys of weights, in 16 bytes
         const uint64_t v = tc_desc(values0 + vr.slot * L::kTile, 16384);
-        const uint64_t hi = (uint64_t)(((p0 + (r & 1) * 2 * L::kP) >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(NP * 16 >> 4) << 32) | (1ull << 46) | (L::kSwizzle << 61);
+        const uint64_t hi = (uint64_t)(((p0 + r % kB * 2 * L::kP) >> 4) & 0x3FFFu) | (1ull << 16) | ((uint64_t)(NP * 16 >> 4) << 32) | (1ull << 46) | (L::kSwizzle << 61);
 #pragma unroll
         for (int ks = 0; ks < kTcKeys / 8; ++ks)  // the upper halves, then the lower
           tc_mma_f16(tmem + 2 * NP, v + (uint64_t)((ks & 7) * 128), hi + (uint64_t)((ks & 7) * kStep + (ks >> 3) * (L::kP >> 4)), idesc_o, p.i > 0 || ks > 0);
-        tc_commit(&bars.p_free[r & 1]);
+        tc_commit(&bars.p_free[r % kB]);
         tc_commit(&bars.v_free[vr.slot]);
       }
       __syncwarp();
@@ -696,7 +704,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
 #pragma unroll
         for (int c = 0; c < NP; ++c) l[c] = 0.0f;
         sync();  // (the last share's numbers have been read)
-        if (tid < NP) s_ref[tid] = tid < rows ? -INFINITY : INFINITY;  // (columns without a row: weights of 0)
+        if (tid < NP) s_ref[tid] = tid < rows ? -INFINITY : INFINITY, s_base2[tid] = tid < rows ? 0.0f : -INFINITY;  // (columns without a row: weights of 0)
         sync();
       }
       ok = ok && all_wait(&bars.s_full[r & 1], (uint32_t)(r >> 1) & 1u);
@@ -723,7 +731,11 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
       for (int c0 = 0; c0 < NP; c0 += kC) {
         load(c0);
 #pragma unroll
-        for (int i = 0; i < kC; ++i) over = over || fmaf(__uint_as_float(v[i]), scale, -8.0f) > s_ref[c0 + i];
+        for (int i = 0; i < kC; i += 4) {
+          const float4 ref = *reinterpret_cast<const float4*>(s_ref + c0 + i);
+          over |= fmaf(__uint_as_float(v[i]), scale, -8.0f) > ref.x | fmaf(__uint_as_float(v[i + 1]), scale, -8.0f) > ref.y |
+                  fmaf(__uint_as_float(v[i + 2]), scale, -8.0f) > ref.z | fmaf(__uint_as_float(v[i + 3]), scale, -8.0f) > ref.w;
+        }
       }
       if (any(over)) {  // some row's maximum has outgrown its reference (always in an item's first block, unless nothing is seen)
 #pragma unroll
@@ -742,6 +754,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
           const float old = s_ref[tid], top = fmaxf(fmaxf(s_max[0][tid], s_max[1][tid]), fmaxf(s_max[2][tid], s_max[3][tid])) * scale, now = fmaxf(old, top);
           s_alpha[tid] = now == -INFINITY ? 1.0f : exp2f(old - now);
           s_ref[tid] = now;
+          s_base2[tid] = now == -INFINITY ? 0.0f : -now;
         } else if (tid < NP) {
           s_alpha[tid] = 1.0f;
         }
@@ -749,7 +762,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
 #pragma unroll
         for (int c = 0; c < NP; ++c) l[c] *= s_alpha[c];
         if (p.i > 0) {  // behind the products of the block before
-          ok = ok && all_wait(&bars.p_free[(r - 1) & 1], (uint32_t)((r - 1) >> 1) & 1u);
+          ok = ok && all_wait(&bars.p_free[(r - 1) % kB], (uint32_t)((r - 1) / kB) & 1u);
           tc_fence_after();
 #pragma unroll
           for (int c0 = 0; c0 < NP; c0 += 16) {
@@ -763,8 +776,8 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
           tmem_st_wait();
         }
       }
-      if (r >= 2) ok = ok && all_wait(&bars.p_free[r & 1], (uint32_t)((r >> 1) - 1) & 1u);  // the products of two blocks before: their weights' place
-      const uint32_t row = p0 + (r & 1) * 2 * L::kP + tid * NP * 2;
+      if (r >= kB) ok = ok && all_wait(&bars.p_free[r % kB], (uint32_t)(r / kB - 1) & 1u);  // the products that read these weights' place
+      const uint32_t row = p0 + r % kB * 2 * L::kP + tid * NP * 2;
 #pragma unroll
       for (int c0 = 0; c0 < NP; c0 += kC) {
         if (NP > kC) load(c0);
@@ -774,8 +787,8 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int k = c + 2 * i;
-            const float r0 = s_ref[c0 + k], r1 = s_ref[c0 + k + 1];
-            const float w0 = paged_exp2(fmaf(__uint_as_float(v[k]), scale, r0 == -INFINITY ? 0.0f : -r0)), w1 = paged_exp2(fmaf(__uint_as_float(v[k + 1]), scale, r1 == -INFINITY ? 0.0f : -r1));
+            const float2 base = *reinterpret_cast<const float2*>(s_base2 + c0 + k);
+            const float w0 = paged_exp2(fmaf(__uint_as_float(v[k]), scale, base.x)), w1 = paged_exp2(fmaf(__uint_as_float(v[k + 1]), scale, base.y));
             l[c0 + k] += w0, l[c0 + k + 1] += w1;
             hi[i] = Num<T>::pack(w0, w1);
             const float2 h = Num<T>::unpack(hi[i]);
@@ -808,7 +821,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
           s_alpha[tid] = !g.whole ? f : g.p_first + tok < 0 ? 0.0f : f / sum;
           if (!g.whole) w.part_ml[slot + tid] = make_float2(most, sum);
         }
-        ok = ok && all_wait(&bars.p_free[r & 1], (uint32_t)(r >> 1) & 1u);
+        ok = ok && all_wait(&bars.p_free[r % kB], (uint32_t)(r / kB) & 1u);
         tc_fence_after();
         sync();
         if (tid < D && ok) {
