@@ -60,46 +60,50 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]
       : "memory");
 }
 
-// One row's scores of a block (128 columns of tensor memory in registers): bias and mask.  first, last: positions of the rows that
-// are worked on together.
+__device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
+
+// One row's scores of a block in tensor memory: bias and mask (written back) and the largest.  first, last: positions of the rows that
+// are worked on together.  Loops over columns are short on purpose: a launch starts with a cold instruction cache.
 template <bool BIAS>
-__device__ __forceinline__ void weigh_block(const Paged& a, uint32_t (&v)[4][32], const float* bias, int pos, int first, int last, int j0) {
-  if (BIAS) {
-    const float far = bias ? bias[a.bias_max] * kPagedLog2e : 0.0f;
-    const bool near = first - (j0 + kTcKeys - 1) < a.bias_max;  // some distance has a bias of its own
+__device__ __forceinline__ float weigh_block(const Paged& a, uint32_t s_col, const float* bias, int pos, int first, int last, int j0) {
+  const bool masked = first < 0 || !seen_by_all(a, first, last, j0, j0 + kTcKeys - 1);
+  const int hi = pos - j0, lo = a.window ? hi - a.window : -1, kp = a.window ? a.keep - j0 : 0;  // column i: i <= hi and (i > lo or i < kp)
+  const bool near = BIAS && first - (j0 + kTcKeys - 1) < a.bias_max;                               // some distance has a bias of its own
+  const float far = BIAS && bias ? bias[a.bias_max] * kPagedLog2e : 0.0f;
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 128; c += 64) {
+    uint32_t v[2][32];
+    tmem_ld32(s_col + c, v[0]);
+    tmem_ld32(s_col + c + 32, v[1]);
+    tmem_ld_wait();
+    if (BIAS || masked) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const float b = near && bias ? __ldg(bias + max(0, min(pos - (j0 + c * 32 + i), a.bias_max))) * kPagedLog2e : far;
-        v[c][i] = __float_as_uint(fmaf(__uint_as_float(v[c][i]), a.scale2, b));
+      for (int i = 0; i < 64; ++i) {
+        uint32_t& x = v[i >> 5][i & 31];
+        if (BIAS) {
+          const float b = near && bias ? __ldg(bias + max(0, min(hi - c - i, a.bias_max))) * kPagedLog2e : far;
+          x = __float_as_uint(fmaf(__uint_as_float(x), a.scale2, b));
+        }
+        if (masked && !(c + i <= hi && (c + i > lo || c + i < kp))) x = 0xff800000u;
       }
+      tmem_st32(s_col + c, v[0]);
+      tmem_st32(s_col + c + 32, v[1]);
+    }
+    float mx[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mx[i] = fmaxf(__uint_as_float(v[0][i]), __uint_as_float(v[1][i]));
+#pragma unroll
+    for (int i = 4; i < 32; ++i) mx[i & 3] = fmaxf(fmaxf(mx[i & 3], __uint_as_float(v[0][i])), __uint_as_float(v[1][i]));
+    top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
   }
-  if (first < 0 || !seen_by_all(a, first, last, j0, j0 + kTcKeys - 1)) {
-    const int hi = pos - j0, lo = a.window ? hi - a.window : -1, kp = a.window ? a.keep - j0 : 0;  // column i: i <= hi and (i > lo or i < kp)
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const int col = c * 32 + i;
-        if (!(col <= hi && (col > lo || col < kp))) v[c][i] = 0xff800000u;
-      }
-  }
-}
-__device__ __forceinline__ float row_top(const uint32_t (&v)[4][32]) {
-  float mx[4];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    mx[c] = __uint_as_float(v[c][0]);
-#pragma unroll
-    for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(v[c][i]));
-  }
-  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+  if (BIAS || masked) tmem_st_wait();
+  return top;
 }
 // O of the row times alpha, in tensor memory
 template <int D>
 __device__ __forceinline__ void rescale(uint32_t o_col, float alpha) {
-#pragma unroll
+#pragma unroll 1
   for (int c = 0; c < D / 32; ++c) {
     uint32_t o[32];
     tmem_ld32(o_col + c * 32, o);
@@ -111,18 +115,24 @@ __device__ __forceinline__ void rescale(uint32_t o_col, float alpha) {
 }
 // weights 2^(score scale + base) in 16 bits over the scores' columns; their sum
 template <class T>
-__device__ __forceinline__ float put_weights(const uint32_t (&v)[4][32], uint32_t s_col, float scale, float base) {
+__device__ __forceinline__ float put_weights(uint32_t s_col, float scale, float base) {
   float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+  for (int c = 0; c < 128; c += 64) {
+    uint32_t v[2][32], w[2][16];
+    tmem_ld32(s_col + c, v[0]);
+    tmem_ld32(s_col + c + 32, v[1]);
+    tmem_ld_wait();
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    uint32_t w[16];
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float p0 = paged_exp2(fmaf(__uint_as_float(v[c][2 * i]), scale, base)), p1 = paged_exp2(fmaf(__uint_as_float(v[c][2 * i + 1]), scale, base));
-      sum[i & 3] += p0 + p1;
-      w[i] = Num<T>::pack(p0, p1);
+      for (int i = 0; i < 16; ++i) {
+        const float p0 = paged_exp2(fmaf(__uint_as_float(v[h][2 * i]), scale, base)), p1 = paged_exp2(fmaf(__uint_as_float(v[h][2 * i + 1]), scale, base));
+        sum[i & 3] += p0 + p1;
+        w[h][i] = Num<T>::pack(p0, p1);
+      }
+      tmem_st16(s_col + c / 2 + h * 16, w[h]);
     }
-    tmem_st16(s_col + c * 16, w);
   }
   return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
@@ -142,6 +152,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
   __shared__ volatile int s_bad, s_gave_up;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const uint32_t smem0 = (smem_u32(tc_smem_raw) + 1023u) & ~1023u, keys0 = smem0 + 2 * L::kTile, values0 = keys0 + L::kK * L::kTile;
+  if (tid < 3) tma_prefetch_map(tid == 0 ? &qmap : tid == 1 ? &kmap : &vmap);
   pdl_launch_dependents();
   pdl_wait_prior();
   const int toks = 128 / a.group, kvh = blockIdx.x % a.kv_heads;
@@ -174,6 +185,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
     return pos0 < 0 || !seen_by_all(a, pos0, p_last, j0, j0 + kTcKeys - 1);
   };
   auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity)) return true;
     if (s_gave_up) return false;
     if (mbar_wait_bounded(bar, parity)) return true;
     s_gave_up = 1;
@@ -181,7 +193,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
   };
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == 8) {
       // ---------------------------------------------------------- copies
       if (nt) {
@@ -259,11 +270,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
           for (int t = 0; t < tiles; ++t) scores(t, 0, t == tiles - 1);
         }
         for (int j = 0; j < nt && ok; ++j) {
+          // (what is there long before the weights is waited for before them)
+          ok = all_wait(&bars.v_full[j % L::kV], turn(j, L::kV)) && all_wait(&bars.v_fixed[j % L::kV], turn(j, L::kV));
+          if (ok && j + 1 < nt) ok = all_wait(&bars.k_full[(j + 1) % L::kK], turn(j + 1, L::kK));
           for (int t = 0; t < tiles && ok; ++t) {
             ok = all_wait(&bars.p_ready[t], (uint32_t)j & 1u);
-            if (t == 0 && ok) {
-              ok = all_wait(&bars.v_full[j % L::kV], turn(j, L::kV)) && all_wait(&bars.v_fixed[j % L::kV], turn(j, L::kV));
-            }
             if (!ok) break;
             tc_fence_after();
             if (issuer) {
@@ -275,13 +286,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
               if (j == nt - 1) tc_commit(&bars.o_done[t]);
             }
             __syncwarp();
-            if (j + 1 < nt) {
-              if (t == 0) ok = all_wait(&bars.k_full[(j + 1) % L::kK], turn(j + 1, L::kK));
-              if (ok) {
-                tc_fence_after();
-                scores(t, j + 1, t == tiles - 1);
-              }
-            }
+            if (j + 1 < nt) scores(t, j + 1, t == tiles - 1);
           }
         }
       }
@@ -298,7 +303,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
           const bool some = seen_by_some(seen, j0 + r);
           if (some && pos0 >= 0 && seen_by_all(a, pos0, p_last, j0 + r, j0 + r)) continue;
           for (int c = 0; c < D / 8; ++c) {
-            const uint32_t at = block + (c / 8) * 16384 + r * 128 + (c % 8) * 16;  // (any order: every piece of the row is visited)
+            const uint32_t at = block + (c / 8) * 16384 + r * 128 + (((c % 8) ^ (r & 7)) * 16);
             if (some) {
               uint4 x;
               asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory");
@@ -324,7 +329,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
   }
 
   // ------------------------------------------------------------ weights: one row per thread
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
   {
     const int t = warp >> 2, r = tid & 127, tok = r / a.group, hg = r - tok * a.group, head = kvh * a.group + hg;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_col = tmem + t * 128 + lanes, o_col = tmem + 256 + t * D + lanes;
@@ -340,12 +344,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
     for (int j = 0; j < n; ++j) {
       ok = ok && __all_sync(0xffffffffu, wait(&bars.s_full[t], (uint32_t)j & 1u));
       tc_fence_after();
-      uint32_t v[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(s_col + c * 32, v[c]);
-      tmem_ld_wait();
-      weigh_block<BIAS>(a, v, bias, pos, first, last, block_key<kTcKeys>(seen, j));
-      const float top = row_top(v);
+      const float top = weigh_block<BIAS>(a, s_col, bias, pos, first, last, block_key<kTcKeys>(seen, j));
       if (__any_sync(0xffffffffu, live && top > m + grown)) {
         const float m_new = fmaxf(m, top), alpha = m_new == -INFINITY ? 1.0f : paged_exp2((m - m_new) * scale);
         m = m_new;
@@ -354,7 +353,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
           rescale<D>(o_col, alpha);
         }
       }
-      l += put_weights<T>(v, s_col, scale, m == -INFINITY ? 0.0f : -m * scale);
+      l += put_weights<T>(s_col, scale, m == -INFINITY ? 0.0f : -m * scale);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -501,6 +500,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
     tmem_alloc(&s_tmem, L::kColumns);
     tmem_relinquish();
   }
+  if (tid < 3) tma_prefetch_map(tid == 0 ? &qmap : tid == 1 ? &kmap : &vmap);
   pdl_launch_dependents();
   pdl_wait_prior();
   sum_blocks<kTcKeys, kDecThreads>(a, s_base);
