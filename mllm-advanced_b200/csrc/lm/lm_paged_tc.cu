@@ -113,10 +113,57 @@ __device__ __forceinline__ void rescale(uint32_t o_col, float alpha) {
     tmem_st32(o_col + c * 32, o);
   }
 }
-// weights 2^(score scale + base) in 16 bits over the scores' columns; their sum
+// Two fp32 numbers in a register pair: one instruction for both.
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 pair_parts(uint64_t p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x of two numbers up to 127 without the special-function unit, 2^-18 of the result off at most: x = n + f with n whole (the addition
+// leaves n + 127 in the low bits of its sum) and |f| <= 1/2; a polynomial of degree 4 for 2^f (least largest relative error, fitted by
+// reweighted least squares) times the number whose exponent is n.  Below 2^-126, 0; NaN stays NaN.
+__device__ __forceinline__ float2 pair_exp2(uint64_t x) {
+  float2 v = pair_parts(x);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(-127.0f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(-127.0f));
+  x = pair_of(v.x, v.y);
+  const uint64_t t = pair_add(x, pair_of(12583039.0f, 12583039.0f));  // 1.5 2^23 + 127
+  const uint64_t f = pair_add(x, pair_mul(pair_add(t, pair_of(-12583039.0f, -12583039.0f)), pair_of(-1.0f, -1.0f)));
+  uint64_t p = pair_fma(f, pair_of(0.009570102207362652f, 0.009570102207362652f), pair_of(0.05591785907745361f, 0.05591785907745361f));
+  p = pair_fma(p, f, pair_of(0.240247443318367f, 0.240247443318367f));
+  p = pair_fma(p, f, pair_of(0.6931217908859253f, 0.6931217908859253f));
+  p = pair_fma(p, f, pair_of(0.9999992847442627f, 0.9999992847442627f));
+  const float2 n = pair_parts(t);
+  return pair_parts(pair_mul(p, pair_of(__uint_as_float(__float_as_uint(n.x) << 23), __uint_as_float(__float_as_uint(n.y) << 23))));
+}
+
+// weights 2^(score scale + base) in 16 bits over the scores' columns; their sum.  The special-function unit takes 1024 cycles for a
+// tile's exponentials, as long as both products; every kPoly-th pair goes through the other pipes instead.
+constexpr int kPoly = 4;
 template <class T>
 __device__ __forceinline__ float put_weights(uint32_t s_col, float scale, float base) {
-  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const uint64_t scale2 = pair_of(scale, scale), base2 = pair_of(base, base);
+  uint64_t sum[2] = {0, 0};
 #pragma unroll 1
   for (int c = 0; c < 128; c += 64) {
     uint32_t v[2][32], w[2][16];
@@ -127,14 +174,22 @@ __device__ __forceinline__ float put_weights(uint32_t s_col, float scale, float 
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float p0 = paged_exp2(fmaf(__uint_as_float(v[h][2 * i]), scale, base)), p1 = paged_exp2(fmaf(__uint_as_float(v[h][2 * i + 1]), scale, base));
-        sum[i & 3] += p0 + p1;
-        w[h][i] = Num<T>::pack(p0, p1);
+        const uint64_t x = pair_fma(pair_of(__uint_as_float(v[h][2 * i]), __uint_as_float(v[h][2 * i + 1])), scale2, base2);
+        float2 e;
+        if (i % kPoly == kPoly - 1) {
+          e = pair_exp2(x);
+        } else {
+          const float2 y = pair_parts(x);
+          e = make_float2(paged_exp2(y.x), paged_exp2(y.y));
+        }
+        sum[i & 1] = pair_add(sum[i & 1], pair_of(e.x, e.y));
+        w[h][i] = Num<T>::pack(e.x, e.y);
       }
       tmem_st16(s_col + c / 2 + h * 16, w[h]);
     }
   }
-  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  const float2 total = pair_parts(pair_add(sum[0], sum[1]));
+  return total.x + total.y;
 }
 
 struct TcBarriers {
