@@ -72,15 +72,16 @@ template <bool VEC>
 __device__ __forceinline__ int element(int i, int e) { return VEC ? i + e : i + e * kRowThreads; }
 
 // ------------------------------------------------------------------------------------------ probabilities
-// grid (cluster, rows): every CTA reads its part of the row once, all loads in flight, and keeps it in registers; weights are taken
-// against the part's own maximum, so that one exchange in the cluster (maximum, sum) settles the row.  Bound by memory: 8
-// bytes a number.  384 rows of 151936: 452 us with three passes of scalar loads over the row.
+// grid (cluster, rows): every CTA reads its part of the row once, all loads in flight, and keeps it in registers.  A thread takes its
+// weights against its own maximum; the warps' maxima and sums go to every CTA of the cluster, so that one barrier settles the
+// row.  Bound by memory, 8 bytes a number, and by what a CTA does between its loads and its stores (two of them share an SM).  384
+// rows of 151936: 452 us with three passes of scalar loads over the row, 115 with four barriers and exact exponentials.
 template <class T, int ITEMS, bool VEC>
 __global__ void __launch_bounds__(kRowThreads, 2) lm_probability_rows_kernel(const T* __restrict__ logits, long long ld, int vocab, int per, float inv_t, bool greedy,
                                                                           float* __restrict__ out, long long ld_out) {
-  __shared__ float s_red[kRowWarps], s_max, s_sum;
-  __shared__ int s_at[kRowWarps], s_first;
+  __shared__ float2 s_pairs[8 * kRowWarps];  // {maximum, sum or place} of every warp of the cluster
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, ctas = gridDim.x, part = blockIdx.x;
+  cluster_arrive_relaxed();
   pdl_launch_dependents();
   pdl_wait_prior();
   const T* z = logits + blockIdx.y * ld;
@@ -94,75 +95,66 @@ __global__ void __launch_bounds__(kRowThreads, 2) lm_probability_rows_kernel(con
   for (int k = 0; k < ITEMS; ++k)
 #pragma unroll
     for (int e = 0; e < 4; ++e) odd = odd || !(x[k][e] < INFINITY), mx = fmaxf(mx, x[k][e]);
+  const float t2 = fminf(inv_t * kPagedLog2e, 3.402823466e+38f), base = mx > -INFINITY ? mx : 0.0f;
+  float top = mx, second = 0.0f;  // of the warp
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  if (lane == 0) s_red[warp] = mx;
-  odd = __syncthreads_or(odd);
-#pragma unroll
-  for (int w = 0; w < kRowWarps; ++w) mx = fmaxf(mx, s_red[w]);
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (greedy) {
     int at = 0x7fffffff;
 #pragma unroll
-    for (int k = ITEMS - 1; k >= 0; --k)
-#pragma unroll
-      for (int e = 3; e >= 0; --e)
-        if (x[k][e] == mx && mx > -INFINITY) at = min(at, element<VEC>(item_at<VEC>(v0, k, tid), e));
-    at = __reduce_min_sync(0xffffffffu, at);
-    if (lane == 0) s_at[warp] = at;
-    __syncthreads();
-    if (tid == 0) {
-      for (int w = 0; w < kRowWarps; ++w) at = min(at, s_at[w]);
-      s_first = at, s_max = mx;
-    }
-    cluster_sync_all();
-    float best = -INFINITY;
-    for (int r = 0; r < ctas; ++r) {
-      const float m = ld_remote(&s_max, r);
-      if (m > best) best = m, at = ld_remote(&s_first, r);  // (parts in order: the first of equals stays)
-    }
-    if (!(best > -INFINITY)) at = -1;
-#pragma unroll
     for (int k = 0; k < ITEMS; ++k)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[k][e] = element<VEC>(item_at<VEC>(v0, k, tid), e) == at ? 1.0f : 0.0f;
+      for (int e = 0; e < 4; ++e)
+        if (x[k][e] == top) at = min(at, element<VEC>(item_at<VEC>(v0, k, tid), e));
+    second = __int_as_float((int)__reduce_min_sync(0xffffffffu, (unsigned)at));
   } else {
-    const float base = mx > -INFINITY ? mx : 0.0f;
     float sum = 0.0f;
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[k][e] = expf((x[k][e] - base) * inv_t);
+        x[k][e] = paged_exp2((x[k][e] - base) * t2);
         sum += x[k][e];
       }
+    sum = odd ? __int_as_float(0x7fffffff) : sum * paged_exp2((base - (top > -INFINITY ? top : 0.0f)) * t2);  // (a NaN here is one everywhere)
+    if (mx == -INFINITY && !odd) sum = 0.0f;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    __syncthreads();
-    if (lane == 0) s_red[warp] = sum;
-    __syncthreads();
-    if (tid == 0) {
-      sum = 0.0f;
-      for (int w = 0; w < kRowWarps; ++w) sum += s_red[w];
-      s_max = mx, s_sum = odd ? __int_as_float(0x7fffffff) : sum;  // (a NaN here is one everywhere)
-    }
-    cluster_sync_all();
-    float m_r[8], s_r[8], top = -INFINITY, total = 0.0f;
+    second = sum;
+  }
+  cluster_wait();  // every CTA has begun
+  if (lane < ctas) {
+    const uint32_t to = map_to_cta(s_pairs + part * kRowWarps + warp, lane);
+    st_cluster_f32(to, top);
+    st_cluster_f32(to + 4, second);
+  }
+  cluster_sync_all();
+  const int n = ctas * kRowWarps;
+  float best = -INFINITY;
+  for (int i = lane; i < n; i += 32) best = fmaxf(best, s_pairs[i].x);
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      m_r[r] = r < ctas ? ld_remote(&s_max, r) : -INFINITY;
-      s_r[r] = r < ctas ? ld_remote(&s_sum, r) : 0.0f;
-      top = fmaxf(top, m_r[r]);
-    }
-    const float at = top > -INFINITY ? top : 0.0f;
-#pragma unroll
-    for (int r = 0; r < 8; ++r) total += expf((m_r[r] - at) * inv_t) * s_r[r];
-    const float f = total == 0.0f ? 0.0f : expf((base - at) * inv_t) / total;  // (0: nothing but -inf)
+  for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+  if (greedy) {
+    int at = 0x7fffffff;
+    for (int i = lane; i < n; i += 32)
+      if (s_pairs[i].x == best && best > -INFINITY) at = min(at, __float_as_int(s_pairs[i].y));
+    at = (int)__reduce_min_sync(0xffffffffu, (unsigned)at);
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[k][e] *= f;
+      for (int e = 0; e < 4; ++e) x[k][e] = element<VEC>(item_at<VEC>(v0, k, tid), e) == at ? 1.0f : 0.0f;
+  } else {
+    const float at = best > -INFINITY ? best : 0.0f;
+    float total = 0.0f;
+    for (int i = lane; i < n; i += 32) total += s_pairs[i].y == 0.0f ? 0.0f : s_pairs[i].y * paged_exp2((s_pairs[i].x - at) * t2);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const float f = total == 0.0f ? 0.0f : paged_exp2((base - at) * t2) / total;  // (0: nothing but -inf)
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[k][e] = mx == -INFINITY && !odd && total == total ? 0.0f : x[k][e] * f;
   }
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA has read the others
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
     const int i = item_at<VEC>(v0, k, tid);
@@ -174,7 +166,6 @@ __global__ void __launch_bounds__(kRowThreads, 2) lm_probability_rows_kernel(con
         if (element<VEC>(i, e) < v1) y[element<VEC>(i, e)] = x[k][e];
     }
   }
-  cluster_wait();
 }
 
 // Longer rows: three passes.
@@ -524,7 +515,7 @@ int mllmb200_lm_verify(const float* target, long long t_seq, long long t_row, co
       smem = (size_t)((per + kRowThreads * 4 - 1) / (kRowThreads * 4)) * kRowWarps * (vec ? 1 : 4) * sizeof(double);
     };
     size();
-    while (ctas < 8 && (smem > 40 * 1024 || ((long long)b.seqs * ctas <= 2 * kSms && vocab > ctas * kRowThreads * 4))) ctas *= 2, size();
+    while (ctas < 8 && (smem > 40 * 1024 || ((long long)b.seqs * ctas * 2 <= 2 * kSms && vocab > ctas * kRowThreads * 4))) ctas *= 2, size();  // (all at once)
     auto go = [&](auto kernel) { return launch_pdl_cluster(kernel, dim3(ctas, b.seqs), dim3(kRowThreads), dim3(ctas, 1, 1), smem, st, b, per); };
     const cudaError_t r = vec ? go(lm_verify_kernel<true>) : go(lm_verify_kernel<false>);
     if (r != cudaSuccess) return MLLMB200_CUDA_ERROR;

@@ -39,23 +39,26 @@ def verify(target, draft, tokens, accept, pick, stream=None):
 
     Returns accepted (int32 [sequences]) and the new tokens (int32 [sequences, drafts + 1]): the accepted ones, the next
     one, -1 behind it."""
-    if target.dim() != 3 or draft.dim() != 3 or tokens.dim() != 2 or accept.dim() != 2:
+    try:
+        seqs, places, vocab = target.shape
+        d_seq, d_row, d_one = draft.stride()
+        tokens_seq, tokens_one = tokens.stride()
+        accept_seq, accept_one = accept.stride()
+    except ValueError:
         _refuse("verify", (lambda: False, "probabilities [sequences, places, vocab], tokens and random numbers [sequences, drafts]"))
-    seqs, places, vocab = target.shape
     k, device = places - 1, target.get_device()
     t_seq, t_row, t_one = target.stride()
-    d_seq, d_row, d_one = draft.stride()
     if not (k >= 0 and draft.shape == (seqs, k, vocab) and tokens.shape == (seqs, k) and accept.shape == (seqs, k) and pick.shape == (seqs,) and
             target.dtype == draft.dtype == accept.dtype == pick.dtype == torch.float32 and tokens.dtype == torch.int32 and t_one == 1 and (k == 0 or d_one == 1) and
-            (k < 2 or (tokens.stride(1) == 1 and accept.stride(1) == 1)) and (seqs < 2 or pick.stride(0) == 1) and device >= 0 and
+            (k < 2 or (tokens_one == 1 and accept_one == 1)) and (seqs < 2 or pick.stride(0) == 1) and device >= 0 and
             draft.get_device() == tokens.get_device() == accept.get_device() == pick.get_device() == device):
         _refuse("verify", (lambda: k >= 0 and draft.shape == (seqs, k, vocab) and tokens.shape == accept.shape == (seqs, k) and pick.shape == (seqs,), "one place more in the target's probabilities than drafts"),
                 (lambda: target.dtype == draft.dtype == accept.dtype == pick.dtype == torch.float32 and tokens.dtype == torch.int32, "tokens in int32, all else in fp32"),
                 (lambda: device >= 0 and all(t.get_device() == device for t in (draft, tokens, accept, pick)), "tensors on one GPU"), (lambda: False, "rows are contiguous"))
 
     def call(s):
-        accepted, out = tokens.new_empty((seqs,)), tokens.new_empty((seqs, places))
-        st = lm.lib().mllmb200_lm_verify(target.data_ptr(), t_seq, t_row, draft.data_ptr(), d_seq, d_row, tokens.data_ptr(), tokens.stride(0), accept.data_ptr(), accept.stride(0),
+        accepted, out = torch.empty_like(pick, dtype=torch.int32), tokens.new_empty((seqs, places))
+        st = lm.lib().mllmb200_lm_verify(target.data_ptr(), t_seq, t_row, draft.data_ptr(), d_seq, d_row, tokens.data_ptr(), tokens_seq, accept.data_ptr(), accept_seq,
                                          pick.data_ptr(), seqs, k, vocab, accepted.data_ptr(), out.data_ptr(), places, s)
         return st, (accepted, out)
     st, o = _on(device, stream, call)

@@ -16,7 +16,7 @@ import struct
 import torch
 
 from . import lm
-from .binding import scratch
+from .binding import _allocator
 
 _PAGES = struct.Struct("@PP6q3P10i")
 _LOOK = struct.Struct("@PP4qPP4if4x")
@@ -52,25 +52,29 @@ def _on(index, stream, call):
 
 
 def _pages(where, k, v, table, lengths, q_start, rows):
+    """(the call's mllmb200_lm_pages as bytes, sequences, kv heads, size of a key, of a value)"""
     dtype, device = _DTYPES.get(k.dtype), k.get_device()
-    if k.dim() != 4 or v.dim() != 4 or table.dim() != 2 or lengths.dim() != 1:
+    try:
+        pages, heads, page, dim = k.shape
+        v_pages, v_heads, v_rows, vdim = v.shape
+        seqs, width = table.shape
+        n_lengths, = lengths.shape
+    except ValueError:
         _refuse(where, (lambda: k.dim() == v.dim() == 4, "keys and values are [pages, kv_heads, page, size]"), (lambda: False, "table is [sequences, pages], lengths [sequences]"))
-    pages, heads, page, dim = k.shape
-    seqs, width = table.shape
     k_page, k_head, k_row, k_one = k.stride()
     v_page, v_head, v_row, v_one = v.stride()
-    vs = v.shape
-    if not (dtype is not None and v.dtype == k.dtype and vs[0] == pages and vs[1] == heads and vs[2] == page and k_one == 1 and v_one == 1 and
-            table.dtype == _INT and lengths.dtype == _INT and lengths.shape[0] == seqs and (seqs < 2 or lengths.stride(0) == 1) and (width < 2 or table.stride(1) == 1) and
+    ld_table, one = table.stride()
+    if not (dtype is not None and v.dtype == k.dtype and v_pages == pages and v_heads == heads and v_rows == page and k_one == 1 and v_one == 1 and
+            table.dtype == _INT and lengths.dtype == _INT and n_lengths == seqs and (seqs < 2 or lengths.stride(0) == 1) and (width < 2 or one == 1) and
             device >= 0 and v.get_device() == device and table.get_device() == device and lengths.get_device() == device and
             (q_start is None or (q_start.dtype == _INT and q_start.dim() == 1 and q_start.shape[0] == seqs + 1 and q_start.stride(0) == 1 and q_start.get_device() == device))):
-        _refuse(where, (lambda: dtype is not None and v.dtype == k.dtype, "keys and values in bf16 or fp16"), (lambda: vs[:3] == k.shape[:3], "keys and values of the same pages"),
+        _refuse(where, (lambda: dtype is not None and v.dtype == k.dtype, "keys and values in bf16 or fp16"), (lambda: v.shape[:3] == k.shape[:3], "keys and values of the same pages"),
                 (lambda: k_one == v_one == 1, "rows of keys and values are contiguous"), (lambda: table.dtype == lengths.dtype == _INT, "table and lengths in int32"),
-                (lambda: lengths.shape[0] == seqs and (seqs < 2 or lengths.stride(0) == 1) and (width < 2 or table.stride(1) == 1), "a length and a contiguous row of the table per sequence"),
+                (lambda: n_lengths == seqs and (seqs < 2 or lengths.stride(0) == 1) and (width < 2 or one == 1), "a length and a contiguous row of the table per sequence"),
                 (lambda: q_start is None or (q_start.dtype == _INT and q_start.shape == (seqs + 1,) and q_start.is_contiguous()), "q_start [sequences + 1] in int32"),
                 (lambda: False, "tensors on one GPU"))
     return _PAGES.pack(k.data_ptr(), v.data_ptr(), k_page, k_head, k_row, v_page, v_head, v_row, table.data_ptr(), lengths.data_ptr(), 0 if q_start is None else q_start.data_ptr(),
-                       dtype, pages, page, heads, dim, vs[3], table.stride(0), width, seqs, rows)
+                       dtype, pages, page, heads, dim, vdim, ld_table, width, seqs, rows), seqs, heads, dim, vdim
 
 
 def append(k_pages, v_pages, k, v, table, lengths, q_start=None, stream=None):
@@ -80,34 +84,34 @@ def append(k_pages, v_pages, k, v, table, lengths, q_start=None, stream=None):
             k.shape[0] == v.shape[0] and k.shape[1] == v.shape[1] == k_pages.shape[1] and k.shape[2] == k_pages.shape[3] and v.shape[2] == v_pages.shape[3] and k.stride(2) == 1 and v.stride(2) == 1):
         _refuse("append", (lambda: k.dim() == v.dim() == 3 and k.dtype == v.dtype == k_pages.dtype and k.device == v.device == k_pages.device, "new keys and values [rows, kv_heads, size] of the cache's type"),
                 (lambda: k.stride(2) == v.stride(2) == 1, "rows of keys and values are contiguous"), (lambda: False, "sizes of keys and values"))
-    pages = _pages("append", k_pages, v_pages, table, lengths, q_start, k.shape[0])
+    pages = _pages("append", k_pages, v_pages, table, lengths, q_start, k.shape[0])[0]
     st = _on(k.get_device(), stream, lambda s: lm.lib().mllmb200_lm_pages_append(pages, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), s))
     if st:
         _fail("append", st)
 
 
 def _attention(where, q, k_pages, v_pages, table, lengths, q_start, scale, window, keep, sink, bias, out, stream):
-    if q.dim() != 3:
+    try:
+        rows, heads, dim = q.shape
+    except ValueError:
         _refuse(where, (lambda: False, "queries [rows, heads, dim]"))
-    rows, heads, dim = q.shape
     q_row, q_head, q_one = q.stride()
     index = q.get_device()
-    pages = _pages(where, k_pages, v_pages, table, lengths, q_start, rows)
-    kv_heads, vdim = k_pages.shape[1], v_pages.shape[3]
-    if not (q.dtype == k_pages.dtype and index == k_pages.get_device() and q_one == 1 and dim == k_pages.shape[3] and
+    pages, seqs, kv_heads, k_dim, vdim = _pages(where, k_pages, v_pages, table, lengths, q_start, rows)
+    if not (q.dtype == k_pages.dtype and index == k_pages.get_device() and q_one == 1 and dim == k_dim and
             (sink is None or (sink.dtype == _F32 and sink.shape == (heads,) and sink.is_contiguous() and sink.get_device() == index)) and
             (bias is None or (bias.dtype == _F32 and bias.dim() == 2 and bias.shape[0] == heads and bias.shape[1] > 0 and bias.is_contiguous() and bias.get_device() == index)) and
             (out is None or (out.shape == (rows, heads, vdim) and out.dtype == q.dtype and out.get_device() == index and out.stride(2) == 1))):
         _refuse(where, (lambda: q.dtype == k_pages.dtype and index == k_pages.get_device() and q_one == 1, "queries of the cache's type and device, rows contiguous"),
-                (lambda: dim == k_pages.shape[3], "size of queries and keys"), (lambda: sink is None or (sink.dtype == _F32 and sink.shape == (heads,) and sink.is_contiguous() and sink.get_device() == index), "sink [heads] in fp32"),
+                (lambda: dim == k_dim, "size of queries and keys"), (lambda: sink is None or (sink.dtype == _F32 and sink.shape == (heads,) and sink.is_contiguous() and sink.get_device() == index), "sink [heads] in fp32"),
                 (lambda: bias is None or (bias.dtype == _F32 and bias.dim() == 2 and bias.shape[0] == heads and bias.shape[1] > 0 and bias.is_contiguous() and bias.get_device() == index), "bias [heads, distances] in fp32"),
                 (lambda: False, "out [rows, heads, vdim] of the queries' type, rows contiguous"))
     L = lm.lib()
     decode = q_start is None
-    key = (decode, rows, heads, kv_heads, dim, vdim, table.shape)
+    key = (decode, rows, heads, kv_heads, dim, vdim, seqs)
 
     def call(s):
-        o = out if out is not None else q.new_empty((rows, heads, vdim))
+        o = out if out is not None else torch.empty_like(q) if vdim == dim and q.is_contiguous() else q.new_empty((rows, heads, vdim))
         o_row, o_head, _ = o.stride()
         look = _LOOK.pack(q.data_ptr(), o.data_ptr(), q_row, q_head, o_row, o_head, 0 if sink is None else sink.data_ptr(), 0 if bias is None else bias.data_ptr(), heads,
                           0 if bias is None else bias.shape[1] - 1, window, keep, dim ** -0.5 if scale is None else scale)
@@ -123,8 +127,12 @@ def _attention(where, q, k_pages, v_pages, table, lengths, q_start, scale, windo
         run = L.mllmb200_lm_attn_decode if decode else L.mllmb200_lm_attn_prompt
         if not need:
             return run(pages, look, None, s), o
-        with scratch(need, s) as ws:
+        take, give = _allocator()  # memory of the call, on its stream
+        ws = take(need, s)
+        try:
             return run(pages, look, ws, s), o
+        finally:
+            give(ws)
     st, o = _on(index, stream, call)
     if st:
         _fail(where, st)
