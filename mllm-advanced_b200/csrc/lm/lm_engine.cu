@@ -417,6 +417,8 @@ int create(Engine* e, const mllmb200_lm_layer* descs) {
       Paged a{};
       a.dim = L.dimp, a.vdim = L.vdimp, a.group = L.d.heads / L.d.kv_heads, a.tokens = 1, a.seqs = c.max_seqs;
       ws = std::max(ws, paged_decode_bytes(a));
+      // (what a step of prompts takes depends on its rows; no step's CTAs and parts are more than the GPU's SMs)
+      ws = std::max(ws, (size_t)kSms * 256 * (L.vdimp * 4 + 8) + kSms * 4);
     }
     int unbounded = 0;
     for (const LayerState& L : e->layers) {
@@ -933,7 +935,7 @@ int paged_mixer(Engine* e, const StepCtx& t, const LayerState& L, const Weights&
     return r.n > 0;
   };
   if (rows(t.page_single)) LM_CUDA(launch_paged_decode(a, false, e->page_ws, e->stream));
-  if (rows(t.page_prompt)) LM_CUDA(launch_paged_prompt(a, false, e->stream));
+  if (rows(t.page_prompt)) LM_CUDA(launch_paged_prompt(a, false, e->page_ws, e->stream));
   return MLLMB200_OK;
 }
 

@@ -505,9 +505,9 @@ cudaError_t launch_paged_decode(const Paged& a, bool f16, void* workspace, cudaS
   auto* ws = static_cast<uint8_t*>(workspace);
   return f16 ? launch_decode<__half>(a, ws, s) : launch_decode<__nv_bfloat16>(a, ws, s);
 }
-cudaError_t launch_paged_prompt(const Paged& a, bool f16, cudaStream_t s) {
+cudaError_t launch_paged_prompt(const Paged& a, bool f16, void* workspace, cudaStream_t s) {
   cudaError_t r = cudaSuccess;
-  if (launch_paged_prompt_tc(a, f16, s, &r)) return r;
+  if (launch_paged_prompt_tc(a, f16, workspace, s, &r)) return r;
   r = configure_prompt();
   if (r != cudaSuccess) return r;
   return f16 ? launch_prompt<__half>(a, s) : launch_prompt<__nv_bfloat16>(a, s);
@@ -563,7 +563,7 @@ int mllmb200_lm_attn_prompt_workspace(const mllmb200_lm_pages* pages, const mllm
   if (!bytes) return MLLMB200_INVALID_ARG;
   const int st = check_look(pages, look, &a);
   if (st != MLLMB200_OK) return st;
-  *bytes = 0;
+  *bytes = paged_prompt_bytes(a);
   return MLLMB200_OK;
 }
 int mllmb200_lm_attn_prompt(const mllmb200_lm_pages* pages, const mllmb200_lm_look* look, void* workspace, void* stream) {
@@ -571,8 +571,8 @@ int mllmb200_lm_attn_prompt(const mllmb200_lm_pages* pages, const mllmb200_lm_lo
   const int st = check_look(pages, look, &a);
   if (st != MLLMB200_OK) return st;
   if (!a.seqs || !a.rows) return MLLMB200_OK;
-  (void)workspace;
-  return status_of(launch_paged_prompt(a, pages->dtype == MLLMB200_LM_F16, static_cast<cudaStream_t>(stream)));
+  if (paged_prompt_bytes(a) && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u))) return MLLMB200_INVALID_ARG;
+  return status_of(launch_paged_prompt(a, pages->dtype == MLLMB200_LM_F16, workspace, static_cast<cudaStream_t>(stream)));
 }
 
 int mllmb200_lm_operator_status(void* stream) {

@@ -215,7 +215,8 @@ cudaError_t once_per_device(std::atomic<unsigned long long>* done, F f) {
 // Checked launches for the engine: sizes and strides as the public calls take them.
 size_t paged_decode_bytes(const Paged& a);  // workspace of launch_paged_decode for a.seqs sequences
 cudaError_t launch_paged_decode(const Paged& a, bool f16, void* workspace, cudaStream_t s);
-cudaError_t launch_paged_prompt(const Paged& a, bool f16, cudaStream_t s);
+size_t paged_prompt_bytes(const Paged& a);
+cudaError_t launch_paged_prompt(const Paged& a, bool f16, void* workspace, cudaStream_t s);
 // Rows of a decode step of sequences with one token each: where their keys and values go, and the lengths with them.
 cudaError_t launch_paged_prep(cudaStream_t s, int n, const int2* row_sp, const int* table, int ld_table, int page, int2* row_page, int* lengths);
 // out fp32 [rows][ld_out] (the checks are those of mllmb200_lm_probabilities)
@@ -226,7 +227,7 @@ cudaError_t launch_probability_rows(const float* logits, long long ld, int rows,
 bool paged_decode_tc_takes(const Paged& a);
 int paged_decode_tc_rows(const Paged& a);  // rows of an item
 bool launch_paged_decode_tc(const Paged& a, bool f16, const DecodeWork& w, int* flags, cudaStream_t s, cudaError_t* launched);
-bool launch_paged_prompt_tc(const Paged& a, bool f16, cudaStream_t s, cudaError_t* launched);
+bool launch_paged_prompt_tc(const Paged& a, bool f16, void* workspace, cudaStream_t s, cudaError_t* launched);
 
 }  // namespace lm
 }  // namespace mllmb200

@@ -192,6 +192,14 @@ __device__ __forceinline__ float put_weights(uint32_t s_col, float scale, float 
   return total.x + total.y;
 }
 
+// Few rows and long contexts: `parts` CTAs (gridDim.y) share a pair of tiles' blocks and leave {maximum, sum} and unnormalized outputs
+// [CTA][part][256 rows]; flags [CTA][part]: 1 where the part has been done again in full (see below).
+struct PromptSplit {
+  float* part_o;
+  float2* part_ml;
+  int *flags, parts;
+};
+
 struct TcBarriers {
   uint64_t q_full, k_full[4], k_free[4], v_full[4], v_free[4], v_fixed[4], s_full[2], p_ready[2], o_done[2];
 };
@@ -199,7 +207,7 @@ struct TcBarriers {
 template <class T, int D, bool BIAS>
 __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const __grid_constant__ Paged a, const __grid_constant__ CUtensorMap qmap,
                                                                            const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                                                                           int piece) {
+                                                                           int piece, PromptSplit w) {
   using L = TcLayout<D>;
   extern __shared__ uint8_t tc_smem_raw[];
   __shared__ TcBarriers bars;
@@ -217,7 +225,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
   const int row0 = seq_rows.x + tile.y * 2 * toks, ntok = min(2 * toks, seq_rows.y - tile.y * 2 * toks);
   const int pos0 = paged_length(a, tile.x) - seq_rows.y + tile.y * 2 * toks, p_last = pos0 + ntok - 1;
   const Seen seen = paged_seen<kTcKeys>(a, pos0, p_last);
-  const int nt = seen.blocks, tiles = ntok > toks ? 2 : 1;
+  const int b0 = (int)((long long)seen.blocks * blockIdx.y / w.parts), nt = (int)((long long)seen.blocks * (blockIdx.y + 1) / w.parts) - b0;  // this CTA's blocks
+  const int tiles = ntok > toks ? 2 : 1;
   if (tid == 0) {
     mbar_init(&bars.q_full, 1);
     for (int i = 0; i < L::kK; ++i) mbar_init(&bars.k_full[i], 1), mbar_init(&bars.k_free[i], 1);
@@ -236,7 +245,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
   const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
   auto turn = [](int j, int n) { return (uint32_t)(j / n) & 1u; };  // parity of a ring's pass
   auto partly = [&](int j) {  // some row does not see some key of block j
-    const int j0 = block_key<kTcKeys>(seen, j);
+    const int j0 = block_key<kTcKeys>(seen, b0 + j);
     return pos0 < 0 || !seen_by_all(a, pos0, p_last, j0, j0 + kTcKeys - 1);
   };
   auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -262,7 +271,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
         auto page_of = [&](int j) {  // lane i: page of piece i of block j, a.pages (zeros) where nothing of it is seen
           int page = a.pages;
           if (j < nt && lane < pieces) {
-            const int key = block_key<kTcKeys>(seen, j) + lane * piece;
+            const int key = block_key<kTcKeys>(seen, b0 + j) + lane * piece;
             if (key <= seen.last && (key + piece > seen.lo || key < seen.head)) {
               const int p = paged_page(a, tile.x, key / a.page);
               if (p >= 0) page = p;
@@ -272,7 +281,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
         };
         int pages = page_of(0);
         for (int j = 0; j < nt && ok; ++j) {
-          const int next = page_of(j + 1), j0 = block_key<kTcKeys>(seen, j);
+          const int next = page_of(j + 1), j0 = block_key<kTcKeys>(seen, b0 + j);
           auto copy = [&](const CUtensorMap* map, uint32_t block, uint64_t* full) {
             if (lane == 0) mbar_arrive_expect_tx(full, L::kTile);
             __syncwarp();
@@ -351,7 +360,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
       for (int j = 0; j < nt && ok; ++j) {
         ok = wait(&bars.v_full[j % L::kV], turn(j, L::kV));
         if (!ok) break;
-        const int j0 = block_key<kTcKeys>(seen, j);
+        const int j0 = block_key<kTcKeys>(seen, b0 + j);
         const uint32_t block = values0 + j % L::kV * L::kTile;
         bool bad = false;
         for (int r = partly(j) ? tid - 320 : kTcKeys; r < kTcKeys; r += 64) {
@@ -399,7 +408,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
     for (int j = 0; j < n; ++j) {
       ok = ok && __all_sync(0xffffffffu, wait(&bars.s_full[t], (uint32_t)j & 1u));
       tc_fence_after();
-      const float top = weigh_block<BIAS>(a, s_col, bias, pos, first, last, block_key<kTcKeys>(seen, j));
+      const float top = weigh_block<BIAS>(a, s_col, bias, pos, first, last, block_key<kTcKeys>(seen, b0 + j));
       if (__any_sync(0xffffffffu, live && top > m + grown)) {
         const float m_new = fmaxf(m, top), alpha = m_new == -INFINITY ? 1.0f : paged_exp2((m - m_new) * scale);
         m = m_new;
@@ -416,30 +425,45 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
     }
     if (n) ok = ok && __all_sync(0xffffffffu, wait(&bars.o_done[t], 0));
     tc_fence_after();
-    if (live && n == 0) {
-      T* out = static_cast<T*>(a.out) + (row0 + t * toks + tok) * a.out_row + head * a.out_head;
-      for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(out + d) = make_uint4(0, 0, 0, 0);
+    const bool split = w.parts > 1;
+    const size_t at = ((size_t)blockIdx.x * w.parts + blockIdx.y) * 256 + tid;  // tid: tile and row
+    T* out = static_cast<T*>(a.out) + (row0 + t * toks + tok) * a.out_row + head * a.out_head;
+    if (n == 0 && live) {
+      if (split) {
+        w.part_ml[at] = make_float2(-INFINITY, 0.0f);
+      } else {
+        for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(out + d) = make_uint4(0, 0, 0, 0);
+      }
     }
     if (n) {
-      const float total = l + paged_exp2(sink - (m == -INFINITY ? 0.0f : m * scale)), inv = pos < 0 ? 0.0f : 1.0f / total;
-#pragma unroll
+      const float total = l + (split ? 0.0f : paged_exp2(sink - (m == -INFINITY ? 0.0f : m * scale))), inv = pos < 0 ? 0.0f : 1.0f / total;
+      if (split && live) w.part_ml[at] = make_float2(m * scale, l);  // base 2
+#pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
         tmem_ld32(o_col + c * 32, o);
         tmem_ld_wait();
-        if (live && ok) {
-          T* out = static_cast<T*>(a.out) + (row0 + t * toks + tok) * a.out_row + head * a.out_head + c * 32;
-          uint32_t w[16];
+        if (!live || !ok) continue;
+        if (split) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = pos < 0 ? 0u : Num<T>::pack(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+          for (int i = 0; i < 8; ++i)
+            reinterpret_cast<uint4*>(w.part_o + at * D + c * 32)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(out + i * 8) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          for (int i = 0; i < 4; ++i) {
+            uint32_t y[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              y[k] = pos < 0 ? 0u : Num<T>::pack(__uint_as_float(o[8 * i + 2 * k]) * inv, __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
+            *reinterpret_cast<uint4*>(out + c * 32 + i * 8) = make_uint4(y[0], y[1], y[2], y[3]);
+          }
         }
       }
     }
   }
   tc_fence_before();
   __syncthreads();
+  if (tid == 0 && w.parts > 1) w.flags[(size_t)blockIdx.x * w.parts + blockIdx.y] = s_bad;
   if (!s_bad) return;
   struct Cta {
     __device__ void sync() const { asm volatile("bar.sync 1, 256;" ::: "memory"); }
@@ -455,6 +479,49 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
   for (int t = 0; t < ntok; t += few) {
     cta.sync();
     paged_prompt_rows<T, D>(a, smem, cta, tid, tile.x, row0 + t, min(few, ntok - t), pos0 + t, kvh);
+  }
+}
+
+// grid (CTAs of the kernel above, 8): a warp joins the parts of four rows.
+template <class T, int D>
+__global__ void __launch_bounds__(256) lm_paged_prompt_join_kernel(Paged a, PromptSplit w) {
+  pdl_launch_dependents();
+  pdl_wait_prior();
+  const int toks = 128 / a.group, kvh = blockIdx.x % a.kv_heads, lane = threadIdx.x & 31;
+  const int2 tile = paged_tile(a, blockIdx.x / a.kv_heads, 2 * toks);
+  if (tile.x < 0) return;
+  for (int i = 0; i < w.parts; ++i)
+    if (w.flags[(size_t)blockIdx.x * w.parts + i]) return;  // done there
+  const int2 rows = paged_rows(a, tile.x);
+  const int first = tile.y * 2 * toks, pos0 = paged_length(a, tile.x) - rows.y + first;
+  for (int u = 0; u < 4; ++u) {
+    const int i = blockIdx.y * 32 + (threadIdx.x >> 5) * 4 + u, r = i & 127, tok = (i >> 7) * toks + r / a.group, head = kvh * a.group + r % a.group;
+    if (r / a.group >= toks || first + tok >= rows.y) continue;
+    auto at = [&](int p) { return ((size_t)blockIdx.x * w.parts + p) * 256 + i; };
+    const float2 ml = lane < w.parts ? w.part_ml[at(lane)] : make_float2(-INFINITY, 0.0f);
+    const float sink = a.sink ? a.sink[head] * kPagedLog2e : -INFINITY;
+    float mx = ml.x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    mx = fmaxf(mx, sink);
+    const float base = mx == -INFINITY ? 0.0f : mx, f = ml.y == 0.0f ? 0.0f : exp2f(ml.x - base);
+    float sum = f * ml.y, v[D / 32] = {};
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int p = 0; p < w.parts; ++p) {
+      const float fp = __shfl_sync(0xffffffffu, f, p);
+      if (fp == 0.0f) continue;  // (an empty part has left no output)
+      const float* part = w.part_o + at(p) * D + lane * (D / 32);
+#pragma unroll
+      for (int k = 0; k < D / 32; k += 2) {
+        const float2 x = *reinterpret_cast<const float2*>(part + k);
+        v[k] = fmaf(fp, x.x, v[k]), v[k + 1] = fmaf(fp, x.y, v[k + 1]);
+      }
+    }
+    const float inv = 1.0f / (sum + exp2f(sink - base));
+    T* out = static_cast<T*>(a.out) + (rows.x + first + tok) * a.out_row + head * a.out_head + lane * (D / 32);
+#pragma unroll
+    for (int k = 0; k < D / 32; k += 2) *reinterpret_cast<uint32_t*>(out + k) = pos0 + tok < 0 ? 0u : Num<T>::pack(v[k] * inv, v[k + 1] * inv);
   }
 }
 
@@ -941,14 +1008,31 @@ cudaError_t configure() {
   static std::atomic<unsigned long long> done{0};
   return once_per_device(&done, [] { return cudaFuncSetAttribute(lm_paged_prompt_tc_kernel<T, D, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<D>::kBytes); });
 }
-template <class T, int D>
-cudaError_t launch(const Paged& a, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, int piece, cudaStream_t s) {
+long long prompt_ctas(const Paged& a) {
   const int toks = 2 * (128 / a.group);
-  const long long tiles = std::min((long long)a.rows, a.rows / toks + (long long)a.seqs);
-  auto go = [&](auto kernel, cudaError_t r) {
-    return r != cudaSuccess ? r : launch_pdl(kernel, dim3((unsigned)(tiles * a.kv_heads)), dim3(kTcThreads), TcLayout<D>::kBytes, s, a, q, k, v, piece);
-  };
-  return a.bias ? go(lm_paged_prompt_tc_kernel<T, D, true>, configure<T, D, true>()) : go(lm_paged_prompt_tc_kernel<T, D, false>, configure<T, D, false>());
+  return std::min((long long)a.rows, a.rows / toks + (long long)a.seqs) * a.kv_heads;
+}
+// CTAs that share a pair of tiles: as many as the GPU has room for, with four blocks of keys each at least.
+int prompt_parts(const Paged& a) {
+  const long long ctas = prompt_ctas(a), keys = std::min((long long)a.max_pages * a.page, a.window ? (long long)a.window + a.keep + 2 * (128 / a.group) : 1ll << 40);
+  return ctas ? (int)std::max(1ll, std::min({16ll, kSms / ctas, keys / kTcKeys / 4})) : 1;
+}
+size_t prompt_split_rows(const Paged& a, int parts) { return (size_t)prompt_ctas(a) * parts * 256; }
+
+template <class T, int D>
+cudaError_t launch(const Paged& a, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, int piece, void* workspace, cudaStream_t s) {
+  PromptSplit w{};
+  w.parts = prompt_parts(a);
+  if (w.parts > 1) {
+    const size_t rows = prompt_split_rows(a, w.parts);
+    w.part_o = static_cast<float*>(workspace);
+    w.part_ml = reinterpret_cast<float2*>(w.part_o + rows * D);
+    w.flags = reinterpret_cast<int*>(w.part_ml + rows);
+  }
+  const dim3 grid((unsigned)prompt_ctas(a), w.parts);
+  auto go = [&](auto kernel, cudaError_t r) { return r != cudaSuccess ? r : launch_pdl(kernel, grid, dim3(kTcThreads), TcLayout<D>::kBytes, s, a, q, k, v, piece, w); };
+  const cudaError_t r = a.bias ? go(lm_paged_prompt_tc_kernel<T, D, true>, configure<T, D, true>()) : go(lm_paged_prompt_tc_kernel<T, D, false>, configure<T, D, false>());
+  return r != cudaSuccess || w.parts == 1 ? r : launch_pdl(lm_paged_prompt_join_kernel<T, D>, dim3(grid.x, 8), dim3(256), 0, s, a, w);
 }
 
 template <class T, int D, int NP, bool BIAS>
@@ -988,15 +1072,20 @@ bool make_maps(const Paged& a, bool f16, int toks, Maps* m) {
 
 }  // namespace
 
+bool prompt_tc_takes(const Paged& a) { return a.dim == a.vdim && (a.dim == 64 || a.dim == 128) && a.rows > 0 && prompt_ctas(a) <= 0x7fffffffll; }
+size_t paged_prompt_bytes(const Paged& a) {
+  if (!prompt_tc_takes(a)) return 0;
+  const int parts = prompt_parts(a);
+  return parts > 1 ? prompt_split_rows(a, parts) * (a.dim * 4 + sizeof(float2)) + (size_t)prompt_ctas(a) * parts * sizeof(int) : 0;
+}
 // Whether the kernel takes these sizes (and the tensor maps, these addresses and strides); `launched` says what became of it.
-bool launch_paged_prompt_tc(const Paged& a, bool f16, cudaStream_t s, cudaError_t* launched) {
-  if (a.dim != a.vdim || (a.dim != 64 && a.dim != 128) || !(a.scale2 > 1e-30f) || !(a.scale2 < 1e30f)) return false;
+bool launch_paged_prompt_tc(const Paged& a, bool f16, void* workspace, cudaStream_t s, cudaError_t* launched) {
+  if (!prompt_tc_takes(a) || !(a.scale2 > 1e-30f) || !(a.scale2 < 1e30f)) return false;
   const int toks = 128 / a.group;
-  if (((long long)a.rows / (2 * toks) + a.seqs) * a.kv_heads > 0x7fffffffll) return false;
   Maps m;
   if (!make_maps(a, f16, toks, &m)) return false;
-  *launched = f16 ? (a.dim == 64 ? launch<__half, 64>(a, m.q, m.k, m.v, m.piece, s) : launch<__half, 128>(a, m.q, m.k, m.v, m.piece, s))
-                  : (a.dim == 64 ? launch<__nv_bfloat16, 64>(a, m.q, m.k, m.v, m.piece, s) : launch<__nv_bfloat16, 128>(a, m.q, m.k, m.v, m.piece, s));
+  *launched = f16 ? (a.dim == 64 ? launch<__half, 64>(a, m.q, m.k, m.v, m.piece, workspace, s) : launch<__half, 128>(a, m.q, m.k, m.v, m.piece, workspace, s))
+                  : (a.dim == 64 ? launch<__nv_bfloat16, 64>(a, m.q, m.k, m.v, m.piece, workspace, s) : launch<__nv_bfloat16, 128>(a, m.q, m.k, m.v, m.piece, workspace, s));
   return true;
 }
 

@@ -108,7 +108,7 @@ def _attention(where, q, k_pages, v_pages, table, lengths, q_start, scale, windo
                 (lambda: False, "out [rows, heads, vdim] of the queries' type, rows contiguous"))
     L = lm.lib()
     decode = q_start is None
-    key = (decode, rows, heads, kv_heads, dim, vdim, seqs)
+    key = (decode, rows, heads, kv_heads, dim, vdim, seqs) if decode else (rows, heads, kv_heads, dim, vdim, table.shape, k_pages.shape[2], window, keep)
 
     def call(s):
         o = out if out is not None else torch.empty_like(q) if vdim == dim and q.is_contiguous() else q.new_empty((rows, heads, vdim))

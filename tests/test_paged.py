@@ -225,6 +225,30 @@ def test_prompt_many_heads_layouts_sequences():
     run_prompt([n + i % 30 for i, n in enumerate(counts)], counts, 2, 1, 64, 64, 16, BF16)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths, counts", [([3000], [9]), ([2100, 4, 0, 1300], [30, 4, 0, 1]), ([700, 3, 1500], [5, 7, 40])])
+@pytest.mark.parametrize("heads, kv, dim, page", [(12, 2, 128, 48), (14, 2, 64, 16), (4, 4, 128, 64)])
+@pytest.mark.parametrize("window, keep, rel", [(0, 0, False), (1100, 3, True)])
+def test_prompt_few_rows_of_long_contexts(lengths, counts, heads, kv, dim, page, window, keep, rel):
+    """The lengths are split and joined."""
+    run_prompt(lengths, counts, heads, kv, dim, dim, page, BF16, window, keep, rel, seed=heads)
+
+
+@pytest.mark.gpu
+def test_prompt_values_of_unseen_keys_where_lengths_are_split():
+    c = Cache([2000, 900], 2, 64, 64, 16, BF16, 3)
+    q = rand((12, 4, 64), BF16, 4)
+    want, spread, big = attention64(c, [6, 6], q)
+    for t in (c.k, c.v):
+        t[c.table_h[0, 1996 // 16], :, 1996 % 16] = float("nan")  # seen by the tokens at 1996 .. 1999 of sequence 0
+    c.on_gpu()
+    start = torch.tensor([0, 6, 12], dtype=torch.int32, device="cuda")
+    got = paged.prompt_attention(q.cuda(), c.k, c.v, c.table, c.lengths, start)
+    clean = [0, 1] + list(range(6, 12))
+    check(got[clean], want[clean], spread[clean], big, 64, BF16, True)
+    assert not torch.isfinite(got[2:6].float()).any()
+
+
 # ------------------------------------------------------------------------------------------------ append, and a run of them together
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, FP16])
