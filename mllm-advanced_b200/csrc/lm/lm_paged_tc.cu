@@ -24,12 +24,18 @@ namespace {
 
 constexpr int kTcKeys = 128, kTcThreads = 384;
 
-template <int D>
+template <int D, bool BIAS>
 struct TcLayout {
-  static constexpr int kTile = 128 * D * 2;                 // a block of keys or values, and a tile of queries
-  static constexpr int kK = D == 128 ? 3 : 4, kV = D == 128 ? 2 : 4;  // blocks of keys, of values
-  static constexpr int kBytes = (2 + kK + kV) * kTile + 1024;  // (queries and ring on 1024 bytes)
+  static constexpr int kTile = 128 * D * 2;  // a block of keys or values, and a tile of queries
+  static constexpr int kK = D == 128 ? (BIAS ? 2 : 3) : BIAS ? 3 : 4, kV = D == 128 ? 2 : BIAS ? 3 : 4;  // blocks of keys, of values
+  static constexpr int kTable = BIAS ? 30 * 1024 : 0;                                                    // the group's bias tables, if they fit
+  static constexpr int kBytes = (2 + kK + kV) * kTile + kTable + 1024;                                   // (queries and ring on 1024 bytes)
 };
+// Floats from one head's bias table to the next in shared memory: the rows of a warp (all heads of some tokens) read from banks of their own.
+__host__ __device__ inline int bias_pitch(int bias_max, int group) {
+  const int want = group < 32 ? (32 + group - 1) / group : 1;
+  return (bias_max + 32 - want) / 32 * 32 + want;  // at least bias_max + 1
+}
 
 template <class T>
 __device__ __forceinline__ uint32_t tc_idesc(int n, bool b_mn) {  // fp32 sums, M = 128
@@ -65,11 +71,11 @@ __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) { asm v
 // One row's scores of a block in tensor memory: bias and mask (written back) and the largest.  first, last: positions of the rows that
 // are worked on together.  Loops over columns are short on purpose: a launch starts with a cold instruction cache.
 template <bool BIAS>
-__device__ __forceinline__ float weigh_block(const Paged& a, uint32_t s_col, const float* bias, int pos, int first, int last, int j0) {
+__device__ __forceinline__ float weigh_block(const Paged& a, uint32_t s_col, const float* bias, float bias_scale, int pos, int first, int last, int j0) {
   const bool masked = first < 0 || !seen_by_all(a, first, last, j0, j0 + kTcKeys - 1);
   const int hi = pos - j0, lo = a.window ? hi - a.window : -1, kp = a.window ? a.keep - j0 : 0;  // column i: i <= hi and (i > lo or i < kp)
   const bool near = BIAS && first - (j0 + kTcKeys - 1) < a.bias_max;                               // some distance has a bias of its own
-  const float far = BIAS && bias ? bias[a.bias_max] * kPagedLog2e : 0.0f;
+  const float far = BIAS ? bias[a.bias_max] * bias_scale : 0.0f;
   float top = -INFINITY;
 #pragma unroll 1
   for (int c = 0; c < 128; c += 64) {
@@ -77,16 +83,27 @@ __device__ __forceinline__ float weigh_block(const Paged& a, uint32_t s_col, con
     tmem_ld32(s_col + c, v[0]);
     tmem_ld32(s_col + c + 32, v[1]);
     tmem_ld_wait();
-    if (BIAS || masked) {
+    if (BIAS) {
+      if (near) {
 #pragma unroll
-      for (int i = 0; i < 64; ++i) {
-        uint32_t& x = v[i >> 5][i & 31];
-        if (BIAS) {
-          const float b = near && bias ? __ldg(bias + max(0, min(hi - c - i, a.bias_max))) * kPagedLog2e : far;
-          x = __float_as_uint(fmaf(__uint_as_float(x), a.scale2, b));
+        for (int i = 0; i < 64; ++i) {
+          uint32_t& x = v[i >> 5][i & 31];
+          x = __float_as_uint(fmaf(__uint_as_float(x), a.scale2, bias[max(0, min(hi - c - i, a.bias_max))] * bias_scale));
         }
-        if (masked && !(c + i <= hi && (c + i > lo || c + i < kp))) x = 0xff800000u;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) {
+          uint32_t& x = v[i >> 5][i & 31];
+          x = __float_as_uint(fmaf(__uint_as_float(x), a.scale2, far));
+        }
       }
+    }
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 64; ++i)
+        if (!(c + i <= hi && (c + i > lo || c + i < kp))) v[i >> 5][i & 31] = 0xff800000u;
+    }
+    if (BIAS || masked) {
       tmem_st32(s_col + c, v[0]);
       tmem_st32(s_col + c + 32, v[1]);
     }
@@ -208,7 +225,7 @@ template <class T, int D, bool BIAS>
 __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const __grid_constant__ Paged a, const __grid_constant__ CUtensorMap qmap,
                                                                            const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                                                                            int piece, PromptSplit w) {
-  using L = TcLayout<D>;
+  using L = TcLayout<D, BIAS>;
   extern __shared__ uint8_t tc_smem_raw[];
   __shared__ TcBarriers bars;
   __shared__ uint32_t s_tmem;
@@ -239,6 +256,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
     tmem_alloc(&s_tmem, 512);
     tmem_relinquish();
   }
+  const int pitch = BIAS ? bias_pitch(a.bias_max, a.group) : 0;
+  const bool staged = BIAS && (size_t)pitch * a.group * 4 <= (size_t)L::kTable;
+  float* table = reinterpret_cast<float*>(tc_smem_raw + (values0 + L::kV * L::kTile - smem_u32(tc_smem_raw)));
+  if (staged)
+    for (int h = warp; h < a.group; h += kTcThreads / 32)
+      for (int i = lane; i <= a.bias_max; i += 32) table[h * pitch + i] = a.bias[(size_t)(kvh * a.group + h) * (a.bias_max + 1) + i] * kPagedLog2e;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -399,7 +422,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
     const bool live = tok < toks && t * toks + tok < ntok;
     const int pos = live ? pos0 + t * toks + tok : -1;
     const int first = pos0 + t * toks, last = min(p_last, first + toks - 1);  // of this tile
-    const float* bias = BIAS && live ? a.bias + (size_t)head * (a.bias_max + 1) : nullptr;
+    // (a row that is not there reads the first one's)
+    const float* bias = !BIAS ? nullptr : staged ? table + (live ? hg * pitch : 0) : a.bias + (size_t)(live ? head : 0) * (a.bias_max + 1);
     const float sink = a.sink && live ? a.sink[head] * kPagedLog2e : -INFINITY;
     const float scale = BIAS ? 1.0f : a.scale2, grown = 8.0f / scale;  // BIAS: scores are scaled before their maximum
     float m = -INFINITY, l = 0.0f;
@@ -408,7 +432,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
     for (int j = 0; j < n; ++j) {
       ok = ok && __all_sync(0xffffffffu, wait(&bars.s_full[t], (uint32_t)j & 1u));
       tc_fence_after();
-      const float top = weigh_block<BIAS>(a, s_col, bias, pos, first, last, block_key<kTcKeys>(seen, b0 + j));
+      const float top = weigh_block<BIAS>(a, s_col, bias, staged ? 1.0f : kPagedLog2e, pos, first, last, block_key<kTcKeys>(seen, b0 + j));
       if (__any_sync(0xffffffffu, live && top > m + grown)) {
         const float m_new = fmaxf(m, top), alpha = m_new == -INFINITY ? 1.0f : paged_exp2((m - m_new) * scale);
         m = m_new;
@@ -601,7 +625,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
   __shared__ DecBarriers<D, NP> bars;
   __shared__ int s_base[kDecSeqs + 1];
   __shared__ float s_max[4][NP];
-  __shared__ __align__(16) float s_ref[NP], s_alpha[NP], s_base2[NP];  // the rows' maxima by warp; the one in use, times scale (base 2); what is added to scores
+  __shared__ __align__(16) float s_ref[NP], s_alpha[NP], s_base2[NP], s_far[BIAS ? NP : 1];  // the rows' maxima by warp; the one in use, times scale (base 2); what is added to scores; the bias of far keys
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_bad, s_gave_up;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -827,31 +851,51 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
         for (int c = 0; c < NP; ++c) l[c] = 0.0f;
         sync();  // (the last share's numbers have been read)
         if (tid < NP) s_ref[tid] = tid < rows ? -INFINITY : INFINITY, s_base2[tid] = tid < rows ? 0.0f : -INFINITY;  // (columns without a row: weights of 0)
+        if (BIAS && tid < NP) s_far[tid] = tid < rows ? a.bias[(size_t)(g.kvh * a.group + tid % a.group) * (a.bias_max + 1) + a.bias_max] * kPagedLog2e : 0.0f;
         sync();
       }
       ok = ok && all_wait(&bars.s_full[r & 1], (uint32_t)(r >> 1) & 1u);
       tc_fence_after();
       bool over = false;
       uint32_t v[kC];
-      auto load = [&](int c0) {  // columns c0 .. c0 + kC - 1: scores, with bias and mask
+      const bool near = BIAS && g.p_first - (j - tid + kTcKeys - 1) < a.bias_max;  // some distance has a bias of its own
+      auto load = [&](int c0) {  // columns c0 .. c0 + kC - 1
         if constexpr (kC == 16) tmem_ld16(s_col + c0, v);
         else tmem_ld32(s_col + c0, v);
         tmem_ld_wait();
-        if (BIAS || masked) {
+      };
+      auto prepare = [&](int c0) {  // bias and mask
+        if (BIAS) {
+          if (near) {
+            int tok = c0 / a.group, hg = c0 - tok * a.group;
+#pragma unroll
+            for (int i = 0; i < kC; ++i) {
+              const float* table = a.bias + (size_t)(g.kvh * a.group + hg) * (a.bias_max + 1);
+              const float b = c0 + i < rows ? __ldg(table + max(0, min(g.p_first + tok - j, a.bias_max))) * kPagedLog2e : 0.0f;
+              v[i] = __float_as_uint(fmaf(__uint_as_float(v[i]), a.scale2, b));
+              if (++hg == a.group) hg = 0, ++tok;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < kC; ++i) v[i] = __float_as_uint(fmaf(__uint_as_float(v[i]), a.scale2, s_far[c0 + i]));
+          }
+        }
+        if (masked) {
           int tok = c0 / a.group, hg = c0 - tok * a.group;
 #pragma unroll
           for (int i = 0; i < kC; ++i) {
-            const int pos = g.p_first + tok;
-            float x = __uint_as_float(v[i]);
-            if (BIAS && c0 + i < rows) x = fmaf(x, a.scale2, __ldg(a.bias + (size_t)(g.kvh * a.group + hg) * (a.bias_max + 1) + max(0, min(pos - j, a.bias_max))) * kPagedLog2e);
-            v[i] = masked && !seen_by(a, pos, j) ? 0xff800000u : __float_as_uint(x);
+            if (!seen_by(a, g.p_first + tok, j)) v[i] = 0xff800000u;
             if (++hg == a.group) hg = 0, ++tok;
           }
+        }
+        if constexpr (NP > kC) {
+          if (BIAS || masked) tmem_st32(s_col + c0, v);  // (they are read again)
         }
       };
 #pragma unroll
       for (int c0 = 0; c0 < NP; c0 += kC) {
         load(c0);
+        prepare(c0);
 #pragma unroll
         for (int i = 0; i < kC; i += 4) {
           const float4 ref = *reinterpret_cast<const float4*>(s_ref + c0 + i);
@@ -859,6 +903,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
                   fmaf(__uint_as_float(v[i + 2]), scale, -8.0f) > ref.z | fmaf(__uint_as_float(v[i + 3]), scale, -8.0f) > ref.w;
         }
       }
+      if (NP > kC && (BIAS || masked)) tmem_st_wait();
       if (any(over)) {  // some row's maximum has outgrown its reference (always in an item's first block, unless nothing is seen)
 #pragma unroll
         for (int c0 = 0; c0 < NP; c0 += kC) {
@@ -1006,7 +1051,7 @@ bool encode(CUtensorMap* map, CUtensorMapDataType type, const void* base, const 
 template <class T, int D, bool BIAS>
 cudaError_t configure() {
   static std::atomic<unsigned long long> done{0};
-  return once_per_device(&done, [] { return cudaFuncSetAttribute(lm_paged_prompt_tc_kernel<T, D, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<D>::kBytes); });
+  return once_per_device(&done, [] { return cudaFuncSetAttribute(lm_paged_prompt_tc_kernel<T, D, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<D, BIAS>::kBytes); });
 }
 long long prompt_ctas(const Paged& a) {
   const int toks = 2 * (128 / a.group);
@@ -1030,8 +1075,9 @@ cudaError_t launch(const Paged& a, const CUtensorMap& q, const CUtensorMap& k, c
     w.flags = reinterpret_cast<int*>(w.part_ml + rows);
   }
   const dim3 grid((unsigned)prompt_ctas(a), w.parts);
-  auto go = [&](auto kernel, cudaError_t r) { return r != cudaSuccess ? r : launch_pdl(kernel, grid, dim3(kTcThreads), TcLayout<D>::kBytes, s, a, q, k, v, piece, w); };
-  const cudaError_t r = a.bias ? go(lm_paged_prompt_tc_kernel<T, D, true>, configure<T, D, true>()) : go(lm_paged_prompt_tc_kernel<T, D, false>, configure<T, D, false>());
+  auto go = [&](auto kernel, size_t smem, cudaError_t r) { return r != cudaSuccess ? r : launch_pdl(kernel, grid, dim3(kTcThreads), smem, s, a, q, k, v, piece, w); };
+  const cudaError_t r = a.bias ? go(lm_paged_prompt_tc_kernel<T, D, true>, TcLayout<D, true>::kBytes, configure<T, D, true>())
+                               : go(lm_paged_prompt_tc_kernel<T, D, false>, TcLayout<D, false>::kBytes, configure<T, D, false>());
   return r != cudaSuccess || w.parts == 1 ? r : launch_pdl(lm_paged_prompt_join_kernel<T, D>, dim3(grid.x, 8), dim3(256), 0, s, a, w);
 }
 
