@@ -148,7 +148,8 @@ MLLMB200_API int mllmb200_lm_check_device_status(void* handle);
 enum { MLLMB200_LM_F16 = 2 };  /* caches and queries in fp16 (beside MLLMB200_LM_BF16) */
 
 /* A layer's cache: position j of sequence s lies in page table[s * ld_table + j / page], row j % page.  Pages may lie in
- * any order; strides are in elements (multiples of 8; rows are contiguous), pointers 16-byte aligned.
+ * any order; strides are in elements (multiples of 8, whatever they are for a dimension of one; rows are contiguous), pointers
+ * 16-byte aligned.
  * Sequence s brings the rows [q_start[s], q_start[s + 1]) of a call (q_start NULL: rows / seqs each) and is
  * lengths[s] tokens long with them: its row t stands at position lengths[s] - n + t.  Rows at negative positions see nothing
  * (attention: zeros) and are not stored; rows from q_start[seqs] on are neither read nor written.

@@ -402,13 +402,16 @@ int check_pages(const mllmb200_lm_pages* p, Paged* a) {
   if (p->dtype != MLLMB200_LM_BF16 && p->dtype != MLLMB200_LM_F16) return MLLMB200_UNSUPPORTED;
   if (p->pages < 1 || p->page < 1 || p->kv_heads < 1 || p->dim < 1 || p->vdim < 1 || p->max_pages < 0 || p->ld_table < 0) return MLLMB200_INVALID_ARG;
   if (p->page % 16 || p->dim % 16 || p->vdim % 16 || p->dim > 256 || p->vdim > 256) return MLLMB200_UNSUPPORTED;
-  if ((long long)p->max_pages * p->page > kLongest) return MLLMB200_UNSUPPORTED;
+  if ((long long)p->max_pages * p->page > kLongest || p->rows > kLongest) return MLLMB200_UNSUPPORTED;
   if (p->seqs && (!p->k || !p->v || !p->lengths || (!p->table && p->max_pages))) return MLLMB200_INVALID_ARG;
-  if (!aligned(p->k, p->k_page, p->k_head, p->k_row) || !aligned(p->v, p->v_page, p->v_head, p->v_row)) return MLLMB200_INVALID_ARG;
-  if (!p->q_start && p->seqs && p->rows % p->seqs) return MLLMB200_INVALID_ARG;
   *a = Paged{};
-  a->k = p->k, a->v = p->v;
   a->k_page = p->k_page, a->k_head = p->k_head, a->k_row = p->k_row, a->v_page = p->v_page, a->v_head = p->v_head, a->v_row = p->v_row;
+  // (the stride of a dimension of one says nothing)
+  if (p->kv_heads == 1) a->k_head = p->k_row, a->v_head = p->v_row;
+  if (p->pages == 1) a->k_page = p->k_row, a->v_page = p->v_row;
+  if (!aligned(p->k, a->k_page, a->k_head, a->k_row) || !aligned(p->v, a->v_page, a->v_head, a->v_row)) return MLLMB200_INVALID_ARG;
+  if (!p->q_start && p->seqs && p->rows % p->seqs) return MLLMB200_INVALID_ARG;
+  a->k = p->k, a->v = p->v;
   a->table = p->table, a->lengths = p->lengths, a->q_start = p->q_start;
   a->pages = p->pages, a->page = p->page, a->kv_heads = p->kv_heads, a->dim = p->dim, a->vdim = p->vdim;
   a->ld_table = p->ld_table, a->max_pages = p->max_pages, a->seqs = p->seqs, a->rows = p->rows;
@@ -422,11 +425,14 @@ int check_look(const mllmb200_lm_pages* p, const mllmb200_lm_look* l, Paged* a) 
   if (l->heads / a->kv_heads > 64) return MLLMB200_UNSUPPORTED;
   if (l->bias && l->bias_max < 0) return MLLMB200_INVALID_ARG;
   if (a->rows && (!l->q || !l->out)) return MLLMB200_INVALID_ARG;
-  if (!aligned(l->q, l->q_row, l->q_head) || !aligned(l->out, l->out_row, l->out_head)) return MLLMB200_INVALID_ARG;
   a->q = l->q, a->out = l->out;
   a->q_row = l->q_row, a->q_head = l->q_head, a->out_row = l->out_row, a->out_head = l->out_head;
+  if (l->heads == 1) a->q_head = a->dim, a->out_head = a->vdim;
+  if (a->rows == 1) a->q_row = (long long)l->heads * a->dim, a->out_row = (long long)l->heads * a->vdim;
+  if (!aligned(l->q, a->q_row, a->q_head) || !aligned(l->out, a->out_row, a->out_head)) return MLLMB200_INVALID_ARG;
   a->sink = l->sink, a->bias = l->bias;
-  a->heads = l->heads, a->group = l->heads / a->kv_heads, a->bias_max = l->bias_max, a->window = l->window, a->keep = l->keep;
+  a->heads = l->heads, a->group = l->heads / a->kv_heads, a->bias_max = l->bias_max;
+  a->window = std::min(l->window, kLongest), a->keep = std::min(l->keep, kLongest);  // (no position is beyond; differences stay in 32 bits)
   a->scale2 = l->scale * kPagedLog2e;
   return MLLMB200_OK;
 }
@@ -453,7 +459,7 @@ cudaError_t launch_decode(Paged a, uint8_t* ws, cudaStream_t s) {
     b.lengths += s0;
     b.table += (size_t)s0 * a.ld_table;
     if (b.q_start) b.q_start += s0, b.q_count += s0;
-    else b.q = static_cast<const T*>(a.q) + (long long)s0 * a.tokens * a.q_row, b.out = static_cast<T*>(a.out) + (long long)s0 * a.tokens * a.out_row;
+    else b.q = static_cast<const T*>(a.q) + (long long)s0 * a.tokens * a.q_row, b.out = static_cast<T*>(a.out) + (long long)s0 * a.tokens * a.out_row, b.rows -= s0 * a.tokens;
     DecodeWork w{reinterpret_cast<float*>(ws), reinterpret_cast<float2*>(ws + d.ml), reinterpret_cast<long long*>(ws + d.base), 0, nullptr};
     int* flags = reinterpret_cast<int*>(ws + d.flags);
     cudaError_t r = cudaSuccess;
@@ -530,6 +536,8 @@ int mllmb200_lm_pages_append(const mllmb200_lm_pages* pages, const void* k, long
   const int st = check_pages(pages, &a);
   if (st != MLLMB200_OK) return st;
   if (!a.seqs || !a.rows) return MLLMB200_OK;
+  if (a.kv_heads == 1) k_head = a.dim, v_head = a.vdim;
+  if (a.rows == 1) k_row = (long long)a.kv_heads * a.dim, v_row = (long long)a.kv_heads * a.vdim;
   if (!k || !v || !aligned(k, k_row, k_head) || !aligned(v, v_row, v_head)) return MLLMB200_INVALID_ARG;
   const int pieces = a.kv_heads * (a.dim + a.vdim) / 8;
   // (one row a thread while that does not fill the GPU: 64 rows take 2.8 us with one, 5.1 with four; 9476 rows of 4 heads of 128 11.4 and 9)

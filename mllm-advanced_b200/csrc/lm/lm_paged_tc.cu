@@ -68,6 +68,8 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]
 
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
+__device__ __forceinline__ uint32_t first_bits(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
+
 // One row's scores of a block in tensor memory: bias and mask (written back) and the largest.  first, last: positions of the rows that
 // are worked on together.  Loops over columns are short on purpose: a launch starts with a cold instruction cache.
 template <bool BIAS>
@@ -100,8 +102,13 @@ __device__ __forceinline__ float weigh_block(const Paged& a, uint32_t s_col, con
     }
     if (masked) {
 #pragma unroll
-      for (int i = 0; i < 64; ++i)
-        if (!(c + i <= hi && (c + i > lo || c + i < kp))) v[i >> 5][i & 31] = 0xff800000u;
+      for (int h = 0; h < 2; ++h) {
+        const int at = c + h * 32;
+        const uint32_t seen = first_bits(hi + 1 - at) & (~first_bits(lo + 1 - at) | first_bits(kp - at));
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (!((seen >> i) & 1u)) v[h][i] = 0xff800000u;
+      }
     }
     if (BIAS || masked) {
       tmem_st32(s_col + c, v[0]);
@@ -233,7 +240,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const uint32_t smem0 = (smem_u32(tc_smem_raw) + 1023u) & ~1023u, keys0 = smem0 + 2 * L::kTile, values0 = keys0 + L::kK * L::kTile;
   if (tid < 3) tma_prefetch_map(tid == 0 ? &qmap : tid == 1 ? &kmap : &vmap);
-  pdl_launch_dependents();
   pdl_wait_prior();
   const int toks = 128 / a.group, kvh = blockIdx.x % a.kv_heads;
   const int2 tile = paged_tile(a, blockIdx.x / a.kv_heads, 2 * toks);
@@ -265,6 +271,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // (not before this CTA has its tensor memory, and not taken before the kernels in front have ended: a kernel that takes some of it and
+  // then waits for another must not keep that one from taking its own)
+  pdl_launch_dependents();
   const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
   auto turn = [](int j, int n) { return (uint32_t)(j / n) & 1u; };  // parity of a ring's pass
   auto partly = [&](int j) {  // some row does not see some key of block j
@@ -642,13 +651,12 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
     s_bad = s_gave_up = 0;
     mbar_fence_init();
   }
+  if (tid < 3) tma_prefetch_map(tid == 0 ? &qmap : tid == 1 ? &kmap : &vmap);
+  pdl_wait_prior();
   if (warp == 5) {
     tmem_alloc(&s_tmem, L::kColumns);
     tmem_relinquish();
   }
-  if (tid < 3) tma_prefetch_map(tid == 0 ? &qmap : tid == 1 ? &kmap : &vmap);
-  pdl_launch_dependents();
-  pdl_wait_prior();
   sum_blocks<kTcKeys, kDecThreads>(a, s_base);
   if (blockIdx.x == 0)
     for (int i = tid; i <= a.seqs; i += kDecThreads) w.base[i] = s_base[i];
@@ -666,6 +674,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_launch_dependents();  // (as above)
   const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return true;

@@ -134,6 +134,70 @@ def test_decode_many_sequences():
 
 
 @pytest.mark.gpu
+def test_decode_many_sequences_in_blocks_of_rows():
+    """Launches of 512 sequences, and more rows of a key head than a block holds (24 heads x 3 tokens)."""
+    lengths = np.random.default_rng(2).integers(0, 40, 530).tolist()
+    run_decode(lengths, 3, 24, 1, 64, 64, 16, BF16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-35, 0.5])
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_scales(scale, tokens):
+    c = Cache([300, 5, 130], 2, 64, 64, 16, BF16, 4)
+    q = rand((3 * tokens, 6, 64), BF16, 5)
+    want = attention64(c, [tokens] * 3, q, scale)
+    c.on_gpu()
+    start = torch.arange(4, dtype=torch.int32, device="cuda") * tokens
+    check(paged.decode_attention(q.cuda(), c.k, c.v, c.table, c.lengths, scale=scale), *want, 64, BF16, False)
+    check(paged.prompt_attention(q.cuda(), c.k, c.v, c.table, c.lengths, start, scale=scale), *want, 64, BF16, True)
+
+
+@pytest.mark.gpu
+def test_strides_of_dimensions_of_one():
+    """A single key head, a single row, a single head: their strides say nothing and may be anything."""
+    c = Cache([40], 1, 64, 64, 16, BF16, 4)
+    q = rand((1, 1, 64), BF16, 5)
+    want = attention64(c, [1], q)
+    c.on_gpu()
+    odd = lambda t, *strides: torch.as_strided(t, t.shape, strides)
+    k, v = odd(c.k, 16 * 64, 3, 64, 1), odd(c.v, 16 * 64, 5, 64, 1)
+    qd = odd(q.cuda(), 7, 9, 1)
+    start = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    check(paged.decode_attention(qd, k, v, c.table, c.lengths), *want, 64, BF16, False)
+    check(paged.prompt_attention(qd, k, v, c.table, c.lengths, start), *want, 64, BF16, True)
+    before = c.k.clone()
+    paged.append(k, v, odd(q.cuda(), 3, 11, 1), odd(q.cuda(), 3, 11, 1), c.table, c.lengths)
+    at = c.table_h[0, 39 // 16]
+    assert torch.equal(c.k[at, 0, 39 % 16].cpu(), q[0, 0])
+    before[at, 0, 39 % 16] = q[0, 0].cuda()
+    assert torch.equal(torch.nan_to_num(c.k.float(), 9.0), torch.nan_to_num(before.float(), 9.0))
+    # queries shared by all heads (a stride of 0)
+    c = Cache([40, 70], 2, 64, 64, 16, BF16, 6)
+    q = rand((2, 1, 64), BF16, 7)
+    want = attention64(c, [1, 1], q.expand(2, 4, 64))
+    c.on_gpu()
+    check(paged.decode_attention(q.cuda().expand(2, 4, 64), c.k, c.v, c.table, c.lengths), *want, 64, BF16, False)
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    """Calls that run beside one another, each with scratch of its own."""
+    c = Cache([900, 2000, 77], 2, 128, 128, 16, BF16, 8)
+    q = rand((2, 3, 12, 128), BF16, 9).cuda()
+    c.on_gpu()
+    start = torch.tensor([0, 1, 2, 3], dtype=torch.int32, device="cuda")
+    calls = [lambda x, s: paged.decode_attention(x, c.k, c.v, c.table, c.lengths, stream=s), lambda x, s: paged.prompt_attention(x, c.k, c.v, c.table, c.lengths, start, stream=s)]
+    want = [call(x, None) for call, x in zip(calls, q)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[call(x, s) for call, x, s in zip(calls, q, streams)] for _ in range(20)]
+    torch.cuda.synchronize()
+    for pair in got:
+        assert torch.equal(pair[0], want[0]) and torch.equal(pair[1], want[1])
+
+
+@pytest.mark.gpu
 def test_decode_same_bits_and_strides():
     """A sequence's result does not depend on how often it is computed; views of larger tensors give the same bits."""
     c, q, got = run_decode([900, 30, 411], 2, 8, 2, 128, 128, 16, BF16, 100, 5)
@@ -202,7 +266,7 @@ def test_prompt_lengths(lengths, counts, heads, kv, dim, vdim, page):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("dim", [64, 128, 80])
-@pytest.mark.parametrize("window, keep", [(0, 0), (1, 0), (7, 3), (64, 17), (150, 400)])
+@pytest.mark.parametrize("window, keep", [(0, 0), (1, 0), (7, 3), (64, 17), (150, 400), (2 ** 31 - 1, 2 ** 31 - 1)])
 @pytest.mark.parametrize("rel", [False, True])
 def test_prompt_masks(dtype, dim, window, keep, rel):
     run_prompt([400, 1, 0, 90, 66], [150, 1, 0, 2, 66], 8, 2, dim, dim, 32, dtype, window, keep, rel, seed=dim)
@@ -214,6 +278,7 @@ def test_prompt_positions_before_the_start():
     c, q, start, got = run_prompt([3, 20], [9, 20], 4, 2, 64, 64, 16, BF16)
     assert (got[:6] == 0).all()
     run_prompt([3, 20], [9, 20], 4, 2, 64, 64, 16, BF16, 4, 1, True)
+    run_prompt([3, 20], [9, 20], 4, 2, 64, 64, 16, BF16, 2 ** 31 - 1, 0, True)
     run_decode([2, 0, 5], 4, 4, 2, 64, 64, 16, BF16, rel=True)
 
 
