@@ -247,14 +247,15 @@ __global__ void __launch_bounds__(32 * WARPS, 1) lm_paged_decode_kernel(Paged a,
   }
 }
 
-// grid (items of all sequences, rows of an item / 4): a warp joins the shares of a row of an item that lies in several CTAs; zeros
-// for those without keys.
+// grid (items of all sequences, rows of an item x PER / 4): joins the shares of a row of an item that lies in several CTAs, PER warps a row;
+// zeros for those without keys.
 constexpr int kJoinWarps = 4;
-template <class T>
+template <class T, int PER>
 __global__ void __launch_bounds__(32 * kJoinWarps) lm_paged_join_kernel(Paged a, DecodeWork w, int item_rows) {
+  __shared__ float s_v[PER > 1 ? kJoinWarps : 1][256], s_sum[kJoinWarps];
   pdl_launch_dependents();
-  const int items = a.kv_heads * w.row_blocks, s = blockIdx.x / items, item = blockIdx.x - s * items, lane = threadIdx.x & 31;
-  const int kvh = item / w.row_blocks, r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5), row = (item - kvh * w.row_blocks) * item_rows + r;
+  const int items = a.kv_heads * w.row_blocks, s = blockIdx.x / items, item = blockIdx.x - s * items, warp = PER > 1 ? threadIdx.x >> 5 : 0, lane = threadIdx.x & 31;
+  const int kvh = item / w.row_blocks, r = PER > 1 ? blockIdx.y : blockIdx.y * kJoinWarps + (threadIdx.x >> 5), row = (item - kvh * w.row_blocks) * item_rows + r;
   const int tok = row / a.group, h = kvh * a.group + row - tok * a.group;
   pdl_wait_prior();
   if (r >= item_rows || row >= a.group * a.tokens) return;
@@ -263,7 +264,6 @@ __global__ void __launch_bounds__(32 * kJoinWarps) lm_paged_join_kernel(Paged a,
   if (n == 1) return;  // finished there
   const int2 q_rows = paged_rows(a, s);
   if (tok >= q_rows.y) return;
-  T* out = static_cast<T*>(a.out) + (q_rows.x + tok) * a.out_row + h * a.out_head;
   const bool nothing = n == 0 || paged_length(a, s) - a.tokens + tok < 0;
   auto slot = [&](int i) { return (size_t)(2 * (c0 + i) + (i == 0)) * item_rows + r; };
   const float sink = a.sink ? a.sink[h] * kPagedLog2e : -INFINITY;
@@ -273,17 +273,18 @@ __global__ void __launch_bounds__(32 * kJoinWarps) lm_paged_join_kernel(Paged a,
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   const float base = mx == -INFINITY ? 0.0f : mx;
   float sum = 0.0f, v[8] = {};  // columns 4 lane .. and 128 + 4 lane ..
-  for (int i0 = 0; i0 < n; i0 += 32) {
+  for (int i0 = warp; i0 < n; i0 += 32 * PER) {  // lane l: share i0 + PER l
     float f = 0.0f;
-    if (i0 + lane < n) {
-      const float2 ml = w.part_ml[slot(i0 + lane)];
+    if (i0 + PER * lane < n) {
+      const float2 ml = w.part_ml[slot(i0 + PER * lane)];
       f = exp2f(ml.x - base);
       sum = fmaf(f, ml.y, sum);
     }
-#pragma unroll 4
-    for (int i = 0; i < min(32, n - i0); ++i) {
+    const int here = min(32, (n - i0 + PER - 1) / PER);
+#pragma unroll 8
+    for (int i = 0; i < here; ++i) {
       const float fi = __shfl_sync(0xffffffffu, f, i);
-      const float* part = w.part_o + slot(i0 + i) * a.vdim;
+      const float* part = w.part_o + slot(i0 + PER * i) * a.vdim;
 #pragma unroll
       for (int c = 0; c < 2; ++c)
         if (c * 128 + lane * 4 < a.vdim) {
@@ -295,12 +296,25 @@ __global__ void __launch_bounds__(32 * kJoinWarps) lm_paged_join_kernel(Paged a,
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const float inv = 1.0f / (sum + exp2f(sink - base));
+  T* out = static_cast<T*>(a.out) + (q_rows.x + tok) * a.out_row + h * a.out_head;
+  if constexpr (PER == 1) {
+    const float inv = 1.0f / (sum + exp2f(sink - base));
 #pragma unroll
-  for (int c = 0; c < 2; ++c)
-    if (c * 128 + lane * 4 < a.vdim)
-      *reinterpret_cast<uint2*>(out + c * 128 + lane * 4) =
-          nothing ? make_uint2(0, 0) : make_uint2(Num<T>::pack(v[c * 4] * inv, v[c * 4 + 1] * inv), Num<T>::pack(v[c * 4 + 2] * inv, v[c * 4 + 3] * inv));
+    for (int c = 0; c < 2; ++c)
+      if (c * 128 + lane * 4 < a.vdim)
+        *reinterpret_cast<uint2*>(out + c * 128 + lane * 4) =
+            nothing ? make_uint2(0, 0) : make_uint2(Num<T>::pack(v[c * 4] * inv, v[c * 4 + 1] * inv), Num<T>::pack(v[c * 4 + 2] * inv, v[c * 4 + 3] * inv));
+  } else {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) *reinterpret_cast<float4*>(&s_v[warp][c * 128 + lane * 4]) = make_float4(v[c * 4], v[c * 4 + 1], v[c * 4 + 2], v[c * 4 + 3]);
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    const float inv = 1.0f / ((s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]) + exp2f(sink - base));
+    for (int d = threadIdx.x * 2; d < a.vdim; d += 64 * kJoinWarps) {
+      const float x = (s_v[0][d] + s_v[1][d]) + (s_v[2][d] + s_v[3][d]), y = (s_v[0][d + 1] + s_v[1][d + 1]) + (s_v[2][d + 1] + s_v[3][d + 1]);
+      *reinterpret_cast<uint32_t*>(out + d) = nothing ? 0u : Num<T>::pack(x * inv, y * inv);
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------ prompts, any head size
@@ -443,10 +457,13 @@ int check_decode(const mllmb200_lm_pages* p, const mllmb200_lm_look* l, Paged* a
   return a->tokens > 16 ? MLLMB200_UNSUPPORTED : MLLMB200_OK;
 }
 
+// An item lies in kDecCtas / items CTAs or one more.  One warp a row where that is few (five tokens of 32 sequences with 4 key heads: the
+// whole call 132 us, with four warps 139), four where it is many (one token of one sequence of 60000, 2 key heads: 34.5 and 22.0).
 template <class T>
 cudaError_t join_decode(const Paged& a, const DecodeWork& w, int item_rows, cudaStream_t s) {
-  const int rows = std::min(item_rows, a.group * a.tokens);
-  return launch_pdl(lm_paged_join_kernel<T>, dim3(a.seqs * a.kv_heads * w.row_blocks, (rows + kJoinWarps - 1) / kJoinWarps), dim3(32 * kJoinWarps), 0, s, a, w, item_rows);
+  const int rows = std::min(item_rows, a.group * a.tokens), items = a.seqs * a.kv_heads * w.row_blocks;
+  return items * 8 < kDecCtas ? launch_pdl(lm_paged_join_kernel<T, kJoinWarps>, dim3(items, rows), dim3(32 * kJoinWarps), 0, s, a, w, item_rows)
+                              : launch_pdl(lm_paged_join_kernel<T, 1>, dim3(items, (rows + kJoinWarps - 1) / kJoinWarps), dim3(32 * kJoinWarps), 0, s, a, w, item_rows);
 }
 template <class T>
 cudaError_t launch_decode(Paged a, uint8_t* ws, cudaStream_t s) {

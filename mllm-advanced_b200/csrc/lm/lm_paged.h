@@ -95,9 +95,9 @@ struct DecodeWork {
   int row_blocks;
   const int* redo;  // nullptr: always; else only if one of the CTAs' numbers is not 0
 };
-// (for all threads of a CTA) blocks of every sequence summed up, base[0 .. seqs]
+// (for all threads of a CTA) blocks of every sequence summed up, base[0 .. seqs]; lengths: kept there too unless it is nullptr
 template <int B, int THREADS, class N>
-__device__ __forceinline__ void sum_blocks(const Paged& a, N* base) {
+__device__ __forceinline__ void sum_blocks(const Paged& a, N* base, int* lengths = nullptr) {
   __shared__ N s_warp[THREADS / 32];
   constexpr int kEach = (kDecSeqs + THREADS - 1) / THREADS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, s0 = tid * kEach;
@@ -106,6 +106,7 @@ __device__ __forceinline__ void sum_blocks(const Paged& a, N* base) {
   for (int i = 0; i < kEach; ++i) {
     if (s0 + i < a.seqs) {
       const int len = paged_length(a, s0 + i);
+      if (lengths) lengths[s0 + i] = len;
       run += paged_seen<B>(a, len - a.tokens, len - 1).blocks;
     }
     sum[i] = run;

@@ -572,14 +572,14 @@ struct Share {  // a CTA's part of an item
   bool begins, whole;
   Seen all;  // what the sequence's rows see: the blocks; the item's own rows are at p_first .. p_last
 };
-__device__ __forceinline__ Share share_at(const Paged& a, const int* base, int row_blocks, int tpi, int b, int end) {
+__device__ __forceinline__ Share share_at(const Paged& a, const int* base, const int* lengths, int row_blocks, int tpi, int b, int end) {
   Share g;
   const int items = a.kv_heads * row_blocks;
   int s = 0;
   for (int step = kDecSeqs / 2; step; step /= 2)
     if (s + step < a.seqs && base[s + step] * items <= b) s += step;
   g.seq = s;
-  const int len = paged_length(a, s);
+  const int len = lengths[s];
   g.all = paged_seen<kTcKeys>(a, len - a.tokens, len - 1);
   const int in_seq = b - base[s] * items, item = in_seq / g.all.blocks, rb = item % row_blocks;
   g.blk0 = in_seq - item * g.all.blocks;
@@ -612,7 +612,7 @@ struct DecLayout {
   static constexpr int kP = 128 * NP * 2;       // weights of a block, one half
   static constexpr int kBufs = NP == 16 ? 2 : 1;  // places for queries and for weights: with more rows keys and values need the room more
   static constexpr int kFixed = 1024 + kBufs * (kQ + 2 * kP);
-  static constexpr int kBlocks = (232448 - 5120 - kFixed) / kTile < 12 ? (232448 - 5120 - kFixed) / kTile : 12;  // (5120: the static part)
+  static constexpr int kBlocks = (232448 - 7168 - kFixed) / kTile < 12 ? (232448 - 7168 - kFixed) / kTile : 12;  // (7168: the static part)
   static constexpr int kV = kBlocks / 2, kK = kBlocks - kV;
   static constexpr int kBytes = kFixed + kBlocks * kTile;
   static constexpr int kColumns = NP <= 16 ? 64 : NP <= 32 ? 128 : 256;  // of tensor memory: S twice, O
@@ -632,7 +632,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
   constexpr int kC = NP < 32 ? NP : 32;  // columns handled at a time
   extern __shared__ uint8_t tc_smem_raw[];
   __shared__ DecBarriers<D, NP> bars;
-  __shared__ int s_base[kDecSeqs + 1];
+  __shared__ int s_base[kDecSeqs + 1], s_len[kDecSeqs];
   __shared__ float s_max[4][NP];
   __shared__ __align__(16) float s_ref[NP], s_alpha[NP], s_base2[NP], s_far[BIAS ? NP : 1];  // the rows' maxima by warp; the one in use, times scale (base 2); what is added to scores; the bias of far keys
   __shared__ uint32_t s_tmem;
@@ -657,7 +657,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
     tmem_alloc(&s_tmem, L::kColumns);
     tmem_relinquish();
   }
-  sum_blocks<kTcKeys, kDecThreads>(a, s_base);
+  sum_blocks<kTcKeys, kDecThreads>(a, s_base, s_len);
   if (blockIdx.x == 0)
     for (int i = tid; i <= a.seqs; i += kDecThreads) w.base[i] = s_base[i];
   for (int s = blockIdx.x; s < a.seqs; s += gridDim.x) {  // sequences without keys
@@ -689,7 +689,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
     Share g;
   } p{start, 0, 0, {}};
   auto enter = [&](Place& q) {  // block q.b: its share
-    if (q.i == 0) q.g = share_at(a, s_base, w.row_blocks, tpi, q.b, end);
+    if (q.i == 0) q.g = share_at(a, s_base, s_len, w.row_blocks, tpi, q.b, end);
   };
   auto leave = [&](Place& q) {
     ++q.b;
