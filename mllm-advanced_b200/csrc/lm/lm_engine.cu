@@ -1156,16 +1156,37 @@ void give_pages(Engine* e, int s, int from) {
     if (v[i] >= 0) e->free_pages.push_back(v[i]);
   v.resize(std::min(v.size(), (size_t)from));
 }
-// Gives up the pages that no later token of the slot sees in any layer (what runs on the stream still does, and whoever takes
-// them writes behind it).
-void leave_window(Engine* e, int s) {
-  if (!e->paged || !e->window) return;
-  auto& v = e->slot_pages[s];
-  const int page = e->c.page, first = (e->keep_first + page - 1) / page;
-  for (int i = (e->pos[s] - e->window + 1) / page - 1; i >= first && v[i] >= 0; --i) {
-    e->free_pages.push_back(v[i]);
-    v[i] = -1;
+// Pages that no token of the slot from kRewind before its current end on sees in any layer: places [first, last] of those still held.
+constexpr int kRewind = 64;
+std::pair<int, int> left_behind(const Engine* e, int s) {
+  if (!e->window) return {0, -1};
+  const auto& v = e->slot_pages[s];
+  const int page = e->c.page, last = (e->pos[s] - kRewind - e->window + 1) / page - 1;
+  int first = std::max((e->keep_first + page - 1) / page, 0);
+  while (first <= last && v[first] < 0) ++first;
+  return {first, last};
+}
+// Takes the pages for every slot's first `length` positions, after what the windows have left behind has been given up (what runs on
+// the stream still reads it, and whoever takes it writes behind that).  This happens when a slot moves on, not at a step's end: it
+// can be taken back to where its last step began, and by kRewind tokens.  False, and nothing changed: too few are free.
+bool move_on(Engine* e, int count, const int* slots, const std::vector<int>& length, long long* lacking, long long* there) {
+  *lacking = 0;
+  *there = (long long)e->free_pages.size();
+  for (int i = 0; i < count; ++i) {
+    const auto left = left_behind(e, slots[i]);
+    *lacking += pages_lacking(e, slots[i], length[i]);
+    *there += std::max(0, left.second - left.first + 1);
   }
+  if (*lacking > *there) return false;
+  for (int i = 0; i < count; ++i) {
+    const auto left = left_behind(e, slots[i]);
+    for (int k = left.first; k <= left.second; ++k) {
+      e->free_pages.push_back(e->slot_pages[slots[i]][k]);
+      e->slot_pages[slots[i]][k] = -1;
+    }
+  }
+  for (int i = 0; i < count; ++i) take_pages(e, slots[i], length[i]);
+  return true;
 }
 void table_row(const Engine* e, int s, int* row) {
   for (int i = 0; i < e->max_pages; ++i) row[i] = i < (int)e->slot_pages[s].size() ? e->slot_pages[s][i] : -1;
@@ -1205,10 +1226,10 @@ int step(Engine* e, int n_entries, const int* slots, const int* counts, const in
     if (want[i] < 0 || want[i] >= rows) return fail(e, MLLMB200_INVALID_ARG, "wanted place %d of %d rows", want[i], rows);
 
   if (e->paged) {
-    long long lacking = 0;
-    for (const Entry& en : entries) lacking += pages_lacking(e, en.slot, en.pos0 + en.count);
-    if (lacking > (long long)e->free_pages.size()) return fail(e, MLLMB200_TOO_LARGE, "%lld pages for the step, %zu are free", lacking, e->free_pages.size());
-    for (const Entry& en : entries) take_pages(e, en.slot, en.pos0 + en.count);
+    std::vector<int> ends(n_entries);
+    for (int i = 0; i < n_entries; ++i) ends[i] = entries[i].pos0 + entries[i].count;
+    long long lacking, there;
+    if (!move_on(e, n_entries, slots, ends, &lacking, &there)) return fail(e, MLLMB200_TOO_LARGE, "%lld pages for the step, %lld are free", lacking, there);
   }
 
   std::vector<int2> row_sp(rows), chunks, entry_chunks(n_entries);
@@ -1369,7 +1390,6 @@ int step(Engine* e, int n_entries, const int* slots, const int* counts, const in
     e->pos[en.slot] = en.pos0 + en.count;
     e->tail[en.slot] ^= 1;
     e->ready[en.slot] = do_sample != 0;
-    leave_window(e, en.slot);
   }
   return MLLMB200_OK;
 }
@@ -1414,14 +1434,12 @@ int decode(Engine* e, int count, const int* slots, int steps) {
     longest = std::max(longest, e->pos[s]);
   }
   if (e->paged) {
-    long long lacking = 0;
-    for (int i = 0; i < count; ++i) lacking += pages_lacking(e, slots[i], e->pos[slots[i]] + steps);
-    if (lacking > (long long)e->free_pages.size()) return fail(e, MLLMB200_TOO_LARGE, "%lld pages for the steps, %zu are free", lacking, e->free_pages.size());
+    std::vector<int> ends(count);
+    for (int i = 0; i < count; ++i) ends[i] = e->pos[slots[i]] + steps;
+    long long lacking, there;
+    if (!move_on(e, count, slots, ends, &lacking, &there)) return fail(e, MLLMB200_TOO_LARGE, "%lld pages for the steps, %lld are free", lacking, there);
     std::vector<int> table((size_t)count * e->max_pages);
-    for (int i = 0; i < count; ++i) {
-      take_pages(e, slots[i], e->pos[slots[i]] + steps);
-      table_row(e, slots[i], table.data() + (size_t)i * e->max_pages);
-    }
+    for (int i = 0; i < count; ++i) table_row(e, slots[i], table.data() + (size_t)i * e->max_pages);
     LM_CUDA(cudaMemcpyAsync(e->d_table, table.data(), table.size() * 4, cudaMemcpyHostToDevice, e->stream));  // (from pageable memory: copied when this returns)
   }
   std::vector<int> now(slots, slots + count);
@@ -1460,7 +1478,6 @@ int decode(Engine* e, int count, const int* slots, int steps) {
       e->tail[s] ^= 1;
     }
   }
-  for (int s : now) leave_window(e, s);
   return MLLMB200_OK;
 }
 

@@ -122,12 +122,16 @@ def generate_drafted(model, draft, prompts, max_new, drafts=4, temperature=0.0, 
             raise ValueError("models with retention or an input convolution cannot take drafted tokens back")
     if draft.vocab != model.vocab:
         raise ValueError("the draft model has another vocabulary")
-    if drafts < 1 or drafts + 1 > min(model.max_rows, draft.max_rows):
+    if not 1 <= drafts <= 64 or drafts + 1 > min(model.max_rows, draft.max_rows):  # (models with windows go back by 64 tokens)
         raise ValueError(f"{drafts} drafts a round")
     waiting, running, out = deque(enumerate(prompts)), {}, [None] * len(prompts)
     for p in prompts:
         if not len(p) or max_new < 1 or len(p) + max_new > min(model.max_ctx, draft.max_ctx):
             raise ValueError("a request needs a prompt, at least one new token, and room for both in a slot of both models")
+    held = lambda m, n: -(-(n + max_new) // m.page) if m.page else 0  # pages that a prompt of n tokens and what follows it take
+    for m in (model, draft):
+        if any(held(m, len(p)) > m.pages for p in prompts):
+            raise ValueError(f"a request does not fit {m.pages} pages of {m.page}")
     gen = torch.Generator(device="cuda").manual_seed(seed)
     rand = lambda *shape: torch.rand(shape, generator=gen, device="cuda")
 
@@ -170,6 +174,8 @@ def generate_drafted(model, draft, prompts, max_new, drafts=4, temperature=0.0, 
 
     while waiting or running:
         while waiting:
+            if any(sum(held(m, r.start) for r in running.values()) + held(m, len(waiting[0][1])) > m.pages for m in (model, draft)):
+                break
             slots = model.acquire(), draft.acquire()
             if None in slots:
                 for m, s in zip((model, draft), slots):

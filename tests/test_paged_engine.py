@@ -120,14 +120,16 @@ def test_pages_are_counted_and_given_up(tmp_path):
     m.step([(a, case.tokens(100))])
     # 7 pages; position 100 sees from 31 on (window 70): place 0 holds the first tokens, place 1 (positions 16 .. 31) still shows one
     assert m.free_pages() == 23
-    m.step([(a, case.tokens(29, 1))], [28], sample=True)  # 129 tokens, 9 pages; positions 16 .. 59 are behind every window
-    assert m.free_pages() == 30 - 9 + 2
-    m.decode([a], 63)                       # 192 tokens, 12 pages; 16 .. 122
-    assert m.free_pages() == 30 - 12 + 6
+    m.step([(a, case.tokens(29, 1))], [28], sample=True)  # 129 tokens, 9 pages
+    assert m.free_pages() == 30 - 9
+    m.decode([a], 63)                       # 192 tokens, 12 pages; at 129 nothing was behind a window of 70 and 64 tokens to go back
+    assert m.free_pages() == 30 - 12
+    m.decode([a], 0)                        # 16 .. 58 are behind now: places 1 and 2
+    assert m.free_pages() == 30 - 12 + 2
     b = m.acquire()
     with pytest.raises(lm.EngineError) as e:
         m.step([(b, case.tokens(500, 2))])
-    assert e.value.status == 6 and m.length[b] == 0 and m.free_pages() == 24
+    assert e.value.status == 6 and m.length[b] == 0 and m.free_pages() == 20
     with pytest.raises(lm.EngineError):
         m.decode([a], 400)
     m.step([(b, case.tokens(300, 2))])
@@ -228,6 +230,46 @@ def test_greedy_tokens_with_drafts(other, tmp_path):
         scheduler.generate_drafted(model, draft, [[1]], 300)
     model.close()
     draft.close()
+
+
+@gpu
+def test_drafts_over_pages(tmp_path):
+    """A model of attention layers without a convolution, on pages: taken back and forth over them, one request at a time where the
+    pages hold no more; the tokens are its own greedy ones, but for near ties (a step of other shapes rounds otherwise)."""
+    rng = np.random.default_rng(5)
+    V_, W = 97, 64
+
+    def model(pages, seed):
+        layers = [dict(mixer=lm.ATTENTION, heads=4, kv_heads=2, dim=16, vdim=16, score_scale=0.25, sink=1, bias_rows=8, bias_max=20, window=24, keep=2, ff=48, ff_limit=2.0)] * 2
+        m = lm.LanguageModel(dict(vocab=V_, width=W, conv_taps=0, max_seqs=3, max_ctx=160, max_rows=160, eps=1e-5, logit_scale=1.0, page=16, pages=pages), layers)
+        r = np.random.default_rng(seed)
+        bf = lambda n, k, s=1.0: M.f32_to_bf16((r.standard_normal((n, k)) * s / np.sqrt(k)).astype(np.float32))
+        m.set_tensor(-1, "embed", bf(V_, W, 8.0))
+        m.set_tensor(-1, "head", bf(V_, W, 3.0))
+        m.set_tensor(-1, "final_norm", np.float32(1.0))
+        for i in range(2):
+            for name, n, k in (("q", 64, W), ("k", 32, W), ("v", 32, W), ("o", W, 64), ("gate", 48, W), ("up", 48, W), ("down", W, 48)):
+                m.set_tensor(i, name, bf(n, k))
+            m.set_tensor(i, "rel", r.standard_normal((8, 4)).astype(np.float32))
+            for name in ("norm1", "norm1b", "norm2", "norm2b"):
+                m.set_tensor(i, name, np.float32(1.0))
+        return m
+
+    prompts = [rng.integers(0, V_, n).tolist() for n in (40, 3, 17)]
+    target, small = model(30, 1), model(30, 2)
+    want = scheduler.generate(target, prompts, 40)
+    for pages in (30, 5):  # 80 tokens are 5 pages
+        m = model(pages, 1)
+        got = scheduler.generate_drafted(m, small, prompts, 40, 3)
+        assert m.free_pages() == pages and [len(x) for x in got] == [40] * 3
+        agree = [next((i for i, (a, b) in enumerate(zip(x, y)) if a != b), 40) for x, y in zip(got, want)]
+        assert sum(agree) >= 60, agree
+        m.check_device_status()
+        with pytest.raises(ValueError):
+            scheduler.generate_drafted(m, small, [[1] * 110], 40 if pages == 5 else 60)
+        m.close()
+    target.close()
+    small.close()
 
 
 @gpu
