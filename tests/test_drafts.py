@@ -62,6 +62,20 @@ def test_probabilities(dtype, rows, vocab, t):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("t", [0.0, 0.8])
+def test_probabilities_of_long_rows(t):
+    """Rows beyond what a cluster of CTAs holds."""
+    vocab = 200003
+    z = torch.randn((3, vocab), generator=torch.Generator().manual_seed(4)) * 3
+    z[1, 7], z[1, 150000] = 40.0, 40.0
+    z[2, :] = -float("inf")
+    got, want = drafts.probabilities(z.cuda(), t).cpu().double(), softmax64(z, t)
+    arg = 0.0 if t == 0 else torch.nan_to_num((z.double().max(dim=1, keepdim=True).values - z.double()) / t, 0.0)
+    # (as above; a thread adds up vocab / 2048 weights)
+    assert ((got - want).abs() <= want * 2.0 ** -24 * (6 * arg + 8 + vocab / 2048 + 40) + 1e-37).all()
+
+
+@pytest.mark.gpu
 def test_probabilities_of_masked_rows():
     inf, low = float("inf"), torch.finfo(torch.float32).min
     z = torch.randn(8, 3001)
@@ -125,7 +139,7 @@ def run_verify(target, draft, tokens, accept, pick):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("seqs, k, vocab", [(1, 1, 1), (1, 0, 50), (3, 4, 3), (5, 2, 1025), (2, 40, 300), (64, 5, 999), (7, 3, 32000), (2, 8, 151936), (700, 1, 64)])
+@pytest.mark.parametrize("seqs, k, vocab", [(1, 1, 1), (1, 0, 50), (3, 4, 3), (5, 2, 1025), (2, 40, 300), (64, 5, 999), (7, 3, 32000), (2, 8, 151936), (700, 1, 64), (3, 2, 300001)])
 def test_verify(seqs, k, vocab):
     rng = np.random.default_rng(seqs * 1000 + vocab)
     target, draft = rows(rng, (seqs, k + 1, vocab)), rows(rng, (seqs, k, vocab))
