@@ -11,6 +11,11 @@
 //                   made zeros; where what only some rows see is not finite, a weight of 0 would not hide it: the tile is
 //                   done again row-block by row-block on mma.sync (paged_prompt_rows), which can.
 // The weights' rounding to 16 bits (2^-9 of each, independent) is of the size of the output's own; everything else is fp32.
+// Measured on a B200: 8192 tokens, 16 / 4 heads of 128, causal: 243 us (1.13 PFLOP/s, tensor pipe 53 % active); 2571 rows of five sequences with
+// a window of 512, 12 / 2 heads: 27.  Bound by the chain of a tile: scores, their maximum, weights, product; with two tiles a
+// block takes 3900 cycles of which the products need 2048.  Two tiles and not one, since one tile's products hide the other's
+// weights; not three, since S and O of two fill tensor memory's 512 columns.  Scores handed over by halves of 64 keys were slower (276 us:
+// twice the waits for the same chain).
 #include <algorithm>
 #include <atomic>
 #include <mutex>
