@@ -2,7 +2,9 @@
 // of the vocabulary at a time: a cluster of CTAs per row, each holding its part in shared memory or registers, so that the
 // row is read once; what the parts have to tell one another goes through distributed shared memory.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "../device_common.cuh"
 #include "lm_paged.h"
@@ -41,11 +43,11 @@ __device__ __forceinline__ int ld_remote(const int* local, uint32_t rank) {
 constexpr int kRowThreads = 512, kRowWarps = kRowThreads / 32, kRowItems = 10;  // a CTA's part of a row: up to 10 x 4 numbers a thread
 constexpr int kRowMost = 8 * kRowThreads * 4 * kRowItems;                        // a cluster of 8 CTAs holds rows up to here
 
-// Numbers i .. i + 3 of a row, `fill` from `end` on.  VEC: i is a multiple of 4 and the row lies on 4 numbers; else the four are
-// kRowThreads apart.
+// Numbers i .. i + 3 of a row, `fill` before `begin` and from `end` on.  VEC: i is a multiple of 4 and the row lies on 4 numbers; else
+// the four are kRowThreads apart.
 template <bool VEC, class T>
-__device__ __forceinline__ void load4(const T* row, int i, int end, float fill, float (&v)[4]) {
-  if (VEC && i + 3 < end) {
+__device__ __forceinline__ void load4(const T* row, int i, int begin, int end, float fill, float (&v)[4]) {
+  if (VEC && i >= begin && i + 3 < end) {
     if constexpr (sizeof(T) == 4) {
       const float4 x = *reinterpret_cast<const float4*>(row + i);
       v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
@@ -59,9 +61,20 @@ __device__ __forceinline__ void load4(const T* row, int i, int end, float fill, 
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int at = i + e * (VEC ? 1 : kRowThreads);
-      v[e] = at < end ? to_f32(row[at]) : fill;
+      v[e] = at >= begin && at < end ? to_f32(row[at]) : fill;
     }
   }
+}
+// The same as bits, -inf outside: numbers of 16 bits are taken apart when all loads are under way (384 rows of 151936 in bf16 otherwise
+// wait for one load after the other: 147 us).
+template <class T>
+__device__ __forceinline__ uint2 bits4(const T* row, int i, int begin, int end) {
+  if (i >= begin && i + 3 < end) return *reinterpret_cast<const uint2*>(row + i);
+  const uint32_t low = std::is_same<T, __half>::value ? 0xfc00u : 0xff80u;
+  uint32_t b[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) b[e] = i + e >= begin && i + e < end ? reinterpret_cast<const uint16_t*>(row)[i + e] : low;
+  return make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
 }
 // first number of a thread's item k in a part that starts at v0
 template <bool VEC>
@@ -74,96 +87,162 @@ __device__ __forceinline__ int element(int i, int e) { return VEC ? i + e : i + 
 // ------------------------------------------------------------------------------------------ probabilities
 // grid (cluster, rows): every CTA reads its part of the row once, all loads in flight, and keeps it in registers.  A thread takes its
 // weights against its own maximum; the warps' maxima and sums go to every CTA of the cluster, so that one barrier settles the
-// row.  Bound by memory, 8 bytes a number, and by what a CTA does between its loads and its stores (two of them share an SM).  384
-// rows of 151936: 452 us with three passes of scalar loads over the row, 115 with four barriers and exact exponentials.
-template <class T, int ITEMS, bool VEC>
-__global__ void __launch_bounds__(kRowThreads, 2) lm_probability_rows_kernel(const T* __restrict__ logits, long long ld, int vocab, int per, float inv_t, bool greedy,
-                                                                          float* __restrict__ out, long long ld_out) {
-  __shared__ float2 s_pairs[8 * kRowWarps];  // {maximum, sum or place} of every warp of the cluster
+// row.  Bound by memory, 8 bytes a number, and by what a CTA does between its loads and its stores (two of them share an SM).
+// VEC: rows of logits and of probabilities lie alike in groups of four numbers, a row's first number `sh` places into one.
+// AHEAD: grid (cluster, fewer than the rows): a cluster takes every gridDim.y-th row, and copies the next one into shared memory, each
+// thread its own numbers, as soon as it has the current one in registers.
+// 384 rows of 151936, one call after the other: 95 us, 96 with an odd distance of rows, 94 from bf16.  452 with three passes of scalar loads
+// over the row, 115 with four barriers and exact exponentials, 105 where all warps send to all CTAs and so wait for their stores
+// of the row before, 416 where rows of an odd distance are read number by number.
+template <class T, int ITEMS, bool VEC, bool AHEAD>
+__global__ void __launch_bounds__(kRowThreads, 2) lm_probability_rows_kernel(const T* __restrict__ logits, long long ld, int rows, int vocab, int per, float inv_t,
+                                                                          bool greedy, float* __restrict__ out, long long ld_out) {
+  static_assert(VEC || !AHEAD);
+  extern __shared__ uint4 s_ahead[];                       // AHEAD: four numbers a thread and item
+  __shared__ float2 s_warps[kRowWarps], s_ctas[AHEAD ? 2 : 1][8];  // {maximum, sum or place} of every warp, of every CTA (rows in turn)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, ctas = gridDim.x, part = blockIdx.x;
   cluster_arrive_relaxed();
   pdl_launch_dependents();
   pdl_wait_prior();
-  const T* z = logits + blockIdx.y * ld;
-  float* y = out + blockIdx.y * ld_out;
-  const int v0 = min(part * per, vocab), v1 = min(v0 + per, vocab);
-  float x[ITEMS][4], mx = -INFINITY;
+  constexpr int kEach = 4 * sizeof(T);
+  const uint32_t place = smem_u32(s_ahead);
+  auto shift = [&](const T* z) { return VEC ? (int)(reinterpret_cast<uintptr_t>(z) / sizeof(T) & 3) : 0; };
+  auto request = [&](int row, int me) {
+    const T* z = logits + row * ld;
+    const int sh = shift(z), v1 = min(part * per + per, sh + vocab);
+    z -= sh;
 #pragma unroll
-  for (int k = 0; k < ITEMS; ++k) load4<VEC>(z, item_at<VEC>(v0, k, tid), v1, -INFINITY, x[k]);
-  bool odd = false;  // NaN or +inf
+    for (int k = 0; k < ITEMS; ++k) {
+      const int i = item_at<VEC>(part * per, k, me), n = i >= sh && i + 3 < v1 ? kEach : 0;
+      if constexpr (kEach == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(place + (k * kRowThreads + me) * kEach), "l"(n ? z + i : logits), "r"(n) : "memory");
+      else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(place + (k * kRowThreads + me) * kEach), "l"(n ? z + i : logits), "r"(n) : "memory");
+    }
+    paged_commit();
+  };
+  if (AHEAD) request(blockIdx.y, tid);
+  for (int row = blockIdx.y, turn = 0; row < rows; row += gridDim.y, ++turn) {
+    int me = tid;
+    asm volatile("" : "+r"(me));  // (places are worked out where they are used: there are no registers to keep them)
+    float2* s_pairs = s_ctas[AHEAD ? turn & 1 : 0];
+    const T* z = logits + row * ld;
+    const int sh = shift(z), v0 = part * per, v1 = min(v0 + per, sh + vocab);  // counted from `sh` numbers before the row
+    z -= sh;
+    float x[ITEMS][4], mx = -INFINITY;
+    if (AHEAD) {
+      paged_wait<0>();
 #pragma unroll
-  for (int k = 0; k < ITEMS; ++k)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) odd = odd || !(x[k][e] < INFINITY), mx = fmaxf(mx, x[k][e]);
-  const float t2 = fminf(inv_t * kPagedLog2e, 3.402823466e+38f), base = mx > -INFINITY ? mx : 0.0f;
-  float top = mx, second = 0.0f;  // of the warp
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (greedy) {
-    int at = 0x7fffffff;
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (x[k][e] == top) at = min(at, element<VEC>(item_at<VEC>(v0, k, tid), e));
-    second = __int_as_float((int)__reduce_min_sync(0xffffffffu, (unsigned)at));
-  } else {
-    float sum = 0.0f;
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[k][e] = paged_exp2((x[k][e] - base) * t2);
-        sum += x[k][e];
+      for (int k = 0; k < ITEMS; ++k) {
+        const int i = item_at<VEC>(v0, k, me);
+        if (i >= sh && i + 3 < v1) load4<VEC>(reinterpret_cast<const T*>(s_ahead) + (k * kRowThreads + me) * 4, 0, 0, 4, 0.0f, x[k]);
+        else load4<VEC>(z, i, sh, v1, -INFINITY, x[k]);
       }
-    sum = odd ? __int_as_float(0x7fffffff) : sum * paged_exp2((base - (top > -INFINITY ? top : 0.0f)) * t2);  // (a NaN here is one everywhere)
-    if (mx == -INFINITY && !odd) sum = 0.0f;
+      if (row + gridDim.y < rows) request(row + gridDim.y, me);
+    } else if constexpr (VEC && sizeof(T) == 2) {
+      uint2 bits[ITEMS];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    second = sum;
-  }
-  cluster_wait();  // every CTA has begun
-  if (lane < ctas) {
-    const uint32_t to = map_to_cta(s_pairs + part * kRowWarps + warp, lane);
-    st_cluster_f32(to, top);
-    st_cluster_f32(to + 4, second);
-  }
-  cluster_sync_all();
-  const int n = ctas * kRowWarps;
-  float best = -INFINITY;
-  for (int i = lane; i < n; i += 32) best = fmaxf(best, s_pairs[i].x);
+      for (int k = 0; k < ITEMS; ++k) bits[k] = bits4(z, item_at<VEC>(v0, k, me), sh, v1);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-  if (greedy) {
-    int at = 0x7fffffff;
-    for (int i = lane; i < n; i += 32)
-      if (s_pairs[i].x == best && best > -INFINITY) at = min(at, __float_as_int(s_pairs[i].y));
-    at = (int)__reduce_min_sync(0xffffffffu, (unsigned)at);
+      for (int k = 0; k < ITEMS; ++k)
 #pragma unroll
-    for (int k = 0; k < ITEMS; ++k)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[k][e] = element<VEC>(item_at<VEC>(v0, k, tid), e) == at ? 1.0f : 0.0f;
-  } else {
-    const float at = best > -INFINITY ? best : 0.0f;
-    float total = 0.0f;
-    for (int i = lane; i < n; i += 32) total += s_pairs[i].y == 0.0f ? 0.0f : s_pairs[i].y * paged_exp2((s_pairs[i].x - at) * t2);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const float f = total == 0.0f ? 0.0f : paged_exp2((base - at) * t2) / total;  // (0: nothing but -inf)
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[k][e] = mx == -INFINITY && !odd && total == total ? 0.0f : x[k][e] * f;
-  }
-#pragma unroll
-  for (int k = 0; k < ITEMS; ++k) {
-    const int i = item_at<VEC>(v0, k, tid);
-    if (VEC && i + 3 < v1) {
-      *reinterpret_cast<float4*>(y + i) = make_float4(x[k][0], x[k][1], x[k][2], x[k][3]);
+        for (int e = 0; e < 4; ++e) x[k][e] = to_f32(reinterpret_cast<const T*>(&bits[k])[e]);
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (element<VEC>(i, e) < v1) y[element<VEC>(i, e)] = x[k][e];
+      for (int k = 0; k < ITEMS; ++k) load4<VEC>(z, item_at<VEC>(v0, k, me), sh, v1, -INFINITY, x[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, x[k][e]);
+    const float t2 = fminf(inv_t * kPagedLog2e, 3.402823466e+38f), base = mx > -INFINITY ? mx : 0.0f;
+    float top = mx, second = 0.0f;  // of the warp
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (greedy) {
+      int at = 0x7fffffff;
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (x[k][e] == top) at = min(at, element<VEC>(item_at<VEC>(v0, k, me), e));
+      second = __int_as_float((int)__reduce_min_sync(0xffffffffu, (unsigned)at));
+    } else {
+      float sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[k][e] = paged_exp2((x[k][e] - base) * t2);  // (a NaN, or inf - inf: a NaN, and so the sum, and every probability)
+          sum += x[k][e];
+        }
+      if (sum != 0.0f) sum *= paged_exp2((base - (top > -INFINITY ? top : 0.0f)) * t2);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      second = sum;
+    }
+    // {maximum, sum or place} of those that lanes have
+    auto join = [&](float2 mine) {
+      float best = mine.x;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+      if (greedy) {
+        const unsigned at = mine.x == best && best > -INFINITY ? (unsigned)__float_as_int(mine.y) : 0x7fffffffu;
+        return make_float2(best, __int_as_float((int)__reduce_min_sync(0xffffffffu, at)));
+      }
+      float total = mine.y == 0.0f ? 0.0f : mine.y * paged_exp2((mine.x - (best > -INFINITY ? best : 0.0f)) * t2);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      return make_float2(best, total);
+    };
+    const float2 none = make_float2(-INFINITY, greedy ? __int_as_float(0x7fffffff) : 0.0f);
+    if (lane == 0) s_warps[warp] = make_float2(top, second);
+    if (turn == 0) {
+      __syncwarp();
+      cluster_wait();  // every CTA has begun
+    }
+    __syncthreads();
+    if (warp == 0) {
+      const float2 ours = join(lane < kRowWarps ? s_warps[lane] : none);
+      if (lane < ctas) {
+        const uint32_t to = map_to_cta(s_pairs + part, lane);
+        st_cluster_f32(to, ours.x);
+        st_cluster_f32(to + 4, ours.y);
+      }
+      __syncwarp();
+      cluster_arrive();
+    } else {
+      cluster_arrive_relaxed();  // (with nothing to hand over: it does not wait for the last row's stores)
+    }
+    cluster_wait();
+    asm volatile("" : "+r"(me));
+    const float2 all = join(lane < ctas ? s_pairs[lane] : none);
+    if (greedy) {
+      const int at = __float_as_int(all.y);
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[k][e] = element<VEC>(item_at<VEC>(v0, k, me), e) == at ? 1.0f : 0.0f;
+    } else {
+      const float at = all.x > -INFINITY ? all.x : 0.0f, total = all.y;
+      // (0: nothing but -inf, in the row or among the thread's)
+      const float f = total == 0.0f || (mx == -INFINITY && total == total) ? 0.0f : paged_exp2((base - at) * t2) / total;
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[k][e] *= f;
+    }
+    float* y = out + row * ld_out - sh;
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const int i = item_at<VEC>(v0, k, me);
+      if (VEC && i >= sh && i + 3 < v1) {
+        *reinterpret_cast<float4*>(y + i) = make_float4(x[k][0], x[k][1], x[k][2], x[k][3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (element<VEC>(i, e) >= sh && element<VEC>(i, e) < v1) y[element<VEC>(i, e)] = x[k][e];
+      }
     }
   }
 }
@@ -301,8 +380,8 @@ __global__ void __launch_bounds__(kRowThreads, 2) lm_verify_kernel(VerifyArgs a,
       float x[kAhead][4], y[kAhead][4] = {};
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        load4<VEC>(p, item_at<VEC>(v0, t0 + u, tid), v1, 0.0f, x[u]);
-        if (rest) load4<VEC>(q, item_at<VEC>(v0, t0 + u, tid), v1, 0.0f, y[u]);
+        load4<VEC>(p, item_at<VEC>(v0, t0 + u, tid), 0, v1, 0.0f, x[u]);
+        if (rest) load4<VEC>(q, item_at<VEC>(v0, t0 + u, tid), 0, v1, 0.0f, y[u]);
       }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
@@ -384,8 +463,8 @@ __global__ void __launch_bounds__(kRowThreads, 2) lm_verify_kernel(VerifyArgs a,
     if (which % kRowWarps == warp) {
       const int i = item_at<VEC>(v0, which / kSums, tid), only = which / kRowWarps % 4;
       float x[4], y[4] = {};
-      load4<VEC>(p, i, v1, 0.0f, x);
-      if (rest) load4<VEC>(q, i, v1, 0.0f, y);
+      load4<VEC>(p, i, 0, v1, 0.0f, x);
+      if (rest) load4<VEC>(q, i, 0, v1, 0.0f, y);
       double m[4], up = 0.0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -442,20 +521,52 @@ bool on(const void* p, size_t bytes, long long stride = 0, long long stride2 = 0
   return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride % 4 == 0 && stride2 % 4 == 0;
 }
 
+// Clusters of `ctas` that a device holds at a time, 0 where that is not known.
+template <class T, int ITEMS>
+int resident_clusters(int ctas) {
+  static std::atomic<int> known[64][4];
+  int dev = 0, log = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 0;
+  while (1 << log < ctas) ++log;
+  if ((n = known[dev][log].load(std::memory_order_acquire))) return n;
+  const auto kernel = lm_probability_rows_kernel<T, ITEMS, true, true>;
+  constexpr int smem = ITEMS * kRowThreads * 4 * sizeof(T);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas, 148), cfg.blockDim = dim3(kRowThreads), cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 0;
+  }
+  known[dev][log].store(n, std::memory_order_release);
+  return n;
+}
+
 template <class T>
 cudaError_t launch_probabilities(const void* logits, long long ld, int rows, int vocab, float t, float* out, long long ld_out, cudaStream_t s) {
   const float inv_t = t > 0.0f ? std::fmin(1.0f / t, 3.402823466e+38f) : 0.0f;
-  const bool vec = on(logits, 4 * sizeof(T), ld) && on(out, 16, ld_out);
+  const bool vec = ((reinterpret_cast<uintptr_t>(logits) / sizeof(T) ^ reinterpret_cast<uintptr_t>(out) / 4) & 3) == 0 && (rows == 1 || ((ld ^ ld_out) & 3) == 0);
+  const int places = vocab + (vec && !on(out, 16, rows == 1 ? 0 : ld_out) ? 3 : 0);  // (a row may begin inside a group of four)
   for (int r0 = 0; r0 < rows; r0 += 65535) {
     const int n = std::min(rows - r0, 65535);
     const T* z = static_cast<const T*>(logits) + r0 * ld;
     float* y = out + r0 * ld_out;
     cudaError_t r;
-    if (vocab <= kRowMost) {
-      const RowPlan p = row_plan(n, vocab);
+    if (places <= kRowMost) {
+      const RowPlan p = row_plan(n, places);
       r = with_items(p.items, [&](auto items) {
-        auto go = [&](auto kernel) { return launch_pdl_cluster(kernel, dim3(p.ctas, n), dim3(kRowThreads), dim3(p.ctas, 1, 1), 0, s, z, ld, vocab, p.per, inv_t, t == 0.0f, y, ld_out); };
-        return vec ? go(lm_probability_rows_kernel<T, decltype(items)::value, true>) : go(lm_probability_rows_kernel<T, decltype(items)::value, false>);
+        constexpr int kItems = decltype(items)::value;
+        auto go = [&](auto kernel, int clusters, size_t smem) {
+          return launch_pdl_cluster(kernel, dim3(p.ctas, clusters), dim3(kRowThreads), dim3(p.ctas, 1, 1), smem, s, z, ld, n, vocab, p.per, inv_t, t == 0.0f, y, ld_out);
+        };
+        // (2048 rows of 32000: 89 us with the next row copied ahead, 94 without; 4096 of 2048 22 and 33; clusters of 4 and 8 have enough under way:
+        // 1024 of 65536 110 and 98, 384 of 151936 109 and 95)
+        const int room = vec && p.ctas <= 2 ? resident_clusters<T, kItems>(p.ctas) : 0;
+        if (room && n > room) return go(lm_probability_rows_kernel<T, kItems, true, true>, room, kItems * kRowThreads * 4 * sizeof(T));
+        return vec ? go(lm_probability_rows_kernel<T, kItems, true, false>, n, 0) : go(lm_probability_rows_kernel<T, kItems, false, false>, n, 0);
       });
     } else {
       r = launch_pdl_cluster(lm_probabilities_kernel<T>, dim3(8, n), dim3(kDrThreads), dim3(8, 1, 1), 0, s, z, ld, vocab, inv_t, t == 0.0f, y, ld_out);

@@ -62,6 +62,43 @@ def test_probabilities(dtype, rows, vocab, t):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows, vocab, z_at, z_pad, out_at, out_pad",
+                         [(700, 1003, 0, 0, 0, 0), (400, 32001, 0, 0, 0, 0), (90, 50257, 0, 0, 0, 0), (90, 151935, 1, 2, 5, 2), (400, 32002, 3, 0, 2, 0), (60, 151937, 2, 0, 2, 3), (600, 1, 3, 5, 3, 1)])
+@pytest.mark.parametrize("t", [0.0, 0.8])
+def test_probabilities_of_many_rows(dtype, rows, vocab, z_at, z_pad, out_at, out_pad, t):
+    """More rows than the GPU works on at a time; rows that begin anywhere in groups of four numbers."""
+    g = torch.Generator().manual_seed(rows + vocab)
+    inf = float("inf")
+    z = (torch.randn((rows, vocab), generator=g) * 3).to(dtype)
+    z[rows // 2, vocab // 3:] = -inf
+    z[rows - 1] = torch.finfo(dtype).min
+    z[rows - 2] = -inf
+    z[rows - 3, vocab - 1] = inf
+    z[rows - 4, vocab // 2] = float("nan")
+    apart = torch.full((z_at + rows * (vocab + z_pad),), inf, dtype=dtype, device="cuda")
+    logits = apart[z_at:].view(rows, vocab + z_pad)[:, :vocab]
+    logits.copy_(z)
+    whole = torch.full((out_at + rows * (vocab + out_pad) + 4,), -1.0, device="cuda")
+    out = whole[out_at:out_at + rows * (vocab + out_pad)].view(rows, vocab + out_pad)[:, :vocab]
+    drafts.probabilities(logits, t, out=out)
+    got, want = out.cpu().double(), softmax64(z, t)
+    assert (whole == -1).sum() == out_at + rows * out_pad + 4  # nothing beside the rows
+    if t == 0:
+        assert torch.equal(got, want)
+        return
+    assert got[rows - 3].isnan().all() and got[rows - 4].isnan().all()
+    zd = z.double()
+    arg = torch.nan_to_num((zd.max(dim=1, keepdim=True).values - zd) / t, 0.0, 0.0, 0.0)
+    # In units of 2^-24: an exponent's argument is off by five roundings (difference, 1 / t, log2 e, their product, the whole), 5 |z - m| / t,
+    # and exp2 by 4.  Above the line two exp2, a product and a quotient: 5 arg + 10.  Below it four exp2 (a thread's, warp's, CTA's
+    # and cluster's maximum), the mean of 5 arg under the weights, at most 5 ln(vocab) < 60, and 40 + 15 sums: 131.  1e-37: below 2^-126
+    bound = want * 2.0 ** -24 * (5 * arg + 141) + 1e-37
+    fine = [r for r in range(rows) if r not in (rows - 3, rows - 4)]
+    assert ((got - want).abs() <= bound)[fine].all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("t", [0.0, 0.8])
 def test_probabilities_of_long_rows(t):
     """Rows beyond what a cluster of CTAs holds."""
