@@ -180,6 +180,7 @@ typedef struct mllmb200_lm_look {
   int heads;                         /* a multiple of kv_heads, at most 64 per key head */
   int bias_max, window, keep;
   float scale;
+  int exact;                         /* attn_prompt; 0 or 1, see there */
 } mllmb200_lm_look;
 
 /* New keys [rows][kv_heads][dim] and values [rows][kv_heads][vdim] into the pages (strides as above). */
@@ -190,7 +191,9 @@ MLLMB200_API int mllmb200_lm_pages_append(const mllmb200_lm_pages* pages, const 
 MLLMB200_API int mllmb200_lm_attn_decode_workspace(const mllmb200_lm_pages* pages, const mllmb200_lm_look* look, size_t* bytes);
 MLLMB200_API int mllmb200_lm_attn_decode(const mllmb200_lm_pages* pages, const mllmb200_lm_look* look, void* workspace, void* stream);
 
-/* Any number of tokens of every sequence. */
+/* Any number of tokens of every sequence.  Heads of 64 or 128 on the tensor cores: softmax weights are rounded to the cache's type before they
+ * meet the values (half a step of every weight, an error of the size of the outputs' own rounding), or, look->exact, carried by two numbers of it
+ * (2^-16 and better; a third more time on long prompts).  attn_decode and all other head sizes always carry two. */
 MLLMB200_API int mllmb200_lm_attn_prompt_workspace(const mllmb200_lm_pages* pages, const mllmb200_lm_look* look, size_t* bytes);
 MLLMB200_API int mllmb200_lm_attn_prompt(const mllmb200_lm_pages* pages, const mllmb200_lm_look* look, void* workspace, void* stream);
 

@@ -930,6 +930,7 @@ int paged_mixer(Engine* e, const StepCtx& t, const LayerState& L, const Weights&
   a.bias = d.bias_rows ? w.bias : nullptr;
   a.heads = d.heads, a.group = d.heads / d.kv_heads, a.bias_max = d.bias_max, a.window = d.window, a.keep = d.keep;
   a.scale2 = d.score_scale * kPagedLog2e;
+  a.exact = 1;  // (as attention over slots)
   auto rows = [&](const StepCtx::PagedRows& r) {
     a.seqs = r.n, a.q_start = r.first, a.q_count = r.count, a.lengths = r.lengths, a.table = r.table;
     return r.n > 0;

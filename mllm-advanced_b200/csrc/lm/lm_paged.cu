@@ -448,6 +448,7 @@ int check_look(const mllmb200_lm_pages* p, const mllmb200_lm_look* l, Paged* a) 
   a->heads = l->heads, a->group = l->heads / a->kv_heads, a->bias_max = l->bias_max;
   a->window = std::min(l->window, kLongest), a->keep = std::min(l->keep, kLongest);  // (no position is beyond; differences stay in 32 bits)
   a->scale2 = l->scale * kPagedLog2e;
+  a->exact = l->exact != 0;
   return MLLMB200_OK;
 }
 int check_decode(const mllmb200_lm_pages* p, const mllmb200_lm_look* l, Paged* a) {

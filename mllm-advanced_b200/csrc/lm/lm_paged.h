@@ -24,6 +24,7 @@ struct Paged {
   long long q_row, q_head, out_row, out_head;
   const float *sink, *bias;
   int heads, group, bias_max, window, keep;
+  int exact;           // prompts on tcgen05: weights in two halves of 16 bits
   float scale2;        // scale log2(e): scores are in base 2
 };
 

@@ -2,7 +2,7 @@
 //
 // A CTA owns two tiles of 128 rows; a row is (token, query head) of one kv head, so that all heads of a group share every key
 // and value that is fetched.  Per block of 128 keys and tile: S = Q K^T into tensor memory, softmax weights P in 16 bits over
-// S's own columns, O += P V.  While the weights of one tile are made, the products of the other run:
+// S's own columns, O += P V (64 keys at a time).  While the weights of one tile are made, the products of the other run:
 //   warps 0-3, 4-7  weights of tile 0 and 1, a row per thread; O is rescaled (tensor memory) only when a row's maximum has grown by
 //                   more than 2^8 - weights up to 2^8 are as exact in 16 bits, and their fp32 sum is kept under the same base
 //   warp 8          copies: TMA, pieces of a block that lie in one page, into a ring of keys and one of values
@@ -10,7 +10,10 @@
 //   warps 10-11     values of blocks that some rows do not see in full: rows that no row sees (page tails, other sequences' data) are
 //                   made zeros; where what only some rows see is not finite, a weight of 0 would not hide it: the tile is
 //                   done again row-block by row-block on mma.sync (paged_prompt_rows), which can.
-// The weights' rounding to 16 bits (2^-9 of each, independent) is of the size of the output's own; everything else is fp32.
+// EXACT: a weight is two numbers of 16 bits, the second what the first one's rounding left, and both meet the values.  Without it the weights'
+// rounding (2^-9 of each in bf16, independent) is of the size of the output's own: 2.0e-3 of the 2-norm off instead of 1.5e-3.  The caller
+// chooses: half the products more and their making cost 8192 tokens of 16 / 4 heads of 128 a third (284 and 376 us), and the engine, whose
+// attention over slots carries two numbers, takes EXACT.  Everything else is fp32.
 // Measured on a B200: 8192 tokens, 16 / 4 heads of 128, causal: 243 us (1.13 PFLOP/s, tensor pipe 53 % active); 2571 rows of five sequences with
 // a window of 512, 12 / 2 heads: 27.  Bound by the chain of a tile: scores, their maximum, weights, product; with two tiles a
 // block takes 3900 cycles of which the products need 2048.  Two tiles and not one, since one tile's products hide the other's
@@ -186,21 +189,23 @@ __device__ __forceinline__ float2 pair_exp2(uint64_t x) {
   return pair_parts(pair_mul(p, pair_of(__uint_as_float(__float_as_uint(n.x) << 23), __uint_as_float(__float_as_uint(n.y) << 23))));
 }
 
-// weights 2^(score scale + base) in 16 bits over the scores' columns; their sum.  The special-function unit takes 1024 cycles for a
-// tile's exponentials, as long as both products; every kPoly-th pair goes through the other pipes instead.
+// weights 2^(score scale + base) over the scores' columns: for the 64 keys whose scores lay there 32 columns of weights in 16 bits and, EXACT, 32
+// of what their rounding left, in 16 bits too; their sum.  ready(h): those of keys 64 h and on are there.  The special-function unit takes 1024 cycles for a tile's exponentials, as long as a
+// product of a tile; every kPoly-th pair goes through the other pipes instead.
 constexpr int kPoly = 4;
-template <class T>
-__device__ __forceinline__ float put_weights(uint32_t s_col, float scale, float base) {
+template <class T, bool EXACT, class F>
+__device__ __forceinline__ float put_weights(uint32_t s_col, float scale, float base, F ready) {
   const uint64_t scale2 = pair_of(scale, scale), base2 = pair_of(base, base);
   uint64_t sum[2] = {0, 0};
 #pragma unroll 1
   for (int c = 0; c < 128; c += 64) {
-    uint32_t v[2][32], w[2][16];
+    uint32_t v[2][32];
     tmem_ld32(s_col + c, v[0]);
     tmem_ld32(s_col + c + 32, v[1]);
     tmem_ld_wait();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      uint32_t hi[16], lo[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const uint64_t x = pair_fma(pair_of(__uint_as_float(v[h][2 * i]), __uint_as_float(v[h][2 * i + 1])), scale2, base2);
@@ -212,10 +217,17 @@ __device__ __forceinline__ float put_weights(uint32_t s_col, float scale, float 
           e = make_float2(paged_exp2(y.x), paged_exp2(y.y));
         }
         sum[i & 1] = pair_add(sum[i & 1], pair_of(e.x, e.y));
-        w[h][i] = Num<T>::pack(e.x, e.y);
+        hi[i] = Num<T>::pack(e.x, e.y);
+        if constexpr (EXACT) {
+          const float2 up = Num<T>::unpack(hi[i]);
+          lo[i] = Num<T>::pack(e.x - up.x, e.y - up.y);
+        }
       }
-      tmem_st16(s_col + c / 2 + h * 16, w[h]);
+      tmem_st16(s_col + c + h * 16, hi);
+      if constexpr (EXACT) tmem_st16(s_col + c + 32 + h * 16, lo);
     }
+    tmem_st_wait();
+    ready(c / 64);
   }
   const float2 total = pair_parts(pair_add(sum[0], sum[1]));
   return total.x + total.y;
@@ -230,10 +242,10 @@ struct PromptSplit {
 };
 
 struct TcBarriers {
-  uint64_t q_full, k_full[4], k_free[4], v_full[4], v_free[4], v_fixed[4], s_full[2], p_ready[2], o_done[2];
+  uint64_t q_full, k_full[4], k_free[4], v_full[4], v_free[4], v_fixed[4], s_full[2], p_ready[2][2], o_done[2];
 };
 
-template <class T, int D, bool BIAS>
+template <class T, int D, bool BIAS, bool EXACT>
 __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const __grid_constant__ Paged a, const __grid_constant__ CUtensorMap qmap,
                                                                            const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                                                                            int piece, PromptSplit w) {
@@ -259,7 +271,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
     mbar_init(&bars.q_full, 1);
     for (int i = 0; i < L::kK; ++i) mbar_init(&bars.k_full[i], 1), mbar_init(&bars.k_free[i], 1);
     for (int i = 0; i < L::kV; ++i) mbar_init(&bars.v_full[i], 1), mbar_init(&bars.v_free[i], 1), mbar_init(&bars.v_fixed[i], 2);
-    for (int i = 0; i < 2; ++i) mbar_init(&bars.s_full[i], 1), mbar_init(&bars.p_ready[i], 4), mbar_init(&bars.o_done[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&bars.s_full[i], 1), mbar_init(&bars.p_ready[i][0], 4), mbar_init(&bars.p_ready[i][1], 4), mbar_init(&bars.o_done[i], 1);
     s_bad = s_gave_up = 0;
     mbar_fence_init();
   }
@@ -375,18 +387,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
           ok = all_wait(&bars.v_full[j % L::kV], turn(j, L::kV)) && all_wait(&bars.v_fixed[j % L::kV], turn(j, L::kV));
           if (ok && j + 1 < nt) ok = all_wait(&bars.k_full[(j + 1) % L::kK], turn(j + 1, L::kK));
           for (int t = 0; t < tiles && ok; ++t) {
-            ok = all_wait(&bars.p_ready[t], (uint32_t)j & 1u);
-            if (!ok) break;
-            tc_fence_after();
-            if (issuer) {
-              const uint64_t v = tc_desc(values0 + j % L::kV * L::kTile, 16384);
+            for (int h = 0; h < 2 && ok; ++h) {  // keys 64 h and on: the products of the first 64 run while the other weights are made
+              ok = all_wait(&bars.p_ready[t][h], (uint32_t)j & 1u);
+              if (!ok) break;
+              tc_fence_after();
+              if (issuer) {
+                const uint64_t v = tc_desc(values0 + j % L::kV * L::kTile, 16384);
 #pragma unroll
-              for (int ks = 0; ks < kTcKeys / 16; ++ks)
-                tc_mma_f16_ts(tmem + 256 + t * D, tmem + t * 128 + ks * 8, v + (uint64_t)(ks * 128), idesc_o, j > 0 || ks > 0);
-              if (t == tiles - 1) tc_commit(&bars.v_free[j % L::kV]);
-              if (j == nt - 1) tc_commit(&bars.o_done[t]);
+                for (int ks = 0; ks < (EXACT ? 8 : 4); ++ks)  // the weights, then what their rounding left
+                  tc_mma_f16_ts(tmem + 256 + t * D, tmem + t * 128 + h * 64 + ks * 8, v + (uint64_t)((h * 4 + (ks & 3)) * 128), idesc_o, j > 0 || h > 0 || ks > 0);
+                if (h == 1 && t == tiles - 1) tc_commit(&bars.v_free[j % L::kV]);
+                if (h == 1 && j == nt - 1) tc_commit(&bars.o_done[t]);
+              }
+              __syncwarp();
             }
-            __syncwarp();
+            if (!ok) break;
             if (j + 1 < nt) scores(t, j + 1, t == tiles - 1);
           }
         }
@@ -455,11 +470,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
           rescale<D>(o_col, alpha);
         }
       }
-      l += put_weights<T>(s_col, scale, m == -INFINITY ? 0.0f : -m * scale);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.p_ready[t]);
+      l += put_weights<T, EXACT>(s_col, scale, m == -INFINITY ? 0.0f : -m * scale, [&](int h) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.p_ready[t][h]);
+      });
     }
     if (n) ok = ok && __all_sync(0xffffffffu, wait(&bars.o_done[t], 0));
     tc_fence_after();
@@ -1064,10 +1079,10 @@ bool encode(CUtensorMap* map, CUtensorMapDataType type, const void* base, const 
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class T, int D, bool BIAS>
+template <class T, int D, bool BIAS, bool EXACT>
 cudaError_t configure() {
   static std::atomic<unsigned long long> done{0};
-  return once_per_device(&done, [] { return cudaFuncSetAttribute(lm_paged_prompt_tc_kernel<T, D, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<D, BIAS>::kBytes); });
+  return once_per_device(&done, [] { return cudaFuncSetAttribute(lm_paged_prompt_tc_kernel<T, D, BIAS, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<D, BIAS>::kBytes); });
 }
 long long prompt_ctas(const Paged& a) {
   const int toks = 2 * (128 / a.group);
@@ -1091,9 +1106,14 @@ cudaError_t launch(const Paged& a, const CUtensorMap& q, const CUtensorMap& k, c
     w.flags = reinterpret_cast<int*>(w.part_ml + rows);
   }
   const dim3 grid((unsigned)prompt_ctas(a), w.parts);
-  auto go = [&](auto kernel, size_t smem, cudaError_t r) { return r != cudaSuccess ? r : launch_pdl(kernel, grid, dim3(kTcThreads), smem, s, a, q, k, v, piece, w); };
-  const cudaError_t r = a.bias ? go(lm_paged_prompt_tc_kernel<T, D, true>, TcLayout<D, true>::kBytes, configure<T, D, true>())
-                               : go(lm_paged_prompt_tc_kernel<T, D, false>, TcLayout<D, false>::kBytes, configure<T, D, false>());
+  auto go = [&](auto bias, auto exact) {
+    constexpr bool BIAS = decltype(bias)::value, EXACT = decltype(exact)::value;
+    const cudaError_t c = configure<T, D, BIAS, EXACT>();
+    return c != cudaSuccess ? c : launch_pdl(lm_paged_prompt_tc_kernel<T, D, BIAS, EXACT>, grid, dim3(kTcThreads), TcLayout<D, BIAS>::kBytes, s, a, q, k, v, piece, w);
+  };
+  const std::true_type yes;
+  const std::false_type no;
+  const cudaError_t r = a.bias ? a.exact ? go(yes, yes) : go(yes, no) : a.exact ? go(no, yes) : go(no, no);
   return r != cudaSuccess || w.parts == 1 ? r : launch_pdl(lm_paged_prompt_join_kernel<T, D>, dim3(grid.x, 8), dim3(256), 0, s, a, w);
 }
 

@@ -19,7 +19,7 @@ from . import lm
 from .binding import _allocator
 
 _PAGES = struct.Struct("@PP6q3P10i")
-_LOOK = struct.Struct("@PP4qPP4if4x")
+_LOOK = struct.Struct("@PP4qPP4ifi")
 _DTYPES = {torch.bfloat16: lm.BF16, torch.float16: lm.F16}
 _INT, _F32 = torch.int32, torch.float32
 _sizes = {}  # bytes of workspace by sizes
@@ -91,7 +91,7 @@ def append(k_pages, v_pages, k, v, table, lengths, q_start=None, stream=None):
         _fail("append", st)
 
 
-def _attention(where, q, k_pages, v_pages, table, lengths, q_start, scale, window, keep, sink, bias, out, stream):
+def _attention(where, q, k_pages, v_pages, table, lengths, q_start, scale, window, keep, sink, bias, out, stream, exact):
     try:
         rows, heads, dim = q.shape
     except ValueError:
@@ -116,7 +116,7 @@ def _attention(where, q, k_pages, v_pages, table, lengths, q_start, scale, windo
         o = out if out is not None else torch.empty_like(q) if vdim == dim and whole else q.new_empty((rows, heads, vdim))
         o_row, o_head = (heads * vdim, vdim) if out is None else (out.stride(0), out.stride(1))
         look = _LOOK.pack(q.data_ptr(), o.data_ptr(), q_row, q_head, o_row, o_head, 0 if sink is None else sink.data_ptr(), 0 if bias is None else bias.data_ptr(), heads,
-                          0 if bias is None else bias.shape[1] - 1, window, keep, dim ** -0.5 if scale is None else scale)
+                          0 if bias is None else bias.shape[1] - 1, window, keep, dim ** -0.5 if scale is None else scale, exact)
         need = _sizes.get(key)
         if need is None:  # (a function of the sizes)
             n = C.c_size_t()
@@ -148,15 +148,17 @@ def decode_attention(q, k_pages, v_pages, table, lengths, scale=None, window=0, 
     A token at position i sees key j if j <= i and (no window, or j > i - window, or j < keep).  Scores are scale q.k (default
     dim ** -0.5) + bias[head, min(i - j, distances - 1)]; sink: one more score per head, without a value.  A token that sees
     nothing gives zeros."""
-    return _attention("decode_attention", q, k_pages, v_pages, table, lengths, None, scale, window, keep, sink, bias, out, stream)
+    return _attention("decode_attention", q, k_pages, v_pages, table, lengths, None, scale, window, keep, sink, bias, out, stream, False)
 
 
-def prompt_attention(q, k_pages, v_pages, table, lengths, q_start, scale=None, window=0, keep=0, sink=None, bias=None, out=None, stream=None):
+def prompt_attention(q, k_pages, v_pages, table, lengths, q_start, scale=None, window=0, keep=0, sink=None, bias=None, out=None, stream=None, exact=False):
     """The same for any number of tokens per sequence: sequence s has the rows q_start[s] .. q_start[s + 1] - 1 of q.  Rows behind
-    the last sequence are left as they are in `out`."""
+    the last sequence are left as they are in `out`.  exact: softmax weights meet the values as two numbers of 16 bits, as in
+    decode_attention; without it heads of 64 and 128 round them to one, which errs about as much as the outputs' own rounding and
+    is faster."""
     if q_start is None:
         raise ValueError("prompt_attention: q_start")
-    return _attention("prompt_attention", q, k_pages, v_pages, table, lengths, q_start, scale, window, keep, sink, bias, out, stream)
+    return _attention("prompt_attention", q, k_pages, v_pages, table, lengths, q_start, scale, window, keep, sink, bias, out, stream, bool(exact))
 
 
 def check(stream=None):
