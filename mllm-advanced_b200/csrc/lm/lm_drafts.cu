@@ -40,6 +40,16 @@ __device__ __forceinline__ int ld_remote(const int* local, uint32_t rank) {
   return v;
 }
 
+// Cluster barriers in the form that wants nothing of the warps: what stands before them here depends on the lane, and the .aligned form is
+// only defined where a warp's threads execute it together.
+__device__ __forceinline__ void cluster_here() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_here_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void cluster_all() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ void cluster_meet() {
+  cluster_here();
+  cluster_all();
+}
+
 constexpr int kRowThreads = 512, kRowWarps = kRowThreads / 32, kRowItems = 10;  // a CTA's part of a row: up to 10 x 4 numbers a thread
 constexpr int kRowMost = 8 * kRowThreads * 4 * kRowItems;                        // a cluster of 8 CTAs holds rows up to here
 
@@ -101,7 +111,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) lm_probability_rows_kernel(con
   extern __shared__ uint4 s_ahead[];                       // AHEAD: four numbers a thread and item
   __shared__ float2 s_warps[kRowWarps], s_ctas[AHEAD ? 2 : 1][8];  // {maximum, sum or place} of every warp, of every CTA (rows in turn)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, ctas = gridDim.x, part = blockIdx.x;
-  cluster_arrive_relaxed();
+  cluster_here_relaxed();
   pdl_launch_dependents();
   pdl_wait_prior();
   constexpr int kEach = 4 * sizeof(T);
@@ -199,7 +209,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) lm_probability_rows_kernel(con
     if (lane == 0) s_warps[warp] = make_float2(top, second);
     if (turn == 0) {
       __syncwarp();
-      cluster_wait();  // every CTA has begun
+      cluster_all();  // every CTA has begun
     }
     __syncthreads();
     if (warp == 0) {
@@ -210,11 +220,11 @@ __global__ void __launch_bounds__(kRowThreads, 2) lm_probability_rows_kernel(con
         st_cluster_f32(to + 4, ours.y);
       }
       __syncwarp();
-      cluster_arrive();
+      cluster_here();
     } else {
-      cluster_arrive_relaxed();  // (with nothing to hand over: it does not wait for the last row's stores)
+      cluster_here_relaxed();  // (with nothing to hand over: it does not wait for the last row's stores)
     }
-    cluster_wait();
+    cluster_all();
     asm volatile("" : "+r"(me));
     const float2 all = join(lane < ctas ? s_pairs[lane] : none);
     if (greedy) {
@@ -277,13 +287,13 @@ __global__ void __launch_bounds__(kDrThreads) lm_probabilities_kernel(const T* _
   odd = __syncthreads_or(odd);
   for (int w = 0; w < kDrWarps; ++w) better(mx, at, s_red[w], s_at[w]);
   if (tid == 0) s_max = mx, s_first = at, s_sum = odd ? 1.0f : 0.0f;
-  if (ctas > 1) cluster_sync_all();
+  if (ctas > 1) cluster_meet();
   else __syncthreads();
   for (int r = 0; r < ctas; ++r) {
     better(mx, at, ctas > 1 ? ld_remote(&s_max, r) : s_max, ctas > 1 ? ld_remote(&s_first, r) : s_first);
     odd = odd || (ctas > 1 ? ld_remote(&s_sum, r) : s_sum) != 0.0f;
   }
-  if (ctas > 1) cluster_sync_all();
+  if (ctas > 1) cluster_meet();
   else __syncthreads();
   if (greedy) {
     for (int i = v0 + tid; i < v1; i += kDrThreads) y[i] = i == at ? 1.0f : 0.0f;
@@ -301,11 +311,11 @@ __global__ void __launch_bounds__(kDrThreads) lm_probabilities_kernel(const T* _
     for (int w = 0; w < kDrWarps; ++w) sum += s_red[w];
     s_sum = sum;
   }
-  if (ctas > 1) cluster_sync_all();
+  if (ctas > 1) cluster_meet();
   else __syncthreads();
   sum = 0.0f;
   for (int r = 0; r < ctas; ++r) sum += ctas > 1 ? ld_remote(&s_sum, r) : s_sum;
-  if (ctas > 1) cluster_sync_all();
+  if (ctas > 1) cluster_meet();
   for (int i = v0 + tid; i < v1; i += kDrThreads)
     y[i] = odd ? __int_as_float(0x7fffffff) : mx > -INFINITY ? expf((to_f32(z[i]) - mx) * inv_t) / sum : 0.0f;
 }
@@ -406,7 +416,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) lm_verify_kernel(VerifyArgs a,
       v = warp_sum(v);
       if (lane == 0) s_sum = v;
     }
-    cluster_sync_all();
+    cluster_meet();
     total = before = 0.0;
     for (int r = 0; r < ctas; ++r) {
       const double v = ld_remote(&s_sum, r);
@@ -415,7 +425,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) lm_verify_kernel(VerifyArgs a,
     }
     if (total > 0.0 || !rest) break;
     rest = false;  // refused, and nothing is left of the target's numbers: from the target
-    cluster_sync_all();
+    cluster_meet();
   }
   const double goal = fmin(pick * total, total);
   // the CTA that the draw falls on (pick of 1 and beyond: the last that has mass)
@@ -426,7 +436,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) lm_verify_kernel(VerifyArgs a,
       if (ld_remote(&s_sum, r) > 0.0) last = r;
     mine = last == part;
   }
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA has read the others
+  cluster_here();  // this CTA has read the others
   int* out = a.out + seq * a.ld_out;
   if (part == 0) {
     const int* tokens = a.tokens + seq * a.ld_tokens;
@@ -493,7 +503,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) lm_verify_kernel(VerifyArgs a,
       if (lane == 0) out[n] = found != 0x7fffffff ? found : last;
     }
   }
-  cluster_wait();
+  cluster_all();
 }
 
 // Cluster and items per thread for rows held in registers: as few CTAs as hold the row, more while they do not fill the GPU.
