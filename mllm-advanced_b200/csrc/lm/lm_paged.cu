@@ -181,8 +181,8 @@ __global__ void __launch_bounds__(32 * WARPS, 1) lm_paged_decode_kernel(Paged a,
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
           float alpha[2];
-          if (all) weigh_keys<2, true>(a, sc[t], m[t], l[t], alpha, j0, lane, pos[t], bias[t]);
-          else weigh_keys<2, false>(a, sc[t], m[t], l[t], alpha, j0, lane, pos[t], bias[t]);
+          if (all) weigh_keys<T, 2, true>(a, sc[t], m[t], l[t], alpha, j0, lane, pos[t], bias[t]);
+          else weigh_keys<T, 2, false>(a, sc[t], m[t], l[t], alpha, j0, lane, pos[t], bias[t]);
           if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
 #pragma unroll
             for (int n = 0; n < DV / 8; ++n) o[t][n][0] *= alpha[0], o[t][n][1] *= alpha[0], o[t][n][2] *= alpha[1], o[t][n][3] *= alpha[1];
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) lm_paged_decode_kernel(Paged a,
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int r = t * 16 + (lane >> 2) + i * 8;
-        if ((lane & 3) == 0) s_m[warp][r] = m[t][i], s_l[warp][r] = l[t][i];
+        if ((lane & 3) == 0) s_m[warp][r] = m[t][i] - Num<T>::kLift, s_l[warp][r] = l[t][i];  // (what sums and outputs are relative to)
         float* so = sO + ((size_t)warp * kRows + r) * a.vdim + (lane & 3) * 2;
 #pragma unroll
         for (int n = 0; n < DV / 8; ++n)

@@ -137,7 +137,11 @@ __device__ __forceinline__ int sequence_of(const Paged& a, const long long* base
 }
 __device__ __forceinline__ int owner_of(long long b, long long total, int ctas) { return (int)(((b + 1) * ctas - 1) / total); }
 
-// Numbers of 16 bits on the tensor cores of a warp.
+// Numbers of 16 bits on the tensor cores.  Softmax weights are made relative to a reference that their row's maximum may outgrow by 2^kLag, and
+// stored times 2^kLift.  bf16 has fp32's exponents: no lift, and a reference that seldom moves.  fp16 ends at 65504 and lies 2^-24 apart below
+// 2^-14: of a row with one large weight the others would be lost (their fp32 sum counts them), so the reference stays within 2^3 and weights
+// are lifted to 2^15.  What 16 bits leave of a weight in two numbers is then 2^-22 of it or 2^-37 of the reference, whichever is more (bf16:
+// 2^-17 of it).
 template <class T>
 struct Num;
 template <>
@@ -154,6 +158,7 @@ struct Num<__nv_bfloat16> {
   }
   static __device__ __forceinline__ float2 unpack(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
   static constexpr uint32_t kExponent = 0x7f807f80u;
+  static constexpr float kLag = 8.0f, kLift = 0.0f;
 };
 template <>
 struct Num<__half> {
@@ -172,6 +177,7 @@ struct Num<__half> {
     return __half22float2(h);
   }
   static constexpr uint32_t kExponent = 0x7c007c00u;
+  static constexpr float kLag = 3.0f, kLift = 12.0f;
 };
 // infinity or NaN in either half
 template <class T>

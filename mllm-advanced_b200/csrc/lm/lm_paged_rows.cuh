@@ -9,7 +9,7 @@ namespace lm {
 namespace {
 
 // o += P V for 16 keys at j0 held as B fragments (mv: address of the first), P = hi + lo of the type (its rounding to 16 bits
-// would cost as much as the output's; two halves keep 2^-17 and better).  EDGE: some of the keys are not seen by some of the
+// would cost as much as the output's; what two halves keep stands at Num).  EDGE: some of the keys are not seen by some of the
 // warp's rows, and what their values hold (infinities, NaN) must not reach those rows through a weight of 0: one token
 // of the rows after the other, with the keys that it does not see as zeros.
 template <class T, int DV, bool EDGE>
@@ -55,8 +55,8 @@ __device__ __forceinline__ void weigh_values(const Paged& a, float (&o)[DV / 8][
 }
 
 // Scores (base 2) of 16 x 8 N products of one warp for keys from j0 on: scale, bias, mask; the rows' running maxima and sums,
-// the weights in place of the scores.  ALL: every row sees every key.
-template <int N, bool ALL>
+// the weights, times 2^kLift as their sums, in place of the scores.  ALL: every row sees every key.
+template <class T, int N, bool ALL>
 __device__ __forceinline__ void weigh_keys(const Paged& a, float (&s)[N][4], float (&m)[2], float (&l)[2], float (&alpha)[2], int j0, int lane,
                                            const int (&pos)[2], const float* const (&bias)[2]) {
   float mx[2] = {m[0], m[1]};
@@ -78,7 +78,7 @@ __device__ __forceinline__ void weigh_keys(const Paged& a, float (&s)[N][4], flo
     alpha[r] = paged_exp2(m[r] - base);
     m[r] = mx[r];
     l[r] *= alpha[r];
-    mx[r] = base;
+    mx[r] = base - Num<T>::kLift;
   }
 #pragma unroll
   for (int n = 0; n < N; ++n)
@@ -234,8 +234,8 @@ __device__ __forceinline__ void paged_prompt_rows(const Paged& a, uint8_t* smem,
       }
     }
     float alpha[2];
-    if (w_first >= 0 && seen_by_all(a, w_first, w_last, jw, jw + kHalf - 1)) weigh_keys<kHalf / 8, true>(a, s, m, l, alpha, jw, lane, pos, bias);
-    else weigh_keys<kHalf / 8, false>(a, s, m, l, alpha, jw, lane, pos, bias);
+    if (w_first >= 0 && seen_by_all(a, w_first, w_last, jw, jw + kHalf - 1)) weigh_keys<T, kHalf / 8, true>(a, s, m, l, alpha, jw, lane, pos, bias);
+    else weigh_keys<T, kHalf / 8, false>(a, s, m, l, alpha, jw, lane, pos, bias);
 #pragma unroll
     for (int n = 0; n < DV / 8; ++n) o[n][0] *= alpha[0], o[n][1] *= alpha[0], o[n][2] *= alpha[1], o[n][3] *= alpha[1];
 #pragma unroll
@@ -250,6 +250,7 @@ __device__ __forceinline__ void paged_prompt_rows(const Paged& a, uint8_t* smem,
   paged_wait<0>();
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
+    m[r] -= Num<T>::kLift;  // what sums and outputs are relative to
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
   }

@@ -4,7 +4,7 @@
 // and value that is fetched.  Per block of 128 keys and tile: S = Q K^T into tensor memory, softmax weights P in 16 bits over
 // S's own columns, O += P V (64 keys at a time).  While the weights of one tile are made, the products of the other run:
 //   warps 0-3, 4-7  weights of tile 0 and 1, a row per thread; O is rescaled (tensor memory) only when a row's maximum has grown by
-//                   more than 2^8 - weights up to 2^8 are as exact in 16 bits, and their fp32 sum is kept under the same base
+//                   more than 2^8 (fp16: 2^3) - weights beyond 1 are as exact in 16 bits, and their fp32 sum is kept under the same base
 //   warp 8          copies: TMA, pieces of a block that lie in one page, into a ring of keys and one of values
 //   warp 9          MMA issue, tensor-memory owner
 //   warps 10-11     values of blocks that some rows do not see in full: rows that no row sees (page tails, other sequences' data) are
@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
     // (a row that is not there reads the first one's)
     const float* bias = !BIAS ? nullptr : staged ? table + (live ? hg * pitch : 0) : a.bias + (size_t)(live ? head : 0) * (a.bias_max + 1);
     const float sink = a.sink && live ? a.sink[head] * kPagedLog2e : -INFINITY;
-    const float scale = BIAS ? 1.0f : a.scale2, grown = 8.0f / scale;  // BIAS: scores are scaled before their maximum
+    const float scale = BIAS ? 1.0f : a.scale2, grown = Num<T>::kLag / scale;  // BIAS: scores are scaled before their maximum
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     const int n = t < tiles ? nt : 0;
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
           rescale<D>(o_col, alpha);
         }
       }
-      l += put_weights<T, EXACT>(s_col, scale, m == -INFINITY ? 0.0f : -m * scale, [&](int h) {
+      l += put_weights<T, EXACT>(s_col, scale, m == -INFINITY ? 0.0f : fmaf(-m, scale, Num<T>::kLift), [&](int h) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.p_ready[t][h]);
@@ -489,8 +489,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
       }
     }
     if (n) {
-      const float total = l + (split ? 0.0f : paged_exp2(sink - (m == -INFINITY ? 0.0f : m * scale))), inv = pos < 0 ? 0.0f : 1.0f / total;
-      if (split && live) w.part_ml[at] = make_float2(m * scale, l);  // base 2
+      const float ref = fmaf(m, scale, -Num<T>::kLift);  // what sums and outputs are relative to (base 2)
+      const float total = l + (split ? 0.0f : paged_exp2(sink - (m == -INFINITY ? 0.0f : ref))), inv = pos < 0 ? 0.0f : 1.0f / total;
+      if (split && live) w.part_ml[at] = make_float2(ref, l);
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -583,8 +584,8 @@ __global__ void __launch_bounds__(256) lm_paged_prompt_join_kernel(Paged a, Prom
 // shorter than its way from memory.  So the keys are the wide side of both products: S^T = K Q^T has a key per lane and an item's rows
 // (all heads of a kv head, of up to 64 / group tokens) as its 16, 32 or 64 columns, and O^T += V^T P^T a value's number per lane.
 // Every thread of the four warps has its own key; a row's maximum is looked for across threads only when some score has
-// outgrown the one in use by more than 2^8, and sums are added up across threads at an item's end.  Weights enter as two halves of
-// 16 bits (2^-17 of a weight and better).  A CTA walks an even share of all blocks, copies running ahead over the ends of items:
+// outgrown the one in use by more than 2^8 (fp16: 2^3), and sums are added up across threads at an item's end.  Weights enter as two halves of
+// 16 bits (Num says what they keep).  A CTA walks an even share of all blocks, copies running ahead over the ends of items:
 //   warps 0-3        weights
 //   warp 4, 5, 6     copies; MMA issue (scores a block ahead); values that not every row sees
 // Five tokens of 32 contexts of 8-12 k, 16 / 4 heads of 128: 107-124 us of 129 in all, 658 MB at 5.3-6.1 TB/s (rows as lanes: 158-197, three
@@ -863,6 +864,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
     // ------------------------------------------------------------ weights: one key per thread
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     const float scale = BIAS ? 1.0f : a.scale2;  // BIAS: scores are scaled when it is added
+    constexpr float kLag = Num<T>::kLag, kLift = Num<T>::kLift;
     auto sync = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
     auto any = [](bool v) {
       int r;
@@ -930,8 +932,8 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
 #pragma unroll
         for (int i = 0; i < kC; i += 4) {
           const float4 ref = *reinterpret_cast<const float4*>(s_ref + c0 + i);
-          over |= fmaf(__uint_as_float(v[i]), scale, -8.0f) > ref.x | fmaf(__uint_as_float(v[i + 1]), scale, -8.0f) > ref.y |
-                  fmaf(__uint_as_float(v[i + 2]), scale, -8.0f) > ref.z | fmaf(__uint_as_float(v[i + 3]), scale, -8.0f) > ref.w;
+          over |= fmaf(__uint_as_float(v[i]), scale, -kLag) > ref.x | fmaf(__uint_as_float(v[i + 1]), scale, -kLag) > ref.y |
+                  fmaf(__uint_as_float(v[i + 2]), scale, -kLag) > ref.z | fmaf(__uint_as_float(v[i + 3]), scale, -kLag) > ref.w;
         }
       }
       if (NP > kC && (BIAS || masked)) tmem_st_wait();
@@ -952,7 +954,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
           const float old = s_ref[tid], top = fmaxf(fmaxf(s_max[0][tid], s_max[1][tid]), fmaxf(s_max[2][tid], s_max[3][tid])) * scale, now = fmaxf(old, top);
           s_alpha[tid] = now == -INFINITY ? 1.0f : exp2f(old - now);
           s_ref[tid] = now;
-          s_base2[tid] = now == -INFINITY ? 0.0f : -now;
+          s_base2[tid] = now == -INFINITY ? 0.0f : kLift - now;
         } else if (tid < NP) {
           s_alpha[tid] = 1.0f;
         }
@@ -1014,7 +1016,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
         const size_t slot = (size_t)(2 * blockIdx.x + g.begins) * item_rows;
         if (tid < rows) {
           const int tok = tid / a.group, head = g.kvh * a.group + tid - tok * a.group;
-          const float ref = s_ref[tid], sink = g.whole && a.sink ? a.sink[head] * kPagedLog2e : -INFINITY, most = fmaxf(ref, sink), at = most == -INFINITY ? 0.0f : most;
+          const float ref = s_ref[tid] - kLift, sink = g.whole && a.sink ? a.sink[head] * kPagedLog2e : -INFINITY, most = fmaxf(ref, sink), at = most == -INFINITY ? 0.0f : most;
           const float f = exp2f(ref - at), sum = ((s_max[0][tid] + s_max[1][tid]) + (s_max[2][tid] + s_max[3][tid])) * f + exp2f(sink - at);
           s_alpha[tid] = !g.whole ? f : g.p_first + tok < 0 ? 0.0f : f / sum;
           if (!g.whole) w.part_ml[slot + tid] = make_float2(most, sum);

@@ -8,7 +8,7 @@ import torch
 import lm_case
 import lm_models as M
 from mllm_b200 import paged, registry
-from paged_case import Cache, attention64, check
+from paged_case import HALF_STEP, Cache, attention64, check
 
 BF16, FP16 = torch.bfloat16, torch.float16
 
@@ -54,3 +54,38 @@ def test_engine_prefill_on_pages_is_as_exact_as_on_slots(dim, tmp_path):
         got.append(lm_case.residual_after(case, tokens))
         case.model.close()
     assert np.linalg.norm(got[1] - got[0]) <= 2.0 ** -11 * np.linalg.norm(got[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 80])
+@pytest.mark.parametrize("top, late", [(18.0, False), (14.0, True)])
+@pytest.mark.parametrize("value", [0.0, 1.0])
+def test_many_small_weights_beside_a_large_one(dtype, dim, top, late, value):
+    """A key whose score lies 14 or 18 above those of 65535 others: their weights, near 2^-20 and 2^-26 of its, sum up to what fp16 must not
+    lose.  In fp16 a weight in two numbers is off by 2^-37 of the reference at most, whose own weight is at least 1 in the sum."""
+    n = 65536
+    c = Cache([64], 1, dim, dim, 64, dtype, 1)  # (its values are made anew below)
+    c.lengths_h, pages = [n], n // 64
+    c.keys, c.values = [torch.zeros(n, 1, dim, dtype=dtype)], [torch.ones(n, 1, dim, dtype=dtype)]
+    at = n - 40 if late else 0
+    c.keys[0][at, 0, 0], c.values[0][at] = top, value
+    order = np.random.default_rng(2).permutation(pages)
+    c.table_h, c.pages = np.ascontiguousarray(order[None].astype(np.int32)), pages
+    c.k, c.v = (torch.empty(pages, 1, 64, dim, dtype=dtype) for _ in range(2))
+    for pool, flat in ((c.k, c.keys[0]), (c.v, c.values[0])):
+        pool[torch.from_numpy(order)] = flat.view(pages, 64, 1, dim).transpose(1, 2)
+    q = torch.zeros(3, 2, dim, dtype=dtype)
+    q[:, :, 0] = 1.0
+    want, spread, big = attention64(c, [3], q, 1.0)
+    c.on_gpu()
+    start = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    for got, one in ((paged.decode_attention(q.cuda(), c.k, c.v, c.table, c.lengths, scale=1.0), False),
+                     (paged.prompt_attention(q.cuda(), c.k, c.v, c.table, c.lengths, start, scale=1.0), True),
+                     (paged.prompt_attention(q.cuda(), c.k, c.v, c.table, c.lengths, start, scale=1.0, exact=True), False)):
+        half = HALF_STEP[dtype]
+        bound = half * want.abs() * 1.01 + spread * ((half if one else 0.0) + 2.0 ** -16 + 2 * (dim / 16 + 4) * 2.0 ** -23 * big) + \
+            (n * 2.0 ** -37 if dtype == FP16 else 0.0)
+        off = (got.cpu().double() - want).abs()
+        assert (off <= bound).all(), (float(off.max()), float(bound.min()), float(want.min()))
+    paged.check()
