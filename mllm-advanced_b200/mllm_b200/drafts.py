@@ -13,15 +13,16 @@ def probabilities(logits, temperature=1.0, out=None, stream=None):
     """Rows of logits [rows, vocab] (fp32, bf16 or fp16) to probabilities in fp32: exp((z - max z) / temperature) over their sum;
     temperature 0: 1 at the first largest.  -inf gives 0, a row of nothing else zeros; NaN or +inf make their row NaN."""
     dtype = _DTYPES.get(logits.dtype)
+    distance = None if out is None or logits.dim() != 2 else lm.row_distance("probabilities", out, *logits.shape)
     if not (logits.dim() == 2 and logits.stride(1) == 1 and dtype is not None and logits.is_cuda):
         _refuse("probabilities", (lambda: False, "logits [rows, vocab] in fp32, bf16 or fp16 on the GPU, rows contiguous"))
     rows, vocab = logits.shape
-    if out is not None and not (out.shape == (rows, vocab) and out.dtype == torch.float32 and out.get_device() == logits.get_device() and out.stride(1) == 1):
-        _refuse("probabilities", (lambda: False, "out like the logits, in fp32"))
+    if out is not None and out.get_device() != logits.get_device():
+        _refuse("probabilities", (lambda: False, "out on the logits' GPU"))
 
     def call(s):
         o = out if out is not None else logits.new_empty((rows, vocab), dtype=torch.float32)
-        return lm.lib().mllmb200_lm_probabilities(logits.data_ptr(), dtype, logits.stride(0), rows, vocab, temperature, o.data_ptr(), max(o.stride(0), vocab), s), o
+        return lm.lib().mllmb200_lm_probabilities(logits.data_ptr(), dtype, logits.stride(0), rows, vocab, temperature, o.data_ptr(), distance or vocab, s), o
     st, o = _on(logits.get_device(), stream, call)
     if st:
         _fail("probabilities", st)

@@ -91,6 +91,15 @@ def distance_buckets(bias_rows, bias_max, count):
     return out
 
 
+def row_distance(where, out, rows, vocab):
+    """Numbers from one row of `out`, fp32 [rows, vocab], to the next; a single row's stride says nothing."""
+    if out.shape != (rows, vocab) or str(out.dtype) != "torch.float32" or out.stride(1) != 1:
+        raise ValueError(f"{where}: out [{rows}, {vocab}] in fp32, rows contiguous")
+    if rows > 1 and out.stride(0) < vocab:
+        raise ValueError(f"{where}: rows of out overlap")
+    return out.stride(0) if rows > 1 else vocab
+
+
 def _ints(a):
     return np.ascontiguousarray(a, np.int32)
 
@@ -187,12 +196,13 @@ class LanguageModel:
         tokens, want = _ints(np.concatenate([np.asarray(t, np.int32) for _, t in entries])), _ints(want)
         if out is None:
             out = torch.empty((len(want), self.vocab), dtype=torch.float32, device="cuda")
-        if out.shape != (len(want), self.vocab) or out.dtype != torch.float32 or out.stride(1) != 1 or not out.is_cuda:
-            raise ValueError("step_probabilities: out [wanted, vocab] in fp32 on the GPU")
+        distance = row_distance("step_probabilities", out, len(want), self.vocab)
+        if out.get_device() != torch.cuda.current_device():
+            raise ValueError("step_probabilities: out on the model's GPU")
         mine, here = self.stream(), torch.cuda.current_stream()
         mine.wait_stream(here)  # whoever still uses out's memory
         self._check(self._L.mllmb200_lm_step_probabilities(self._h, len(slots), slots.ctypes.data, counts.ctypes.data, tokens.ctypes.data, len(want), want.ctypes.data,
-                                                           temperature, out.data_ptr(), max(out.stride(0), self.vocab)), "step_probabilities")
+                                                           temperature, out.data_ptr(), distance), "step_probabilities")
         here.wait_stream(mine)
         for s, n in zip(slots, counts):
             self.length[s] += int(n)

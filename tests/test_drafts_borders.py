@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from mllm_b200 import drafts
+import taralix_models as TM
+from mllm_b200 import drafts, lm, registry
 from test_drafts import rows, run_verify, softmax64
 
 
@@ -40,3 +41,36 @@ def test_probabilities_after_work_of_single_lanes(rows_, vocab, t):
     assert torch.allclose(first.double().sum(dim=1).cpu(), torch.ones(rows_, dtype=torch.float64), atol=1e-4)
     for _ in range(20):
         assert torch.equal(drafts.probabilities(z, t), first)
+
+
+def test_rows_of_out_that_overlap_are_refused():
+    """Shape and contiguous rows are not enough: rows nearer than vocab (an expanded row) would be written behind the tensor's end."""
+    z = torch.zeros(4, 10)
+    for out in (torch.zeros(1, 10).expand(4, 10), torch.zeros(40).as_strided((4, 10), (9, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            drafts.probabilities(z, out=out)
+        with pytest.raises(ValueError, match="overlap"):
+            lm.row_distance("step_probabilities", out, 4, 10)
+    for out in (torch.zeros(4, 9), torch.zeros(4, 10).double(), torch.zeros(10, 4).T, torch.zeros(40)):
+        with pytest.raises(ValueError, match="out \\["):
+            lm.row_distance("step_probabilities", out, 4, 10)
+    assert lm.row_distance("", torch.zeros(4, 12)[:, 1:11], 4, 10) == 12 and lm.row_distance("", torch.zeros(1, 10).as_strided((1, 10), (3, 1)), 1, 10) == 10
+    assert lm.row_distance("", torch.zeros(0, 10), 0, 10) == 10
+
+
+@pytest.mark.gpu
+def test_overlapping_rows_of_out_are_refused_on_the_gpu(tmp_path):
+    z = torch.randn(4, 10, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        drafts.probabilities(z, out=torch.zeros(1, 10, device="cuda").expand(4, 10))
+    cfg = TM.config(64, 211, [TM.layer(TM.mixer(3, 20, 28, 36), TM.dense(72))])
+    m, _ = registry.load(TM.write(tmp_path, cfg, TM.weights(cfg, 3)), "float32", 1, 64, 64)
+    s = m.acquire()
+    for out in (torch.zeros(1, 211, device="cuda").expand(3, 211), torch.zeros(3, 211)):
+        with pytest.raises(ValueError):
+            m.step_probabilities([(s, [1, 2, 3])], [0, 1, 2], out=out)
+    assert m.length[s] == 0
+    out = torch.zeros(2, 300, device="cuda")
+    m.step_probabilities([(s, [1, 2, 3])], [0, 2], out=out[:, :211])
+    assert (out[:, 211:] == 0).all() and torch.allclose(out.sum(dim=1), torch.ones(2, device="cuda"), atol=1e-5)
+    m.close()
