@@ -253,6 +253,7 @@ int create(Engine* e, const mllmb200_lm_layer* descs) {
   if (c.page < 0 || c.pages < 0 || (c.page == 0) != (c.pages == 0)) return fail(e, MLLMB200_INVALID_ARG, "%d pages of %d tokens", c.pages, c.page);
   e->paged = c.page > 0;
   if (e->paged && (e->f32 || c.page % 16)) return fail(e, MLLMB200_UNSUPPORTED, "pages hold bf16, a multiple of 16 tokens each");
+  if (e->paged && (long long)c.max_ctx + c.page > kLongest) return fail(e, MLLMB200_UNSUPPORTED, "pages of %d tokens for %d positions", c.page, c.max_ctx);
   e->widthp = pad_to(c.width, 64);
   if (e->widthp > 8192 || (size_t)c.conv_taps * e->widthp * 4 > kNormSmemMax) return fail(e, MLLMB200_UNSUPPORTED, "width %d with %d taps", c.width, c.conv_taps);
   LM_CUDA(cudaStreamCreateWithFlags(&e->stream, cudaStreamNonBlocking));
@@ -277,6 +278,7 @@ int create(Engine* e, const mllmb200_lm_layer* descs) {
     LayerState& L = e->layers[i];
     LM_OK(check_layer(e, i, descs[i]));
     L.d = descs[i];
+    L.d.window = std::min(L.d.window, c.max_ctx), L.d.keep = std::min(L.d.keep, c.max_ctx);  // (no position lies beyond; sums with them stay in 32 bits)
     L.src = L.d.weights_of < 0 ? i : e->layers[L.d.weights_of].src;
     L.dimp = pad_to(L.d.dim, 16);
     L.vdimp = pad_to(L.d.vdim, 16);
