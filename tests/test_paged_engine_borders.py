@@ -11,7 +11,7 @@ sys.path.insert(0, os.path.join(ROOT, "oracle"))
 import lm_case  # noqa: E402
 import lm_models as M  # noqa: E402
 import vupuzen_oracle as V  # noqa: E402
-from mllm_b200 import lm, registry, vupuzen  # noqa: E402
+from mllm_b200 import lm, registry, scheduler, vupuzen  # noqa: E402
 
 gpu = pytest.mark.gpu
 MOST = 2 ** 31 - 1
@@ -47,3 +47,50 @@ def test_windows_and_first_tokens_of_any_size(windows, tmp_path):
     case.check(np.concatenate(got), want)
     m.check_device_status()
     m.close()
+
+
+@gpu
+def test_taken_back_after_pages_were_given_up(tmp_path):
+    """What the windows have left behind by 64 tokens is gone; the last 64 tokens, and those of the last step, can be taken back."""
+    case = Case(tmp_path, ((24, 2), (20, 1)), 40)
+    m, tokens = case.model, case.tokens(320)
+    want, s = case.oracle(tokens), case.model.acquire()
+    for a, b in ((0, 90), (90, 150), (150, 160), (160, 170)):
+        got = m.step([(s, tokens[a:b])], range(b - a))
+        case.check(got, want[a:b])
+    # before the last step the slot held 160 tokens: of positions up to 160 - 64 - 24 = 72 places 1 .. 3 (16 .. 63) went
+    assert m.free_pages() == 40 - 11 + 3
+    m.truncate(s, 106)  # 64 tokens
+    case.check(m.step([(s, tokens[106:170])], range(64)), want[106:170])
+    m.truncate(s, 160)
+    with pytest.raises(lm.EngineError) as e:  # a token at 70 sees from 47 on
+        m.truncate(s, 70)
+    assert e.value.status == 1 and m.free_pages() == 40 - 10 + 3 and m.length[s] == 160
+    case.check(m.step([(s, tokens[160:300])], range(140)), want[160:300])
+    m.truncate(s, 160)  # where the last step began
+    case.check(m.step([(s, tokens[160:320])], range(160)), want[160:320])
+    m.truncate(s, 0)
+    assert m.free_pages() == 40
+    case.check(m.step([(s, tokens[:30])], range(30)), want[:30])
+    m.check_device_status()
+    m.close()
+
+
+@gpu
+def test_drafts_behind_long_prompts_over_windows(tmp_path):
+    """Prompts that the windows have left pages of, one request after the other: the model's own greedy tokens, but for near ties (a step
+    of other shapes rounds otherwise)."""
+    case = Case(tmp_path / "a", ((24, 2), (20, 1)), 60)
+    other = Case(tmp_path / "b", ((24, 2), (20, 1)), 60)
+    prompts = [case.tokens(n, seed=n) for n in (140, 230, 101)]
+    want = scheduler.generate(case.model, prompts, 90)
+    got = scheduler.generate_drafted(case.model, other.model, prompts, 90, 5)
+    assert case.model.free_pages() == other.model.free_pages() == 60 and [len(x) for x in got] == [90] * 3
+    for prompt, x, y in zip(prompts, got, want):
+        logits = case.oracle(prompt + x[:-1])[len(prompt) - 1:]
+        gap = logits.max(axis=1) - logits[np.arange(90), x]
+        assert gap.max() < 0.5 * np.sqrt(np.mean(logits ** 2)) and (gap == 0).mean() > 0.8
+        assert x[0] == y[0]
+    for c in (case, other):
+        c.model.check_device_status()
+        c.model.close()
