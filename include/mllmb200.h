@@ -444,7 +444,7 @@ MLLMB200_API int mllmb200_selftest_prompt_attention(const float* q_dev, const fl
                                                     float* cache_k_dev, float* cache_v_dev, float* out_dev, void* stream);
 
 /* Device-side status word (bounded waits that ran out, bad tile headers).  Synchronizes `stream`,
- * reads and clears the word.  0 = clean. */
+ * reads and clears what was found on the current device, on any stream; one kind a call, another that was found is told by the next.  0 = clean. */
 MLLMB200_API int mllmb200_check_device_status(void* stream);
 
 #ifdef __cplusplus

@@ -215,7 +215,9 @@ MLLMB200_API int mllmb200_lm_verify(const float* target, long long t_seq, long l
                                     long long ld_accept, const float* pick, int seqs, int drafts, int vocab, int* accepted,
                                     int* out, long long ld_out, void* stream);
 
-/* Synchronizes the stream; reads and clears what these operators found wrong on the device. */
+/* Waits for the stream; reads and clears what these operators found wrong on the current device, on any stream (calls that are
+ * checked one by one are checked before the next is made).  One kind a call: another that was found is told by the next.
+ * The engines' status (mllmb200_lm_check_device_status) is apart from this. */
 MLLMB200_API int mllmb200_lm_operator_status(void* stream);
 
 /* Host only: the distance buckets of a bias table, out[n] for n in [0, count). */

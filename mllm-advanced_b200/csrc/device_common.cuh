@@ -15,6 +15,8 @@ enum : unsigned {
   kDevStatusBadHeader = 2u,  // tiled buffer header does not match the call's N/K
   kDevStatusBadPage = 4u,    // page number or length outside of a paged cache
 };
+// Operators on a caller's memory report the same bits this many places higher: they are read and cleared by themselves.
+constexpr unsigned kDevStatusOfOperators = 8;
 
 extern __device__ unsigned int g_device_status;
 
@@ -51,12 +53,12 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 // Waits for the phase with the given parity, at most ~2^31 clock ticks (about a second).
 // Returns false and raises the timeout bit in the status word when the wait runs out, so a
 // lost copy shows up as an error code on the host instead of a hung GPU.
-__device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, long long limit_ticks = 1ll << 31) {
+__device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, long long limit_ticks = 1ll << 31, unsigned bit = kDevStatusTimeout) {
   if (mbar_try_wait(bar, parity)) return true;
   const long long t0 = clock64();
   while (!mbar_try_wait(bar, parity)) {
     if (clock64() - t0 > limit_ticks) {
-      atomicOr(&g_device_status, kDevStatusTimeout);
+      atomicOr(&g_device_status, bit);
       return false;
     }
   }

@@ -7,7 +7,7 @@
 #include "lm_paged_rows.cuh"
 
 namespace mllmb200 {
-cudaError_t read_device_status(cudaStream_t, int* status);
+cudaError_t read_operator_status(cudaStream_t, int* status);
 
 namespace lm {
 namespace {
@@ -430,6 +430,7 @@ int check_pages(const mllmb200_lm_pages* p, Paged* a) {
   a->pages = p->pages, a->page = p->page, a->kv_heads = p->kv_heads, a->dim = p->dim, a->vdim = p->vdim;
   a->ld_table = p->ld_table, a->max_pages = p->max_pages, a->seqs = p->seqs, a->rows = p->rows;
   a->tokens = p->q_start || !p->seqs ? 0 : p->rows / p->seqs;
+  a->reports = kDevStatusOfOperators;
   return MLLMB200_OK;
 }
 int check_look(const mllmb200_lm_pages* p, const mllmb200_lm_look* l, Paged* a) {
@@ -603,7 +604,7 @@ int mllmb200_lm_attn_prompt(const mllmb200_lm_pages* pages, const mllmb200_lm_lo
 
 int mllmb200_lm_operator_status(void* stream) {
   int status = MLLMB200_OK;
-  return read_device_status(static_cast<cudaStream_t>(stream), &status) == cudaSuccess ? status : MLLMB200_CUDA_ERROR;
+  return read_operator_status(static_cast<cudaStream_t>(stream), &status) == cudaSuccess ? status : MLLMB200_CUDA_ERROR;
 }
 
 }  // extern "C"

@@ -297,10 +297,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
     const int j0 = block_key<kTcKeys>(seen, b0 + j);
     return pos0 < 0 || !seen_by_all(a, pos0, p_last, j0, j0 + kTcKeys - 1);
   };
+  auto bounded = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, 1ll << 31, kDevStatusTimeout << a.reports); };
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return true;
     if (s_gave_up) return false;
-    if (mbar_wait_bounded(bar, parity)) return true;
+    if (bounded(bar, parity)) return true;
     s_gave_up = 1;
     return false;
   };
@@ -353,9 +354,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
           pages = next;
         }
         if (!ok) {  // nothing in flight when the CTA leaves
-          mbar_wait_bounded(&bars.q_full, 0);
-          for (int j = max(0, n_k - L::kK); j < n_k; ++j) mbar_wait_bounded(&bars.k_full[j % L::kK], turn(j, L::kK));
-          for (int j = max(0, n_v - L::kV); j < n_v; ++j) mbar_wait_bounded(&bars.v_full[j % L::kV], turn(j, L::kV));
+          bounded(&bars.q_full, 0);
+          for (int j = max(0, n_k - L::kK); j < n_k; ++j) bounded(&bars.k_full[j % L::kK], turn(j, L::kK));
+          for (int j = max(0, n_v - L::kV); j < n_v; ++j) bounded(&bars.v_full[j % L::kV], turn(j, L::kV));
         }
       }
     } else if (warp == 9) {
@@ -699,10 +700,11 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
   tc_fence_after();
   pdl_launch_dependents();  // (as above)
   const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+  auto bounded = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, 1ll << 31, kDevStatusTimeout << a.reports); };
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return true;
     if (s_gave_up) return false;
-    if (mbar_wait_bounded(bar, parity)) return true;
+    if (bounded(bar, parity)) return true;
     s_gave_up = 1;
     return false;
   };
@@ -768,9 +770,9 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
       leave(p);
     }
     if (!ok) {  // nothing in flight when the CTA leaves
-      for (int i = max(0, kr.count - L::kK); i < kr.count; ++i) mbar_wait_bounded(&bars.k_full[i % L::kK], (uint32_t)(i / L::kK) & 1u);
-      for (int i = max(0, vr.count - L::kV); i < vr.count; ++i) mbar_wait_bounded(&bars.v_full[i % L::kV], (uint32_t)(i / L::kV) & 1u);
-      for (int i = max(0, p.sg + 1 - kB); i <= p.sg; ++i) mbar_wait_bounded(&bars.q_full[i % kB], (uint32_t)(i / kB) & 1u);
+      for (int i = max(0, kr.count - L::kK); i < kr.count; ++i) bounded(&bars.k_full[i % L::kK], (uint32_t)(i / L::kK) & 1u);
+      for (int i = max(0, vr.count - L::kV); i < vr.count; ++i) bounded(&bars.v_full[i % L::kV], (uint32_t)(i / L::kV) & 1u);
+      for (int i = max(0, p.sg + 1 - kB); i <= p.sg; ++i) bounded(&bars.q_full[i % kB], (uint32_t)(i / kB) & 1u);
     }
   } else if (warp == 5) {
     // ------------------------------------------------------------ MMA issue
