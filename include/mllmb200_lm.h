@@ -154,7 +154,8 @@ enum { MLLMB200_LM_F16 = 2 };  /* caches and queries in fp16 (beside MLLMB200_LM
  * lengths[s] tokens long with them: its row t stands at position lengths[s] - n + t.  Rows at negative positions see nothing
  * (attention: zeros) and are not stored; rows from q_start[seqs] on are neither read nor written.
  * A page number outside [0, pages): what the page would hold is taken as zeros and is not stored.  A length beyond
- * max_pages pages counts as max_pages pages.  Both make mllmb200_lm_operator_status report MLLMB200_BAD_PAGE.  Page numbers of
+ * max_pages pages counts as max_pages pages in attention; rows whose position lies beyond them are not stored.  These make
+ * mllmb200_lm_operator_status report MLLMB200_BAD_PAGE.  Page numbers of
  * positions that no row of the call sees are not read. */
 typedef struct mllmb200_lm_pages {
   void *k, *v;                       /* dim numbers per key, vdim per value */

@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(128) lm_pages_append_kernel(Paged a, const voi
     pos[u] = row0 + u < a.rows && t >= 0 && t < n ? t - n : 0;  // (0: behind the last row or the last sequence)
   }
 #pragma unroll
-  for (int u = 0; u < ROWS; ++u) pos[u] = pos[u] < 0 ? paged_length(a, seq[u]) + pos[u] : -1;
+  for (int u = 0; u < ROWS; ++u) pos[u] = pos[u] < 0 ? a.lengths[seq[u]] + pos[u] : -1;  // (uncut: beyond the table is no page, and no other row's)
 #pragma unroll
   for (int u = 0; u < ROWS; ++u) page[u] = pos[u] >= 0 ? paged_page(a, seq[u], pos[u] / a.page) : -1;
 #pragma unroll

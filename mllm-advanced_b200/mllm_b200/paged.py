@@ -80,7 +80,8 @@ def _pages(where, k, v, table, lengths, q_start, rows):
 
 def append(k_pages, v_pages, k, v, table, lengths, q_start=None, stream=None):
     """Rows of new keys [rows, kv_heads, dim] and values [rows, kv_heads, vdim] into their pages.  Sequence s brings the rows
-    q_start[s] .. q_start[s + 1] - 1 (without q_start: as many as every other); rows behind the last sequence are not stored."""
+    q_start[s] .. q_start[s + 1] - 1 (without q_start: as many as every other); rows behind the last sequence, and
+    those whose position the table has no place for, are not stored."""
     if not (k.dim() == 3 and v.dim() == 3 and k_pages.dim() == 4 and v_pages.dim() == 4 and k.dtype == v.dtype == k_pages.dtype and k.get_device() == v.get_device() == k_pages.get_device() and
             k.shape[0] == v.shape[0] and k.shape[1] == v.shape[1] == k_pages.shape[1] and k.shape[2] == k_pages.shape[3] and v.shape[2] == v_pages.shape[3] and k.stride(2) == 1 and v.stride(2) == 1):
         _refuse("append", (lambda: k.dim() == v.dim() == 3 and k.dtype == v.dtype == k_pages.dtype and k.device == v.device == k_pages.device, "new keys and values [rows, kv_heads, size] of the cache's type"),
