@@ -23,7 +23,7 @@ def probabilities(logits, temperature=1.0, out=None, stream=None):
     def call(s):
         o = out if out is not None else logits.new_empty((rows, vocab), dtype=torch.float32)
         return lm.lib().mllmb200_lm_probabilities(logits.data_ptr(), dtype, logits.stride(0), rows, vocab, temperature, o.data_ptr(), distance or vocab, s), o
-    st, o = _on(logits.get_device(), stream, call)
+    st, o = _on(logits.get_device(), stream, call, logits, out)
     if st:
         _fail("probabilities", st)
     return o
@@ -62,7 +62,7 @@ def verify(target, draft, tokens, accept, pick, stream=None):
         st = lm.lib().mllmb200_lm_verify(target.data_ptr(), t_seq, t_row, draft.data_ptr(), d_seq, d_row, tokens.data_ptr(), tokens_seq, accept.data_ptr(), accept_seq,
                                          pick.data_ptr(), seqs, k, vocab, accepted.data_ptr(), out.data_ptr(), places, s)
         return st, (accepted, out)
-    st, o = _on(device, stream, call)
+    st, o = _on(device, stream, call, target, draft, tokens, accept, pick)
     if st:
         _fail("verify", st)
     return o

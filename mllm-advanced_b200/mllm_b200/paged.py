@@ -8,8 +8,8 @@ row j % page; pages may lie in any order.  lengths[s] counts the tokens of a seq
 at positions lengths[s] - n and on.  table, lengths and q_start are int32 tensors on the device, and are read there: a
 captured call replays with what they hold then.
 
-Calls run on the current stream of the tensors' device, or on `stream` (the tensors must be ready there); `out` is allocated
-there too.  What the device finds wrong (page numbers, lengths) is reported by `check`."""
+Calls run on the current stream of the tensors' device, or on `stream` of that device (the tensors must be ready there); `out` is
+allocated there too.  What the device finds wrong (page numbers, lengths) is reported by `check`."""
 import ctypes as C
 import struct
 
@@ -43,12 +43,22 @@ except AttributeError:  # (names that torch does not promise)
     _device, _raw_stream = torch.cuda.current_device, lambda index: torch.cuda.current_stream(index).cuda_stream
 
 
-def _on(index, stream, call):
-    """call(raw stream) with the tensors' device as the current one."""
-    if stream is None and index == _device():
-        return call(_raw_stream(index))
-    with torch.cuda.device(index) if stream is None else torch.cuda.stream(stream):
-        return call(_raw_stream(index) if stream is None else stream.cuda_stream)
+def _on(index, stream, call, *tensors):
+    """call(raw stream) with the tensors' device as the current one.  On a stream of the caller's the tensors' memory stays theirs until
+    that stream is through, whatever becomes of the tensors meanwhile."""
+    if stream is None:
+        if index == _device():
+            return call(_raw_stream(index))
+        with torch.cuda.device(index):
+            return call(_raw_stream(index))
+    if stream.device.index != index:
+        raise ValueError(f"a stream of {stream.device} for tensors of cuda:{index}")
+    with torch.cuda.stream(stream):
+        result = call(stream.cuda_stream)
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
+    return result
 
 
 def _pages(where, k, v, table, lengths, q_start, rows):
@@ -87,7 +97,8 @@ def append(k_pages, v_pages, k, v, table, lengths, q_start=None, stream=None):
         _refuse("append", (lambda: k.dim() == v.dim() == 3 and k.dtype == v.dtype == k_pages.dtype and k.device == v.device == k_pages.device, "new keys and values [rows, kv_heads, size] of the cache's type"),
                 (lambda: k.stride(2) == v.stride(2) == 1, "rows of keys and values are contiguous"), (lambda: False, "sizes of keys and values"))
     pages = _pages("append", k_pages, v_pages, table, lengths, q_start, k.shape[0])[0]
-    st = _on(k.get_device(), stream, lambda s: lm.lib().mllmb200_lm_pages_append(pages, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), s))
+    st = _on(k.get_device(), stream, lambda s: lm.lib().mllmb200_lm_pages_append(pages, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), s),
+             k_pages, v_pages, k, v, table, lengths, q_start)
     if st:
         _fail("append", st)
 
@@ -136,7 +147,7 @@ def _attention(where, q, k_pages, v_pages, table, lengths, q_start, scale, windo
             return run(pages, look, ws, s), o
         finally:
             give(ws)
-    st, o = _on(index, stream, call)
+    st, o = _on(index, stream, call, q, k_pages, v_pages, table, lengths, q_start, sink, bias, out)
     if st:
         _fail(where, st)
     return o
@@ -163,7 +174,9 @@ def prompt_attention(q, k_pages, v_pages, table, lengths, q_start, scale=None, w
 
 
 def check(stream=None):
-    """Waits for the stream; raises if a call met a page number or a length outside of its cache."""
-    st = lm.lib().mllmb200_lm_operator_status((stream or torch.cuda.current_stream()).cuda_stream)
+    """Waits for the stream; raises if a call on its device met a page number or a length outside of its cache."""
+    stream = stream or torch.cuda.current_stream()
+    with torch.cuda.device(stream.device):
+        st = lm.lib().mllmb200_lm_operator_status(stream.cuda_stream)
     if st:
         _fail("paged operators", st)

@@ -1,9 +1,9 @@
 """Operators over pages at their borders: lengths beyond a table, tensors of other streams, odd arguments."""
-import numpy as np
+import contextlib
 import pytest
 import torch
 
-from mllm_b200 import lm, paged
+from mllm_b200 import drafts, lm, paged
 from paged_case import Cache
 
 BF16 = torch.bfloat16
@@ -37,3 +37,71 @@ def test_rows_beyond_a_full_table_are_not_stored(beyond, count, ragged):
     assert e.value.status == 7
     for got, w in zip((c.k, c.v), want):
         assert torch.equal(torch.nan_to_num(got.cpu().float(), 11.0), torch.nan_to_num(w.float(), 11.0))
+
+
+class FakeStream:
+    """A stream as the calls see it, without a GPU."""
+
+    def __init__(self, index, cuda_stream=77):
+        self.device, self.cuda_stream, self.device_index = torch.device("cuda", index), cuda_stream, index
+
+
+def test_a_stream_of_the_callers_keeps_the_tensors(monkeypatch):
+    kept = []
+
+    class Tensor:
+        def record_stream(self, s):
+            kept.append((self, s))
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: contextlib.nullcontext())
+    s, tensors = FakeStream(0), [Tensor(), None, Tensor()]
+    assert paged._on(0, s, lambda raw: raw + 1, *tensors) == 78
+    assert kept == [(tensors[0], s), (tensors[2], s)]
+    ran = []
+    with pytest.raises(ValueError, match="cuda:1 for tensors of cuda:0"):
+        paged._on(0, FakeStream(1), ran.append, *tensors)
+    assert not ran and len(kept) == 2
+
+
+def test_check_asks_the_streams_device(monkeypatch):
+    asked = []
+
+    class Device(contextlib.nullcontext):
+        def __init__(self, device):
+            super().__init__()
+            asked.append(device)
+
+    class Library:
+        def mllmb200_lm_operator_status(self, raw):
+            asked.append(raw)
+            return 7
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(lm, "lib", Library)
+    with pytest.raises(lm.EngineError):
+        paged.check(FakeStream(1))
+    assert asked == [torch.device("cuda", 1), 77]
+
+
+@pytest.mark.gpu
+def test_tensors_dropped_behind_a_call_on_a_stream():
+    """Temporaries of calls on a stream that is busy: their memory is not handed out while it is read."""
+    c = Cache([300, 40], 2, 64, 64, 16, BF16, 14).on_gpu()
+    q, z = rand((2, 4, 64), BF16, 15).cuda(), torch.randn(3, 5000, device="cuda")
+    start = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    want = [paged.decode_attention(q, c.k, c.v, c.table, c.lengths), paged.prompt_attention(q, c.k, c.v, c.table, c.lengths, start), drafts.probabilities(z)]
+    side = torch.cuda.Stream()
+    for i in range(3):
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+        args = (z.clone(),) if i == 2 else (q.clone(), c.k, c.v, c.table.clone(), c.lengths.clone())
+        ready = torch.cuda.Event()
+        ready.record()
+        call = [paged.decode_attention, lambda *a, stream: paged.prompt_attention(*a, start, stream=stream), drafts.probabilities][i]
+        side.wait_event(ready)
+        got = call(*args, stream=side)
+        shapes = [(a.shape, a.dtype) for a in args]
+        del args
+        junk = [torch.empty(shape, dtype=dtype, device="cuda").fill_(3) for shape, dtype in shapes for _ in range(4)]
+        torch.cuda.synchronize()
+        assert torch.equal(got, want[i])
+        del junk
