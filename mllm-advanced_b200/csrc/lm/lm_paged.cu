@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) lm_paged_decode_kernel(Paged a,
     const int slot = 2 * blockIdx.x + begins, n_rows = min(kRows, rows - r0);
     for (int i = tid; i < n_rows * a.vdim; i += kDecThreads) {
       const int r = i / a.vdim, d = i - r * a.vdim, tok = (r0 + r) / a.group, h = kvh * a.group + r0 + r - tok * a.group;
-      const float sink = whole && a.sink ? a.sink[h] * kPagedLog2e : -INFINITY;
+      const float sink = whole && a.sink ? in_base2(a.sink[h]) : -INFINITY;
       float mx = sink;
 #pragma unroll
       for (int u = 0; u < kDecWarps; ++u) mx = fmaxf(mx, s_m[u][r]);
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) lm_paged_join_kernel(Paged a,
   if (tok >= q_rows.y) return;
   const bool nothing = n == 0 || paged_length(a, s) - a.tokens + tok < 0;
   auto slot = [&](int i) { return (size_t)(2 * (c0 + i) + (i == 0)) * item_rows + r; };
-  const float sink = a.sink ? a.sink[h] * kPagedLog2e : -INFINITY;
+  const float sink = a.sink ? in_base2(a.sink[h]) : -INFINITY;
   float mx = sink;
   for (int i = lane; i < n; i += 32) mx = fmaxf(mx, w.part_ml[slot(i)].x);
 #pragma unroll

@@ -66,7 +66,7 @@ __device__ __forceinline__ void weigh_keys(const Paged& a, float (&s)[N][4], flo
     for (int i = 0; i < 4; ++i) {
       const int j = j0 + n * 8 + (lane & 3) * 2 + (i & 1), r = i >> 1;
       float x = s[n][i] * a.scale2;
-      if (a.bias && bias[r]) x = fmaf(__ldg(bias[r] + max(0, min(pos[r] - j, a.bias_max))), kPagedLog2e, x);
+      if (a.bias && bias[r]) x += in_base2(__ldg(bias[r] + max(0, min(pos[r] - j, a.bias_max))));
       s[n][i] = ALL || seen_by(a, pos[r], j) ? x : -INFINITY;
       mx[r] = fmaxf(mx[r], s[n][i]);
     }
@@ -272,7 +272,7 @@ __device__ __forceinline__ void paged_prompt_rows(const Paged& a, uint8_t* smem,
   for (int r = 0; r < 2; ++r) {
     if (tok_r[r] >= ntok) continue;
     const int row = wrow + (lane >> 2) + r * 8, h = kvh * a.group + hg_r[r];
-    const float sink = a.sink ? a.sink[h] * kPagedLog2e : -INFINITY, mt = fmaxf(fmaxf(m[r], s_m[row]), sink);
+    const float sink = a.sink ? in_base2(a.sink[h]) : -INFINITY, mt = fmaxf(fmaxf(m[r], s_m[row]), sink);
     const float base = mt == -INFINITY ? 0.0f : mt, f0 = exp2f(m[r] - base), f1 = exp2f(s_m[row] - base);
     const float sum = l[r] * f0 + s_l[row] * f1 + exp2f(sink - base), inv = pos[r] < 0 ? 0.0f : 1.0f / sum;
     const float* so = sO + (size_t)row * a.vdim + (lane & 3) * 2;

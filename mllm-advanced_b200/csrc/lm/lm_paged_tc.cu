@@ -78,14 +78,14 @@ __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) { asm v
 
 __device__ __forceinline__ uint32_t first_bits(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
 
-// One row's scores of a block in tensor memory: bias and mask (written back) and the largest.  first, last: positions of the rows that
+// One row's scores of a block in tensor memory: bias (staged: in shared memory) and mask (written back) and the largest.  first, last: positions of the rows that
 // are worked on together.  Loops over columns are short on purpose: a launch starts with a cold instruction cache.
 template <bool BIAS>
-__device__ __forceinline__ float weigh_block(const Paged& a, uint32_t s_col, const float* bias, float bias_scale, int pos, int first, int last, int j0) {
+__device__ __forceinline__ float weigh_block(const Paged& a, uint32_t s_col, const float* bias, bool staged, int pos, int first, int last, int j0) {
   const bool masked = first < 0 || !seen_by_all(a, first, last, j0, j0 + kTcKeys - 1);
   const int hi = pos - j0, lo = a.window ? hi - a.window : -1, kp = a.window ? a.keep - j0 : 0;  // column i: i <= hi and (i > lo or i < kp)
   const bool near = BIAS && first - (j0 + kTcKeys - 1) < a.bias_max;                               // some distance has a bias of its own
-  const float far = BIAS ? bias[a.bias_max] * bias_scale : 0.0f;
+  const float far = !BIAS ? 0.0f : staged ? bias[a.bias_max] : in_base2(bias[a.bias_max]);
   float top = -INFINITY;
 #pragma unroll 1
   for (int c = 0; c < 128; c += 64) {
@@ -95,11 +95,15 @@ __device__ __forceinline__ float weigh_block(const Paged& a, uint32_t s_col, con
     tmem_ld_wait();
     if (BIAS) {
       if (near) {
+        auto add = [&](auto base2) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
-          uint32_t& x = v[i >> 5][i & 31];
-          x = __float_as_uint(fmaf(__uint_as_float(x), a.scale2, bias[max(0, min(hi - c - i, a.bias_max))] * bias_scale));
-        }
+          for (int i = 0; i < 64; ++i) {
+            uint32_t& x = v[i >> 5][i & 31];
+            x = __float_as_uint(fmaf(__uint_as_float(x), a.scale2, base2(bias[max(0, min(hi - c - i, a.bias_max))])));
+          }
+        };
+        if (staged) add([](float b) { return b; });  // (a table in shared memory is in base 2)
+        else add(in_base2);
       } else {
 #pragma unroll
         for (int i = 0; i < 64; ++i) {
@@ -284,7 +288,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
   float* table = reinterpret_cast<float*>(tc_smem_raw + (values0 + L::kV * L::kTile - smem_u32(tc_smem_raw)));
   if (staged)
     for (int h = warp; h < a.group; h += kTcThreads / 32)
-      for (int i = lane; i <= a.bias_max; i += 32) table[h * pitch + i] = a.bias[(size_t)(kvh * a.group + h) * (a.bias_max + 1) + i] * kPagedLog2e;
+      for (int i = lane; i <= a.bias_max; i += 32) table[h * pitch + i] = in_base2(a.bias[(size_t)(kvh * a.group + h) * (a.bias_max + 1) + i]);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -454,7 +458,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
     const int first = pos0 + t * toks, last = min(p_last, first + toks - 1);  // of this tile
     // (a row that is not there reads the first one's)
     const float* bias = !BIAS ? nullptr : staged ? table + (live ? hg * pitch : 0) : a.bias + (size_t)(live ? head : 0) * (a.bias_max + 1);
-    const float sink = a.sink && live ? a.sink[head] * kPagedLog2e : -INFINITY;
+    const float sink = a.sink && live ? in_base2(a.sink[head]) : -INFINITY;
     const float scale = BIAS ? 1.0f : a.scale2, grown = Num<T>::kLag / scale;  // BIAS: scores are scaled before their maximum
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
@@ -462,7 +466,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
     for (int j = 0; j < n; ++j) {
       ok = ok && __all_sync(0xffffffffu, wait(&bars.s_full[t], (uint32_t)j & 1u));
       tc_fence_after();
-      const float top = weigh_block<BIAS>(a, s_col, bias, staged ? 1.0f : kPagedLog2e, pos, first, last, block_key<kTcKeys>(seen, b0 + j));
+      const float top = weigh_block<BIAS>(a, s_col, bias, staged, pos, first, last, block_key<kTcKeys>(seen, b0 + j));
       if (__any_sync(0xffffffffu, live && top > m + grown)) {
         const float m_new = fmaxf(m, top), alpha = m_new == -INFINITY ? 1.0f : paged_exp2((m - m_new) * scale);
         m = m_new;
@@ -554,7 +558,7 @@ __global__ void __launch_bounds__(256) lm_paged_prompt_join_kernel(Paged a, Prom
     if (r / a.group >= toks || first + tok >= rows.y) continue;
     auto at = [&](int p) { return ((size_t)blockIdx.x * w.parts + p) * 256 + i; };
     const float2 ml = lane < w.parts ? w.part_ml[at(lane)] : make_float2(-INFINITY, 0.0f);
-    const float sink = a.sink ? a.sink[head] * kPagedLog2e : -INFINITY;
+    const float sink = a.sink ? in_base2(a.sink[head]) : -INFINITY;
     float mx = ml.x;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -886,7 +890,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
         for (int c = 0; c < NP; ++c) l[c] = 0.0f;
         sync();  // (the last share's numbers have been read)
         if (tid < NP) s_ref[tid] = tid < rows ? -INFINITY : INFINITY, s_base2[tid] = tid < rows ? 0.0f : -INFINITY;  // (columns without a row: weights of 0)
-        if (BIAS && tid < NP) s_far[tid] = tid < rows ? a.bias[(size_t)(g.kvh * a.group + tid % a.group) * (a.bias_max + 1) + a.bias_max] * kPagedLog2e : 0.0f;
+        if (BIAS && tid < NP) s_far[tid] = tid < rows ? in_base2(a.bias[(size_t)(g.kvh * a.group + tid % a.group) * (a.bias_max + 1) + a.bias_max]) : 0.0f;
         sync();
       }
       ok = ok && all_wait(&bars.s_full[r & 1], (uint32_t)(r >> 1) & 1u);
@@ -906,7 +910,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
 #pragma unroll
             for (int i = 0; i < kC; ++i) {
               const float* table = a.bias + (size_t)(g.kvh * a.group + hg) * (a.bias_max + 1);
-              const float b = c0 + i < rows ? __ldg(table + max(0, min(g.p_first + tok - j, a.bias_max))) * kPagedLog2e : 0.0f;
+              const float b = c0 + i < rows ? in_base2(__ldg(table + max(0, min(g.p_first + tok - j, a.bias_max)))) : 0.0f;
               v[i] = __float_as_uint(fmaf(__uint_as_float(v[i]), a.scale2, b));
               if (++hg == a.group) hg = 0, ++tok;
             }
@@ -1018,7 +1022,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
         const size_t slot = (size_t)(2 * blockIdx.x + g.begins) * item_rows;
         if (tid < rows) {
           const int tok = tid / a.group, head = g.kvh * a.group + tid - tok * a.group;
-          const float ref = s_ref[tid] - kLift, sink = g.whole && a.sink ? a.sink[head] * kPagedLog2e : -INFINITY, most = fmaxf(ref, sink), at = most == -INFINITY ? 0.0f : most;
+          const float ref = s_ref[tid] - kLift, sink = g.whole && a.sink ? in_base2(a.sink[head]) : -INFINITY, most = fmaxf(ref, sink), at = most == -INFINITY ? 0.0f : most;
           const float f = exp2f(ref - at), sum = ((s_max[0][tid] + s_max[1][tid]) + (s_max[2][tid] + s_max[3][tid])) * f + exp2f(sink - at);
           s_alpha[tid] = !g.whole ? f : g.p_first + tok < 0 ? 0.0f : f / sum;
           if (!g.whole) w.part_ml[slot + tid] = make_float2(most, sum);

@@ -89,3 +89,32 @@ def test_many_small_weights_beside_a_large_one(dtype, dim, top, late, value):
         off = (got.cpu().double() - want).abs()
         assert (off <= bound).all(), (float(off.max()), float(bound.min()), float(want.min()))
     paged.check()
+
+
+LOWEST = torch.finfo(torch.float32).min
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim, dtype", [(64, BF16), (128, FP16), (80, BF16)])
+@pytest.mark.parametrize("distances", [40, 3001])
+@pytest.mark.parametrize("sink", [None, 0.5, LOWEST])
+def test_biases_of_the_lowest_value(dim, dtype, distances, sink):
+    """Distance biases that say "as good as unseen" by the type's lowest number: all of them (a row shares its weight out evenly), the
+    near ones (short rows have nothing else), the far ones.  Lowest plus a score is lowest again, in 32 bits and in 64."""
+    lengths, counts, heads = [700, 9, 300, 4], [150, 9, 2, 4], 8
+    c = Cache(lengths, 2, dim, dim, 32, dtype, 6)
+    bias = rand((heads, distances), torch.float32, 7)
+    bias[0::4] = LOWEST
+    bias[1::4, :20] = LOWEST
+    bias[2::4, 20:] = LOWEST
+    sinks = None if sink is None else torch.full((heads,), sink)
+    start, cuda = starts(counts), lambda t: None if t is None else t.cuda()
+    q = rand((sum(counts), heads, dim), dtype, 8)
+    want = attention64(c, counts, q, None, 0, 0, sinks, bias)
+    few = rand((12, heads, dim), dtype, 9)
+    want_few = attention64(c, [3] * 4, few, None, 0, 0, sinks, bias)
+    c.on_gpu()
+    look = dict(sink=cuda(sinks), bias=bias.cuda())
+    check(paged.prompt_attention(q.cuda(), c.k, c.v, c.table, c.lengths, start, **look), *want, dim, dtype, True)
+    check(paged.decode_attention(few.cuda(), c.k, c.v, c.table, c.lengths, **look), *want_few, dim, dtype, False)
+    paged.check()
