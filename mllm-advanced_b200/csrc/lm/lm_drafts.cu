@@ -124,10 +124,11 @@ __global__ void __launch_bounds__(kRowThreads, 2) lm_probability_rows_kernel(con
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
       const int i = item_at<VEC>(part * per, k, me), n = i >= sh && i + 3 < v1 ? kEach : 0;
+      const T* from = z + (n ? i : 0);  // (a group of four begins there also where nothing is read)
       if constexpr (kEach == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(place + (k * kRowThreads + me) * kEach), "l"(n ? z + i : logits), "r"(n) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(place + (k * kRowThreads + me) * kEach), "l"(from), "r"(n) : "memory");
       else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(place + (k * kRowThreads + me) * kEach), "l"(n ? z + i : logits), "r"(n) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(place + (k * kRowThreads + me) * kEach), "l"(from), "r"(n) : "memory");
     }
     paged_commit();
   };

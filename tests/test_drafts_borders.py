@@ -74,3 +74,18 @@ def test_overlapping_rows_of_out_are_refused_on_the_gpu(tmp_path):
     m.step_probabilities([(s, [1, 2, 3])], [0, 2], out=out[:, :211])
     assert (out[:, 211:] == 0).all() and torch.allclose(out.sum(dim=1), torch.ones(2, device="cuda"), atol=1e-5)
     m.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("at", [1, 2, 3])
+def test_many_rows_from_an_odd_address(dtype, at):
+    """Rows that are copied ahead from memory that begins inside a group of four numbers."""
+    rows_, vocab, ld = 700, 1003, 1004
+    logits = torch.randn(at + rows_ * ld, generator=torch.Generator().manual_seed(at)).to(dtype).cuda()[at:].view(rows_, ld)[:, :vocab]
+    whole = torch.full((at + rows_ * ld,), -1.0, device="cuda")
+    out = drafts.probabilities(logits, 0.8, out=whole[at:].view(rows_, ld)[:, :vocab])
+    # (the groups fall otherwise, and with them the order of sums and the threads' maxima: 2^-24 (5 arg + 141) on either side, arg < 12)
+    want = drafts.probabilities(logits.contiguous(), 0.8)
+    assert ((out - want).abs() <= want * 2.0 ** -24 * 2 * (5 * 12 + 141)).all()
+    assert (whole[:at] == -1).all() and (whole[at:].view(rows_, ld)[:, vocab:] == -1).all()
