@@ -200,7 +200,7 @@ MLLMB200_API int mllmb200_lm_attn_prompt(const mllmb200_lm_pages* pages, const m
 
 /* Rows of logits to probabilities: exp((z - max z) / temperature) over their sum; temperature 0: 1 at the first largest.
  * -inf gives 0; a row of nothing but -inf, zeros; a row with NaN or +inf, NaN (temperature 0: NaN is passed over).
- * dtype: MLLMB200_LM_F32, _BF16 or _F16; out fp32. */
+ * dtype: MLLMB200_LM_F32, _BF16 or _F16; out fp32.  vocab: at most 2^30. */
 MLLMB200_API int mllmb200_lm_probabilities(const void* logits, int dtype, long long ld, int rows, int vocab, float temperature,
                                            float* out, long long ld_out, void* stream);
 

@@ -606,6 +606,7 @@ int mllmb200_lm_probabilities(const void* logits, int dtype, long long ld, int r
                               void* stream) {
   if (rows < 0 || vocab < 1 || ld < 0 || ld_out < vocab || !(temperature >= 0.0f) || std::isinf(temperature)) return MLLMB200_INVALID_ARG;
   if (dtype != MLLMB200_LM_F32 && dtype != MLLMB200_LM_BF16 && dtype != MLLMB200_LM_F16) return MLLMB200_UNSUPPORTED;
+  if (vocab > 1 << 30) return MLLMB200_UNSUPPORTED;  // (places in a row, and steps beyond them, are counted in 32 bits)
   if (!rows) return MLLMB200_OK;
   if (!logits || !out) return MLLMB200_INVALID_ARG;
   auto s = static_cast<cudaStream_t>(stream);

@@ -89,3 +89,9 @@ def test_many_rows_from_an_odd_address(dtype, at):
     want = drafts.probabilities(logits.contiguous(), 0.8)
     assert ((out - want).abs() <= want * 2.0 ** -24 * 2 * (5 * 12 + 141)).all()
     assert (whole[:at] == -1).all() and (whole[at:].view(rows_, ld)[:, vocab:] == -1).all()
+
+
+def test_rows_longer_than_32_bits_count_are_refused():
+    L = lm.lib()
+    for vocab in (2 ** 30 + 1, 2 ** 31 - 1):
+        assert L.mllmb200_lm_probabilities(4096, lm.F32, 2 ** 31, 1, vocab, 1.0, 4096, 2 ** 31, None) == 2
