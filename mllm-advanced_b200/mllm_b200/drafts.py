@@ -14,7 +14,7 @@ def probabilities(logits, temperature=1.0, out=None, stream=None):
     temperature 0: 1 at the first largest.  -inf gives 0, a row of nothing else zeros; NaN or +inf make their row NaN."""
     dtype = _DTYPES.get(logits.dtype)
     distance = None if out is None or logits.dim() != 2 else lm.row_distance("probabilities", out, *logits.shape)
-    if not (logits.dim() == 2 and logits.stride(1) == 1 and dtype is not None and logits.is_cuda):
+    if not (logits.dim() == 2 and (logits.shape[1] < 2 or logits.stride(1) == 1) and dtype is not None and logits.is_cuda):
         _refuse("probabilities", (lambda: False, "logits [rows, vocab] in fp32, bf16 or fp16 on the GPU, rows contiguous"))
     rows, vocab = logits.shape
     if out is not None and out.get_device() != logits.get_device():
@@ -50,7 +50,7 @@ def verify(target, draft, tokens, accept, pick, stream=None):
     k, device = places - 1, target.get_device()
     t_seq, t_row, t_one = target.stride()
     if not (k >= 0 and draft.shape == (seqs, k, vocab) and tokens.shape == (seqs, k) and accept.shape == (seqs, k) and pick.shape == (seqs,) and
-            target.dtype == draft.dtype == accept.dtype == pick.dtype == torch.float32 and tokens.dtype == torch.int32 and t_one == 1 and (k == 0 or d_one == 1) and
+            target.dtype == draft.dtype == accept.dtype == pick.dtype == torch.float32 and tokens.dtype == torch.int32 and (vocab < 2 or (t_one == 1 and (k == 0 or d_one == 1))) and
             (k < 2 or (tokens_one == 1 and accept_one == 1)) and (seqs < 2 or pick.stride(0) == 1) and device >= 0 and
             draft.get_device() == tokens.get_device() == accept.get_device() == pick.get_device() == device):
         _refuse("verify", (lambda: k >= 0 and draft.shape == (seqs, k, vocab) and tokens.shape == accept.shape == (seqs, k) and pick.shape == (seqs,), "one place more in the target's probabilities than drafts"),

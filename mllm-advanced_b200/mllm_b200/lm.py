@@ -93,7 +93,7 @@ def distance_buckets(bias_rows, bias_max, count):
 
 def row_distance(where, out, rows, vocab):
     """Numbers from one row of `out`, fp32 [rows, vocab], to the next; a single row's stride says nothing."""
-    if out.shape != (rows, vocab) or str(out.dtype) != "torch.float32" or out.stride(1) != 1:
+    if out.shape != (rows, vocab) or str(out.dtype) != "torch.float32" or (vocab > 1 and out.stride(1) != 1):
         raise ValueError(f"{where}: out [{rows}, {vocab}] in fp32, rows contiguous")
     if rows > 1 and out.stride(0) < vocab:
         raise ValueError(f"{where}: rows of out overlap")

@@ -95,3 +95,15 @@ def test_rows_longer_than_32_bits_count_are_refused():
     L = lm.lib()
     for vocab in (2 ** 30 + 1, 2 ** 31 - 1):
         assert L.mllmb200_lm_probabilities(4096, lm.F32, 2 ** 31, 1, vocab, 1.0, 4096, 2 ** 31, None) == 2
+
+
+@pytest.mark.gpu
+def test_strides_of_a_vocabulary_of_one():
+    """A dimension of one may have any stride."""
+    odd = lambda t, *strides: torch.as_strided(t, t.shape, strides)
+    z, out = torch.randn(3, 1, device="cuda"), torch.zeros(3, 1, device="cuda")
+    assert (drafts.probabilities(odd(z, 1, 7), 0.5, out=odd(out, 1, 5)) == 1.0).all() and (out == 1.0).all()
+    p = torch.ones(2, 2, 1, device="cuda")
+    acc, new = drafts.verify(odd(p, 2, 1, 9), odd(p[:, :1].contiguous(), 1, 1, 4), torch.zeros(2, 1, dtype=torch.int32, device="cuda"), torch.zeros(2, 1, device="cuda") + 0.5,
+                             torch.zeros(2, device="cuda") + 0.5)
+    assert acc.tolist() == [1, 1] and new.tolist() == [[0, 0], [0, 0]]
