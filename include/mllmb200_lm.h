@@ -174,7 +174,7 @@ typedef struct mllmb200_lm_pages {
  * summed in fp32. */
 typedef struct mllmb200_lm_look {
   const void* q;                     /* [rows][heads][dim] */
-  void* out;                         /* [rows][heads][vdim] */
+  void* out;                         /* [rows][heads][vdim], not where q lies */
   long long q_row, q_head, out_row, out_head;
   const float* sink;                 /* [heads] or NULL */
   const float* bias;                 /* [heads][bias_max + 1] or NULL */

@@ -103,6 +103,11 @@ def append(k_pages, v_pages, k, v, table, lengths, q_start=None, stream=None):
         _fail("append", st)
 
 
+def _apart(out, q):
+    """Whether every place of `out` is there once, and not where the queries lie (a block of rows may be done again from them)."""
+    return out.numel() == 0 or (out.data_ptr() != q.data_ptr() and all(n < 2 or s for n, s in zip(out.shape, out.stride())))
+
+
 def _attention(where, q, k_pages, v_pages, table, lengths, q_start, scale, window, keep, sink, bias, out, stream, exact):
     try:
         rows, heads, dim = q.shape
@@ -115,11 +120,11 @@ def _attention(where, q, k_pages, v_pages, table, lengths, q_start, scale, windo
     if not (q.dtype == k_pages.dtype and index == k_pages.get_device() and q_one == 1 and dim == k_dim and
             (sink is None or (sink.dtype == _F32 and sink.shape == (heads,) and sink.is_contiguous() and sink.get_device() == index)) and
             (bias is None or (bias.dtype == _F32 and bias.dim() == 2 and bias.shape[0] == heads and bias.shape[1] > 0 and bias.is_contiguous() and bias.get_device() == index)) and
-            (out is None or (out.shape == (rows, heads, vdim) and out.dtype == q.dtype and out.get_device() == index and out.stride(2) == 1))):
+            (out is None or (out.shape == (rows, heads, vdim) and out.dtype == q.dtype and out.get_device() == index and out.stride(2) == 1 and _apart(out, q)))):
         _refuse(where, (lambda: q.dtype == k_pages.dtype and index == k_pages.get_device() and q_one == 1, "queries of the cache's type and device, rows contiguous"),
                 (lambda: dim == k_dim, "size of queries and keys"), (lambda: sink is None or (sink.dtype == _F32 and sink.shape == (heads,) and sink.is_contiguous() and sink.get_device() == index), "sink [heads] in fp32"),
                 (lambda: bias is None or (bias.dtype == _F32 and bias.dim() == 2 and bias.shape[0] == heads and bias.shape[1] > 0 and bias.is_contiguous() and bias.get_device() == index), "bias [heads, distances] in fp32"),
-                (lambda: False, "out [rows, heads, vdim] of the queries' type, rows contiguous"))
+                (lambda: False, "out [rows, heads, vdim] of the queries' type, rows contiguous, every place once and not the queries' own"))
     L = lm.lib()
     decode = q_start is None
     key = (decode, rows, heads, kv_heads, dim, vdim, seqs) if decode else (rows, heads, kv_heads, dim, vdim, table.shape, k_pages.shape[2], window, keep)
@@ -159,7 +164,7 @@ def decode_attention(q, k_pages, v_pages, table, lengths, scale=None, window=0, 
 
     A token at position i sees key j if j <= i and (no window, or j > i - window, or j < keep).  Scores are scale q.k (default
     dim ** -0.5) + bias[head, min(i - j, distances - 1)]; sink: one more score per head, without a value.  A token that sees
-    nothing gives zeros."""
+    nothing gives zeros.  `out` must not overlap the queries."""
     return _attention("decode_attention", q, k_pages, v_pages, table, lengths, None, scale, window, keep, sink, bias, out, stream, False)
 
 

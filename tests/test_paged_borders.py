@@ -105,3 +105,21 @@ def test_tensors_dropped_behind_a_call_on_a_stream():
         torch.cuda.synchronize()
         assert torch.equal(got, want[i])
         del junk
+
+
+def test_outputs_that_overlap():
+    q = torch.zeros(3, 4, 64)
+    assert paged._apart(torch.zeros(3, 4, 64), q) and paged._apart(torch.zeros(6, 9, 64)[::2, 1:5], q) and paged._apart(torch.zeros(64).expand(1, 1, 64), q)
+    assert not paged._apart(q, q) and not paged._apart(torch.zeros(1, 4, 64).expand(3, 4, 64), q) and not paged._apart(torch.zeros(3, 1, 64).expand(3, 4, 64), q)
+    assert paged._apart(q[:0], q)
+
+
+@pytest.mark.gpu
+def test_outputs_that_overlap_are_refused():
+    c = Cache([30, 40], 2, 64, 64, 16, BF16, 14).on_gpu()
+    q, start = rand((2, 4, 64), BF16, 15).cuda(), torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    for out in (q, torch.zeros(1, 4, 64, dtype=BF16, device="cuda").expand(2, 4, 64)):
+        with pytest.raises(ValueError, match="every place once"):
+            paged.decode_attention(q, c.k, c.v, c.table, c.lengths, out=out)
+        with pytest.raises(ValueError, match="every place once"):
+            paged.prompt_attention(q, c.k, c.v, c.table, c.lengths, start, out=out)
