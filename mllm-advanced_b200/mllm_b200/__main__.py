@@ -50,7 +50,13 @@ def trace(args):
 
 
 def main(argv=None):
-    args = parser().parse_args(argv)
+    ap = parser()
+    args = ap.parse_args(argv)
+    if args.command == "generate":
+        if args.pages and not args.page:
+            ap.error("--pages says nothing without --page")
+        if args.temperature and not args.draft:
+            ap.error("--temperature wants --draft: without it generation is greedy")
     from . import registry
     if args.command == "info":
         cfg = registry.read_config(args.model)
