@@ -1541,6 +1541,18 @@ int mllmb200_lm_create(const mllmb200_lm_config* cfg, const mllmb200_lm_layer* l
   *handle = e;
   return MLLMB200_OK;
 }
+// The symbol of callers whose structures end in front of `page` and `window`.
+#undef mllmb200_lm_create
+MLLMB200_API int mllmb200_lm_create(const void* cfg, const void* layers, void** handle) {
+  if (!cfg || !layers || !handle) return MLLMB200_INVALID_ARG;
+  constexpr size_t kConfig = offsetof(mllmb200_lm_config, page), kLayer = (offsetof(mllmb200_lm_layer, window) + alignof(mllmb200_lm_layer) - 1) / alignof(mllmb200_lm_layer) * alignof(mllmb200_lm_layer);
+  mllmb200_lm_config c{};
+  std::memcpy(&c, cfg, kConfig);
+  if (c.layers < 1) return MLLMB200_INVALID_ARG;
+  std::vector<mllmb200_lm_layer> all(c.layers);
+  for (int i = 0; i < c.layers; ++i) std::memcpy(&all[i], static_cast<const char*>(layers) + i * kLayer, offsetof(mllmb200_lm_layer, window));
+  return mllmb200_lm_create_paged(&c, all.data(), handle);
+}
 void mllmb200_lm_destroy(void* handle) {
   if (handle) destroy(from(handle));
 }

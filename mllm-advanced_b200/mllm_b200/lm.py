@@ -59,7 +59,7 @@ def lib():
         raise ImportError(f"{lib_path()} is missing: build it with mllm-advanced_b200/build.sh lm; there is no CPU fallback")
     L = C.CDLL(lib_path())
     vp, ci, ll = C.c_void_p, C.c_int, C.c_longlong
-    sig = {"create": [C.POINTER(Config), C.POINTER(Layer), C.POINTER(vp)], "set_tensor": [vp, ci, ci, vp, ci, ci],
+    sig = {"create_paged": [C.POINTER(Config), C.POINTER(Layer), C.POINTER(vp)], "set_tensor": [vp, ci, ci, vp, ci, ci],
            "set_expert": [vp, ci, ci, ci, vp, ci, ci],
            "step": [vp, ci, vp, vp, vp, ci, vp, vp, ci], "decode": [vp, ci, vp, ci], "free_slot": [vp, ci],
            "step_probabilities": [vp, ci, vp, vp, vp, ci, vp, C.c_float, vp, ll], "truncate": [vp, ci, ci], "free_pages": [vp, vp],
@@ -118,7 +118,7 @@ class LanguageModel:
         self.page, self.pages = self.config["page"], self.config["pages"]
         self._L, self._h = lib(), C.c_void_p()
         descs = (Layer * len(layers))(*[Layer(**d) for d in self.layers])
-        st = self._L.mllmb200_lm_create(C.byref(Config(**self.config)), descs, C.byref(self._h))
+        st = self._L.mllmb200_lm_create_paged(C.byref(Config(**self.config)), descs, C.byref(self._h))
         if st:
             raise EngineError(st, "create", self._L.mllmb200_lm_last_error(None).decode())
         self.length = [0] * self.max_seqs

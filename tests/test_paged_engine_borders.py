@@ -1,9 +1,11 @@
 """The language-model engine on pages at its borders: windows of any size, slots taken back after their windows have left pages behind."""
+import ctypes as C
 import os
 import sys
 
 import numpy as np
 import pytest
+import torch
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, os.path.join(ROOT, "oracle"))
@@ -94,3 +96,41 @@ def test_drafts_behind_long_prompts_over_windows(tmp_path):
     for c in (case, other):
         c.model.check_device_status()
         c.model.close()
+
+
+# the structures of callers that were built before there were pages
+class OldConfig(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("vocab", "width", "layers", "dtype", "conv_taps", "max_seqs", "max_ctx", "max_rows")] + \
+               [("eps", C.c_float), ("logit_scale", C.c_float), ("norm_place", C.c_int), ("residual_scale", C.c_float)]
+
+
+class OldLayer(C.Structure):
+    _fields_ = lm.Layer._fields_[:-2]
+
+
+def old_structures(layers):
+    cfg = M.config(64, 50, [M.layer("attention", M.attention(2, 1, 16, 16, 37), 32)] * layers)
+    now = [{"sink": 0, "bias_rows": 0, "bias_max": 0, "rot_dims": 0, "rot_base": 1.0, "ff": 0, "ff_limit": 0.0, "score_scale": 1.0, "weights_of": -1, "kv_rank": 0,
+            "kv_from": -1, "act": lm.CLAMPED, "experts": 0, "top": 0, **d} for d in vupuzen.layers_from_config(cfg, lambda i: 10)]
+    names = [n for n, *_ in OldLayer._fields_]
+    descs = (OldLayer * layers)(*[OldLayer(**{n: d[n] for n in names}) for d in now])
+    c = {**vupuzen.model_config(cfg, 1, 64, 64), "layers": layers, "dtype": lm.BF16, "norm_place": lm.NORM_SANDWICH, "residual_scale": 1.0}
+    return OldConfig(**{n: c[n] for n, *_ in OldConfig._fields_}), descs
+
+
+@pytest.mark.parametrize("layers", [1, 5])
+def test_structures_of_older_callers(layers):
+    """What lies behind a shorter structure is not read as pages: the model is as good as it was then (without a GPU: as far as its
+    sizes are looked at)."""
+    assert C.sizeof(OldLayer) < C.sizeof(lm.Layer)
+    config, descs = old_structures(layers)
+    noise = (C.c_char * 4096).from_buffer(bytearray(b"\xff" * 4096))
+    C.memmove(noise, C.byref(config), C.sizeof(config))
+    C.memmove(C.byref(noise, 2048), descs, C.sizeof(descs))
+    h, L = C.c_void_p(), C.CDLL(lm.lib_path())
+    st = L.mllmb200_lm_create(noise, C.byref(noise, 2048), C.byref(h))
+    assert st == (0 if torch.cuda.is_available() else 3)
+    if st == 0:
+        n = C.c_int()
+        assert L.mllmb200_lm_free_pages(h, C.byref(n)) == 0 and n.value == 0
+        L.mllmb200_lm_destroy(h)
