@@ -6,6 +6,11 @@ generate_drafted samples at a temperature, with a second model that proposes tok
 from collections import deque
 
 
+def pages_to_come(model, slot, most):
+    """Pages that a slot has still to take until it holds `most`."""
+    return most - -(-model.length[slot] // model.page)
+
+
 class Request:
     def __init__(self, prompt, max_new, stop=()):
         self.prompt, self.max_new, self.stop = [int(t) for t in prompt], int(max_new), frozenset(stop)
@@ -25,8 +30,12 @@ class Scheduler:
         self.page, self.pages = getattr(model, "page", 0), getattr(model, "pages", 0)
 
     def _pages(self, r):
-        """Pages that a request holds at most (a model with pages: what is admitted always finds them)."""
+        """Pages that a request holds at most."""
         return (len(r.prompt) + r.max_new + self.page - 1) // self.page if self.page else 0
+
+    def _room(self, r):
+        """Whether a request finds its pages beside what those that run have still to take, whoever else holds some."""
+        return not self.page or sum(pages_to_come(self.model, x.slot, self._pages(x)) for x in self.running) + self._pages(r) <= self.model.free_pages()
 
     def submit(self, prompt, max_new, stop=()):
         r = Request(prompt, max_new, stop)
@@ -41,7 +50,7 @@ class Scheduler:
 
     def _admit(self):
         while self.waiting:
-            if sum(self._pages(r) for r in self.running) + self._pages(self.waiting[0]) > self.pages:
+            if not self._room(self.waiting[0]):
                 return
             slot = self.model.acquire()
             if slot is None:
@@ -92,6 +101,8 @@ class Scheduler:
         """Until every submitted request is finished."""
         while self.waiting or self.running:
             self._admit()
+            if not self.running:
+                raise RuntimeError("no slot or too few pages for a request: others hold them")
             if any(r.done < len(r.prompt) for r in self.running):
                 self._mixed_step()
             else:
@@ -129,9 +140,15 @@ def generate_drafted(model, draft, prompts, max_new, drafts=4, temperature=0.0, 
         if not len(p) or max_new < 1 or len(p) + max_new > min(model.max_ctx, draft.max_ctx):
             raise ValueError("a request needs a prompt, at least one new token, and room for both in a slot of both models")
     held = lambda m, n: -(-(n + max_new) // m.page) if m.page else 0  # pages that a prompt of n tokens and what follows it take
+    roles = lambda m: (m is model) + (m is draft)
     for m in (model, draft):
-        if any(held(m, len(p)) > m.pages for p in prompts):
+        if any(held(m, len(p)) * roles(m) > m.pages for p in prompts):
             raise ValueError(f"a request does not fit {m.pages} pages of {m.page}")
+
+    def room(m, n):  # whether a prompt of n tokens finds its pages beside what the others have still to take
+        to_come = lambda r: sum(pages_to_come(m, s, held(m, r.start)) for x, s in ((model, r.slot), (draft, r.draft_slot)) if x is m)
+        return not m.page or sum(map(to_come, running.values())) + held(m, n) * roles(m) <= m.free_pages()
+
     gen = torch.Generator(device="cuda").manual_seed(seed)
     rand = lambda *shape: torch.rand(shape, generator=gen, device="cuda")
 
@@ -174,7 +191,7 @@ def generate_drafted(model, draft, prompts, max_new, drafts=4, temperature=0.0, 
 
     while waiting or running:
         while waiting:
-            if any(sum(held(m, r.start) for r in running.values()) + held(m, len(waiting[0][1])) > m.pages for m in (model, draft)):
+            if not all(room(m, len(waiting[0][1])) for m in (model, draft)):
                 break
             slots = model.acquire(), draft.acquire()
             if None in slots:
@@ -185,6 +202,8 @@ def generate_drafted(model, draft, prompts, max_new, drafts=4, temperature=0.0, 
             i, p = waiting.popleft()
             running[i] = _Drafted(p, max_new, stop, slots)
             read(model, slots[0], running[i].tokens[:-1])
+        if not running:
+            raise RuntimeError("no slot or too few pages for a request: others hold them")
         batch = list(running.values())
         most = max(1, min(model.max_rows // (drafts + 1), draft.max_rows))
         for b in range(0, len(batch), most):
