@@ -189,30 +189,36 @@ def generate_drafted(model, draft, prompts, max_new, drafts=4, temperature=0.0, 
                 if not r.finished:
                     r.tokens.append(t)
 
-    while waiting or running:
-        while waiting:
-            if not all(room(m, len(waiting[0][1])) for m in (model, draft)):
-                break
-            slots = model.acquire(), draft.acquire()
-            if None in slots:
-                for m, s in zip((model, draft), slots):
-                    if s is not None:
-                        m.release(s)
-                break
-            i, p = waiting.popleft()
-            running[i] = _Drafted(p, max_new, stop, slots)
-            read(model, slots[0], running[i].tokens[:-1])
-        if not running:
-            raise RuntimeError("no slot or too few pages for a request: others hold them")
-        batch = list(running.values())
-        most = max(1, min(model.max_rows // (drafts + 1), draft.max_rows))
-        for b in range(0, len(batch), most):
-            round_of(batch[b:b + most])
-        for i in [i for i, r in running.items() if r.finished]:
-            r = running.pop(i)
-            out[i] = r.tokens[r.start:]
+    try:
+        while waiting or running:
+            while waiting:
+                if not all(room(m, len(waiting[0][1])) for m in (model, draft)):
+                    break
+                slots = model.acquire(), draft.acquire()
+                if None in slots:
+                    for m, s in zip((model, draft), slots):
+                        if s is not None:
+                            m.release(s)
+                    break
+                i, p = waiting.popleft()
+                running[i] = _Drafted(p, max_new, stop, slots)
+                read(model, slots[0], running[i].tokens[:-1])
+            if not running:
+                raise RuntimeError("no slot or too few pages for a request: others hold them")
+            batch = list(running.values())
+            most = max(1, min(model.max_rows // (drafts + 1), draft.max_rows))
+            for b in range(0, len(batch), most):
+                round_of(batch[b:b + most])
+            for i in [i for i, r in running.items() if r.finished]:
+                r = running.pop(i)
+                out[i] = r.tokens[r.start:]
+                model.release(r.slot)
+                draft.release(r.draft_slot)
+    except BaseException:
+        for r in running.values():
             model.release(r.slot)
             draft.release(r.draft_slot)
+        raise
     return out
 
 
