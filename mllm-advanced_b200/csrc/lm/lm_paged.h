@@ -30,12 +30,12 @@ struct Paged {
 };
 
 constexpr float kPagedLog2e = 1.4426950408889634f;
-// A bias or a sink for scores in base 2.  What is finite stays finite: a type's lowest value stands for "as good as unseen", and a row that
-// has nothing else shares its weight out evenly.
+// A bias or a sink for scores in base 2.  The type's lowest value stays finite: it stands for "as good as unseen", and a row that has nothing
+// else shares its weight out evenly.  (-inf and NaN stay what they are.)
 __device__ __forceinline__ float in_base2(float x) {
-  constexpr float kMost = 3.402823466e+38f;
-  const float y = x * kPagedLog2e;
-  return fabsf(x) <= kMost ? fminf(fmaxf(y, -kMost), kMost) : y;
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x * kPagedLog2e), "f"(fminf(x, -3.402823466e+38f)));
+  return y;
 }
 constexpr int kLongest = 1 << 30;  // positions that a table's row can name, at most
 
