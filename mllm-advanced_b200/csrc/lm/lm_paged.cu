@@ -430,7 +430,7 @@ int check_pages(const mllmb200_lm_pages* p, Paged* a) {
   a->pages = p->pages, a->page = p->page, a->kv_heads = p->kv_heads, a->dim = p->dim, a->vdim = p->vdim;
   a->ld_table = p->ld_table, a->max_pages = p->max_pages, a->seqs = p->seqs, a->rows = p->rows;
   a->tokens = p->q_start || !p->seqs ? 0 : p->rows / p->seqs;
-  a->reports = kDevStatusOfOperators;
+  a->bad_page <<= kDevStatusOfOperators, a->timeout <<= kDevStatusOfOperators;
   return MLLMB200_OK;
 }
 int check_look(const mllmb200_lm_pages* p, const mllmb200_lm_look* l, Paged* a) {

@@ -26,7 +26,7 @@ struct Paged {
   int heads, group, bias_max, window, keep;
   int exact;           // prompts on tcgen05: weights in two halves of 16 bits
   float scale2;        // scale log2(e): scores are in base 2
-  unsigned reports;    // places by which this call's bits of the status word are shifted: 0 in the engine, else kDevStatusOfOperators
+  unsigned bad_page = kDevStatusBadPage, timeout = kDevStatusTimeout;  // what this call reports in the status word: the engine's bits, or the operators'
 };
 
 constexpr float kPagedLog2e = 1.4426950408889634f;
@@ -42,14 +42,14 @@ constexpr int kLongest = 1 << 30;  // positions that a table's row can name, at 
 // A sequence's length, cut to what its row of the table can name.
 __device__ __forceinline__ int paged_length(const Paged& a, int s) {
   const int n = a.lengths[s], most = a.max_pages * a.page;
-  if (n > most) atomicOr(&g_device_status, kDevStatusBadPage << a.reports);
+  if (n > most) atomicOr(&g_device_status, a.bad_page);
   return max(0, min(n, most));
 }
 // Page number of a table place, or -1.
 __device__ __forceinline__ int paged_page(const Paged& a, int s, int place) {
   int p = place < a.max_pages ? __ldg(a.table + (size_t)s * a.ld_table + place) : -1;
   if (p < 0 || p >= a.pages) {
-    atomicOr(&g_device_status, kDevStatusBadPage << a.reports);
+    atomicOr(&g_device_status, a.bad_page);
     p = -1;
   }
   return p;

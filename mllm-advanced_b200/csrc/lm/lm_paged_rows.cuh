@@ -60,13 +60,22 @@ template <class T, int N, bool ALL>
 __device__ __forceinline__ void weigh_keys(const Paged& a, float (&s)[N][4], float (&m)[2], float (&l)[2], float (&alpha)[2], int j0, int lane,
                                            const int (&pos)[2], const float* const (&bias)[2]) {
   float mx[2] = {m[0], m[1]};
+  const float scale = a.bias ? 1.0f : a.scale2;
+  if (a.bias) {  // (apart: without biases its instructions would cost 2-4 % all the same)
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = j0 + n * 8 + (lane & 3) * 2 + (i & 1), r = i >> 1;
+        s[n][i] = fmaf(s[n][i], a.scale2, bias[r] ? in_base2(__ldg(bias[r] + max(0, min(pos[r] - j, a.bias_max)))) : 0.0f);
+      }
+  }
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int j = j0 + n * 8 + (lane & 3) * 2 + (i & 1), r = i >> 1;
-      float x = s[n][i] * a.scale2;
-      if (a.bias && bias[r]) x += in_base2(__ldg(bias[r] + max(0, min(pos[r] - j, a.bias_max))));
+      const float x = s[n][i] * scale;
       s[n][i] = ALL || seen_by(a, pos[r], j) ? x : -INFINITY;
       mx[r] = fmaxf(mx[r], s[n][i]);
     }

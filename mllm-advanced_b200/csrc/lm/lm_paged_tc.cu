@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) lm_paged_prompt_tc_kernel(const
     const int j0 = block_key<kTcKeys>(seen, b0 + j);
     return pos0 < 0 || !seen_by_all(a, pos0, p_last, j0, j0 + kTcKeys - 1);
   };
-  auto bounded = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, 1ll << 31, kDevStatusTimeout << a.reports); };
+  auto bounded = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, 1ll << 31, a.timeout); };
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return true;
     if (s_gave_up) return false;
@@ -704,7 +704,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) lm_paged_decode_tc_kernel(cons
   tc_fence_after();
   pdl_launch_dependents();  // (as above)
   const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
-  auto bounded = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, 1ll << 31, kDevStatusTimeout << a.reports); };
+  auto bounded = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, 1ll << 31, a.timeout); };
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return true;
     if (s_gave_up) return false;
