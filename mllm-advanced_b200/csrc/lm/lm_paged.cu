@@ -424,7 +424,7 @@ int check_pages(const mllmb200_lm_pages* p, Paged* a) {
   if (p->kv_heads == 1) a->k_head = p->k_row, a->v_head = p->v_row;
   if (p->pages == 1) a->k_page = p->k_row, a->v_page = p->v_row;
   if (!aligned(p->k, a->k_page, a->k_head, a->k_row) || !aligned(p->v, a->v_page, a->v_head, a->v_row)) return MLLMB200_INVALID_ARG;
-  if (!p->q_start && p->seqs && p->rows % p->seqs) return MLLMB200_INVALID_ARG;
+  if (!p->q_start && (p->seqs ? p->rows % p->seqs : p->rows)) return MLLMB200_INVALID_ARG;  // (rows that are nobody's would be left as they are)
   a->k = p->k, a->v = p->v;
   a->table = p->table, a->lengths = p->lengths, a->q_start = p->q_start;
   a->pages = p->pages, a->page = p->page, a->kv_heads = p->kv_heads, a->dim = p->dim, a->vdim = p->vdim;

@@ -1,10 +1,12 @@
 """Operators over pages at their borders: lengths beyond a table, tensors of other streams, odd arguments."""
 import contextlib
+import ctypes as C
 import pytest
 import torch
 
 from mllm_b200 import drafts, lm, paged
 from paged_case import Cache
+from test_paged import good
 
 BF16 = torch.bfloat16
 
@@ -123,3 +125,14 @@ def test_outputs_that_overlap_are_refused():
             paged.decode_attention(q, c.k, c.v, c.table, c.lengths, out=out)
         with pytest.raises(ValueError, match="every place once"):
             paged.prompt_attention(q, c.k, c.v, c.table, c.lengths, start, out=out)
+
+
+def test_rows_without_sequences_are_refused():
+    """Rows that belong to no sequence have no answer; with row starts they lie behind the last sequence and are left as they are."""
+    p, look = good()
+    p.seqs, L, size = 0, lm.lib(), C.c_size_t()
+    assert L.mllmb200_lm_attn_decode_workspace(bytes(p), bytes(look), C.byref(size)) == 1
+    assert L.mllmb200_lm_attn_decode(bytes(p), bytes(look), 4096, None) == 1
+    assert L.mllmb200_lm_pages_append(bytes(p), 4096, 128, 64, 4096, 128, 64, None) == 1
+    p.q_start = 4096
+    assert L.mllmb200_lm_attn_prompt(bytes(p), bytes(look), 4096, None) == 0
