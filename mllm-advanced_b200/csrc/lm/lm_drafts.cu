@@ -101,6 +101,8 @@ __device__ __forceinline__ int element(int i, int e) { return VEC ? i + e : i + 
 // VEC: rows of logits and of probabilities lie alike in groups of four numbers, a row's first number `sh` places into one.
 // AHEAD: grid (cluster, fewer than the rows): a cluster takes every gridDim.y-th row, and copies the next one into shared memory, each
 // thread its own numbers, as soon as it has the current one in registers.
+// Everything is fp32.  A number passes two exponentials of the special-function unit (2^-22 of the result each), a sum up to four: 1.08e-7 of
+// the 2-norm off; with the library's exponential for the numbers 1.06e-7, and 3 % slower.
 // 384 rows of 151936, one call after the other: 95 us, 96 with an odd distance of rows, 94 from bf16.  452 with three passes of scalar loads
 // over the row, 115 with four barriers and exact exponentials, 105 where all warps send to all CTAs and so wait for their stores
 // of the row before, 416 where rows of an odd distance are read number by number.

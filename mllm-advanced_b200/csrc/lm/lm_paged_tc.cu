@@ -12,13 +12,13 @@
 //                   done again row-block by row-block on mma.sync (paged_prompt_rows), which can.
 // EXACT: a weight is two numbers of 16 bits, the second what the first one's rounding left, and both meet the values.  Without it the weights'
 // rounding (2^-9 of each in bf16, independent) is of the size of the output's own: 2.0e-3 of the 2-norm off instead of 1.5e-3.  The caller
-// chooses: half the products more and their making cost 8192 tokens of 16 / 4 heads of 128 a third (284 and 376 us), and the engine, whose
+// chooses: half the products more and their making cost 8192 tokens of 16 / 4 heads of 128 a third (284 and 376 us a call), and the engine, whose
 // attention over slots carries two numbers, takes EXACT.  Everything else is fp32.
-// Measured on a B200: 8192 tokens, 16 / 4 heads of 128, causal: 243 us (1.13 PFLOP/s, tensor pipe 53 % active); 2571 rows of five sequences with
-// a window of 512, 12 / 2 heads: 27.  Bound by the chain of a tile: scores, their maximum, weights, product; with two tiles a
+// Measured on a B200: 8192 tokens, 16 / 4 heads of 128, causal: 277-284 us a call with inputs from memory (0.97 PFLOP/s, tensor pipe 52 %
+// active; EXACT 60 %), 243 (1.13 PFLOP/s; EXACT 323) back to back in a graph; 2571 rows of five sequences with a window of 512, 12 / 2 heads: 27.  Bound by the chain of a tile: scores, their maximum, weights, product; with two tiles a
 // block takes 3900 cycles of which the products need 2048.  Two tiles and not one, since one tile's products hide the other's
-// weights; not three, since S and O of two fill tensor memory's 512 columns.  Scores handed over by halves of 64 keys were slower (276 us:
-// twice the waits for the same chain).
+// weights; not three, since S and O of two fill tensor memory's 512 columns.  Scores handed over by halves of 64 keys were slower (276 us
+// in that graph: twice the waits for the same chain).
 #include <algorithm>
 #include <atomic>
 #include <mutex>
