@@ -1,4 +1,6 @@
 """How exactly the softmax weights of attention over pages enter the product with the values."""
+import os
+import re
 import types
 
 import numpy as np
@@ -118,3 +120,26 @@ def test_biases_of_the_lowest_value(dim, dtype, distances, sink):
     check(paged.prompt_attention(q.cuda(), c.k, c.v, c.table, c.lengths, start, **look), *want, dim, dtype, True)
     check(paged.decode_attention(few.cuda(), c.k, c.v, c.table, c.lengths, **look), *want_few, dim, dtype, False)
     paged.check()
+
+
+def test_polynomial_of_the_exponential():
+    """The exponential that every fourth pair of weights takes (pair_exp2 of lm_paged_tc.cu, its constants read from there), in fp32 as the
+    kernel computes it: off by 2^-18 of the result at most, 0 below 2^-126."""
+    source = open(os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "mllm-advanced_b200", "csrc", "lm", "lm_paged_tc.cu")).read()
+    body = source[source.index("float2 pair_exp2("):source.index("// weights 2^(score scale + base)")]
+    c = [np.float32(x) for x in re.findall(r"pair_of\((0\.\d+)f, \1f\)", body)]
+    big = np.float32(re.search(r"pair_of\((\d+\.0)f", body).group(1))
+    assert len(c) == 5 and big == np.float32(1.5 * 2 ** 23 + 127)
+    fma = lambda a, b, d: (a.astype(np.float64) * np.float64(b) + np.float64(d)).astype(np.float32)  # (a product of two is exact in 64 bits)
+    mul = lambda a, b: a.astype(np.float64) * b.astype(np.float64)
+    x = np.concatenate([np.linspace(-126, 16, 2_000_003), np.linspace(-2, 2, 500_001)]).astype(np.float32)
+    t = x + big
+    f = x - (t - big)
+    p = fma(f, c[0], c[1])
+    for k in c[2:]:
+        p = (mul(p, f) + np.float64(k)).astype(np.float32)
+    got = mul(p, (t.view(np.uint32) << 23).view(np.float32))
+    want = np.exp2(x.astype(np.float64))
+    assert np.abs(got / want - 1).max() <= 2.0 ** -18
+    t = np.float32(-127) + big
+    assert (np.array([t]).view(np.uint32) << 23).view(np.float32)[0] == 0
