@@ -112,7 +112,8 @@ MLLMB200_API int mllmb200_lm_step_probabilities(void* handle, int entries, const
 
 /* Takes a slot back to its first `length` tokens (drafted tokens that did not stand).  MLLMB200_UNSUPPORTED where layers
  * have state that cannot go back (retention, an input convolution); MLLMB200_INVALID_ARG beyond the slot's tokens, or where
- * pages that the tokens would see again have been given up (never for the last 64 tokens, nor for those of the last step). */
+ * pages that the tokens would see again have been given up: never down to 64 tokens before the place where the slot's furthest step (or
+ * decode) began, however often it is taken back meanwhile.  Nothing is changed then. */
 MLLMB200_API int mllmb200_lm_truncate(void* handle, int slot, int length);
 
 /* Pages that no slot holds (0 without pages). */

@@ -1171,7 +1171,7 @@ std::pair<int, int> left_behind(const Engine* e, int s) {
 }
 // Takes the pages for every slot's first `length` positions, after what the windows have left behind has been given up (what runs on
 // the stream still reads it, and whoever takes it writes behind that).  This happens when a slot moves on, not at a step's end: it
-// can be taken back to where its last step began, and by kRewind tokens.  False, and nothing changed: too few are free.
+// can be taken back to kRewind tokens before where its furthest step began.  False, and nothing changed: too few are free.
 bool move_on(Engine* e, int count, const int* slots, const std::vector<int>& length, long long* lacking, long long* there) {
   *lacking = 0;
   *there = (long long)e->free_pages.size();

@@ -209,7 +209,8 @@ class LanguageModel:
         return out
 
     def truncate(self, slot, length):
-        """Takes a slot back to its first `length` tokens (not with retention or an input convolution)."""
+        """Takes a slot back to its first `length` tokens (not with retention or an input convolution; where every layer has a window, as far as
+        64 tokens before the place where its furthest step or decode began, and further while the pages are there)."""
         self._check(self._L.mllmb200_lm_truncate(self._h, slot, length), "truncate")
         self.length[slot] = length
 

@@ -79,6 +79,26 @@ def test_taken_back_after_pages_were_given_up(tmp_path):
 
 
 @gpu
+def test_taken_back_several_times(tmp_path):
+    """How far a slot can be taken back goes by its furthest step, not by where it is when it is taken back."""
+    case = Case(tmp_path, ((24, 2), (20, 1)), 40)
+    m, tokens = case.model, case.tokens(230)
+    want, s = case.oracle(tokens), case.model.acquire()
+    for a, b in ((0, 150), (150, 190), (190, 200)):
+        m.step([(s, tokens[a:b])])
+    free = m.free_pages()
+    m.truncate(s, 160)
+    m.step([(s, tokens[160:161])])
+    m.truncate(s, 126)  # the furthest step began at 190
+    assert m.free_pages() == free + 13 - 8
+    with pytest.raises(lm.EngineError) as e:  # (64 tokens of where it is now, but what they see went when it moved on from 190)
+        m.truncate(s, 62)
+    assert e.value.status == 1 and m.length[s] == 126 and m.free_pages() == free + 13 - 8
+    case.check(m.step([(s, tokens[126:230])], range(104)), want[126:230])
+    m.close()
+
+
+@gpu
 def test_drafts_behind_long_prompts_over_windows(tmp_path):
     """Prompts that the windows have left pages of, one request after the other: the model's own greedy tokens, but for near ties (a step
     of other shapes rounds otherwise)."""
