@@ -85,7 +85,8 @@ enum {
 };
 
 /* (Structures grow at their ends, and the symbol says which ones are meant: what was built before `page` and `window` were there calls the
- * symbol mllmb200_lm_create with structures that end in front of them.) */
+ * symbol mllmb200_lm_create with structures that end in front of them.  A program that was built with `page` and the old symbol has to be
+ * built again.) */
 #define mllmb200_lm_create mllmb200_lm_create_paged
 MLLMB200_API int mllmb200_lm_create(const mllmb200_lm_config* cfg, const mllmb200_lm_layer* layers, void** handle);
 MLLMB200_API void mllmb200_lm_destroy(void* handle);
